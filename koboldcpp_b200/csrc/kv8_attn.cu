@@ -1,0 +1,583 @@
+// kv8_attn.cu -- attention over the paged 8-bit cache (include/b200_kv8.h: b200_op_kv8_attn).
+#include <cfloat>
+#include <type_traits>
+
+#include "kv8.cuh"
+
+namespace b200 {
+namespace kv8 {
+
+// ------------------------------------------------------------------------------------------------ shared by the kernels
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+// x < 2^e for the magnitude with these bits, e >= -100
+__device__ __forceinline__ int exponent_above(unsigned bits) { return max((int)(bits >> 23) - 126, -100); }
+__device__ __forceinline__ unsigned pack_half(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const unsigned *>(&h);
+}
+// what the f16 pair `hi` leaves over of (a, b), as another pair
+__device__ __forceinline__ unsigned pack_rest(float a, float b, unsigned hi) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+    return pack_half(a - f.x, b - f.y);
+}
+// Four int8 as f16, exactly: a byte with its sign flipped is x + 128, behind 0x64 it is the f16 1024 + 128 + x.
+__device__ __forceinline__ unsigned less_1152(unsigned u) {
+    const unsigned c = 0x64806480u;
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&u), *reinterpret_cast<const __half2 *>(&c));
+    return *reinterpret_cast<const unsigned *>(&r);
+}
+__device__ __forceinline__ void int4_to_half(unsigned w, unsigned &lo, unsigned &hi) {
+    w ^= 0x80808080u;
+    lo = less_1152(prmt(w, 0x64646464u, 0x4140));
+    hi = less_1152(prmt(w, 0x64646464u, 0x4342));
+}
+// value i of two words as a pair, i = 0 .. 3: the k side of an MMA's second operand runs along the keys, which lie in different rows
+__device__ __forceinline__ void pairs_to_half(unsigned a, unsigned b, unsigned (&p)[4]) {
+    const unsigned lo = prmt(a, b, 0x5140) ^ 0x80808080u, hi = prmt(a, b, 0x7362) ^ 0x80808080u;
+    p[0] = less_1152(prmt(lo, 0x64646464u, 0x4140));
+    p[1] = less_1152(prmt(lo, 0x64646464u, 0x4342));
+    p[2] = less_1152(prmt(hi, 0x64646464u, 0x4140));
+    p[3] = less_1152(prmt(hi, 0x64646464u, 0x4342));
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 16 values of a row of q or dst, whose type is an argument
+__device__ __forceinline__ void row_load16(const void *row, int type, int64_t at, float (&x)[16]) {
+    if (type == B200_TYPE_F32) load16<float, false>(reinterpret_cast<const float *>(row) + at, x);
+    else if (type == B200_TYPE_F16) load16<__half, false>(reinterpret_cast<const __half *>(row) + at, x);
+    else load16<__nv_bfloat16, false>(reinterpret_cast<const __nv_bfloat16 *>(row) + at, x);
+}
+__device__ __forceinline__ void row_put(void *row, int type, int64_t at, float x) {
+    if (type == B200_TYPE_F32) reinterpret_cast<float *>(row)[at] = x;
+    else if (type == B200_TYPE_F16) reinterpret_cast<__half *>(row)[at] = __float2half_rn(x);
+    else reinterpret_cast<__nv_bfloat16 *>(row)[at] = __float2bfloat16_rn(x);
+}
+__device__ __forceinline__ bool visible(int key, int pos, int window, int keep_first) { return key <= pos && (window <= 0 || pos - key < window || key < keep_first); }
+
+// whether a query sees any of the 16 keys from `key` on, whose page is there if bit 0 of `there` is set
+__device__ __forceinline__ bool half_seen(int key, int pos, int there, int window, int keep_first) {
+    return (there & 1) && key <= pos && (window <= 0 || pos - (key + 15) < window || key < keep_first);
+}
+
+constexpr float LOG2E = 1.4426950408889634f;
+// Weights enter the second product times 2^HEAD (f16 holds 2^-24 .. 2^16); the maximum that the exponent subtracts follows the true one only when that
+// has grown by more than SLACK, so a weight is below 2^(HEAD + SLACK).
+constexpr int HEAD = 6;
+constexpr float SLACK = 8.0f;
+
+struct AttnArgs {
+    b200_kv8_attn_args a;
+    Step step;
+    int *counters;    // one per CTA, zero between calls
+    float *partials;  // two per CTA
+    int group;        // query heads per kv head
+};
+
+// ------------------------------------------------------------------------------------------------ few query rows a sequence
+// The rows of a kv head (tokens times the query heads that share it) come in blocks of R; a block against UNIT keys is a unit of work.  The units of all
+// sequences, heads and blocks are numbered, and each CTA takes an equal run of them, whatever the sequences' lengths.  Within a unit each of four
+// warps takes 32 keys of its own: pages come by cp.async, three stages deep, 16-byte pieces exchanged within a row so that both products read
+// them without conflicts; int8 becomes f16 in registers, in the layout of the MMA's second operand.  R = 8 rows of f32 fill the 16 rows of the MMA as
+// two f16 each (the upper halves and what those leave over), so full precision costs nothing; with one f16 a value R is 16.
+// Warps keep maximum, sum and result of their own and meet in shared memory at the end of a run of units of one block; runs of one block in
+// several CTAs meet in global memory, where the last one to arrive adds them in the order of the CTAs.
+// Scales: a key's joins its score; a value's joins its weight, relative to the power of two above the largest one that the row has seen.
+constexpr int RW_WARPS = 4, RW_TILE = 32, RW_UNIT = RW_WARPS * RW_TILE;
+template <int C> constexpr int rw_stages() { return C == 256 ? 2 : 3; }
+template <int C> constexpr int rw_stage_bytes() { return RW_TILE * 2 * C + 32; }  // keys, values, 2 scales of each, which pages are there
+template <int C> constexpr int rw_per_sm() { return C == 64 ? 4 : C == 128 ? 2 : 1; }
+template <int C> constexpr size_t rw_smem() { return (size_t)RW_WARPS * rw_stages<C>() * rw_stage_bytes<C>(); }
+
+// where piece c (16 bytes) of row r of a tile lies
+template <int C>
+__device__ __forceinline__ int rw_piece(int r, int c) {
+    if constexpr (C == 64) return (r >> 1) * 128 + ((((r & 1) << 2 | c) ^ ((r >> 1 & 3) << 1)) << 4);
+    else return r * C + (((c & ~7) | ((c & 7) ^ ((r & 1) << 2 | (r >> 1 & 3)))) << 4);
+}
+
+template <int C, int TERMS>
+__global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_kernel(const __grid_constant__ AttnArgs args) {
+    pdl_enter();
+    constexpr int R = 16 / TERMS, NR = 2 / TERMS;  // rows of a block; a thread's rows in the MMA's result
+    constexpr int NT = C / 8, STAGES = rw_stages<C>(), STAGE = rw_stage_bytes<C>();
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ long long sum_s[B200_KV8_MAX_SEQ];  // units of the sequences up to this one
+    __shared__ long long warp_sum_s[RW_WARPS];
+    __shared__ float top_s[RW_WARPS][16], total_s[RW_WARPS][16], fac_s[RW_WARPS][16];
+    __shared__ int power_s[RW_WARPS][16], last_s;
+    const b200_kv8_attn_args &a = args.a;
+    const b200_kv8_cache &c = a.cache;
+    const Step &st = args.step;
+    const int32_t *info = behind(st.info), *table = behind(st.table);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tg = lane & 3;
+    const int ps = c.page_size, group = args.group;
+
+    struct Span { int keep, first, units, blocks; };  // units of kept first tokens; number of the first unit behind them; units; blocks of rows
+    auto span_of = [&](const Seq &q) {
+        Span s;
+        s.first = a.window > 0 ? max(0, q.held + 1 - a.window) / RW_UNIT : 0;
+        s.keep = a.window > 0 ? min((int)(((int64_t)max(a.keep_first, 0) + RW_UNIT - 1) / RW_UNIT), s.first) : 0;
+        s.units = s.keep + (int)(((int64_t)q.held + q.count + RW_UNIT - 1) / RW_UNIT) - s.first;
+        s.blocks = (int)(((int64_t)q.count * group + R - 1) / R);
+        return s;
+    };
+    // ---- all sequences' units, summed up
+    {
+        const int each = (st.n_seq + RW_WARPS * 32 - 1) / (RW_WARPS * 32), s0 = tid * each;
+        long long mine = 0;
+        for (int s = s0; s < min(s0 + each, st.n_seq); s++) {
+            const Seq q = seq_of(st, info, s);
+            const Span sp = span_of(q);
+            mine += (long long)sp.units * sp.blocks * c.n_head_kv;
+            sum_s[s] = mine;
+        }
+        long long inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) { const long long y = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += y; }
+        if (lane == 31) warp_sum_s[warp] = inc;
+        __syncthreads();
+        long long before = inc - mine;
+        for (int w = 0; w < warp; w++) before += warp_sum_s[w];
+        for (int s = s0; s < min(s0 + each, st.n_seq); s++) sum_s[s] += before;
+        __syncthreads();
+    }
+    const long long all = sum_s[st.n_seq - 1];
+    const long long ctas = min((long long)gridDim.x, all);
+    if ((long long)blockIdx.x >= ctas) return;
+    const long long u_end = all * (blockIdx.x + 1) / ctas;
+
+    for (long long u = all * blockIdx.x / ctas; u < u_end;) {
+        int s = 0;
+        for (int lo = 0, n = st.n_seq; n > 0;) {  // the first sequence whose sum is above u
+            const int half = n / 2;
+            if (sum_s[lo + half] > u) n = half; else { lo += half + 1; n -= half + 1; }
+            s = lo;
+        }
+        const Seq q = seq_of(st, info, s);
+        const Span sp = span_of(q);
+        const long long rem = u - (s ? sum_s[s - 1] : 0), item = rem / sp.units;
+        const int unit0 = (int)(rem % sp.units), n_here = (int)min((long long)(sp.units - unit0), u_end - u);
+        const int h = (int)(item / sp.blocks), row0 = (int)(item % sp.blocks) * R, n_rows = min(R, q.count * group - row0);
+        const int len = q.held + q.count;
+        const int pos_lo = q.held + row0 / group, pos_hi = q.held + (row0 + n_rows - 1) / group;
+
+        // ---- stages of pages
+        unsigned char *mine = smem + (size_t)warp * STAGES * STAGE;
+        auto key_of = [&](int t) {  // the first of this warp's keys of unit t of the run
+            const int n = unit0 + t;
+            return (n < sp.keep ? n : n - sp.keep + sp.first) * RW_UNIT + warp * RW_TILE;
+        };
+        auto fetch = [&](int t) {  // lanes 0 and 1: the pages of the two 16s of keys
+            const int key = key_of(t) + lane * 16;
+            return lane < 2 && t < n_here && key < len ? page_of(st, table, q.row, key / ps) : -1;
+        };
+        auto issue = [&](int t, int pages) {
+            if (t < n_here) {
+                unsigned char *stage = mine + (t % STAGES) * STAGE;
+                const int key = key_of(t);
+                constexpr int PER_ROW = C / 16, ROWS = 32 / PER_ROW;  // lanes of a row, rows at once
+                const int piece = lane % PER_ROW;
+                int there = 0;
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const int page = __shfl_sync(0xffffffffu, pages, half);
+                    if (page < 0) continue;
+                    there |= 1 << half;
+                    const unsigned char *record = reinterpret_cast<const unsigned char *>(c.pages) + (size_t)page * record_bytes(c);
+                    const int64_t row = (int64_t)h * ps + (key + 16 * half) % ps;
+                    const unsigned char *kp = record + row * c.dim + piece * 16, *vp = record + v_at(c) + row * c.vdim + piece * 16;
+#pragma unroll
+                    for (int i = 0; i < 16 / ROWS; i++) {
+                        const int r = lane / PER_ROW + i * ROWS, at = rw_piece<C>(16 * half + r, piece);
+                        if (piece * 16 < c.dim) cp_async16(stage + at, kp + r * c.dim);
+                        if (piece * 16 < c.vdim) cp_async16(stage + RW_TILE * C + at, vp + r * c.vdim);
+                    }
+                    if (lane < 2) cp_async4(stage + RW_TILE * 2 * C + 8 * half + 4 * lane, record + scales_at(c) + ((size_t)lane * c.n_head_kv + h) * 4);
+                }
+                if (lane == 0) *reinterpret_cast<int *>(stage + RW_TILE * 2 * C + 16) = there;
+            }
+            cp_async_commit();
+        };
+        int first_pages[STAGES];
+#pragma unroll
+        for (int i = 0; i < STAGES; i++) first_pages[i] = fetch(i);
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; i++) issue(i, first_pages[i]);
+        int next_pages = first_pages[STAGES - 1];
+
+        // ---- this block's rows of q as the first operand, each relative to the power of two above its largest value
+        unsigned qf[C / 16][4];
+        float row_scale[NR];
+        int pos[NR];
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            const int row = g + 8 * r;
+            float x[C / 64][16];
+            unsigned loud = 0;
+            pos[r] = -1;  // (no such row: sees nothing)
+            if (row < n_rows) {
+                const int i = (row0 + row) / group, head = h * group + (row0 + row) % group;
+                pos[r] = q.held + i;
+#pragma unroll
+                for (int hf = 0; hf < C / 64; hf++) {
+                    const int at = 16 * (tg + 4 * hf);
+                    if (at < c.dim) row_load16(behind(a.q), a.type, (int64_t)(q.first + i) * a.q_stride + (int64_t)head * c.dim + at, x[hf]);
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        if (at >= c.dim) x[hf][e] = 0.f;
+                        loud = max(loud, __float_as_uint(x[hf][e]) & 0x7fffffffu);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int hf = 0; hf < C / 64; hf++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[hf][e] = 0.f;
+            }
+            loud = max(loud, __shfl_xor_sync(0xffffffffu, loud, 1));
+            loud = max(loud, __shfl_xor_sync(0xffffffffu, loud, 2));
+            const int e = exponent_above(loud);
+            const float down = pow2i(min(14 - e, 126));
+            row_scale[r] = loud >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : a.scale * pow2i(max(e - 14, -126)) * (a.softcap > 0.f ? 1.0f / a.softcap : LOG2E);
+#pragma unroll
+            for (int hf = 0; hf < C / 64; hf++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float x0 = x[hf][4 * j] * down, x1 = x[hf][4 * j + 1] * down, x2 = x[hf][4 * j + 2] * down, x3 = x[hf][4 * j + 3] * down;
+                    unsigned *f = qf[hf * 4 + j];
+                    const unsigned lo = pack_half(x0, x1), hi = pack_half(x2, x3);
+                    f[r] = lo;
+                    f[2 + r] = hi;
+                    if constexpr (TERMS == 2) { f[1] = pack_rest(x0, x1, lo); f[3] = pack_rest(x2, x3, hi); }
+                }
+        }
+
+        float o[NT][4], m[NR], l[NR];
+        int power[NR];  // the scales of the values that a row has seen are below 2^power
+#pragma unroll
+        for (int i = 0; i < NT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+#pragma unroll
+        for (int r = 0; r < NR; r++) { m[r] = -INFINITY; l[r] = 0.f; power[r] = -100; }
+
+        for (int t = 0; t < n_here; t++) {
+            cp_async_wait<STAGES - 2>();
+            __syncwarp();
+            issue(t + STAGES - 1, next_pages);
+            next_pages = fetch(t + STAGES);
+            const unsigned char *stage = mine + (t % STAGES) * STAGE;
+            const int key0 = key_of(t);
+            const int there = *reinterpret_cast<const volatile int *>(stage + RW_TILE * 2 * C + 16);
+            if (key0 > pos_hi || there == 0) continue;
+            // ---- scores
+            float sc[4][4];
+#pragma unroll
+            for (int n = 0; n < 4; n++) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+#pragma unroll
+            for (int hf = 0; hf < C / 64; hf++) {
+                if (hf * 64 >= c.dim) break;
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(stage + rw_piece<C>(8 * n + g, tg + 4 * hf));
+                    const unsigned ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        unsigned b0, b1;
+                        int4_to_half(ws[j], b0, b1);
+                        mma_f16(sc[n], qf[hf * 4 + j], b0, b1);
+                    }
+                }
+            }
+            const float4 scales = *reinterpret_cast<const float4 *>(stage + RW_TILE * 2 * C);  // keys, values of the first 16, then of the others
+            float p[NR][8];
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const float ks = n < 2 ? scales.x : scales.z;
+                    if constexpr (TERMS == 2) p[0][2 * n + e] = (sc[n][e] + sc[n][2 + e]) * (row_scale[0] * ks);
+                    else { p[0][2 * n + e] = sc[n][e] * (row_scale[0] * ks); p[NR - 1][2 * n + e] = sc[n][2 + e] * (row_scale[NR - 1] * ks); }
+                }
+            if (a.softcap > 0.f) {
+#pragma unroll
+                for (int r = 0; r < NR; r++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) p[r][i] = a.softcap * LOG2E * tanhf(p[r][i]);
+            }
+            const bool whole = there == 3 && n_rows == R && key0 + RW_TILE - 1 <= pos_lo && (a.window <= 0 || pos_hi - key0 < a.window);
+            if (!whole) {
+#pragma unroll
+                for (int r = 0; r < NR; r++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int key = key0 + 8 * (i / 2) + 2 * tg + i % 2;
+                        if (!((there >> (i / 4) & 1) && visible(key, pos[r], a.window, a.keep_first))) p[r][i] = -INFINITY;
+                    }
+            }
+            // ---- maxima, weights
+            float corr[NR], common[NR];
+            bool grown = false;
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                float top = fmaxf(fmaxf(fmaxf(p[r][0], p[r][1]), fmaxf(p[r][2], p[r][3])), fmaxf(fmaxf(p[r][4], p[r][5]), fmaxf(p[r][6], p[r][7])));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                corr[r] = common[r] = 1.0f;
+                if (top > m[r] + SLACK) {  // (m = -inf: as soon as a key is seen)
+                    corr[r] = ex2(m[r] - top);
+                    m[r] = top;
+                    grown = true;
+                }
+            }
+            // the values' scales that a row sees: a new largest one moves its accumulators' power of two
+            float vs[NR][2];
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                vs[r][0] = half_seen(key0, pos[r], there, a.window, a.keep_first) ? scales.y : 0.f;
+                vs[r][1] = half_seen(key0 + 16, pos[r], there >> 1, a.window, a.keep_first) ? scales.w : 0.f;
+                const float loudest = fmaxf(vs[r][0], vs[r][1]);  // (a NaN only if both are)
+                const int now = exponent_above(loudest <= FLT_MAX ? __float_as_uint(loudest) & 0x7fffffffu : 0u);
+                if (now > power[r]) {
+                    common[r] = pow2i(max(power[r] - now, -126));
+                    power[r] = now;
+                    grown = true;
+                }
+            }
+            if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+                for (int r = 0; r < NR; r++) { l[r] *= corr[r]; corr[r] *= common[r]; }
+#pragma unroll
+                for (int i = 0; i < NT; i++) { o[i][0] *= corr[0]; o[i][1] *= corr[0]; o[i][2] *= corr[NR - 1]; o[i][3] *= corr[NR - 1]; }
+            }
+            unsigned pf[2][4];  // the weights as the second product's first operand, for the two 16s of keys
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                const float mb = m[r] == -INFINITY ? 0.f : m[r], unit = pow2i(HEAD - power[r]), vs0 = vs[r][0] * unit, vs1 = vs[r][1] * unit;
+                float w[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float e = ex2(p[r][i] - mb);
+                    l[r] += e;
+                    w[i] = (p[r][i] == -INFINITY) ? 0.f : e * (i < 4 ? vs0 : vs1);  // (a page whose scale is NaN: not for rows that do not see it)
+                }
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const unsigned x = pack_half(w[4 * half], w[4 * half + 1]), y = pack_half(w[4 * half + 2], w[4 * half + 3]);
+                    pf[half][r] = x;
+                    pf[half][2 + r] = y;
+                    if constexpr (TERMS == 2) {
+                        pf[half][1] = pack_rest(w[4 * half], w[4 * half + 1], x);
+                        pf[half][3] = pack_rest(w[4 * half + 2], w[4 * half + 3], y);
+                    }
+                }
+            }
+            // ---- weights times values: thread g brings the dims of its own 8 (C = 64) or 16 bytes (and those 128 further on) of keys 2 tg, 2 tg + 1, 2 tg + 8, 2 tg + 9
+            const unsigned char *sv = stage + RW_TILE * C;
+            constexpr int BYTES = C == 64 ? 8 : 16;
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+#pragma unroll
+                for (int cb = 0; cb < (C == 256 ? 2 : 1); cb++) {
+                    const int piece = C == 64 ? g >> 1 : (g >> 1 | (g & 1) << 2) + 8 * cb, inside = C == 64 ? (g & 1) * 8 : 0;
+                    unsigned wv[4][BYTES / 4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const unsigned char *at = sv + rw_piece<C>(16 * half + 2 * tg + (k & 1) + (k >> 1) * 8, piece) + inside;
+                        if constexpr (C == 64) {
+                            const uint2 v = *reinterpret_cast<const uint2 *>(at);
+                            wv[k][0] = v.x; wv[k][1] = v.y;
+                        } else {
+                            const uint4 v = *reinterpret_cast<const uint4 *>(at);
+                            wv[k][0] = v.x; wv[k][1] = v.y; wv[k][2] = v.z; wv[k][3] = v.w;
+                        }
+                    }
+#pragma unroll
+                    for (int w = 0; w < BYTES / 4; w++) {
+                        unsigned b0[4], b1[4];
+                        pairs_to_half(wv[0][w], wv[1][w], b0);
+                        pairs_to_half(wv[2][w], wv[3][w], b1);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) mma_f16(o[16 * cb + 4 * w + j], pf[half], b0[j], b1[j]);
+                    }
+                }
+            }
+        }
+        cp_async_wait<0>();
+        __syncthreads();
+
+        // ---- the warps meet: rows [warp][R][C] where the stages were
+        float *so = reinterpret_cast<float *>(smem);
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            if (tg == 0) { top_s[warp][g + 8 * r] = m[r]; total_s[warp][g + 8 * r] = l[r]; power_s[warp][g + 8 * r] = power[r]; }
+        }
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+            // (columns 2 tg and 2 tg + 1 of tile i)
+            const int d0 = C == 64 ? 16 * tg + i : 128 * (i / 16) + 16 * tg + i % 16, d1 = C == 64 ? d0 + 8 : d0 + 64;
+            float *at = so + ((size_t)warp * R + g) * C;
+            if constexpr (TERMS == 2) { at[d0] = o[i][0] + o[i][2]; at[d1] = o[i][1] + o[i][3]; }
+            else { at[d0] = o[i][0]; at[d1] = o[i][1]; at[8 * C + d0] = o[i][2]; at[8 * C + d1] = o[i][3]; }
+        }
+        __syncthreads();
+        if (tid < R) {
+            float top = -INFINITY, total = 0.f;
+#pragma unroll
+            for (int w = 0; w < RW_WARPS; w++) top = fmaxf(top, top_s[w][tid]);
+#pragma unroll
+            for (int w = 0; w < RW_WARPS; w++) {
+                const float f = top_s[w][tid] == -INFINITY ? (total_s[w][tid] == 0.f ? 0.f : 1.0f) : ex2(top_s[w][tid] - top);  // (a sum without a maximum is NaN: it stays)
+                total += total_s[w][tid] * f;
+                fac_s[w][tid] = f * pow2i(power_s[w][tid] - HEAD);
+            }
+            top_s[0][tid] = top;
+            total_s[0][tid] = total;
+        }
+        __syncthreads();
+        auto sum_of = [&](int r, int d) {
+            float x = 0.f;
+#pragma unroll
+            for (int w = 0; w < RW_WARPS; w++) x += so[((size_t)w * R + r) * C + d] * fac_s[w][r];
+            return x;
+        };
+        // a row's share of 1 / (sum and sink), for results relative to maximum `top`
+        auto finish = [&](int r, float top, float total) {
+            const int head = h * group + (row0 + r) % group;
+            const float sink = a.sink ? a.sink[head] * LOG2E : -INFINITY;
+            const float mm = fmaxf(top, sink);
+            const float f = top == -INFINITY ? (total == 0.f ? 0.f : 1.0f) : ex2(top - mm);
+            const float sum = total * f + (sink == -INFINITY ? 0.f : ex2(sink - mm));
+            return sum == 0.f ? 0.f : f / sum;
+        };
+        auto put = [&](int r, int d, float x) {
+            const int i = (row0 + r) / group, head = h * group + (row0 + r) % group;
+            row_put(a.dst, a.type, (int64_t)(q.first + i) * a.dst_stride + (int64_t)head * c.vdim + d, x);
+        };
+        if (n_here == sp.units) {
+            for (int i = tid; i < n_rows * c.vdim; i += RW_WARPS * 32) {
+                const int r = i / c.vdim, d = i % c.vdim;
+                put(r, d, sum_of(r, d) * finish(r, top_s[0][r], total_s[0][r]));
+            }
+        } else {
+            // ---- part of a block: what began in an earlier CTA is this one's partial 0, what it begins itself its partial 1
+            const long long begin = u - unit0, end = begin + sp.units;
+            auto cta_of = [&](long long unit) { return (int)(((unit + 1) * ctas - 1) / all); };
+            const int c0 = cta_of(begin), parts = cta_of(end - 1) - c0 + 1;
+            constexpr int PART = R * (C + 2);
+            auto part_at = [&](int k) { return args.partials + ((size_t)(c0 + k) * 2 + (k == 0 ? 1 : 0)) * PART; };
+            float *out = part_at((int)blockIdx.x - c0);
+            if (tid < R) { out[tid] = top_s[0][tid]; out[R + tid] = total_s[0][tid]; }
+            for (int i = tid; i < R * c.vdim; i += RW_WARPS * 32) {
+                const int r = i / c.vdim, d = i % c.vdim;
+                out[2 * R + r * C + d] = sum_of(r, d);
+            }
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                last_s = atomicAdd(&args.counters[c0], 1) == parts - 1;
+                if (last_s) args.counters[c0] = 0;
+                __threadfence();
+            }
+            __syncthreads();
+            if (last_s) {
+                float *fac = so;  // [parts][R]
+                for (int r = warp; r < n_rows; r += RW_WARPS) {  // a warp a row: maximum, then the parts' shares
+                    float top = -INFINITY, total = 0.f;
+                    for (int k = lane; k < parts; k += 32) top = fmaxf(top, __ldcg(part_at(k) + r));
+                    top = warp_max(top);
+                    for (int k = lane; k < parts; k += 32) {
+                        const float mk = __ldcg(part_at(k) + r), lk = __ldcg(part_at(k) + R + r);
+                        const float f = mk == -INFINITY ? (lk == 0.f ? 0.f : 1.0f) : ex2(mk - top);
+                        fac[k * R + r] = f;
+                        total += lk * f;
+                    }
+                    total = warp_sum(total);
+                    __syncwarp();
+                    const float f = finish(r, top, total);
+                    for (int k = lane; k < parts; k += 32) fac[k * R + r] *= f;
+                }
+                __syncthreads();
+                for (int i = tid; i < n_rows * c.vdim; i += RW_WARPS * 32) {
+                    const int r = i / c.vdim, d = i % c.vdim;
+                    float x = 0.f;
+#pragma unroll 4
+                    for (int k = 0; k < parts; k++) x += __ldcg(part_at(k) + 2 * R + r * C + d) * fac[k * R + r];
+                    put(r, d, x);
+                }
+            }
+        }
+        __syncthreads();  // (the stages are free again)
+        u += n_here;
+    }
+}
+
+static int attn_class(const b200_kv8_cache &c) { const int d = c.dim > c.vdim ? c.dim : c.vdim; return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+static int rows_grid(const b200_kv8_cache &c) {
+    const int k = attn_class(c);
+    return sm_count() * (k == 64 ? rw_per_sm<64>() : k == 128 ? rw_per_sm<128>() : rw_per_sm<256>());
+}
+static size_t rows_counter_bytes(int grid) { return ((size_t)grid * 4 + 255) / 256 * 256; }
+template <int C, int TERMS>
+static int launch_rows(const AttnArgs &args, cudaStream_t st) {
+    static bool done[16] = {};  // cudaFuncSetAttribute is per device
+    int dev = 0;
+    B200_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev >= 16 || !done[dev]) {
+        B200_CUDA_TRY(cudaFuncSetAttribute(kv8_attn_rows_kernel<C, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rw_smem<C>()));
+        if (dev < 16) done[dev] = true;
+    }
+    B200_CUDA_TRY(launch_chained(kv8_attn_rows_kernel<C, TERMS>, (unsigned)rows_grid(args.a.cache), RW_WARPS * 32, rw_smem<C>(), st, args));
+    return B200_OK;
+}
+
+static int check_attn(const b200_kv8_attn_args *a, const char *who) {
+    OPX_REQUIRE(a, B200_ERR_INVALID, "%s: NULL arguments", who);
+    const int rc = check_step(&a->cache, a->seq_info, a->table, a->table_stride, a->n_rows, a->n_seq, a->n_tokens, a->type, who);
+    if (rc != B200_OK) return rc;
+    const b200_kv8_cache &c = a->cache;
+    OPX_REQUIRE(a->n_head > 0 && a->n_head % c.n_head_kv == 0, B200_ERR_INVALID, "%s: %d query heads over %d kv heads", who, a->n_head, c.n_head_kv);
+    OPX_REQUIRE(a->window >= 0 && a->keep_first >= 0, B200_ERR_INVALID, "%s: window %d, keep_first %d", who, a->window, a->keep_first);
+    OPX_REQUIRE(a->scale == a->scale && a->softcap >= 0.0f && a->softcap <= FLT_MAX, B200_ERR_INVALID, "%s: scale or softcap", who);
+    if (a->n_tokens == 0 || a->n_seq == 0) return B200_OK;
+    OPX_REQUIRE(a->q && a->dst, B200_ERR_INVALID, "%s: NULL q or dst", who);
+    OPX_REQUIRE(a->q_stride >= (int64_t)a->n_head * c.dim && a->dst_stride >= (int64_t)a->n_head * c.vdim, B200_ERR_INVALID, "%s: rows of q or dst overlap (strides %lld, %lld)", who,
+                (long long)a->q_stride, (long long)a->dst_stride);
+    return B200_OK;
+}
+static bool one_term(const b200_kv8_attn_args *a) { return a->type != B200_TYPE_F32 || a->f16_products != 0; }
+
+}  // namespace kv8
+}  // namespace b200
+
+using namespace b200;
+using namespace b200::kv8;
+
+extern "C" {
+
+size_t b200_kv8_attn_workspace_bytes(const b200_kv8_attn_args *a) {
+    if (!a || b200_kv8_page_bytes(a->cache.page_size, a->cache.n_head_kv, a->cache.dim, a->cache.vdim) == 0) return 0;
+    const int grid = rows_grid(a->cache);
+    return rows_counter_bytes(grid) + (size_t)grid * 2 * (one_term(a) ? 16 : 8) * (attn_class(a->cache) + 2) * 4;
+}
+
+int b200_op_kv8_attn(const b200_kv8_attn_args *a, void *workspace, size_t workspace_bytes, b200_stream_t stream) {
+    const char *who = "b200_op_kv8_attn";
+    const int rc = check_attn(a, who);
+    if (rc != B200_OK || a->n_tokens == 0 || a->n_seq == 0) return rc;
+    OPX_REQUIRE(workspace && workspace_bytes >= b200_kv8_attn_workspace_bytes(a) && (uintptr_t)workspace % 16 == 0, B200_ERR_INVALID, "%s: workspace of %zu bytes, 16-byte aligned", who,
+                b200_kv8_attn_workspace_bytes(a));
+    const b200_kv8_cache &c = a->cache;
+    AttnArgs args = {*a, {a->seq_info, a->table, a->table_stride, a->n_rows, a->n_seq, a->n_tokens, c.n_pages, c.page_size}, (int *)workspace,
+                     (float *)((char *)workspace + rows_counter_bytes(rows_grid(c))), a->n_head / c.n_head_kv};
+    const cudaStream_t st = (cudaStream_t)stream;
+    const int k = attn_class(c);
+    if (one_term(a)) return k == 64 ? launch_rows<64, 1>(args, st) : k == 128 ? launch_rows<128, 1>(args, st) : launch_rows<256, 1>(args, st);
+    return k == 64 ? launch_rows<64, 2>(args, st) : k == 128 ? launch_rows<128, 2>(args, st) : launch_rows<256, 2>(args, st);
+}
+
+}  // extern "C"

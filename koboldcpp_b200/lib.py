@@ -155,6 +155,35 @@ class TimeMixArgs(C.Structure):
                 ("dst", C.c_void_p), ("dst_stride", C.c_int64), ("heads", C.c_int32), ("dim", C.c_int32)]
 
 
+class Kv8Cache(C.Structure):
+    """b200_kv8_cache (include/b200_kv8.h): a pool of pages of keys and values in 8 bits."""
+    _fields_ = [("pages", C.c_void_p), ("n_pages", C.c_int32), ("page_size", C.c_int32), ("n_head_kv", C.c_int32), ("dim", C.c_int32), ("vdim", C.c_int32), ("_pad", C.c_int32)]
+
+
+class Kv8StoreArgs(C.Structure):
+    """b200_kv8_store_args (include/b200_kv8.h); strides in values."""
+    _fields_ = [("cache", Kv8Cache), ("k", C.c_void_p), ("k_stride", C.c_int64), ("v", C.c_void_p), ("v_stride", C.c_int64), ("seq_info", C.c_void_p), ("table", C.c_void_p),
+                ("table_stride", C.c_int64), ("n_rows", C.c_int32), ("n_seq", C.c_int32), ("n_tokens", C.c_int32), ("type", C.c_int32)]
+
+
+class Kv8LoadArgs(C.Structure):
+    """b200_kv8_load_args (include/b200_kv8.h); strides in values."""
+    _fields_ = Kv8StoreArgs._fields_
+
+
+class Kv8AttnArgs(C.Structure):
+    """b200_kv8_attn_args (include/b200_kv8.h); strides in values."""
+    _fields_ = [("cache", Kv8Cache), ("q", C.c_void_p), ("q_stride", C.c_int64), ("dst", C.c_void_p), ("dst_stride", C.c_int64), ("seq_info", C.c_void_p), ("table", C.c_void_p),
+                ("table_stride", C.c_int64), ("n_rows", C.c_int32), ("n_seq", C.c_int32), ("n_tokens", C.c_int32), ("max_new", C.c_int32), ("n_head", C.c_int32), ("type", C.c_int32),
+                ("sink", C.c_void_p), ("window", C.c_int32), ("keep_first", C.c_int32), ("scale", C.c_float), ("softcap", C.c_float), ("f16_products", C.c_int32)]
+
+
+class Kv8Map(C.Structure):
+    """b200_kv8_map (include/b200_kv8.h): which row holds which pages."""
+    _fields_ = [("table", C.c_void_p), ("table_stride", C.c_int64), ("len", C.c_void_p), ("refs", C.c_void_p), ("n_rows", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32),
+                ("_pad", C.c_int32)]
+
+
 _SIGS = {
     # name: (restype, argtypes)
     "b200_last_error": (C.c_char_p, []),
@@ -261,6 +290,22 @@ _OPS_SIGS = {
     "b200_op_time_mix_scan": (C.c_int, [C.POINTER(TimeMixArgs), C.c_void_p]),
 }
 
+# include/b200_kv8.h
+_KV8_SIGS = {
+    "b200_kv8_page_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
+    "b200_op_kv8_store": (C.c_int, [C.POINTER(Kv8StoreArgs), C.c_void_p]),
+    "b200_op_kv8_load": (C.c_int, [C.POINTER(Kv8LoadArgs), C.c_void_p]),
+    "b200_kv8_attn_workspace_bytes": (C.c_size_t, [C.POINTER(Kv8AttnArgs)]),
+    "b200_op_kv8_attn": (C.c_int, [C.POINTER(Kv8AttnArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "b200_op_kv8_cut": (C.c_int, [C.POINTER(Kv8Map), C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]),
+    "b200_op_kv8_fork": (C.c_int, [C.POINTER(Kv8Map), C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p]),
+    "b200_kv8_grow_workspace_bytes": (C.c_size_t, [C.c_int32]),
+    "b200_op_kv8_grow": (C.c_int, [C.POINTER(Kv8Map), C.POINTER(Kv8Cache), C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "b200_kv8_compact_workspace_bytes": (C.c_size_t, [C.c_int32]),
+    "b200_op_kv8_compact": (C.c_int, [C.POINTER(Kv8Map), C.POINTER(Kv8Cache), C.c_int32, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "b200_op_kv8_copy_pages": (C.c_int, [C.POINTER(Kv8Cache), C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]),
+}
+
 _lib = None
 
 
@@ -274,7 +319,7 @@ def load(path: Path | None = None):
     if not p.exists():
         raise B200Error(f"{p} not found: build it with `python -m koboldcpp_b200.build` (nvcc, sm_100a)")
     L = C.CDLL(str(p))
-    for name, (res, args) in list(_SIGS.items()) + list(_OPS_SIGS.items()):
+    for name, (res, args) in list(_SIGS.items()) + list(_OPS_SIGS.items()) + list(_KV8_SIGS.items()):
         f = getattr(L, name)  # AttributeError if the library does not export a declared symbol
         f.restype = res
         f.argtypes = args
