@@ -37,72 +37,12 @@ constexpr float FT_SLACK = 8.0f;
 template <int D> constexpr int ft_tile_bytes() { return D / 64 * FT_PANEL; }
 template <int D> constexpr size_t ft_smem(int n_tiles) { return 1024 + (size_t)((D / 64 + 1) * FT_Q_PANEL) + (size_t)(2 * FT_NB) * ft_tile_bytes<D>() + (size_t)n_tiles * 4 + (size_t)(n_tiles + 2) * 4; }
 
-__device__ __forceinline__ void tmem_st32(unsigned taddr, const unsigned (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-        "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// D (TMEM) += A . B: A in TMEM (16-bit values, two a column), B in shared memory
-__device__ __forceinline__ void ft_mma_ts(unsigned d, unsigned a, unsigned long long b, unsigned idesc, unsigned accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
-        "}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// 32 accumulator columns without waiting for them (tmem_wait_ld)
-__device__ __forceinline__ void tmem_ld32_async(unsigned taddr, float *v) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
-          "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]),
-          "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
-        : "r"(taddr)
-        : "memory");
-}
-template <int N>
-__device__ __forceinline__ void tmem_wait_ld(float (&v)[N]) {  // (v: nothing that reads it may move in front of the wait)
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < N; i++) asm volatile("" : "+f"(v[i]));
-}
 // operand whose 64-value rows run along the other dimension (MN-major): panels of 64 values FT_PANEL apart, groups of 8 rows 1024 bytes apart
-__device__ __forceinline__ unsigned long long ft_desc_mn(unsigned smem_addr) {
-    unsigned long long d = 0;
-    d |= (unsigned long long)((smem_addr & 0x3FFFFu) >> 4);
-    d |= (unsigned long long)(FT_PANEL >> 4) << 16;
-    d |= (unsigned long long)(1024 >> 4) << 32;
-    d |= (unsigned long long)1 << 46;
-    d |= (unsigned long long)2 << 61;
-    return d;
-}
+__device__ __forceinline__ unsigned long long ft_desc_mn(unsigned smem_addr) { return umma_desc_mn_sw128(smem_addr, FT_PANEL); }
 // f16 operands, f32 results, 128 rows; B along K (K-major) or not
 __host__ __device__ constexpr unsigned ft_idesc(int n, bool b_mn) { return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((unsigned)(n >> 3) << 17) | ((unsigned)(FT_COLS >> 4) << 24); }
 __device__ __forceinline__ float ft_slope(const FaParams &p, int h) {
     return p.max_bias > 0.0f ? (h < p.n_head_log2 ? powf(p.m0, (float)(h + 1)) : powf(p.m1, (float)(2 * (h - p.n_head_log2) + 1))) : 1.0f;
-}
-// two f32 at a time: one issue slot for both
-__device__ __forceinline__ float2 ft_fma2(float2 x, float2 y, float2 z) {
-    float2 r;
-    asm("{\n.reg .b64 a, b, c;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\nfma.rn.f32x2 a, a, b, c;\nmov.b64 {%0, %1}, a;\n}\n"
-        : "=f"(r.x), "=f"(r.y) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y), "f"(z.x), "f"(z.y));
-    return r;
-}
-__device__ __forceinline__ float2 ft_add2(float2 x, float2 y) {
-    float2 r;
-    asm("{\n.reg .b64 a, b;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.f32x2 a, a, b;\nmov.b64 {%0, %1}, a;\n}\n" : "=f"(r.x), "=f"(r.y) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
-    return r;
 }
 // what two pairs of f16 leave over of four floats; its square is added to energy
 __device__ __forceinline__ void ft_rest(float4 &x, unsigned h0, unsigned h1, float2 &energy) {

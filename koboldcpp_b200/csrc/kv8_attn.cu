@@ -10,6 +10,8 @@ namespace kv8 {
 // ------------------------------------------------------------------------------------------------ shared by the kernels
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+// tanh(x) = 1 - 2 / (1 + e^(2x)), off by about 2^-22 (of 1, not of the result) for any x
+__device__ __forceinline__ float tanh_fast(float x) { return 1.0f - __fdividef(2.0f, 1.0f + ex2(x * 2.8853900817779268f)); }
 // x < 2^e for the magnitude with these bits, e >= -100
 __device__ __forceinline__ int exponent_above(unsigned bits) { return max((int)(bits >> 23) - 126, -100); }
 __device__ __forceinline__ unsigned pack_half(float a, float b) {
@@ -41,7 +43,7 @@ __device__ __forceinline__ void pairs_to_half(unsigned a, unsigned b, unsigned (
     p[3] = less_1152(prmt(hi, 0x64646464u, 0x4342));
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -75,6 +77,7 @@ struct AttnArgs {
     int *counters;    // one per CTA, zero between calls
     float *partials;  // two per CTA
     int group;        // query heads per kv head
+    int rows_most;    // sequences with more query rows a kv head (tokens times group) are the prompt kernel's; negative: there is none
 };
 
 // ------------------------------------------------------------------------------------------------ few query rows a sequence
@@ -122,7 +125,8 @@ __global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_k
         s.first = a.window > 0 ? max(0, q.held + 1 - a.window) / RW_UNIT : 0;
         s.keep = a.window > 0 ? min((int)(((int64_t)max(a.keep_first, 0) + RW_UNIT - 1) / RW_UNIT), s.first) : 0;
         s.units = s.keep + (int)(((int64_t)q.held + q.count + RW_UNIT - 1) / RW_UNIT) - s.first;
-        s.blocks = (int)(((int64_t)q.count * group + R - 1) / R);
+        const int64_t rows = (int64_t)q.count * group;
+        s.blocks = args.rows_most >= 0 && rows > args.rows_most ? 0 : (int)((rows + R - 1) / R);
         return s;
     };
     // ---- all sequences' units, summed up
@@ -279,17 +283,17 @@ __global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_k
 #pragma unroll
             for (int hf = 0; hf < C / 64; hf++) {
                 if (hf * 64 >= c.dim) break;
+                uint4 w[4];
 #pragma unroll
-                for (int n = 0; n < 4; n++) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(stage + rw_piece<C>(8 * n + g, tg + 4 * hf));
-                    const unsigned ws[4] = {w.x, w.y, w.z, w.w};
+                for (int n = 0; n < 4; n++) w[n] = *reinterpret_cast<const uint4 *>(stage + rw_piece<C>(8 * n + g, tg + 4 * hf));
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int n = 0; n < 4; n++) {
                         unsigned b0, b1;
-                        int4_to_half(ws[j], b0, b1);
+                        int4_to_half(j == 0 ? w[n].x : j == 1 ? w[n].y : j == 2 ? w[n].z : w[n].w, b0, b1);
                         mma_f16(sc[n], qf[hf * 4 + j], b0, b1);
                     }
-                }
             }
             const float4 scales = *reinterpret_cast<const float4 *>(stage + RW_TILE * 2 * C);  // keys, values of the first 16, then of the others
             float p[NR][8];
@@ -302,10 +306,11 @@ __global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_k
                     else { p[0][2 * n + e] = sc[n][e] * (row_scale[0] * ks); p[NR - 1][2 * n + e] = sc[n][2 + e] * (row_scale[NR - 1] * ks); }
                 }
             if (a.softcap > 0.f) {
+                const float cap_log2 = a.softcap * LOG2E;
 #pragma unroll
                 for (int r = 0; r < NR; r++)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) p[r][i] = a.softcap * LOG2E * tanhf(p[r][i]);
+                    for (int i = 0; i < 8; i++) p[r][i] = cap_log2 * tanh_fast(p[r][i]);
             }
             const bool whole = there == 3 && n_rows == R && key0 + RW_TILE - 1 <= pos_lo && (a.window <= 0 || pos_hi - key0 < a.window);
             if (!whole) {
@@ -516,6 +521,14 @@ __global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_k
     }
 }
 
+}  // namespace kv8
+}  // namespace b200
+
+#include "kv8_attn_tc.cuh"
+
+namespace b200 {
+namespace kv8 {
+
 static int attn_class(const b200_kv8_cache &c) { const int d = c.dim > c.vdim ? c.dim : c.vdim; return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 static int rows_grid(const b200_kv8_cache &c) {
     const int k = attn_class(c);
@@ -549,7 +562,20 @@ static int check_attn(const b200_kv8_attn_args *a, const char *who) {
                 (long long)a->q_stride, (long long)a->dst_stride);
     return B200_OK;
 }
+// Sequences of more query rows a kv head than this go to the tensor cores' kernel, if the heads are of its sizes.
+constexpr int ROWS_MOST = 64;
 static bool one_term(const b200_kv8_attn_args *a) { return a->type != B200_TYPE_F32 || a->f16_products != 0; }
+
+// 256 rows a CTA where that many CTAs fill the device, else 128
+static int launch_prompt(const AttnArgs &args, bool vec, int k, bool one, long long limit, cudaStream_t st) {
+    const bool two = (int64_t)args.a.n_tokens * args.group * args.a.cache.n_head_kv >= (int64_t)sm_count() * 2 * KT_ROWS;
+    if (k == 64) {
+        if (two) return one ? launch_tc<64, 2, 1>(args, vec, limit, st) : launch_tc<64, 2, 2>(args, vec, limit, st);
+        return one ? launch_tc<64, 1, 1>(args, vec, limit, st) : launch_tc<64, 1, 2>(args, vec, limit, st);
+    }
+    if (two) return one ? launch_tc<128, 2, 1>(args, vec, limit, st) : launch_tc<128, 2, 2>(args, vec, limit, st);
+    return one ? launch_tc<128, 1, 1>(args, vec, limit, st) : launch_tc<128, 1, 2>(args, vec, limit, st);
+}
 
 }  // namespace kv8
 }  // namespace b200
@@ -573,9 +599,16 @@ int b200_op_kv8_attn(const b200_kv8_attn_args *a, void *workspace, size_t worksp
                 b200_kv8_attn_workspace_bytes(a));
     const b200_kv8_cache &c = a->cache;
     AttnArgs args = {*a, {a->seq_info, a->table, a->table_stride, a->n_rows, a->n_seq, a->n_tokens, c.n_pages, c.page_size}, (int *)workspace,
-                     (float *)((char *)workspace + rows_counter_bytes(rows_grid(c))), a->n_head / c.n_head_kv};
+                     (float *)((char *)workspace + rows_counter_bytes(rows_grid(c))), a->n_head / c.n_head_kv, -1};
     const cudaStream_t st = (cudaStream_t)stream;
     const int k = attn_class(c);
+    const int64_t longest = (int64_t)(a->max_new > 0 && a->max_new < a->n_tokens ? a->max_new : a->n_tokens) * args.group;  // query rows a kv head of one sequence, at most
+    if (k <= 128 && longest > ROWS_MOST && (int64_t)a->n_tokens * args.group < (1ll << 30)) {
+        args.rows_most = ROWS_MOST;
+        const bool vec = rows_aligned(a->q, a->q_stride, a->type) && rows_aligned(a->dst, a->dst_stride, a->type), one = one_term(a);
+        const int rc2 = launch_prompt(args, vec, k, one, PAIR_WAIT_LIMIT, st);
+        if (rc2 != B200_OK) return rc2;
+    }
     if (one_term(a)) return k == 64 ? launch_rows<64, 1>(args, st) : k == 128 ? launch_rows<128, 1>(args, st) : launch_rows<256, 1>(args, st);
     return k == 64 ? launch_rows<64, 2>(args, st) : k == 128 ? launch_rows<128, 2>(args, st) : launch_rows<256, 2>(args, st);
 }

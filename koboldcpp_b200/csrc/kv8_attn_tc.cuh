@@ -1,0 +1,437 @@
+// kv8_attn_tc.cuh -- attention of many new tokens over the paged 8-bit cache on the 5th-generation tensor cores (heads of up to 128).  Included by kv8_attn.cu.
+//
+// A CTA serves GROUPS times 128 query rows of one kv head (tokens times the query heads that share it) and walks over tiles of 64 keys:
+//   S = Q . K^T      tcgen05, both operands in shared memory as f16, into TMEM
+//   P = 2^(c S - m)  a thread a row, no exchange between lanes; P goes back to TMEM as f16, in place of S
+//   O += P . V       A = P from TMEM, B = V as it lies in the page (keys are the strided side), O stays in TMEM
+// Four warps turn int8 keys and values into f16 once for all the CTA's rows: pieces of 16 bytes come from the pages into registers a tile ahead, and leave for
+// shared memory in the 128-byte swizzle that the products read.  int8 is exact in f16, so with TERMS = 2 only Q and P have to be taken apart (upper halves
+// and what those leave over, a second product each) for results as f32 gives them; 64 columns of S are just two times 32 of P.
+// Softmax: four warps a group of 128 rows.  The maximum that the exponent subtracts follows the true one only when that has grown by SLACK, so O is hardly
+// ever rescaled.  A key's scale joins its score, a value's its weight, relative to the power of two above the largest that the row has seen; the softmax
+// warps bring the scales of their tile's four 16s of keys themselves, a tile ahead.
+// Every S has two buffers a group: products run while the softmax is busy with the tile before.
+// Waits have a limit, as in the prompt GEMM: a role that gives up sets `failed`, the others follow, and the status word is set.
+#pragma once
+#include "tcgen05.cuh"
+
+namespace b200 {
+namespace kv8 {
+
+constexpr int KT_ROWS = 128, KT_KEYS = 64, KT_CONVERT = 4;
+constexpr int KT_Q_PANEL = KT_ROWS * 128, KT_PANEL = KT_KEYS * 128;  // panels of 64 values, 128 bytes a row
+template <int GROUPS> constexpr int kt_threads() { return (GROUPS * 4 + 2 + KT_CONVERT) * 32; }
+template <int GROUPS, int TERMS> constexpr int kt_buffers() { return GROUPS * TERMS == 4 ? 3 : 4; }  // of K and V
+template <int C, int GROUPS, int TERMS> constexpr size_t kt_smem() {
+    return 1024 + (size_t)GROUPS * TERMS * (C / 64) * KT_Q_PANEL + (size_t)kt_buffers<GROUPS, TERMS>() * 2 * (C / 64) * KT_PANEL;
+}
+// f16 operands, f32 results, 128 rows
+__device__ __forceinline__ unsigned kt_idesc(int n, bool b_mn) { return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((unsigned)(n >> 3) << 17) | ((unsigned)(KT_ROWS >> 4) << 24); }
+__device__ __forceinline__ float2 mul2(float2 x, float2 y) {
+    float2 r;
+    asm("{\n.reg .b64 a, b;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 a, a, b;\nmov.b64 {%0, %1}, a;\n}\n" : "=f"(r.x), "=f"(r.y) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+    return r;
+}
+// accumulators of a row times alpha
+template <int C>
+__device__ __noinline__ void kt_rescale(unsigned o_at, float alpha) {
+#pragma unroll 1
+    for (int ch = 0; ch < C / 32; ch++) {
+        float v[32];
+        unsigned x[32];
+        tmem_ld32(o_at + 32 * ch, v);
+#pragma unroll
+        for (int i = 0; i < 32; i++) x[i] = __float_as_uint(v[i] * alpha);
+        tmem_st32(o_at + 32 * ch, x);
+    }
+}
+// a whole warp waits
+template <int SLEEP>
+__device__ __forceinline__ bool kt_wait(unsigned long long *bar, int parity, volatile int *failed, long long limit) {
+    return __all_sync(0xffffffffu, pair_wait<SLEEP>(smem_u32(bar), (unsigned)parity, failed, limit));
+}
+
+template <int C, int GROUPS, int TERMS>
+__global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(const __grid_constant__ AttnArgs args, bool vec, long long limit, int *timeout) {
+    constexpr int NB = kt_buffers<GROUPS, TERMS>(), PANELS = C / 64, BLOCK = GROUPS * KT_ROWS, SOFTMAX = GROUPS * 4;
+    constexpr int TILE = PANELS * KT_PANEL;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *smem = reinterpret_cast<unsigned char *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ __align__(8) unsigned long long k_full[NB], k_free[NB], v_full[NB], v_free[NB], s_full[GROUPS][2], p_full[GROUPS][2], o_done[GROUPS][2];
+    __shared__ unsigned tmem_base_s;
+    __shared__ volatile int failed;
+    const b200_kv8_attn_args &a = args.a;
+    const b200_kv8_cache &c = a.cache;
+    const Step &st = args.step;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const int group = args.group, ps = c.page_size, h = blockIdx.y;
+    pdl_enter();
+    const int32_t *info = behind(st.info), *table = behind(st.table);
+    // block j of rows belongs to the sequence s with first_s group / BLOCK + s <= j (long causal walks first)
+    const int j = (int)(gridDim.x - 1 - blockIdx.x);
+    auto first_block = [&](int first, int s) { return (int)((int64_t)first * group / BLOCK) + s; };
+    const int s = find_seq(info, st.n_seq, j, first_block);
+    const Seq q = seq_of(st, info, s);
+    const int64_t row0_64 = (int64_t)(j - first_block(q.first, s)) * BLOCK, rows_64 = (int64_t)q.count * group;
+    if (rows_64 <= args.rows_most || row0_64 < 0 || row0_64 >= rows_64) return;  // (another kernel's, or no block)
+    const int row0 = (int)row0_64, n_rows = (int)min((int64_t)BLOCK, rows_64 - row0_64);
+    const int pos_lo = q.held + row0 / group, pos_hi = q.held + (row0 + n_rows - 1) / group;
+    // tiles: those of the kept first tokens, then from the window's on
+    const int first_tile = a.window > 0 ? max(0, pos_lo + 1 - a.window) / KT_KEYS : 0;
+    const int keep_tiles = a.window > 0 ? min((int)(((int64_t)max(a.keep_first, 0) + KT_KEYS - 1) / KT_KEYS), first_tile) : 0;
+    const int n_tiles = keep_tiles + pos_hi / KT_KEYS + 1 - first_tile;
+    auto key_of = [&](int t) { return (t < keep_tiles ? t : t - keep_tiles + first_tile) * KT_KEYS; };
+    unsigned char *sq = smem, *sk = sq + GROUPS * TERMS * PANELS * KT_Q_PANEL, *sv = sk + NB * TILE;
+
+    if (tid == 0) {
+        for (int i = 0; i < NB; i++) { mbar_init(&k_full[i], KT_CONVERT); mbar_init(&k_free[i], 1); mbar_init(&v_full[i], KT_CONVERT); mbar_init(&v_free[i], 1); }
+        for (int i = 0; i < 2 * GROUPS; i++) { mbar_init(&s_full[i >> 1][i & 1], 1); mbar_init(&p_full[i >> 1][i & 1], 4); mbar_init(&o_done[i >> 1][i & 1], 1); }
+        mbar_fence_init();
+        failed = 0;
+    }
+    constexpr unsigned TMEM = GROUPS == 2 ? 512 : 256;  // S: two buffers of 64 columns a group; then O
+    if (warp == SOFTMAX) tmem_alloc(&tmem_base_s, TMEM);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = tmem_base_s, tmem_o = tmem + GROUPS * 2 * KT_KEYS;
+
+    if (warp < SOFTMAX) {
+        // ===== a row of Q as f16, relative to the power of two above its largest value
+        const int w = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane, row = w * KT_ROWS + r;
+        const bool mine = row < n_rows;
+        const int i_tok = mine ? (row0 + row) / group : 0, head = h * group + (mine ? (row0 + row) % group : 0);
+        const int64_t q_at = (int64_t)(q.first + i_tok) * a.q_stride + (int64_t)head * c.dim;
+        const void *qp = behind(a.q);
+        auto piece = [&](int p, float (&x)[16]) {
+            if (a.type == B200_TYPE_F32) vec ? load16<float, true>(reinterpret_cast<const float *>(qp) + q_at + 16 * p, x) : load16<float, false>(reinterpret_cast<const float *>(qp) + q_at + 16 * p, x);
+            else if (a.type == B200_TYPE_F16) vec ? load16<__half, true>(reinterpret_cast<const __half *>(qp) + q_at + 16 * p, x) : load16<__half, false>(reinterpret_cast<const __half *>(qp) + q_at + 16 * p, x);
+            else vec ? load16<__nv_bfloat16, true>(reinterpret_cast<const __nv_bfloat16 *>(qp) + q_at + 16 * p, x) : load16<__nv_bfloat16, false>(reinterpret_cast<const __nv_bfloat16 *>(qp) + q_at + 16 * p, x);
+        };
+        unsigned loud = 0;
+        for (int p = 0; mine && p < c.dim / 16; p++) {
+            float x[16];
+            piece(p, x);
+#pragma unroll
+            for (int e = 0; e < 16; e++) loud = max(loud, __float_as_uint(x[e]) & 0x7fffffffu);
+        }
+        const int e_q = exponent_above(loud);
+        const float down = pow2i(min(14 - e_q, 126));
+        const float row_scale = loud >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : a.scale * pow2i(max(e_q - 14, -126)) * (a.softcap > 0.f ? 1.0f / a.softcap : LOG2E);
+        for (int p = 0; p < c.dim / 16; p++) {
+            float x[16];
+            if (mine) piece(p, x);
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[e] = mine ? x[e] * down : 0.f;
+            unsigned hi[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) hi[e] = pack_half(x[2 * e], x[2 * e + 1]);
+            unsigned char *at = sq + ((w * TERMS) * PANELS + p / 4) * KT_Q_PANEL + r * 128;
+            const int c0 = ((p % 4) * 2) ^ (r & 7);
+            *reinterpret_cast<uint4 *>(at + c0 * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4 *>(at + (c0 ^ 1) * 16) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+            if constexpr (TERMS == 2) {
+                at += PANELS * KT_Q_PANEL;
+                *reinterpret_cast<uint4 *>(at + c0 * 16) = make_uint4(pack_rest(x[0], x[1], hi[0]), pack_rest(x[2], x[3], hi[1]), pack_rest(x[4], x[5], hi[2]), pack_rest(x[6], x[7], hi[3]));
+                *reinterpret_cast<uint4 *>(at + (c0 ^ 1) * 16) = make_uint4(pack_rest(x[8], x[9], hi[4]), pack_rest(x[10], x[11], hi[5]), pack_rest(x[12], x[13], hi[6]), pack_rest(x[14], x[15], hi[7]));
+            }
+        }
+        fence_proxy_async_smem();
+        asm volatile("bar.arrive 2, %0;" ::"n"(SOFTMAX * 32 + 32) : "memory");
+
+        const int pos = mine ? q.held + i_tok : -1;
+        // positions of this warp's rows (none: pos_hi_w < pos_lo_w)
+        const int w0 = w * KT_ROWS + quarter * 32, w1 = min(w0 + 31, n_rows - 1);
+        const int pos_lo_w = w0 < n_rows ? q.held + (row0 + w0) / group : 0, pos_hi_w = w0 < n_rows ? q.held + (row0 + w1) / group : -1;
+        const bool all_rows = w0 + 31 < n_rows;
+        const unsigned lanes = (unsigned)(quarter * 32) << 16, o_at = tmem_o + (unsigned)(w * C) + lanes;
+        // lane l & 3 of a tile's 16s of keys: page a tile ahead, then its scales (lanes 0 .. 3 the keys', 4 .. 7 the values')
+        auto page_ahead = [&](int t) {
+            const int key = t < n_tiles ? key_of(t) + 16 * (lane & 3) : 0x7fffffff;
+            return key <= pos_hi ? page_of(st, table, q.row, key / ps) : -1;
+        };
+        auto scale_ahead = [&](int page) {
+            if (page < 0 || lane >= 8) return 0.f;
+            const unsigned char *record = reinterpret_cast<const unsigned char *>(c.pages) + (size_t)page * record_bytes(c) + scales_at(c);
+            return *(reinterpret_cast<const volatile float *>(record) + (lane >> 2) * c.n_head_kv + h);
+        };
+        int page = page_ahead(0), page_next = page_ahead(1);
+        float scale = scale_ahead(page);
+        float m = -INFINITY, l = 0.f;
+        int power = -100;
+        bool ok = true;
+        for (int t = 0; t < n_tiles; t++) {
+            const int b = t & 1, key0 = key_of(t);
+            const unsigned s_at = tmem + (unsigned)((w * 2 + b) * KT_KEYS) + lanes;
+            const int there = (int)(__ballot_sync(0xffffffffu, page >= 0) & 15u);
+            float ks[4], vs[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) { ks[i] = __shfl_sync(0xffffffffu, scale, i) * row_scale; vs[i] = __shfl_sync(0xffffffffu, scale, 4 + i); }
+            page = page_next;
+            scale = scale_ahead(page);
+            page_next = page_ahead(t + 2);
+            ok = kt_wait<20>(&s_full[w][b], (t >> 1) & 1, &failed, limit);
+            if (!ok) break;
+            tc_fence_after();
+            unsigned x[32];
+            const bool hidden = there == 0 || key0 > pos_hi_w || (a.window > 0 && pos_lo_w - (key0 + KT_KEYS - 1) >= a.window && key0 >= a.keep_first);
+            if (hidden) {
+#pragma unroll
+                for (int i = 0; i < 32; i++) x[i] = 0u;
+                tmem_st32(s_at, x);
+                if constexpr (TERMS == 2) tmem_st32(s_at + 32, x);
+            } else {
+                float v[64];
+                tmem_ld32_async(s_at, v);
+                tmem_ld32_async(s_at + 32, v + 32);
+                const bool whole = there == 15 && all_rows && key0 + KT_KEYS - 1 <= pos_lo_w && (a.window <= 0 || pos_hi_w - key0 < a.window);
+                tmem_wait_ld(v);
+                // the common tile keeps the raw products; ks takes them to scores times log2 e
+                if (!whole || a.softcap > 0.f || !(a.scale > 0.f)) {
+#pragma unroll
+                    for (int i = 0; i < 64; i++) v[i] *= ks[i / 16];
+                    if (a.softcap > 0.f) {
+                        const float cap_log2 = a.softcap * LOG2E;
+#pragma unroll
+                        for (int i = 0; i < 64; i++) v[i] = cap_log2 * tanh_fast(v[i]);
+                    }
+                    if (!whole) {
+#pragma unroll
+                        for (int i = 0; i < 64; i++) if (!((there >> (i / 16) & 1) && visible(key0 + i, pos, a.window, a.keep_first))) v[i] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) ks[i] = 1.0f;
+                }
+                float top = -INFINITY, loudest = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float t0 = v[16 * i], t1 = v[16 * i + 1];
+#pragma unroll
+                    for (int e = 2; e < 16; e += 2) { t0 = fmaxf(t0, v[16 * i + e]); t1 = fmaxf(t1, v[16 * i + e + 1]); }
+                    top = fmaxf(top, fmaxf(t0, t1) * ks[i]);
+                    if (!whole && !half_seen(key0 + 16 * i, pos, there >> i, a.window, a.keep_first)) vs[i] = 0.f;
+                    loudest = fmaxf(loudest, vs[i]);  // (passes over NaN)
+                }
+                const bool grown = top > m + SLACK;  // (m = -inf: as soon as a key is seen)
+                const int now = exponent_above(__float_as_uint(loudest));
+                if (__any_sync(0xffffffffu, grown || now > power)) {
+                    float alpha = grown ? ex2(m - top) : 1.0f;
+                    if (grown) { m = top; l *= alpha; }
+                    if (now > power) { alpha *= pow2i(max(power - now, -126)); power = now; }
+                    if (t > 0) {
+                        ok = kt_wait<20>(&o_done[w][b ^ 1], ((t - 1) >> 1) & 1, &failed, limit);  // (the second product of the tile before may be under way)
+                        if (!ok) break;
+                        tc_fence_after();
+                        kt_rescale<C>(o_at, alpha);
+                    }
+                }
+                const float mb = m == -INFINITY ? 0.f : m, unit = pow2i(HEAD - power);
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int i = 0; i < 64; i += 2) {
+                    const float2 e = ft_fma2(make_float2(v[i], v[i + 1]), make_float2(ks[i / 16], ks[i / 16]), make_float2(-mb, -mb));
+                    v[i] = ex2(e.x);
+                    v[i + 1] = ex2(e.y);
+                    sum[i / 2 & 1] = ft_add2(sum[i / 2 & 1], make_float2(v[i], v[i + 1]));
+                }
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                unsigned y[32];
+#pragma unroll
+                for (int i = 0; i < 64; i += 2) {
+                    const float f = vs[i / 16] * unit;
+                    float2 e = mul2(make_float2(v[i], v[i + 1]), make_float2(f, f));
+                    if (!whole) {  // (a weight of 0 stays 0, whatever the scale of its page)
+                        e.x = v[i] == 0.f ? 0.f : e.x;
+                        e.y = v[i + 1] == 0.f ? 0.f : e.y;
+                    }
+                    x[i / 2] = pack_half(e.x, e.y);
+                    if constexpr (TERMS == 2) y[i / 2] = pack_rest(e.x, e.y, x[i / 2]);
+                }
+                tmem_st32(s_at, x);  // (over scores that have been read)
+                if constexpr (TERMS == 2) tmem_st32(s_at + 32, y);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[w][b]);
+        }
+        // ===== results
+        ok = ok && kt_wait<20>(&o_done[w][(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, &failed, limit);
+        tc_fence_after();
+        if (ok) {
+            const float sink = a.sink ? a.sink[head] * LOG2E : -INFINITY;
+            const float mm = fmaxf(m, sink), f = m == -INFINITY ? (l == 0.f ? 0.f : 1.0f) : ex2(m - mm);
+            const float sum = l * f + (sink == -INFINITY ? 0.f : ex2(sink - mm));
+            const float inv = sum == 0.f ? 0.f : f / sum, back = pow2i(power - HEAD);
+            const int64_t out_at = (int64_t)(q.first + i_tok) * a.dst_stride + (int64_t)head * c.vdim;
+#pragma unroll 1
+            for (int ch = 0; ch < c.vdim; ch += 32) {
+                float v[32];
+                tmem_ld32(o_at + ch, v);
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    if (!mine || ch + 16 * half >= c.vdim) continue;
+                    float y[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) y[e] = sum == 0.f ? 0.f : v[16 * half + e] * back * inv;
+                    const int64_t at = out_at + ch + 16 * half;
+                    if (a.type == B200_TYPE_F32) vec ? store16<float, true>(reinterpret_cast<float *>(a.dst) + at, y) : store16<float, false>(reinterpret_cast<float *>(a.dst) + at, y);
+                    else if (a.type == B200_TYPE_F16) vec ? store16<__half, true>(reinterpret_cast<__half *>(a.dst) + at, y) : store16<__half, false>(reinterpret_cast<__half *>(a.dst) + at, y);
+                    else vec ? store16<__nv_bfloat16, true>(reinterpret_cast<__nv_bfloat16 *>(a.dst) + at, y) : store16<__nv_bfloat16, false>(reinterpret_cast<__nv_bfloat16 *>(a.dst) + at, y);
+                }
+            }
+        }
+    } else if (warp == SOFTMAX) {
+        // ===== first products
+        asm volatile("bar.sync 2, %0;" ::"n"(SOFTMAX * 32 + 32) : "memory");
+        const bool elected = elect_lane();
+        const unsigned long long qd = umma_desc_sw128(smem_u32(sq)), kd0 = umma_desc_sw128(smem_u32(sk));
+        const int steps = c.dim / 16;
+        for (int t = 0; t < n_tiles; t++) {
+            const int b = t & 1, nb = t % NB;
+            if (!kt_wait<0>(&k_full[nb], (t / NB) & 1, &failed, limit)) break;
+            bool ok = true;
+#pragma unroll
+            for (int w = 0; w < GROUPS; w++) {
+                if (t >= 2) ok = kt_wait<0>(&o_done[w][b], ((t >> 1) & 1) ^ 1, &failed, limit);  // the weights of tile t - 2 have been used
+                if (!ok) break;
+                tc_fence_after();
+                if (elected) {
+                    const unsigned sd = tmem + (unsigned)((w * 2 + b) * KT_KEYS);
+#pragma unroll
+                    for (int term = 0; term < TERMS; term++)
+#pragma unroll
+                        for (int k = 0; k < C / 16; k++) {
+                            if (k >= steps) break;
+                            tc_mma_bf16(sd, qd + (unsigned)(((w * TERMS + term) * PANELS + k / 4) * (KT_Q_PANEL >> 4) + 2 * (k % 4)), kd0 + (unsigned)(nb * (TILE >> 4) + k / 4 * (KT_PANEL >> 4) + 2 * (k % 4)),
+                                        kt_idesc(KT_KEYS, false), term + k != 0);
+                        }
+                    tc_commit(&s_full[w][b]);
+                    if (w == GROUPS - 1) tc_commit(&k_free[nb]);
+                }
+                __syncwarp();
+            }
+            if (!ok) break;
+        }
+        __syncwarp();
+    } else if (warp == SOFTMAX + 1) {
+        // ===== second products
+        const bool elected = elect_lane();
+        const unsigned long long vd0 = umma_desc_mn_sw128(smem_u32(sv), KT_PANEL);
+        const unsigned idesc = kt_idesc(c.vdim, true);
+        for (int t = 0; t < n_tiles; t++) {
+            const int b = t & 1, nb = t % NB;
+            if (!kt_wait<0>(&v_full[nb], (t / NB) & 1, &failed, limit)) break;
+            bool ok = true;
+#pragma unroll
+            for (int w = 0; w < GROUPS; w++) {
+                ok = kt_wait<0>(&p_full[w][b], (t >> 1) & 1, &failed, limit);
+                if (!ok) break;
+                tc_fence_after();
+                if (elected) {
+                    const unsigned pd = tmem + (unsigned)((w * 2 + b) * KT_KEYS), out = tmem_o + (unsigned)(w * C);
+#pragma unroll
+                    for (int term = 0; term < TERMS; term++)
+#pragma unroll
+                        for (int k = 0; k < KT_KEYS / 16; k++)
+                            ft_mma_ts(out, pd + 32 * term + 8 * k, vd0 + (unsigned)(nb * (TILE >> 4) + k * (2048 >> 4)), idesc, t + term + k != 0);
+                    tc_commit(&o_done[w][b]);
+                    if (w == GROUPS - 1) tc_commit(&v_free[nb]);
+                }
+                __syncwarp();
+            }
+            if (!ok) break;
+        }
+        __syncwarp();
+    } else {
+        // ===== int8 to f16: of a tile's rows (keys), PIECES pieces of 16 values each
+        constexpr int PIECES = C / 16, ROWS = KT_CONVERT * 32 / PIECES, U = KT_KEYS / ROWS;  // rows at once, rounds
+        const int id = tid - (SOFTMAX + 2) * 32, piece = id % PIECES, row = id / PIECES;
+        const size_t record = record_bytes(c);
+        const unsigned char *base = reinterpret_cast<const unsigned char *>(c.pages), *base_v = base + v_at(c);
+        const bool has_k = piece * 16 < c.dim, has_v = piece * 16 < c.vdim;
+        const int shift = 31 - __clz(ps);
+        auto pages_ahead = [&](int t) {  // lane & 3: the pages of a tile's 16s of keys
+            const int key = t < n_tiles ? key_of(t) + 16 * (lane & 3) : 0x7fffffff;
+            return key <= pos_hi ? page_of(st, table, q.row, key >> shift) : -1;
+        };
+        auto fetch = [&](uint4 (&raw)[U], int t, int pages, const unsigned char *from, int size, bool has) {  // pages that are not there: zeros
+            const int key0 = t < n_tiles ? key_of(t) : 0;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int rr = row + u * ROWS, page = __shfl_sync(0xffffffffu, pages, rr >> 4);
+                raw[u] = make_uint4(0u, 0u, 0u, 0u);
+                if (page >= 0 && has) raw[u] = ld_behind(reinterpret_cast<const uint4 *>(from + (size_t)page * record + ((size_t)h * ps + ((key0 + rr) & (ps - 1))) * size + piece * 16));
+            }
+        };
+        auto put = [&](const uint4 (&raw)[U], unsigned char *tile) {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int rr = row + u * ROWS;
+                const unsigned w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+                unsigned f[8];
+#pragma unroll
+                for (int e = 0; e < 4; e++) int4_to_half(w[e], f[2 * e], f[2 * e + 1]);
+                unsigned char *at = tile + piece / 4 * KT_PANEL + rr * 128;
+                // (the two panels lie on the same banks: theirs are written in turn)
+                const int odd = piece >> 2 & 1, c0 = ((piece % 4) * 2 + odd) ^ (rr & 7);
+                *reinterpret_cast<uint4 *>(at + c0 * 16) = odd ? make_uint4(f[4], f[5], f[6], f[7]) : make_uint4(f[0], f[1], f[2], f[3]);
+                *reinterpret_cast<uint4 *>(at + (c0 ^ 1) * 16) = odd ? make_uint4(f[0], f[1], f[2], f[3]) : make_uint4(f[4], f[5], f[6], f[7]);
+            }
+        };
+        uint4 kr[U], vr[U];
+        int pages = pages_ahead(0);
+        fetch(kr, 0, pages, base, c.dim, has_k);
+        fetch(vr, 0, pages, base_v, c.vdim, has_v);
+        pages = pages_ahead(1);
+        for (int t = 0; t < n_tiles; t++) {
+            const int nb = t % NB, parity = ((t / NB) & 1) ^ 1;
+            if (t >= NB && !kt_wait<20>(&k_free[nb], parity, &failed, limit)) break;
+            put(kr, sk + nb * TILE);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&k_full[nb]);
+            fetch(kr, t + 1, pages, base, c.dim, has_k);
+            if (t >= NB && !kt_wait<20>(&v_free[nb], parity, &failed, limit)) break;
+            put(vr, sv + nb * TILE);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&v_full[nb]);
+            fetch(vr, t + 1, pages, base_v, c.vdim, has_v);
+            pages = pages_ahead(t + 2);
+        }
+        __syncwarp();
+    }
+    __syncwarp();
+    __syncthreads();
+    if (failed) {  // MMAs that were requested end within this time
+        if (tid == 0) atomicExch(timeout, 1);
+        for (const long long t0 = clock64(); clock64() - t0 < 4000000LL;) {}
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == SOFTMAX) {
+        tc_fence_after();
+        tmem_dealloc(tmem, TMEM);
+    }
+}
+
+template <int C, int GROUPS, int TERMS>
+static int launch_tc(const AttnArgs &args, bool vec, long long limit, cudaStream_t st) {
+    int *status = nullptr;
+    const int rc = gemm_status_word(&status);
+    if (rc != B200_OK) return rc;
+    static bool done[16] = {};  // cudaFuncSetAttribute is per device
+    int dev = 0;
+    B200_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev >= 16 || !done[dev]) {
+        B200_CUDA_TRY(cudaFuncSetAttribute(kv8_attn_tc_kernel<C, GROUPS, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kt_smem<C, GROUPS, TERMS>()));
+        if (dev < 16) done[dev] = true;
+    }
+    const dim3 grid((unsigned)((int64_t)args.a.n_tokens * args.group / (GROUPS * KT_ROWS) + args.a.n_seq), (unsigned)args.a.cache.n_head_kv);
+    B200_CUDA_TRY(launch_chained(kv8_attn_tc_kernel<C, GROUPS, TERMS>, grid, kt_threads<GROUPS>(), kt_smem<C, GROUPS, TERMS>(), st, args, vec, limit, status));
+    return B200_OK;
+}
+
+}  // namespace kv8
+}  // namespace b200
