@@ -58,11 +58,14 @@ __device__ __forceinline__ void row_put(void *row, int type, int64_t at, float x
     else if (type == B200_TYPE_F16) reinterpret_cast<__half *>(row)[at] = __float2half_rn(x);
     else reinterpret_cast<__nv_bfloat16 *>(row)[at] = __float2bfloat16_rn(x);
 }
-__device__ __forceinline__ bool visible(int key, int pos, int window, int keep_first) { return key <= pos && (window <= 0 || pos - key < window || key < keep_first); }
-
-// whether a query sees any of the 16 keys from `key` on, whose page is there if bit 0 of `there` is set
-__device__ __forceinline__ bool half_seen(int key, int pos, int there, int window, int keep_first) {
-    return (there & 1) && key <= pos && (window <= 0 || pos - (key + 15) < window || key < keep_first);
+// bits below n of 32
+__device__ __forceinline__ unsigned below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }
+// Which of the 32 keys from `key` on a query sees: those up to its own position, and of them those within the window or among the first that stay.  `there`:
+// bits 0 and 1, whether the pages of the two 16s are there.
+__device__ __forceinline__ unsigned seen_keys(int key, int pos, int there, int window, int keep_first) {
+    unsigned seen = below(pos + 1 - key);
+    if (window > 0) seen &= ~below(pos + 1 - window - key) | below(keep_first - key);
+    return seen & ((there & 1 ? 0xffffu : 0u) | (there & 2 ? 0xffff0000u : 0u));
 }
 
 constexpr float LOG2E = 1.4426950408889634f;
@@ -77,6 +80,7 @@ struct AttnArgs {
     int *counters;    // one per CTA, zero between calls
     float *partials;  // two per CTA
     int group;        // query heads per kv head
+    unsigned group_div;  // ceil(2^32 / group): __umulhi(x, group_div) = x / group for x < 2^32 / group
     int rows_most;    // sequences with more query rows a kv head (tokens times group) are the prompt kernel's; negative: there is none
 };
 
@@ -313,14 +317,14 @@ __global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_k
                     for (int i = 0; i < 8; i++) p[r][i] = cap_log2 * tanh_fast(p[r][i]);
             }
             const bool whole = there == 3 && n_rows == R && key0 + RW_TILE - 1 <= pos_lo && (a.window <= 0 || pos_hi - key0 < a.window);
-            if (!whole) {
+            unsigned seen[NR];
 #pragma unroll
-                for (int r = 0; r < NR; r++)
+            for (int r = 0; r < NR; r++) {
+                seen[r] = whole ? 0xffffffffu : seen_keys(key0, pos[r], there, a.window, a.keep_first);
+                if (whole) continue;
+                const unsigned own = seen[r] >> (2 * tg);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int key = key0 + 8 * (i / 2) + 2 * tg + i % 2;
-                        if (!((there >> (i / 4) & 1) && visible(key, pos[r], a.window, a.keep_first))) p[r][i] = -INFINITY;
-                    }
+                for (int i = 0; i < 8; i++) p[r][i] = own >> (8 * (i / 2) + i % 2) & 1u ? p[r][i] : -INFINITY;
             }
             // ---- maxima, weights
             float corr[NR], common[NR];
@@ -341,8 +345,8 @@ __global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_k
             float vs[NR][2];
 #pragma unroll
             for (int r = 0; r < NR; r++) {
-                vs[r][0] = half_seen(key0, pos[r], there, a.window, a.keep_first) ? scales.y : 0.f;
-                vs[r][1] = half_seen(key0 + 16, pos[r], there >> 1, a.window, a.keep_first) ? scales.w : 0.f;
+                vs[r][0] = seen[r] & 0xffffu ? scales.y : 0.f;
+                vs[r][1] = seen[r] & 0xffff0000u ? scales.w : 0.f;
                 const float loudest = fmaxf(vs[r][0], vs[r][1]);  // (a NaN only if both are)
                 const int now = exponent_above(loudest <= FLT_MAX ? __float_as_uint(loudest) & 0x7fffffffu : 0u);
                 if (now > power[r]) {
@@ -599,7 +603,8 @@ int b200_op_kv8_attn(const b200_kv8_attn_args *a, void *workspace, size_t worksp
                 b200_kv8_attn_workspace_bytes(a));
     const b200_kv8_cache &c = a->cache;
     AttnArgs args = {*a, {a->seq_info, a->table, a->table_stride, a->n_rows, a->n_seq, a->n_tokens, c.n_pages, c.page_size}, (int *)workspace,
-                     (float *)((char *)workspace + rows_counter_bytes(rows_grid(c))), a->n_head / c.n_head_kv, -1};
+                     (float *)((char *)workspace + rows_counter_bytes(rows_grid(c))), a->n_head / c.n_head_kv, 0, -1};
+    args.group_div = (unsigned)(((1ull << 32) + args.group - 1) / args.group);
     const cudaStream_t st = (cudaStream_t)stream;
     const int k = attn_class(c);
     const int64_t longest = (int64_t)(a->max_new > 0 && a->max_new < a->n_tokens ? a->max_new : a->n_tokens) * args.group;  // query rows a kv head of one sequence, at most

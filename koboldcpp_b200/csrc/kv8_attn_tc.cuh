@@ -8,8 +8,7 @@
 // shared memory in the 128-byte swizzle that the products read.  int8 is exact in f16, so with TERMS = 2 only Q and P have to be taken apart (upper halves
 // and what those leave over, a second product each) for results as f32 gives them; 64 columns of S are just two times 32 of P.
 // Softmax: four warps a group of 128 rows.  The maximum that the exponent subtracts follows the true one only when that has grown by SLACK, so O is hardly
-// ever rescaled.  A key's scale joins its score, a value's its weight, relative to the power of two above the largest that the row has seen; the softmax
-// warps bring the scales of their tile's four 16s of keys themselves, a tile ahead.
+// ever rescaled.  A key's scale joins its score, a value's its weight, relative to the power of two above the largest that the row has seen.
 // Every S has two buffers a group: products run while the softmax is busy with the tile before.
 // Waits have a limit, as in the prompt GEMM: a role that gives up sets `failed`, the others follow, and the status word is set.
 #pragma once
@@ -19,8 +18,9 @@ namespace b200 {
 namespace kv8 {
 
 constexpr int KT_ROWS = 128, KT_KEYS = 64, KT_CONVERT = 4;
+constexpr int KT_RING = 8;  // scales of so many tiles: a tile's are written when the weights of the tile NB + 2 before it have been used
 constexpr int KT_Q_PANEL = KT_ROWS * 128, KT_PANEL = KT_KEYS * 128;  // panels of 64 values, 128 bytes a row
-template <int GROUPS> constexpr int kt_threads() { return (GROUPS * 4 + 2 + KT_CONVERT) * 32; }
+template <int GROUPS> constexpr int kt_threads() { return (GROUPS * 6 + KT_CONVERT) * 32; }
 template <int GROUPS, int TERMS> constexpr int kt_buffers() { return GROUPS * TERMS == 4 ? 3 : 4; }  // of K and V
 template <int C, int GROUPS, int TERMS> constexpr size_t kt_smem() {
     return 1024 + (size_t)GROUPS * TERMS * (C / 64) * KT_Q_PANEL + (size_t)kt_buffers<GROUPS, TERMS>() * 2 * (C / 64) * KT_PANEL;
@@ -51,6 +51,49 @@ __device__ __forceinline__ bool kt_wait(unsigned long long *bar, int parity, vol
     return __all_sync(0xffffffffu, pair_wait<SLEEP>(smem_u32(bar), (unsigned)parity, failed, limit));
 }
 
+// 8 values of a row as they lie there (16 bits: in the first of the two); zeros where there are none
+__device__ __forceinline__ void row_load8(const void *row, int type, int64_t at, bool there, bool vec, uint4 (&u)[2]) {
+    u[0] = u[1] = make_uint4(0u, 0u, 0u, 0u);
+    if (!there) return;
+    const unsigned char *p = reinterpret_cast<const unsigned char *>(row) + at * (type == B200_TYPE_F32 ? 4 : 2);
+    if (vec) {
+        u[0] = reinterpret_cast<const uint4 *>(p)[0];
+        if (type == B200_TYPE_F32) u[1] = reinterpret_cast<const uint4 *>(p)[1];
+    } else if (type == B200_TYPE_F32) {
+        const unsigned *f = reinterpret_cast<const unsigned *>(p);
+        u[0] = make_uint4(f[0], f[1], f[2], f[3]);
+        u[1] = make_uint4(f[4], f[5], f[6], f[7]);
+    } else {
+        const unsigned short *f = reinterpret_cast<const unsigned short *>(p);
+        u[0] = make_uint4(f[0] | (unsigned)f[1] << 16, f[2] | (unsigned)f[3] << 16, f[4] | (unsigned)f[5] << 16, f[6] | (unsigned)f[7] << 16);
+    }
+}
+__device__ __forceinline__ void row_values8(const uint4 (&u)[2], int type, float (&x)[8]) {
+    const unsigned w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
+    if (type == B200_TYPE_F32) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = __uint_as_float(w[e]);
+    } else if (type == B200_TYPE_F16) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = h2f((unsigned short)(w[e / 2] >> (16 * (e & 1))));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    }
+}
+__device__ __forceinline__ void row_store4(void *row, int type, int64_t at, bool vec, float4 y) {
+    if (!vec) {
+        row_put(row, type, at, y.x); row_put(row, type, at + 1, y.y); row_put(row, type, at + 2, y.z); row_put(row, type, at + 3, y.w);
+    } else if (type == B200_TYPE_F32) {
+        *reinterpret_cast<float4 *>(reinterpret_cast<float *>(row) + at) = y;
+    } else if (type == B200_TYPE_F16) {
+        *reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(row) + at) = make_uint2(pack_half(y.x, y.y), pack_half(y.z, y.w));
+    } else {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
+        *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(row) + at) = make_uint2(*reinterpret_cast<const unsigned *>(&a), *reinterpret_cast<const unsigned *>(&b));
+    }
+}
+
 template <int C, int GROUPS, int TERMS>
 __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(const __grid_constant__ AttnArgs args, bool vec, long long limit, int *timeout) {
     constexpr int NB = kt_buffers<GROUPS, TERMS>(), PANELS = C / 64, BLOCK = GROUPS * KT_ROWS, SOFTMAX = GROUPS * 4;
@@ -59,16 +102,20 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
     unsigned char *smem = reinterpret_cast<unsigned char *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ __align__(8) unsigned long long k_full[NB], k_free[NB], v_full[NB], v_free[NB], s_full[GROUPS][2], p_full[GROUPS][2], o_done[GROUPS][2];
     __shared__ unsigned tmem_base_s;
+    __shared__ float row_scale_s[BLOCK];
+    __shared__ __align__(16) float scales_s[KT_RING][8];  // of a tile's four 16s of keys: the keys', the values'
+    __shared__ int there_s[KT_RING];                      // bit i: their page is there
+    __shared__ __align__(8) unsigned long long scales_full[KT_RING];
     __shared__ volatile int failed;
     const b200_kv8_attn_args &a = args.a;
     const b200_kv8_cache &c = a.cache;
     const Step &st = args.step;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    const int group = args.group, ps = c.page_size, h = blockIdx.y;
+    const int group = args.group, ps = c.page_size, h = (int)(blockIdx.x % (unsigned)c.n_head_kv);
     pdl_enter();
     const int32_t *info = behind(st.info), *table = behind(st.table);
-    // block j of rows belongs to the sequence s with first_s group / BLOCK + s <= j (long causal walks first)
-    const int j = (int)(gridDim.x - 1 - blockIdx.x);
+    // block j of rows belongs to the sequence s with first_s group / BLOCK + s <= j (long causal walks first, of all heads)
+    const int j = (int)((gridDim.x - 1 - blockIdx.x) / (unsigned)c.n_head_kv);
     auto first_block = [&](int first, int s) { return (int)((int64_t)first * group / BLOCK) + s; };
     const int s = find_seq(info, st.n_seq, j, first_block);
     const Seq q = seq_of(st, info, s);
@@ -76,6 +123,9 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
     if (rows_64 <= args.rows_most || row0_64 < 0 || row0_64 >= rows_64) return;  // (another kernel's, or no block)
     const int row0 = (int)row0_64, n_rows = (int)min((int64_t)BLOCK, rows_64 - row0_64);
     const int pos_lo = q.held + row0 / group, pos_hi = q.held + (row0 + n_rows - 1) / group;
+    // local row r is query head head0 + r - token(r) * group of token tok0 + token(r)
+    const int tok0 = row0 / group, head0 = row0 - tok0 * group;
+    auto token = [&](int r) { return group == 1 ? r : (int)__umulhi((unsigned)(head0 + r), args.group_div); };
     // tiles: those of the kept first tokens, then from the window's on
     const int first_tile = a.window > 0 ? max(0, pos_lo + 1 - a.window) / KT_KEYS : 0;
     const int keep_tiles = a.window > 0 ? min((int)(((int64_t)max(a.keep_first, 0) + KT_KEYS - 1) / KT_KEYS), first_tile) : 0;
@@ -84,7 +134,8 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
     unsigned char *sq = smem, *sk = sq + GROUPS * TERMS * PANELS * KT_Q_PANEL, *sv = sk + NB * TILE;
 
     if (tid == 0) {
-        for (int i = 0; i < NB; i++) { mbar_init(&k_full[i], KT_CONVERT); mbar_init(&k_free[i], 1); mbar_init(&v_full[i], KT_CONVERT); mbar_init(&v_free[i], 1); }
+        for (int i = 0; i < NB; i++) { mbar_init(&k_full[i], KT_CONVERT); mbar_init(&k_free[i], GROUPS); mbar_init(&v_full[i], KT_CONVERT); mbar_init(&v_free[i], GROUPS); }
+        for (int i = 0; i < KT_RING; i++) mbar_init(&scales_full[i], 1);
         for (int i = 0; i < 2 * GROUPS; i++) { mbar_init(&s_full[i >> 1][i & 1], 1); mbar_init(&p_full[i >> 1][i & 1], 4); mbar_init(&o_done[i >> 1][i & 1], 1); }
         mbar_fence_init();
         failed = 0;
@@ -97,80 +148,72 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
     const unsigned tmem = tmem_base_s, tmem_o = tmem + GROUPS * 2 * KT_KEYS;
 
     if (warp < SOFTMAX) {
-        // ===== a row of Q as f16, relative to the power of two above its largest value
+        // ===== Q as f16, a row relative to the power of two above its largest value: a thread takes 8 dims, piece number `piece` of a row, of every ROWS-th row
         const int w = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane, row = w * KT_ROWS + r;
-        const bool mine = row < n_rows;
-        const int i_tok = mine ? (row0 + row) / group : 0, head = h * group + (mine ? (row0 + row) % group : 0);
-        const int64_t q_at = (int64_t)(q.first + i_tok) * a.q_stride + (int64_t)head * c.dim;
-        const void *qp = behind(a.q);
-        auto piece = [&](int p, float (&x)[16]) {
-            if (a.type == B200_TYPE_F32) vec ? load16<float, true>(reinterpret_cast<const float *>(qp) + q_at + 16 * p, x) : load16<float, false>(reinterpret_cast<const float *>(qp) + q_at + 16 * p, x);
-            else if (a.type == B200_TYPE_F16) vec ? load16<__half, true>(reinterpret_cast<const __half *>(qp) + q_at + 16 * p, x) : load16<__half, false>(reinterpret_cast<const __half *>(qp) + q_at + 16 * p, x);
-            else vec ? load16<__nv_bfloat16, true>(reinterpret_cast<const __nv_bfloat16 *>(qp) + q_at + 16 * p, x) : load16<__nv_bfloat16, false>(reinterpret_cast<const __nv_bfloat16 *>(qp) + q_at + 16 * p, x);
-        };
-        unsigned loud = 0;
-        for (int p = 0; mine && p < c.dim / 16; p++) {
-            float x[16];
-            piece(p, x);
+        {
+            constexpr int PIECES = C / 8, ROWS = SOFTMAX * 32 / PIECES, AT_ONCE = 8;
+            const int piece = tid % PIECES;
+            const bool there = piece * 8 < c.dim;
+            const void *qp = behind(a.q);
+            unsigned char *at = sq + piece / 8 * KT_Q_PANEL;
+#pragma unroll 1
+            for (int r0 = tid / PIECES; r0 < BLOCK; r0 += AT_ONCE * ROWS) {
+                uint4 raw[AT_ONCE][2];
 #pragma unroll
-            for (int e = 0; e < 16; e++) loud = max(loud, __float_as_uint(x[e]) & 0x7fffffffu);
-        }
-        const int e_q = exponent_above(loud);
-        const float down = pow2i(min(14 - e_q, 126));
-        const float row_scale = loud >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : a.scale * pow2i(max(e_q - 14, -126)) * (a.softcap > 0.f ? 1.0f / a.softcap : LOG2E);
-        for (int p = 0; p < c.dim / 16; p++) {
-            float x[16];
-            if (mine) piece(p, x);
+                for (int k = 0; k < AT_ONCE; k++) {
+                    const int rr = r0 + k * ROWS, tok = token(rr);
+                    row_load8(qp, a.type, (int64_t)(q.first + tok0 + tok) * a.q_stride + (int64_t)(h * group + head0 + rr - tok * group) * c.dim + piece * 8, rr < n_rows && there, vec, raw[k]);
+                }
 #pragma unroll
-            for (int e = 0; e < 16; e++) x[e] = mine ? x[e] * down : 0.f;
-            unsigned hi[8];
+                for (int k = 0; k < AT_ONCE; k++) {
+                    const int rr = r0 + k * ROWS, rw = rr % KT_ROWS;
+                    float x[8];
+                    row_values8(raw[k], a.type, x);
+                    unsigned loud = 0;
 #pragma unroll
-            for (int e = 0; e < 8; e++) hi[e] = pack_half(x[2 * e], x[2 * e + 1]);
-            unsigned char *at = sq + ((w * TERMS) * PANELS + p / 4) * KT_Q_PANEL + r * 128;
-            const int c0 = ((p % 4) * 2) ^ (r & 7);
-            *reinterpret_cast<uint4 *>(at + c0 * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4 *>(at + (c0 ^ 1) * 16) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
-            if constexpr (TERMS == 2) {
-                at += PANELS * KT_Q_PANEL;
-                *reinterpret_cast<uint4 *>(at + c0 * 16) = make_uint4(pack_rest(x[0], x[1], hi[0]), pack_rest(x[2], x[3], hi[1]), pack_rest(x[4], x[5], hi[2]), pack_rest(x[6], x[7], hi[3]));
-                *reinterpret_cast<uint4 *>(at + (c0 ^ 1) * 16) = make_uint4(pack_rest(x[8], x[9], hi[4]), pack_rest(x[10], x[11], hi[5]), pack_rest(x[12], x[13], hi[6]), pack_rest(x[14], x[15], hi[7]));
+                    for (int e = 0; e < 8; e++) loud = max(loud, __float_as_uint(x[e]) & 0x7fffffffu);
+#pragma unroll
+                    for (int o = 1; o < PIECES; o *= 2) loud = max(loud, __shfl_xor_sync(0xffffffffu, loud, o));
+                    const int e_q = exponent_above(loud);
+                    const float down = pow2i(min(14 - e_q, 126));
+                    if (piece == 0)
+                        row_scale_s[rr] = loud >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : a.scale * pow2i(max(e_q - 14, -126)) * (a.softcap > 0.f ? 1.0f / a.softcap : LOG2E);
+                    unsigned hi[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) hi[e] = pack_half(x[2 * e] *= down, x[2 * e + 1] *= down);
+                    unsigned char *to = at + rr / KT_ROWS * (TERMS * PANELS * KT_Q_PANEL) + rw * 128 + (((piece % 8) ^ (rw & 7)) << 4);
+                    *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if constexpr (TERMS == 2)
+                        *reinterpret_cast<uint4 *>(to + PANELS * KT_Q_PANEL) = make_uint4(pack_rest(x[0], x[1], hi[0]), pack_rest(x[2], x[3], hi[1]), pack_rest(x[4], x[5], hi[2]),
+                                                                                        pack_rest(x[6], x[7], hi[3]));
+                }
             }
         }
         fence_proxy_async_smem();
-        asm volatile("bar.arrive 2, %0;" ::"n"(SOFTMAX * 32 + 32) : "memory");
+        asm volatile("bar.arrive 2, %0;" ::"n"((SOFTMAX + GROUPS) * 32) : "memory");
+        asm volatile("bar.sync 3, %0;" ::"n"(SOFTMAX * 32) : "memory");  // (the rows' scales)
 
+        const bool mine = row < n_rows;
+        const int i_tok = tok0 + (mine ? token(row) : 0), head = h * group + (mine ? head0 + row - token(row) * group : 0);
+        const float row_scale = row_scale_s[row];
         const int pos = mine ? q.held + i_tok : -1;
         // positions of this warp's rows (none: pos_hi_w < pos_lo_w)
         const int w0 = w * KT_ROWS + quarter * 32, w1 = min(w0 + 31, n_rows - 1);
         const int pos_lo_w = w0 < n_rows ? q.held + (row0 + w0) / group : 0, pos_hi_w = w0 < n_rows ? q.held + (row0 + w1) / group : -1;
         const bool all_rows = w0 + 31 < n_rows;
         const unsigned lanes = (unsigned)(quarter * 32) << 16, o_at = tmem_o + (unsigned)(w * C) + lanes;
-        // lane l & 3 of a tile's 16s of keys: page a tile ahead, then its scales (lanes 0 .. 3 the keys', 4 .. 7 the values')
-        auto page_ahead = [&](int t) {
-            const int key = t < n_tiles ? key_of(t) + 16 * (lane & 3) : 0x7fffffff;
-            return key <= pos_hi ? page_of(st, table, q.row, key / ps) : -1;
-        };
-        auto scale_ahead = [&](int page) {
-            if (page < 0 || lane >= 8) return 0.f;
-            const unsigned char *record = reinterpret_cast<const unsigned char *>(c.pages) + (size_t)page * record_bytes(c) + scales_at(c);
-            return *(reinterpret_cast<const volatile float *>(record) + (lane >> 2) * c.n_head_kv + h);
-        };
-        int page = page_ahead(0), page_next = page_ahead(1);
-        float scale = scale_ahead(page);
         float m = -INFINITY, l = 0.f;
         int power = -100;
         bool ok = true;
         for (int t = 0; t < n_tiles; t++) {
             const int b = t & 1, key0 = key_of(t);
             const unsigned s_at = tmem + (unsigned)((w * 2 + b) * KT_KEYS) + lanes;
-            const int there = (int)(__ballot_sync(0xffffffffu, page >= 0) & 15u);
-            float ks[4], vs[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) { ks[i] = __shfl_sync(0xffffffffu, scale, i) * row_scale; vs[i] = __shfl_sync(0xffffffffu, scale, 4 + i); }
-            page = page_next;
-            scale = scale_ahead(page);
-            page_next = page_ahead(t + 2);
-            ok = kt_wait<20>(&s_full[w][b], (t >> 1) & 1, &failed, limit);
+            ok = kt_wait<0>(&scales_full[t % KT_RING], (t / KT_RING) & 1, &failed, limit);
+            if (!ok) break;
+            const int there = there_s[t % KT_RING];
+            const float4 k4 = *reinterpret_cast<const float4 *>(&scales_s[t % KT_RING][0]), v4 = *reinterpret_cast<const float4 *>(&scales_s[t % KT_RING][4]);
+            float ks[4] = {k4.x * row_scale, k4.y * row_scale, k4.z * row_scale, k4.w * row_scale}, vs[4] = {v4.x, v4.y, v4.z, v4.w};
+            ok = kt_wait<0>(&s_full[w][b], (t >> 1) & 1, &failed, limit);
             if (!ok) break;
             tc_fence_after();
             unsigned x[32];
@@ -186,6 +229,7 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
                 tmem_ld32_async(s_at + 32, v + 32);
                 const bool whole = there == 15 && all_rows && key0 + KT_KEYS - 1 <= pos_lo_w && (a.window <= 0 || pos_hi_w - key0 < a.window);
                 tmem_wait_ld(v);
+                unsigned seen[2] = {0xffffffffu, 0xffffffffu};
                 // the common tile keeps the raw products; ks takes them to scores times log2 e
                 if (!whole || a.softcap > 0.f || !(a.scale > 0.f)) {
 #pragma unroll
@@ -196,8 +240,10 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
                         for (int i = 0; i < 64; i++) v[i] = cap_log2 * tanh_fast(v[i]);
                     }
                     if (!whole) {
+                        seen[0] = seen_keys(key0, pos, there, a.window, a.keep_first);
+                        seen[1] = seen_keys(key0 + 32, pos, there >> 2, a.window, a.keep_first);
 #pragma unroll
-                        for (int i = 0; i < 64; i++) if (!((there >> (i / 16) & 1) && visible(key0 + i, pos, a.window, a.keep_first))) v[i] = -INFINITY;
+                        for (int i = 0; i < 64; i++) v[i] = seen[i / 32] >> (i % 32) & 1u ? v[i] : -INFINITY;
                     }
 #pragma unroll
                     for (int i = 0; i < 4; i++) ks[i] = 1.0f;
@@ -209,7 +255,7 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
 #pragma unroll
                     for (int e = 2; e < 16; e += 2) { t0 = fmaxf(t0, v[16 * i + e]); t1 = fmaxf(t1, v[16 * i + e + 1]); }
                     top = fmaxf(top, fmaxf(t0, t1) * ks[i]);
-                    if (!whole && !half_seen(key0 + 16 * i, pos, there >> i, a.window, a.keep_first)) vs[i] = 0.f;
+                    vs[i] = seen[i / 2] >> (16 * (i & 1)) & 0xffffu ? vs[i] : 0.f;
                     loudest = fmaxf(loudest, vs[i]);  // (passes over NaN)
                 }
                 const bool grown = top > m + SLACK;  // (m = -inf: as soon as a key is seen)
@@ -263,90 +309,100 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
             const float mm = fmaxf(m, sink), f = m == -INFINITY ? (l == 0.f ? 0.f : 1.0f) : ex2(m - mm);
             const float sum = l * f + (sink == -INFINITY ? 0.f : ex2(sink - mm));
             const float inv = sum == 0.f ? 0.f : f / sum, back = pow2i(power - HEAD);
-            const int64_t out_at = (int64_t)(q.first + i_tok) * a.dst_stride + (int64_t)head * c.vdim;
+            const float share = sum == 0.f ? 0.f : inv * back;
+            // 32 columns at a time through shared memory (where this warp's rows of Q were), so that a row's stores lie side by side
+            unsigned char *stage = sq + w * TERMS * PANELS * KT_Q_PANEL + quarter * 4096;
+            const int e = lane & 7;
+            int64_t at[8];  // where this lane's part of the rows 4 k + lane / 8 goes; -1: no such row
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int rb = w0 + 4 * k + (lane >> 3), tok = token(rb);
+                at[k] = rb < n_rows ? (int64_t)(q.first + tok0 + tok) * a.dst_stride + (int64_t)(h * group + head0 + rb - tok * group) * c.vdim + 4 * e : -1;
+            }
 #pragma unroll 1
             for (int ch = 0; ch < c.vdim; ch += 32) {
                 float v[32];
                 tmem_ld32(o_at + ch, v);
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    if (!mine || ch + 16 * half >= c.vdim) continue;
-                    float y[16];
-#pragma unroll
-                    for (int e = 0; e < 16; e++) y[e] = sum == 0.f ? 0.f : v[16 * half + e] * back * inv;
-                    const int64_t at = out_at + ch + 16 * half;
-                    if (a.type == B200_TYPE_F32) vec ? store16<float, true>(reinterpret_cast<float *>(a.dst) + at, y) : store16<float, false>(reinterpret_cast<float *>(a.dst) + at, y);
-                    else if (a.type == B200_TYPE_F16) vec ? store16<__half, true>(reinterpret_cast<__half *>(a.dst) + at, y) : store16<__half, false>(reinterpret_cast<__half *>(a.dst) + at, y);
-                    else vec ? store16<__nv_bfloat16, true>(reinterpret_cast<__nv_bfloat16 *>(a.dst) + at, y) : store16<__nv_bfloat16, false>(reinterpret_cast<__nv_bfloat16 *>(a.dst) + at, y);
+                for (int i = 0; i < 8; i++) {
+                    float4 y = make_float4(v[4 * i] * share, v[4 * i + 1] * share, v[4 * i + 2] * share, v[4 * i + 3] * share);
+                    if (share == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);  // (nothing was seen)
+                    *reinterpret_cast<float4 *>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = y;
                 }
+                __syncwarp();
+                if (ch + 4 * e < c.vdim) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const int rr = 4 * k + (lane >> 3);
+                        const float4 y = *reinterpret_cast<const float4 *>(stage + rr * 128 + ((e ^ (rr & 7)) << 4));
+                        if (at[k] >= 0) row_store4(a.dst, a.type, at[k] + ch, vec, y);
+                    }
+                }
+                __syncwarp();
             }
         }
-    } else if (warp == SOFTMAX) {
-        // ===== first products
-        asm volatile("bar.sync 2, %0;" ::"n"(SOFTMAX * 32 + 32) : "memory");
+    } else if (warp < SOFTMAX + GROUPS) {
+        // ===== first products of a group
+        const int w = warp - SOFTMAX;
+        asm volatile("bar.sync 2, %0;" ::"n"((SOFTMAX + GROUPS) * 32) : "memory");
         const bool elected = elect_lane();
-        const unsigned long long qd = umma_desc_sw128(smem_u32(sq)), kd0 = umma_desc_sw128(smem_u32(sk));
+        const unsigned long long qd = umma_desc_sw128(smem_u32(sq)) + (unsigned)(w * TERMS * PANELS * (KT_Q_PANEL >> 4)), kd0 = umma_desc_sw128(smem_u32(sk));
         const int steps = c.dim / 16;
         for (int t = 0; t < n_tiles; t++) {
             const int b = t & 1, nb = t % NB;
             if (!kt_wait<0>(&k_full[nb], (t / NB) & 1, &failed, limit)) break;
-            bool ok = true;
-#pragma unroll
-            for (int w = 0; w < GROUPS; w++) {
-                if (t >= 2) ok = kt_wait<0>(&o_done[w][b], ((t >> 1) & 1) ^ 1, &failed, limit);  // the weights of tile t - 2 have been used
-                if (!ok) break;
-                tc_fence_after();
-                if (elected) {
-                    const unsigned sd = tmem + (unsigned)((w * 2 + b) * KT_KEYS);
+            if (t >= 2 && !kt_wait<0>(&o_done[w][b], ((t >> 1) & 1) ^ 1, &failed, limit)) break;  // the weights of tile t - 2 have been used
+            tc_fence_after();
+            if (elected) {
+                const unsigned sd = tmem + (unsigned)((w * 2 + b) * KT_KEYS);
+                const unsigned long long kd = kd0 + (unsigned)(nb * (TILE >> 4));
+                if (steps == C / 16) {
 #pragma unroll
                     for (int term = 0; term < TERMS; term++)
 #pragma unroll
-                        for (int k = 0; k < C / 16; k++) {
-                            if (k >= steps) break;
-                            tc_mma_bf16(sd, qd + (unsigned)(((w * TERMS + term) * PANELS + k / 4) * (KT_Q_PANEL >> 4) + 2 * (k % 4)), kd0 + (unsigned)(nb * (TILE >> 4) + k / 4 * (KT_PANEL >> 4) + 2 * (k % 4)),
-                                        kt_idesc(KT_KEYS, false), term + k != 0);
-                        }
-                    tc_commit(&s_full[w][b]);
-                    if (w == GROUPS - 1) tc_commit(&k_free[nb]);
+                        for (int k = 0; k < C / 16; k++)
+                            tc_mma_bf16(sd, qd + (unsigned)((term * PANELS + k / 4) * (KT_Q_PANEL >> 4) + 2 * (k % 4)), kd + (unsigned)(k / 4 * (KT_PANEL >> 4) + 2 * (k % 4)), kt_idesc(KT_KEYS, false), term + k != 0);
+                } else {
+#pragma unroll 1
+                    for (int i = 0; i < TERMS * steps; i++) {
+                        const int term = i >= steps, k = i - term * steps;
+                        tc_mma_bf16(sd, qd + (unsigned)((term * PANELS + k / 4) * (KT_Q_PANEL >> 4) + 2 * (k % 4)), kd + (unsigned)(k / 4 * (KT_PANEL >> 4) + 2 * (k % 4)), kt_idesc(KT_KEYS, false), i != 0);
+                    }
                 }
-                __syncwarp();
+                tc_commit(&s_full[w][b]);
+                tc_commit(&k_free[nb]);
             }
-            if (!ok) break;
+            __syncwarp();
         }
         __syncwarp();
-    } else if (warp == SOFTMAX + 1) {
-        // ===== second products
+    } else if (warp < SOFTMAX + 2 * GROUPS) {
+        // ===== second products of a group
+        const int w = warp - SOFTMAX - GROUPS;
         const bool elected = elect_lane();
         const unsigned long long vd0 = umma_desc_mn_sw128(smem_u32(sv), KT_PANEL);
-        const unsigned idesc = kt_idesc(c.vdim, true);
+        const unsigned idesc = kt_idesc(c.vdim, true), out = tmem_o + (unsigned)(w * C);
         for (int t = 0; t < n_tiles; t++) {
             const int b = t & 1, nb = t % NB;
             if (!kt_wait<0>(&v_full[nb], (t / NB) & 1, &failed, limit)) break;
-            bool ok = true;
+            if (!kt_wait<0>(&p_full[w][b], (t >> 1) & 1, &failed, limit)) break;
+            tc_fence_after();
+            if (elected) {
+                const unsigned pd = tmem + (unsigned)((w * 2 + b) * KT_KEYS);
+                const unsigned long long vd = vd0 + (unsigned)(nb * (TILE >> 4));
 #pragma unroll
-            for (int w = 0; w < GROUPS; w++) {
-                ok = kt_wait<0>(&p_full[w][b], (t >> 1) & 1, &failed, limit);
-                if (!ok) break;
-                tc_fence_after();
-                if (elected) {
-                    const unsigned pd = tmem + (unsigned)((w * 2 + b) * KT_KEYS), out = tmem_o + (unsigned)(w * C);
+                for (int term = 0; term < TERMS; term++)
 #pragma unroll
-                    for (int term = 0; term < TERMS; term++)
-#pragma unroll
-                        for (int k = 0; k < KT_KEYS / 16; k++)
-                            ft_mma_ts(out, pd + 32 * term + 8 * k, vd0 + (unsigned)(nb * (TILE >> 4) + k * (2048 >> 4)), idesc, t + term + k != 0);
-                    tc_commit(&o_done[w][b]);
-                    if (w == GROUPS - 1) tc_commit(&v_free[nb]);
-                }
-                __syncwarp();
+                    for (int k = 0; k < KT_KEYS / 16; k++) ft_mma_ts(out, pd + 32 * term + 8 * k, vd + (unsigned)(k * (2048 >> 4)), idesc, t + term + k != 0);
+                tc_commit(&o_done[w][b]);
+                tc_commit(&v_free[nb]);
             }
-            if (!ok) break;
+            __syncwarp();
         }
         __syncwarp();
     } else {
         // ===== int8 to f16: of a tile's rows (keys), PIECES pieces of 16 values each
         constexpr int PIECES = C / 16, ROWS = KT_CONVERT * 32 / PIECES, U = KT_KEYS / ROWS;  // rows at once, rounds
-        const int id = tid - (SOFTMAX + 2) * 32, piece = id % PIECES, row = id / PIECES;
+        const int id = tid - (SOFTMAX + 2 * GROUPS) * 32, piece = id % PIECES, row = id / PIECES;
         const size_t record = record_bytes(c);
         const unsigned char *base = reinterpret_cast<const unsigned char *>(c.pages), *base_v = base + v_at(c);
         const bool has_k = piece * 16 < c.dim, has_v = piece * 16 < c.vdim;
@@ -379,20 +435,33 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
                 *reinterpret_cast<uint4 *>(at + (c0 ^ 1) * 16) = odd ? make_uint4(f[0], f[1], f[2], f[3]) : make_uint4(f[4], f[5], f[6], f[7]);
             }
         };
+        // (first warp) lanes 0 .. 3 the keys' scales of a tile's 16s, 4 .. 7 the values'
+        auto scale_ahead = [&](int page) {
+            if (id >= 8 || page < 0) return 0.f;
+            const volatile float *at = reinterpret_cast<const volatile float *>(base + (size_t)page * record + scales_at(c));
+            return at[(id >> 2) * c.n_head_kv + h];
+        };
         uint4 kr[U], vr[U];
         int pages = pages_ahead(0);
+        float scale = scale_ahead(pages);
+        int there = (int)(__ballot_sync(0xffffffffu, pages >= 0) & 15u);
         fetch(kr, 0, pages, base, c.dim, has_k);
         fetch(vr, 0, pages, base_v, c.vdim, has_v);
         pages = pages_ahead(1);
         for (int t = 0; t < n_tiles; t++) {
             const int nb = t % NB, parity = ((t / NB) & 1) ^ 1;
-            if (t >= NB && !kt_wait<20>(&k_free[nb], parity, &failed, limit)) break;
+            if (t >= NB && !kt_wait<0>(&k_free[nb], parity, &failed, limit)) break;
+            if (id < 8) scales_s[t % KT_RING][id] = scale;
+            if (id == 0) there_s[t % KT_RING] = there;
             put(kr, sk + nb * TILE);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&k_full[nb]);
+            if (id == 0) mbar_arrive(&scales_full[t % KT_RING]);
+            scale = scale_ahead(pages);
+            there = (int)(__ballot_sync(0xffffffffu, pages >= 0) & 15u);
             fetch(kr, t + 1, pages, base, c.dim, has_k);
-            if (t >= NB && !kt_wait<20>(&v_free[nb], parity, &failed, limit)) break;
+            if (t >= NB && !kt_wait<0>(&v_free[nb], parity, &failed, limit)) break;
             put(vr, sv + nb * TILE);
             fence_proxy_async_smem();
             __syncwarp();
@@ -428,7 +497,7 @@ static int launch_tc(const AttnArgs &args, bool vec, long long limit, cudaStream
         B200_CUDA_TRY(cudaFuncSetAttribute(kv8_attn_tc_kernel<C, GROUPS, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kt_smem<C, GROUPS, TERMS>()));
         if (dev < 16) done[dev] = true;
     }
-    const dim3 grid((unsigned)((int64_t)args.a.n_tokens * args.group / (GROUPS * KT_ROWS) + args.a.n_seq), (unsigned)args.a.cache.n_head_kv);
+    const unsigned grid = (unsigned)(((int64_t)args.a.n_tokens * args.group / (GROUPS * KT_ROWS) + args.a.n_seq) * args.a.cache.n_head_kv);
     B200_CUDA_TRY(launch_chained(kv8_attn_tc_kernel<C, GROUPS, TERMS>, grid, kt_threads<GROUPS>(), kt_smem<C, GROUPS, TERMS>(), st, args, vec, limit, status));
     return B200_OK;
 }
