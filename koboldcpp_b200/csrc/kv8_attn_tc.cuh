@@ -4,7 +4,7 @@
 //   S = Q . K^T      tcgen05, both operands in shared memory as f16, into TMEM
 //   P = 2^(c S - m)  a thread a row, no exchange between lanes; P goes back to TMEM as f16, in place of S
 //   O += P . V       A = P from TMEM, B = V as it lies in the page (keys are the strided side), O stays in TMEM
-// Four warps turn int8 keys and values into f16 once for all the CTA's rows: pieces of 16 bytes come from the pages into registers a tile ahead, and leave for
+// Eight warps turn int8 keys and values into f16 once for all the CTA's rows: pieces of 16 bytes come from the pages into registers a tile ahead, and leave for
 // shared memory in the 128-byte swizzle that the products read.  int8 is exact in f16, so with TERMS = 2 only Q and P have to be taken apart (upper halves
 // and what those leave over, a second product each) for results as f32 gives them; 64 columns of S are just two times 32 of P.
 // Softmax: four warps a group of 128 rows.  The maximum that the exponent subtracts follows the true one only when that has grown by SLACK, so O is hardly
@@ -17,10 +17,10 @@
 namespace b200 {
 namespace kv8 {
 
-constexpr int KT_ROWS = 128, KT_KEYS = 64, KT_CONVERT = 4;
+constexpr int KT_ROWS = 128, KT_KEYS = 64;
 constexpr int KT_RING = 8;  // scales of so many tiles: a tile's are written when the weights of the tile NB + 2 before it have been used
 constexpr int KT_Q_PANEL = KT_ROWS * 128, KT_PANEL = KT_KEYS * 128;  // panels of 64 values, 128 bytes a row
-template <int GROUPS> constexpr int kt_threads() { return (GROUPS * 6 + KT_CONVERT) * 32; }
+template <int GROUPS> constexpr int kt_threads() { return (GROUPS * 4 + 4 + 8) * 32; }  // softmax; products (one warp a group and product); conversion of keys and of values
 template <int GROUPS, int TERMS> constexpr int kt_buffers() { return GROUPS * TERMS == 4 ? 3 : 4; }  // of K and V
 template <int C, int GROUPS, int TERMS> constexpr size_t kt_smem() {
     return 1024 + (size_t)GROUPS * TERMS * (C / 64) * KT_Q_PANEL + (size_t)kt_buffers<GROUPS, TERMS>() * 2 * (C / 64) * KT_PANEL;
@@ -44,6 +44,14 @@ __device__ __noinline__ void kt_rescale(unsigned o_at, float alpha) {
         for (int i = 0; i < 32; i++) x[i] = __float_as_uint(v[i] * alpha);
         tmem_st32(o_at + 32 * ch, x);
     }
+}
+// A thread's registers from here on, by groups of four warps.  A launch has 96 a thread for 20 warps, 61,440 in all: 8 softmax warps of 144, 8 converting ones of 72
+// and 4 of 48 take just those (12 warps of 128 each with one group of rows: 49,152 of its 65,536).
+constexpr int KT_REGS_SOFTMAX = 144, KT_REGS_CONVERT = 72, KT_REGS_PRODUCTS = 48;
+template <int N, bool MORE>
+__device__ __forceinline__ void kt_registers() {
+    if constexpr (MORE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 // a whole warp waits
 template <int SLEEP>
@@ -96,7 +104,7 @@ __device__ __forceinline__ void row_store4(void *row, int type, int64_t at, bool
 
 template <int C, int GROUPS, int TERMS>
 __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(const __grid_constant__ AttnArgs args, bool vec, long long limit, int *timeout) {
-    constexpr int NB = kt_buffers<GROUPS, TERMS>(), PANELS = C / 64, BLOCK = GROUPS * KT_ROWS, SOFTMAX = GROUPS * 4;
+    constexpr int NB = kt_buffers<GROUPS, TERMS>(), PANELS = C / 64, BLOCK = GROUPS * KT_ROWS, SOFTMAX = GROUPS * 4, CONVERT = SOFTMAX + 4;
     constexpr int TILE = PANELS * KT_PANEL;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -134,7 +142,7 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
     unsigned char *sq = smem, *sk = sq + GROUPS * TERMS * PANELS * KT_Q_PANEL, *sv = sk + NB * TILE;
 
     if (tid == 0) {
-        for (int i = 0; i < NB; i++) { mbar_init(&k_full[i], KT_CONVERT); mbar_init(&k_free[i], GROUPS); mbar_init(&v_full[i], KT_CONVERT); mbar_init(&v_free[i], GROUPS); }
+        for (int i = 0; i < NB; i++) { mbar_init(&k_full[i], 4); mbar_init(&k_free[i], GROUPS); mbar_init(&v_full[i], 4); mbar_init(&v_free[i], GROUPS); }
         for (int i = 0; i < KT_RING; i++) mbar_init(&scales_full[i], 1);
         for (int i = 0; i < 2 * GROUPS; i++) { mbar_init(&s_full[i >> 1][i & 1], 1); mbar_init(&p_full[i >> 1][i & 1], 4); mbar_init(&o_done[i >> 1][i & 1], 1); }
         mbar_fence_init();
@@ -148,6 +156,7 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
     const unsigned tmem = tmem_base_s, tmem_o = tmem + GROUPS * 2 * KT_KEYS;
 
     if (warp < SOFTMAX) {
+        kt_registers<KT_REGS_SOFTMAX, true>();
         // ===== Q as f16, a row relative to the power of two above its largest value: a thread takes 8 dims, piece number `piece` of a row, of every ROWS-th row
         const int w = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane, row = w * KT_ROWS + r;
         {
@@ -341,135 +350,143 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
                 __syncwarp();
             }
         }
-    } else if (warp < SOFTMAX + GROUPS) {
-        // ===== first products of a group
-        const int w = warp - SOFTMAX;
-        asm volatile("bar.sync 2, %0;" ::"n"((SOFTMAX + GROUPS) * 32) : "memory");
-        const bool elected = elect_lane();
-        const unsigned long long qd = umma_desc_sw128(smem_u32(sq)) + (unsigned)(w * TERMS * PANELS * (KT_Q_PANEL >> 4)), kd0 = umma_desc_sw128(smem_u32(sk));
-        const int steps = c.dim / 16;
-        for (int t = 0; t < n_tiles; t++) {
-            const int b = t & 1, nb = t % NB;
-            if (!kt_wait<0>(&k_full[nb], (t / NB) & 1, &failed, limit)) break;
-            if (t >= 2 && !kt_wait<0>(&o_done[w][b], ((t >> 1) & 1) ^ 1, &failed, limit)) break;  // the weights of tile t - 2 have been used
-            tc_fence_after();
-            if (elected) {
-                const unsigned sd = tmem + (unsigned)((w * 2 + b) * KT_KEYS);
-                const unsigned long long kd = kd0 + (unsigned)(nb * (TILE >> 4));
-                if (steps == C / 16) {
-#pragma unroll
-                    for (int term = 0; term < TERMS; term++)
-#pragma unroll
-                        for (int k = 0; k < C / 16; k++)
-                            tc_mma_bf16(sd, qd + (unsigned)((term * PANELS + k / 4) * (KT_Q_PANEL >> 4) + 2 * (k % 4)), kd + (unsigned)(k / 4 * (KT_PANEL >> 4) + 2 * (k % 4)), kt_idesc(KT_KEYS, false), term + k != 0);
-                } else {
-#pragma unroll 1
-                    for (int i = 0; i < TERMS * steps; i++) {
-                        const int term = i >= steps, k = i - term * steps;
-                        tc_mma_bf16(sd, qd + (unsigned)((term * PANELS + k / 4) * (KT_Q_PANEL >> 4) + 2 * (k % 4)), kd + (unsigned)(k / 4 * (KT_PANEL >> 4) + 2 * (k % 4)), kt_idesc(KT_KEYS, false), i != 0);
-                    }
-                }
-                tc_commit(&s_full[w][b]);
-                tc_commit(&k_free[nb]);
-            }
-            __syncwarp();
-        }
-        __syncwarp();
-    } else if (warp < SOFTMAX + 2 * GROUPS) {
-        // ===== second products of a group
-        const int w = warp - SOFTMAX - GROUPS;
-        const bool elected = elect_lane();
-        const unsigned long long vd0 = umma_desc_mn_sw128(smem_u32(sv), KT_PANEL);
-        const unsigned idesc = kt_idesc(c.vdim, true), out = tmem_o + (unsigned)(w * C);
-        for (int t = 0; t < n_tiles; t++) {
-            const int b = t & 1, nb = t % NB;
-            if (!kt_wait<0>(&v_full[nb], (t / NB) & 1, &failed, limit)) break;
-            if (!kt_wait<0>(&p_full[w][b], (t >> 1) & 1, &failed, limit)) break;
-            tc_fence_after();
-            if (elected) {
-                const unsigned pd = tmem + (unsigned)((w * 2 + b) * KT_KEYS);
-                const unsigned long long vd = vd0 + (unsigned)(nb * (TILE >> 4));
-#pragma unroll
-                for (int term = 0; term < TERMS; term++)
-#pragma unroll
-                    for (int k = 0; k < KT_KEYS / 16; k++) ft_mma_ts(out, pd + 32 * term + 8 * k, vd + (unsigned)(k * (2048 >> 4)), idesc, t + term + k != 0);
-                tc_commit(&o_done[w][b]);
-                tc_commit(&v_free[nb]);
-            }
-            __syncwarp();
-        }
-        __syncwarp();
-    } else {
-        // ===== int8 to f16: of a tile's rows (keys), PIECES pieces of 16 values each
-        constexpr int PIECES = C / 16, ROWS = KT_CONVERT * 32 / PIECES, U = KT_KEYS / ROWS;  // rows at once, rounds
-        const int id = tid - (SOFTMAX + 2 * GROUPS) * 32, piece = id % PIECES, row = id / PIECES;
+    } else if (warp >= CONVERT) {
+        // ===== int8 to f16, four warps for the keys and four for the values: of a tile's rows (keys), PIECES pieces of 16 values each
+        kt_registers<KT_REGS_CONVERT, false>();
+        constexpr int PIECES = C / 16, ROWS = 128 / PIECES, U = KT_KEYS / ROWS;  // rows at once, rounds
+        const bool is_v = warp >= CONVERT + 4;
+        const int id = tid & 127, piece = id % PIECES, row = id / PIECES, size = is_v ? c.vdim : c.dim;
         const size_t record = record_bytes(c);
-        const unsigned char *base = reinterpret_cast<const unsigned char *>(c.pages), *base_v = base + v_at(c);
-        const bool has_k = piece * 16 < c.dim, has_v = piece * 16 < c.vdim;
+        const unsigned char *base = reinterpret_cast<const unsigned char *>(c.pages), *from = base + (is_v ? v_at(c) : 0) + ((size_t)h * ps + row % 16) * size + piece * 16;
+        unsigned char *tiles = is_v ? sv : sk;
+        unsigned long long *full = is_v ? v_full : k_full, *free = is_v ? v_free : k_free;
+        const bool has = piece * 16 < size;
         const int shift = 31 - __clz(ps);
         auto pages_ahead = [&](int t) {  // lane & 3: the pages of a tile's 16s of keys
             const int key = t < n_tiles ? key_of(t) + 16 * (lane & 3) : 0x7fffffff;
             return key <= pos_hi ? page_of(st, table, q.row, key >> shift) : -1;
         };
-        auto fetch = [&](uint4 (&raw)[U], int t, int pages, const unsigned char *from, int size, bool has) {  // pages that are not there: zeros
+        // (first warp of the keys') lanes 0 .. 3 the keys' scales of a tile's 16s, 4 .. 7 the values'
+        const bool scales = warp == CONVERT;
+        auto scale_ahead = [&](int page) {
+            if (lane >= 8 || page < 0) return 0.f;
+            const volatile float *at = reinterpret_cast<const volatile float *>(base + (size_t)page * record + scales_at(c));
+            return at[(lane >> 2) * c.n_head_kv + h];
+        };
+        uint4 raw[U];
+        auto fetch = [&](int t, int pages) {  // pages that are not there: zeros
             const int key0 = t < n_tiles ? key_of(t) : 0;
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const int rr = row + u * ROWS, page = __shfl_sync(0xffffffffu, pages, rr >> 4);
+                const int sixteen = (row + u * ROWS) >> 4, page = __shfl_sync(0xffffffffu, pages, sixteen);
                 raw[u] = make_uint4(0u, 0u, 0u, 0u);
-                if (page >= 0 && has) raw[u] = ld_behind(reinterpret_cast<const uint4 *>(from + (size_t)page * record + ((size_t)h * ps + ((key0 + rr) & (ps - 1))) * size + piece * 16));
+                if (page >= 0 && has) raw[u] = ld_behind(reinterpret_cast<const uint4 *>(from + (size_t)page * record + (unsigned)(((key0 + 16 * sixteen) & (ps - 1)) * size)));
             }
         };
-        auto put = [&](const uint4 (&raw)[U], unsigned char *tile) {
+        int pages = pages_ahead(0);
+        fetch(0, pages);
+        float scale = 0.f;
+        int there = 0;
+        if (scales) {
+            scale = scale_ahead(pages);
+            there = (int)(__ballot_sync(0xffffffffu, pages >= 0) & 15u);
+        }
+        pages = pages_ahead(1);
+        unsigned char *at0 = tiles + piece / 4 * KT_PANEL + row * 128;
+        // (the two panels lie on the same banks: theirs are written in turn)
+        const int odd = piece >> 2 & 1, c0 = (((piece % 4) * 2 + odd) ^ (row & 7)) * 16;  // (ROWS is a multiple of 8)
+        for (int t = 0; t < n_tiles; t++) {
+            const int nb = t % NB;
+            if (t >= NB && !kt_wait<0>(&free[nb], ((t / NB) & 1) ^ 1, &failed, limit)) break;
+            if (scales) {
+                if (lane < 8) scales_s[t % KT_RING][lane] = scale;
+                if (lane == 0) there_s[t % KT_RING] = there;
+            }
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const int rr = row + u * ROWS;
                 const unsigned w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
                 unsigned f[8];
 #pragma unroll
                 for (int e = 0; e < 4; e++) int4_to_half(w[e], f[2 * e], f[2 * e + 1]);
-                unsigned char *at = tile + piece / 4 * KT_PANEL + rr * 128;
-                // (the two panels lie on the same banks: theirs are written in turn)
-                const int odd = piece >> 2 & 1, c0 = ((piece % 4) * 2 + odd) ^ (rr & 7);
-                *reinterpret_cast<uint4 *>(at + c0 * 16) = odd ? make_uint4(f[4], f[5], f[6], f[7]) : make_uint4(f[0], f[1], f[2], f[3]);
-                *reinterpret_cast<uint4 *>(at + (c0 ^ 1) * 16) = odd ? make_uint4(f[0], f[1], f[2], f[3]) : make_uint4(f[4], f[5], f[6], f[7]);
+                unsigned char *at = at0 + nb * TILE + u * ROWS * 128;
+                *reinterpret_cast<uint4 *>(at + c0) = odd ? make_uint4(f[4], f[5], f[6], f[7]) : make_uint4(f[0], f[1], f[2], f[3]);
+                *reinterpret_cast<uint4 *>(at + (c0 ^ 16)) = odd ? make_uint4(f[0], f[1], f[2], f[3]) : make_uint4(f[4], f[5], f[6], f[7]);
             }
-        };
-        // (first warp) lanes 0 .. 3 the keys' scales of a tile's 16s, 4 .. 7 the values'
-        auto scale_ahead = [&](int page) {
-            if (id >= 8 || page < 0) return 0.f;
-            const volatile float *at = reinterpret_cast<const volatile float *>(base + (size_t)page * record + scales_at(c));
-            return at[(id >> 2) * c.n_head_kv + h];
-        };
-        uint4 kr[U], vr[U];
-        int pages = pages_ahead(0);
-        float scale = scale_ahead(pages);
-        int there = (int)(__ballot_sync(0xffffffffu, pages >= 0) & 15u);
-        fetch(kr, 0, pages, base, c.dim, has_k);
-        fetch(vr, 0, pages, base_v, c.vdim, has_v);
-        pages = pages_ahead(1);
-        for (int t = 0; t < n_tiles; t++) {
-            const int nb = t % NB, parity = ((t / NB) & 1) ^ 1;
-            if (t >= NB && !kt_wait<0>(&k_free[nb], parity, &failed, limit)) break;
-            if (id < 8) scales_s[t % KT_RING][id] = scale;
-            if (id == 0) there_s[t % KT_RING] = there;
-            put(kr, sk + nb * TILE);
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&k_full[nb]);
-            if (id == 0) mbar_arrive(&scales_full[t % KT_RING]);
-            scale = scale_ahead(pages);
-            there = (int)(__ballot_sync(0xffffffffu, pages >= 0) & 15u);
-            fetch(kr, t + 1, pages, base, c.dim, has_k);
-            if (t >= NB && !kt_wait<0>(&v_free[nb], parity, &failed, limit)) break;
-            put(vr, sv + nb * TILE);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&v_full[nb]);
-            fetch(vr, t + 1, pages, base_v, c.vdim, has_v);
+            if (lane == 0) {
+                mbar_arrive(&full[nb]);
+                if (scales) mbar_arrive(&scales_full[t % KT_RING]);
+            }
+            fetch(t + 1, pages);
+            if (scales) {
+                scale = scale_ahead(pages);
+                there = (int)(__ballot_sync(0xffffffffu, pages >= 0) & 15u);
+            }
             pages = pages_ahead(t + 2);
         }
         __syncwarp();
+    } else {
+        kt_registers<KT_REGS_PRODUCTS, false>();
+        if (warp < SOFTMAX + GROUPS) {
+            // ===== first products of a group
+            const int w = warp - SOFTMAX;
+            asm volatile("bar.sync 2, %0;" ::"n"((SOFTMAX + GROUPS) * 32) : "memory");
+            const bool elected = elect_lane();
+            const unsigned long long qd = umma_desc_sw128(smem_u32(sq)) + (unsigned)(w * TERMS * PANELS * (KT_Q_PANEL >> 4)), kd0 = umma_desc_sw128(smem_u32(sk));
+            const int steps = c.dim / 16;
+            for (int t = 0; t < n_tiles; t++) {
+                const int b = t & 1, nb = t % NB;
+                if (!kt_wait<0>(&k_full[nb], (t / NB) & 1, &failed, limit)) break;
+                if (t >= 2 && !kt_wait<0>(&o_done[w][b], ((t >> 1) & 1) ^ 1, &failed, limit)) break;  // the weights of tile t - 2 have been used
+                tc_fence_after();
+                if (elected) {
+                    const unsigned sd = tmem + (unsigned)((w * 2 + b) * KT_KEYS);
+                    const unsigned long long kd = kd0 + (unsigned)(nb * (TILE >> 4));
+                    if (steps == C / 16) {
+#pragma unroll
+                        for (int term = 0; term < TERMS; term++)
+#pragma unroll
+                            for (int k = 0; k < C / 16; k++)
+                                tc_mma_bf16(sd, qd + (unsigned)((term * PANELS + k / 4) * (KT_Q_PANEL >> 4) + 2 * (k % 4)), kd + (unsigned)(k / 4 * (KT_PANEL >> 4) + 2 * (k % 4)), kt_idesc(KT_KEYS, false), term + k != 0);
+                    } else {
+#pragma unroll 1
+                        for (int i = 0; i < TERMS * steps; i++) {
+                            const int term = i >= steps, k = i - term * steps;
+                            tc_mma_bf16(sd, qd + (unsigned)((term * PANELS + k / 4) * (KT_Q_PANEL >> 4) + 2 * (k % 4)), kd + (unsigned)(k / 4 * (KT_PANEL >> 4) + 2 * (k % 4)), kt_idesc(KT_KEYS, false), i != 0);
+                        }
+                    }
+                    tc_commit(&s_full[w][b]);
+                    tc_commit(&k_free[nb]);
+                }
+                __syncwarp();
+            }
+            __syncwarp();
+        } else if (warp < SOFTMAX + 2 * GROUPS) {
+            // ===== second products of a group
+            const int w = warp - SOFTMAX - GROUPS;
+            const bool elected = elect_lane();
+            const unsigned long long vd0 = umma_desc_mn_sw128(smem_u32(sv), KT_PANEL);
+            const unsigned idesc = kt_idesc(c.vdim, true), out = tmem_o + (unsigned)(w * C);
+            for (int t = 0; t < n_tiles; t++) {
+                const int b = t & 1, nb = t % NB;
+                if (!kt_wait<0>(&v_full[nb], (t / NB) & 1, &failed, limit)) break;
+                if (!kt_wait<0>(&p_full[w][b], (t >> 1) & 1, &failed, limit)) break;
+                tc_fence_after();
+                if (elected) {
+                    const unsigned pd = tmem + (unsigned)((w * 2 + b) * KT_KEYS);
+                    const unsigned long long vd = vd0 + (unsigned)(nb * (TILE >> 4));
+#pragma unroll
+                    for (int term = 0; term < TERMS; term++)
+#pragma unroll
+                        for (int k = 0; k < KT_KEYS / 16; k++) ft_mma_ts(out, pd + 32 * term + 8 * k, vd + (unsigned)(k * (2048 >> 4)), idesc, t + term + k != 0);
+                    tc_commit(&o_done[w][b]);
+                    tc_commit(&v_free[nb]);
+                }
+                __syncwarp();
+            }
+            __syncwarp();
+        }
     }
     __syncwarp();
     __syncthreads();
