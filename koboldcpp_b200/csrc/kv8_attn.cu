@@ -347,8 +347,11 @@ __global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_k
             for (int r = 0; r < NR; r++) {
                 vs[r][0] = seen[r] & 0xffffu ? scales.y : 0.f;
                 vs[r][1] = seen[r] & 0xffff0000u ? scales.w : 0.f;
-                const float loudest = fmaxf(vs[r][0], vs[r][1]);  // (a NaN only if both are)
-                const int now = exponent_above(loudest <= FLT_MAX ? __float_as_uint(loudest) & 0x7fffffffu : 0u);
+                // a row that sees a page whose scale is NaN: its sum becomes NaN, and with it the row, whatever that page's values are
+                const float broken = 0.f * (vs[r][0] + vs[r][1]);
+                l[r] += broken;
+                if (!(broken == 0.f)) vs[r][0] = vs[r][1] = 0.f;
+                const int now = exponent_above(__float_as_uint(fmaxf(vs[r][0], vs[r][1])) & 0x7fffffffu);
                 if (now > power[r]) {
                     common[r] = pow2i(max(power[r] - now, -126));
                     power[r] = now;
@@ -370,7 +373,7 @@ __global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_k
                 for (int i = 0; i < 8; i++) {
                     const float e = ex2(p[r][i] - mb);
                     l[r] += e;
-                    w[i] = (p[r][i] == -INFINITY) ? 0.f : e * (i < 4 ? vs0 : vs1);  // (a page whose scale is NaN: not for rows that do not see it)
+                    w[i] = e * (i < 4 ? vs0 : vs1);
                 }
 #pragma unroll
                 for (int half = 0; half < 2; half++) {

@@ -32,6 +32,11 @@ __device__ __forceinline__ float2 mul2(float2 x, float2 y) {
     asm("{\n.reg .b64 a, b;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 a, a, b;\nmov.b64 {%0, %1}, a;\n}\n" : "=f"(r.x), "=f"(r.y) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
     return r;
 }
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
 // accumulators of a row times alpha
 template <int C>
 __device__ __noinline__ void kt_rescale(unsigned o_at, float alpha) {
@@ -222,7 +227,7 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
             const int there = there_s[t % KT_RING];
             const float4 k4 = *reinterpret_cast<const float4 *>(&scales_s[t % KT_RING][0]), v4 = *reinterpret_cast<const float4 *>(&scales_s[t % KT_RING][4]);
             float ks[4] = {k4.x * row_scale, k4.y * row_scale, k4.z * row_scale, k4.w * row_scale}, vs[4] = {v4.x, v4.y, v4.z, v4.w};
-            ok = kt_wait<0>(&s_full[w][b], (t >> 1) & 1, &failed, limit);
+            ok = kt_wait<20>(&s_full[w][b], (t >> 1) & 1, &failed, limit);
             if (!ok) break;
             tc_fence_after();
             unsigned x[32];
@@ -260,13 +265,19 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
                 float top = -INFINITY, loudest = 0.f;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    float t0 = v[16 * i], t1 = v[16 * i + 1];
-#pragma unroll
-                    for (int e = 2; e < 16; e += 2) { t0 = fmaxf(t0, v[16 * i + e]); t1 = fmaxf(t1, v[16 * i + e + 1]); }
-                    top = fmaxf(top, fmaxf(t0, t1) * ks[i]);
+                    float t0 = max3(v[16 * i], v[16 * i + 1], v[16 * i + 2]), t1 = max3(v[16 * i + 3], v[16 * i + 4], v[16 * i + 5]);
+                    t0 = max3(t0, v[16 * i + 6], v[16 * i + 7]);
+                    t1 = max3(t1, v[16 * i + 8], v[16 * i + 9]);
+                    t0 = max3(t0, v[16 * i + 10], v[16 * i + 11]);
+                    t1 = max3(t1, v[16 * i + 12], v[16 * i + 13]);
+                    top = fmaxf(top, fmaxf(max3(t0, v[16 * i + 14], v[16 * i + 15]), t1) * ks[i]);
                     vs[i] = seen[i / 2] >> (16 * (i & 1)) & 0xffffu ? vs[i] : 0.f;
                     loudest = fmaxf(loudest, vs[i]);  // (passes over NaN)
                 }
+                // a row that sees a page whose scale is NaN: its sum becomes NaN, and with it the row, whatever that page's values are
+                const float broken = 0.f * ((vs[0] + vs[1]) + (vs[2] + vs[3]));
+                l += broken;
+                if (!(broken == 0.f)) vs[0] = vs[1] = vs[2] = vs[3] = 0.f;
                 const bool grown = top > m + SLACK;  // (m = -inf: as soon as a key is seen)
                 const int now = exponent_above(__float_as_uint(loudest));
                 if (__any_sync(0xffffffffu, grown || now > power)) {
@@ -294,11 +305,7 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
 #pragma unroll
                 for (int i = 0; i < 64; i += 2) {
                     const float f = vs[i / 16] * unit;
-                    float2 e = mul2(make_float2(v[i], v[i + 1]), make_float2(f, f));
-                    if (!whole) {  // (a weight of 0 stays 0, whatever the scale of its page)
-                        e.x = v[i] == 0.f ? 0.f : e.x;
-                        e.y = v[i + 1] == 0.f ? 0.f : e.y;
-                    }
+                    const float2 e = mul2(make_float2(v[i], v[i + 1]), make_float2(f, f));
                     x[i / 2] = pack_half(e.x, e.y);
                     if constexpr (TERMS == 2) y[i / 2] = pack_rest(e.x, e.y, x[i / 2]);
                 }
@@ -353,14 +360,14 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
     } else if (warp >= CONVERT) {
         // ===== int8 to f16, four warps for the keys and four for the values: of a tile's rows (keys), PIECES pieces of 16 values each
         kt_registers<KT_REGS_CONVERT, false>();
-        constexpr int PIECES = C / 16, ROWS = 128 / PIECES, U = KT_KEYS / ROWS;  // rows at once, rounds
+        // (8 neighbouring lanes bring half a panel's row each of two keys: their stores fall on all banks)
+        constexpr int U = 2 * PANELS;  // pieces of a thread: keys id / 4 and 32 further on, of every panel
         const bool is_v = warp >= CONVERT + 4;
-        const int id = tid & 127, piece = id % PIECES, row = id / PIECES, size = is_v ? c.vdim : c.dim;
+        const int id = tid & 127, piece = id & 3, row = id >> 2, size = is_v ? c.vdim : c.dim;
         const size_t record = record_bytes(c);
         const unsigned char *base = reinterpret_cast<const unsigned char *>(c.pages), *from = base + (is_v ? v_at(c) : 0) + ((size_t)h * ps + row % 16) * size + piece * 16;
         unsigned char *tiles = is_v ? sv : sk;
         unsigned long long *full = is_v ? v_full : k_full, *free = is_v ? v_free : k_free;
-        const bool has = piece * 16 < size;
         const int shift = 31 - __clz(ps);
         auto pages_ahead = [&](int t) {  // lane & 3: the pages of a tile's 16s of keys
             const int key = t < n_tiles ? key_of(t) + 16 * (lane & 3) : 0x7fffffff;
@@ -377,10 +384,14 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
         auto fetch = [&](int t, int pages) {  // pages that are not there: zeros
             const int key0 = t < n_tiles ? key_of(t) : 0;
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int sixteen = (row + u * ROWS) >> 4, page = __shfl_sync(0xffffffffu, pages, sixteen);
-                raw[u] = make_uint4(0u, 0u, 0u, 0u);
-                if (page >= 0 && has) raw[u] = ld_behind(reinterpret_cast<const uint4 *>(from + (size_t)page * record + (unsigned)(((key0 + 16 * sixteen) & (ps - 1)) * size)));
+            for (int half = 0; half < 2; half++) {
+                const int sixteen = (row >> 4) + 2 * half, page = __shfl_sync(0xffffffffu, pages, sixteen);
+                const unsigned char *at = from + (size_t)max(page, 0) * record + (unsigned)(((key0 + 16 * sixteen) & (ps - 1)) * size);
+#pragma unroll
+                for (int p = 0; p < PANELS; p++) {
+                    raw[2 * p + half] = make_uint4(0u, 0u, 0u, 0u);
+                    if (page >= 0 && 64 * p + piece * 16 < size) raw[2 * p + half] = ld_behind(reinterpret_cast<const uint4 *>(at + 64 * p));
+                }
             }
         };
         int pages = pages_ahead(0);
@@ -392,12 +403,10 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
             there = (int)(__ballot_sync(0xffffffffu, pages >= 0) & 15u);
         }
         pages = pages_ahead(1);
-        unsigned char *at0 = tiles + piece / 4 * KT_PANEL + row * 128;
-        // (the two panels lie on the same banks: theirs are written in turn)
-        const int odd = piece >> 2 & 1, c0 = (((piece % 4) * 2 + odd) ^ (row & 7)) * 16;  // (ROWS is a multiple of 8)
+        unsigned char *at0 = tiles + row * 128 + (((piece * 2) ^ (row & 7)) << 4);
         for (int t = 0; t < n_tiles; t++) {
             const int nb = t % NB;
-            if (t >= NB && !kt_wait<0>(&free[nb], ((t / NB) & 1) ^ 1, &failed, limit)) break;
+            if (t >= NB && !kt_wait<200>(&free[nb], ((t / NB) & 1) ^ 1, &failed, limit)) break;
             if (scales) {
                 if (lane < 8) scales_s[t % KT_RING][lane] = scale;
                 if (lane == 0) there_s[t % KT_RING] = there;
@@ -408,9 +417,9 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
                 unsigned f[8];
 #pragma unroll
                 for (int e = 0; e < 4; e++) int4_to_half(w[e], f[2 * e], f[2 * e + 1]);
-                unsigned char *at = at0 + nb * TILE + u * ROWS * 128;
-                *reinterpret_cast<uint4 *>(at + c0) = odd ? make_uint4(f[4], f[5], f[6], f[7]) : make_uint4(f[0], f[1], f[2], f[3]);
-                *reinterpret_cast<uint4 *>(at + (c0 ^ 16)) = odd ? make_uint4(f[0], f[1], f[2], f[3]) : make_uint4(f[4], f[5], f[6], f[7]);
+                unsigned char *at = at0 + nb * TILE + u / 2 * KT_PANEL + u % 2 * (32 * 128);
+                *reinterpret_cast<uint4 *>(at) = make_uint4(f[0], f[1], f[2], f[3]);
+                *reinterpret_cast<uint4 *>((unsigned char *)((uintptr_t)at ^ 16)) = make_uint4(f[4], f[5], f[6], f[7]);
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -437,8 +446,8 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
             const int steps = c.dim / 16;
             for (int t = 0; t < n_tiles; t++) {
                 const int b = t & 1, nb = t % NB;
-                if (!kt_wait<0>(&k_full[nb], (t / NB) & 1, &failed, limit)) break;
-                if (t >= 2 && !kt_wait<0>(&o_done[w][b], ((t >> 1) & 1) ^ 1, &failed, limit)) break;  // the weights of tile t - 2 have been used
+                if (!kt_wait<40>(&k_full[nb], (t / NB) & 1, &failed, limit)) break;
+                if (t >= 2 && !kt_wait<40>(&o_done[w][b], ((t >> 1) & 1) ^ 1, &failed, limit)) break;  // the weights of tile t - 2 have been used
                 tc_fence_after();
                 if (elected) {
                     const unsigned sd = tmem + (unsigned)((w * 2 + b) * KT_KEYS);
@@ -470,8 +479,8 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
             const unsigned idesc = kt_idesc(c.vdim, true), out = tmem_o + (unsigned)(w * C);
             for (int t = 0; t < n_tiles; t++) {
                 const int b = t & 1, nb = t % NB;
-                if (!kt_wait<0>(&v_full[nb], (t / NB) & 1, &failed, limit)) break;
-                if (!kt_wait<0>(&p_full[w][b], (t >> 1) & 1, &failed, limit)) break;
+                if (!kt_wait<40>(&v_full[nb], (t / NB) & 1, &failed, limit)) break;
+                if (!kt_wait<40>(&p_full[w][b], (t >> 1) & 1, &failed, limit)) break;
                 tc_fence_after();
                 if (elected) {
                     const unsigned pd = tmem + (unsigned)((w * 2 + b) * KT_KEYS);
