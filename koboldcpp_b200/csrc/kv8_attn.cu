@@ -48,15 +48,29 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const unsigned (&a)[4], u
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // 16 values of a row of q or dst, whose type is an argument
-__device__ __forceinline__ void row_load16(const void *row, int type, int64_t at, float (&x)[16]) {
-    if (type == B200_TYPE_F32) load16<float, false>(reinterpret_cast<const float *>(row) + at, x);
-    else if (type == B200_TYPE_F16) load16<__half, false>(reinterpret_cast<const __half *>(row) + at, x);
-    else load16<__nv_bfloat16, false>(reinterpret_cast<const __nv_bfloat16 *>(row) + at, x);
+template <bool VEC>
+__device__ __forceinline__ void row_load16_(const void *row, int type, int64_t at, float (&x)[16]) {
+    if (type == B200_TYPE_F32) load16<float, VEC>(reinterpret_cast<const float *>(row) + at, x);
+    else if (type == B200_TYPE_F16) load16<__half, VEC>(reinterpret_cast<const __half *>(row) + at, x);
+    else load16<__nv_bfloat16, VEC>(reinterpret_cast<const __nv_bfloat16 *>(row) + at, x);
 }
+__device__ __forceinline__ void row_load16(const void *row, int type, int64_t at, bool vec, float (&x)[16]) { vec ? row_load16_<true>(row, type, at, x) : row_load16_<false>(row, type, at, x); }
 __device__ __forceinline__ void row_put(void *row, int type, int64_t at, float x) {
     if (type == B200_TYPE_F32) reinterpret_cast<float *>(row)[at] = x;
     else if (type == B200_TYPE_F16) reinterpret_cast<__half *>(row)[at] = __float2half_rn(x);
     else reinterpret_cast<__nv_bfloat16 *>(row)[at] = __float2bfloat16_rn(x);
+}
+__device__ __forceinline__ void row_store4(void *row, int type, int64_t at, bool vec, float4 y) {
+    if (!vec) {
+        row_put(row, type, at, y.x); row_put(row, type, at + 1, y.y); row_put(row, type, at + 2, y.z); row_put(row, type, at + 3, y.w);
+    } else if (type == B200_TYPE_F32) {
+        *reinterpret_cast<float4 *>(reinterpret_cast<float *>(row) + at) = y;
+    } else if (type == B200_TYPE_F16) {
+        *reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(row) + at) = make_uint2(pack_half(y.x, y.y), pack_half(y.z, y.w));
+    } else {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
+        *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(row) + at) = make_uint2(*reinterpret_cast<const unsigned *>(&a), *reinterpret_cast<const unsigned *>(&b));
+    }
 }
 // bits below n of 32
 __device__ __forceinline__ unsigned below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }
@@ -93,11 +107,12 @@ struct AttnArgs {
 // Warps keep maximum, sum and result of their own and meet in shared memory at the end of a run of units of one block; runs of one block in
 // several CTAs meet in global memory, where the last one to arrive adds them in the order of the CTAs.
 // Scales: a key's joins its score; a value's joins its weight, relative to the power of two above the largest one that the row has seen.
-constexpr int RW_WARPS = 4, RW_TILE = 32, RW_UNIT = RW_WARPS * RW_TILE;
-template <int C> constexpr int rw_stages() { return C == 256 ? 2 : 3; }
+constexpr int RW_WARPS = 4, RW_TILE = 32, RW_UNIT = RW_WARPS * RW_TILE, RW_THREADS = RW_WARPS * 32;
+constexpr int RW_STAGES = 2, RW_PARTS = 128;
 template <int C> constexpr int rw_stage_bytes() { return RW_TILE * 2 * C + 32; }  // keys, values, 2 scales of each, which pages are there
-template <int C> constexpr int rw_per_sm() { return C == 64 ? 4 : C == 128 ? 2 : 1; }
-template <int C> constexpr size_t rw_smem() { return (size_t)RW_WARPS * rw_stages<C>() * rw_stage_bytes<C>(); }
+template <int C> constexpr int rw_per_sm() { return C == 64 ? 4 : C == 128 ? 3 : 1; }
+template <int C> constexpr int rw_fixed() { return RW_WARPS * RW_STAGES * rw_stage_bytes<C>() + C * 32; }  // stages; q as operands of the first product
+template <int C> constexpr int rw_row() { return C + 16; }  // of a warp's results in shared memory, floats: two neighbouring rows fall on the two halves of the banks
 
 // where piece c (16 bytes) of row r of a tile lies
 template <int C>
@@ -107,21 +122,25 @@ __device__ __forceinline__ int rw_piece(int r, int c) {
 }
 
 template <int C, int TERMS>
-__global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_kernel(const __grid_constant__ AttnArgs args) {
+__global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kernel(const __grid_constant__ AttnArgs args, bool vec) {
     pdl_enter();
     constexpr int R = 16 / TERMS, NR = 2 / TERMS;  // rows of a block; a thread's rows in the MMA's result
-    constexpr int NT = C / 8, STAGES = rw_stages<C>(), STAGE = rw_stage_bytes<C>();
+    constexpr int NT = C / 8, STAGE = rw_stage_bytes<C>(), ROW = rw_row<C>();
+    static_assert(RW_WARPS == 4 && RW_PARTS * R * 8 <= RW_WARPS * RW_STAGES * STAGE, "parts' maxima and sums too");
+    static_assert(RW_WARPS * R * ROW * 4 <= RW_WARPS * RW_STAGES * STAGE, "the warps' results lie where the stages were");
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ long long sum_s[B200_KV8_MAX_SEQ];  // units of the sequences up to this one
+    uint4 *q_s = reinterpret_cast<uint4 *>(smem + RW_WARPS * RW_STAGES * STAGE);                 // [step of 16 dims][lane]
+    long long *sum_s = reinterpret_cast<long long *>(smem + rw_fixed<C>());                      // units of the sequences up to this one
     __shared__ long long warp_sum_s[RW_WARPS];
-    __shared__ float top_s[RW_WARPS][16], total_s[RW_WARPS][16], fac_s[RW_WARPS][16];
-    __shared__ int power_s[RW_WARPS][16], last_s;
+    __shared__ float top_s[RW_WARPS][16], total_s[RW_WARPS][16], fac_s[RW_WARPS][16], share_s[16], scale_s[16];
+    __shared__ int power_s[RW_WARPS][16], most_s[RW_WARPS], last_s;
     const b200_kv8_attn_args &a = args.a;
     const b200_kv8_cache &c = a.cache;
     const Step &st = args.step;
     const int32_t *info = behind(st.info), *table = behind(st.table);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tg = lane & 3;
-    const int ps = c.page_size, group = args.group;
+    const int ps = c.page_size, ps_shift = 31 - __clz(ps), group = args.group;
+    const size_t record = record_bytes(c);
 
     struct Span { int keep, first, units, blocks; };  // units of kept first tokens; number of the first unit behind them; units; blocks of rows
     auto span_of = [&](const Seq &q) {
@@ -135,18 +154,21 @@ __global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_k
     };
     // ---- all sequences' units, summed up
     {
-        const int each = (st.n_seq + RW_WARPS * 32 - 1) / (RW_WARPS * 32), s0 = tid * each;
+        const int each = (st.n_seq + RW_THREADS - 1) / RW_THREADS, s0 = tid * each;
         long long mine = 0;
+        int most = 1;
         for (int s = s0; s < min(s0 + each, st.n_seq); s++) {
             const Seq q = seq_of(st, info, s);
             const Span sp = span_of(q);
             mine += (long long)sp.units * sp.blocks * c.n_head_kv;
+            most = max(most, sp.blocks > 0 ? sp.units : 1);
             sum_s[s] = mine;
         }
         long long inc = mine;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) { const long long y = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += y; }
-        if (lane == 31) warp_sum_s[warp] = inc;
+        most = (int)__reduce_max_sync(0xffffffffu, (unsigned)most);
+        if (lane == 31) { warp_sum_s[warp] = inc; most_s[warp] = most; }
         __syncthreads();
         long long before = inc - mine;
         for (int w = 0; w < warp; w++) before += warp_sum_s[w];
@@ -154,7 +176,8 @@ __global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_k
         __syncthreads();
     }
     const long long all = sum_s[st.n_seq - 1];
-    const long long ctas = min((long long)gridDim.x, all);
+    // (no block in more than RW_PARTS parts: what one CTA adds up at the end)
+    const long long ctas = min(min((long long)gridDim.x, all), max(1ll, (RW_PARTS - 2) * all / max(max(most_s[0], most_s[1]), max(most_s[2], most_s[3]))));
     if ((long long)blockIdx.x >= ctas) return;
     const long long u_end = all * (blockIdx.x + 1) / ctas;
 
@@ -171,21 +194,38 @@ __global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_k
         const int unit0 = (int)(rem % sp.units), n_here = (int)min((long long)(sp.units - unit0), u_end - u);
         const int h = (int)(item / sp.blocks), row0 = (int)(item % sp.blocks) * R, n_rows = min(R, q.count * group - row0);
         const int len = q.held + q.count;
-        const int pos_lo = q.held + row0 / group, pos_hi = q.held + (row0 + n_rows - 1) / group;
+        // row r of the block is query head head0 + r - token(r) * group of token tok0 + token(r)
+        const int tok0 = row0 / group, head0 = row0 - tok0 * group;
+        auto token = [&](int r) { return group == 1 ? r : (int)__umulhi((unsigned)(head0 + r), args.group_div); };
+        const int pos_lo = q.held + tok0, pos_hi = pos_lo + token(n_rows - 1);
+
+        // ---- q: pieces of 16 dims of the block's rows, on their way
+        constexpr int PIECES = C / 16, Q_EACH = (R * PIECES + RW_THREADS - 1) / RW_THREADS;
+        float x[Q_EACH][16];
+#pragma unroll
+        for (int i = 0; i < Q_EACH; i++) {
+            const int at = tid + i * RW_THREADS, r = at / PIECES, piece = at % PIECES;
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[i][e] = 0.f;
+            if (r < n_rows && piece * 16 < c.dim) {
+                const int tok = token(r);
+                row_load16(behind(a.q), a.type, (int64_t)(q.first + tok0 + tok) * a.q_stride + (int64_t)(h * group + head0 + r - tok * group) * c.dim + piece * 16, vec, x[i]);
+            }
+        }
 
         // ---- stages of pages
-        unsigned char *mine = smem + (size_t)warp * STAGES * STAGE;
+        unsigned char *mine = smem + (size_t)warp * RW_STAGES * STAGE;
         auto key_of = [&](int t) {  // the first of this warp's keys of unit t of the run
             const int n = unit0 + t;
             return (n < sp.keep ? n : n - sp.keep + sp.first) * RW_UNIT + warp * RW_TILE;
         };
         auto fetch = [&](int t) {  // lanes 0 and 1: the pages of the two 16s of keys
             const int key = key_of(t) + lane * 16;
-            return lane < 2 && t < n_here && key < len ? page_of(st, table, q.row, key / ps) : -1;
+            return lane < 2 && t < n_here && key < len ? page_of(st, table, q.row, key >> ps_shift) : -1;
         };
         auto issue = [&](int t, int pages) {
             if (t < n_here) {
-                unsigned char *stage = mine + (t % STAGES) * STAGE;
+                unsigned char *stage = mine + (t % RW_STAGES) * STAGE;
                 const int key = key_of(t);
                 constexpr int PER_ROW = C / 16, ROWS = 32 / PER_ROW;  // lanes of a row, rows at once
                 const int piece = lane % PER_ROW;
@@ -195,73 +235,60 @@ __global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_k
                     const int page = __shfl_sync(0xffffffffu, pages, half);
                     if (page < 0) continue;
                     there |= 1 << half;
-                    const unsigned char *record = reinterpret_cast<const unsigned char *>(c.pages) + (size_t)page * record_bytes(c);
-                    const int64_t row = (int64_t)h * ps + (key + 16 * half) % ps;
-                    const unsigned char *kp = record + row * c.dim + piece * 16, *vp = record + v_at(c) + row * c.vdim + piece * 16;
+                    const unsigned char *at_page = reinterpret_cast<const unsigned char *>(c.pages) + (size_t)page * record;
+                    const unsigned row = (unsigned)(h * ps + ((key + 16 * half) & (ps - 1)));
+                    const unsigned char *kp = at_page + row * (unsigned)c.dim + piece * 16, *vp = at_page + v_at(c) + row * (unsigned)c.vdim + piece * 16;
 #pragma unroll
                     for (int i = 0; i < 16 / ROWS; i++) {
                         const int r = lane / PER_ROW + i * ROWS, at = rw_piece<C>(16 * half + r, piece);
                         if (piece * 16 < c.dim) cp_async16(stage + at, kp + r * c.dim);
                         if (piece * 16 < c.vdim) cp_async16(stage + RW_TILE * C + at, vp + r * c.vdim);
                     }
-                    if (lane < 2) cp_async4(stage + RW_TILE * 2 * C + 8 * half + 4 * lane, record + scales_at(c) + ((size_t)lane * c.n_head_kv + h) * 4);
+                    if (lane < 2) cp_async4(stage + RW_TILE * 2 * C + 8 * half + 4 * lane, at_page + scales_at(c) + (unsigned)(lane * c.n_head_kv + h) * 4);
                 }
                 if (lane == 0) *reinterpret_cast<int *>(stage + RW_TILE * 2 * C + 16) = there;
             }
             cp_async_commit();
         };
-        int first_pages[STAGES];
-#pragma unroll
-        for (int i = 0; i < STAGES; i++) first_pages[i] = fetch(i);
-#pragma unroll
-        for (int i = 0; i < STAGES - 1; i++) issue(i, first_pages[i]);
-        int next_pages = first_pages[STAGES - 1];
+        static_assert(RW_STAGES == 2, "one tile on its way, one in use");
+        int next_pages = fetch(1);
+        issue(0, fetch(0));
 
-        // ---- this block's rows of q as the first operand, each relative to the power of two above its largest value
-        unsigned qf[C / 16][4];
+        // ---- q as the first operand, each row relative to the power of two above its largest value: in step 4 (piece / 4) + j thread tg holds the dims 4 j .. 4 j + 3 of
+        // its piece, as the keys' do
+#pragma unroll
+        for (int i = 0; i < Q_EACH; i++) {
+            const int at = tid + i * RW_THREADS, r = at / PIECES, piece = at % PIECES;
+            unsigned loud = 0;
+#pragma unroll
+            for (int e = 0; e < 16; e++) loud = max(loud, __float_as_uint(x[i][e]) & 0x7fffffffu);
+#pragma unroll
+            for (int off = 1; off < PIECES; off *= 2) loud = max(loud, __shfl_xor_sync(0xffffffffu, loud, off));
+            const int e_q = exponent_above(loud);
+            const float down = pow2i(min(14 - e_q, 126));
+            if (r >= R) continue;
+            if (piece == 0) scale_s[r] = loud >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : a.scale * pow2i(max(e_q - 14, -126)) * (a.softcap > 0.f ? 1.0f / a.softcap : LOG2E);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float x0 = x[i][4 * j] * down, x1 = x[i][4 * j + 1] * down, x2 = x[i][4 * j + 2] * down, x3 = x[i][4 * j + 3] * down;
+                const unsigned lo = pack_half(x0, x1), hi = pack_half(x2, x3);
+                uint4 *to = q_s + (piece / 4 * 4 + j) * 32 + (r % 8) * 4 + piece % 4;
+                if constexpr (TERMS == 2) {
+                    *to = make_uint4(lo, pack_rest(x0, x1, lo), hi, pack_rest(x2, x3, hi));
+                } else {
+                    unsigned *w = reinterpret_cast<unsigned *>(to) + r / 8;
+                    w[0] = lo;
+                    w[2] = hi;
+                }
+            }
+        }
+        __syncthreads();
         float row_scale[NR];
         int pos[NR];
 #pragma unroll
         for (int r = 0; r < NR; r++) {
-            const int row = g + 8 * r;
-            float x[C / 64][16];
-            unsigned loud = 0;
-            pos[r] = -1;  // (no such row: sees nothing)
-            if (row < n_rows) {
-                const int i = (row0 + row) / group, head = h * group + (row0 + row) % group;
-                pos[r] = q.held + i;
-#pragma unroll
-                for (int hf = 0; hf < C / 64; hf++) {
-                    const int at = 16 * (tg + 4 * hf);
-                    if (at < c.dim) row_load16(behind(a.q), a.type, (int64_t)(q.first + i) * a.q_stride + (int64_t)head * c.dim + at, x[hf]);
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        if (at >= c.dim) x[hf][e] = 0.f;
-                        loud = max(loud, __float_as_uint(x[hf][e]) & 0x7fffffffu);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int hf = 0; hf < C / 64; hf++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) x[hf][e] = 0.f;
-            }
-            loud = max(loud, __shfl_xor_sync(0xffffffffu, loud, 1));
-            loud = max(loud, __shfl_xor_sync(0xffffffffu, loud, 2));
-            const int e = exponent_above(loud);
-            const float down = pow2i(min(14 - e, 126));
-            row_scale[r] = loud >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : a.scale * pow2i(max(e - 14, -126)) * (a.softcap > 0.f ? 1.0f / a.softcap : LOG2E);
-#pragma unroll
-            for (int hf = 0; hf < C / 64; hf++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float x0 = x[hf][4 * j] * down, x1 = x[hf][4 * j + 1] * down, x2 = x[hf][4 * j + 2] * down, x3 = x[hf][4 * j + 3] * down;
-                    unsigned *f = qf[hf * 4 + j];
-                    const unsigned lo = pack_half(x0, x1), hi = pack_half(x2, x3);
-                    f[r] = lo;
-                    f[2 + r] = hi;
-                    if constexpr (TERMS == 2) { f[1] = pack_rest(x0, x1, lo); f[3] = pack_rest(x2, x3, hi); }
-                }
+            row_scale[r] = scale_s[g + 8 * r];
+            pos[r] = g + 8 * r < n_rows ? pos_lo + token(g + 8 * r) : -1;  // (no such row: sees nothing)
         }
 
         float o[NT][4], m[NR], l[NR];
@@ -272,11 +299,11 @@ __global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_k
         for (int r = 0; r < NR; r++) { m[r] = -INFINITY; l[r] = 0.f; power[r] = -100; }
 
         for (int t = 0; t < n_here; t++) {
-            cp_async_wait<STAGES - 2>();
+            cp_async_wait<0>();
             __syncwarp();
-            issue(t + STAGES - 1, next_pages);
-            next_pages = fetch(t + STAGES);
-            const unsigned char *stage = mine + (t % STAGES) * STAGE;
+            issue(t + 1, next_pages);
+            next_pages = fetch(t + 2);
+            const unsigned char *stage = mine + (t % RW_STAGES) * STAGE;
             const int key0 = key_of(t);
             const int there = *reinterpret_cast<const volatile int *>(stage + RW_TILE * 2 * C + 16);
             if (key0 > pos_hi || there == 0) continue;
@@ -291,13 +318,16 @@ __global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_k
 #pragma unroll
                 for (int n = 0; n < 4; n++) w[n] = *reinterpret_cast<const uint4 *>(stage + rw_piece<C>(8 * n + g, tg + 4 * hf));
 #pragma unroll
-                for (int j = 0; j < 4; j++)
+                for (int j = 0; j < 4; j++) {
+                    const uint4 qv = q_s[(hf * 4 + j) * 32 + lane];
+                    const unsigned qf[4] = {qv.x, qv.y, qv.z, qv.w};
 #pragma unroll
                     for (int n = 0; n < 4; n++) {
                         unsigned b0, b1;
                         int4_to_half(j == 0 ? w[n].x : j == 1 ? w[n].y : j == 2 ? w[n].z : w[n].w, b0, b1);
-                        mma_f16(sc[n], qf[hf * 4 + j], b0, b1);
+                        mma_f16(sc[n], qf, b0, b1);
                     }
+                }
             }
             const float4 scales = *reinterpret_cast<const float4 *>(stage + RW_TILE * 2 * C);  // keys, values of the first 16, then of the others
             float p[NR][8];
@@ -420,8 +450,10 @@ __global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_k
         cp_async_wait<0>();
         __syncthreads();
 
-        // ---- the warps meet: rows [warp][R][C] where the stages were
+        // ---- the warps meet: rows [warp][R][ROW] where the stages were.  Piece p (4 dims) of a row's 16 dims number n is at p ^ n: thread tg's pieces of the same number
+        // fall on different banks
         float *so = reinterpret_cast<float *>(smem);
+        auto place = [&](int d) { return C == 64 ? d : (d & ~15) | (((d >> 2 & 3) ^ (d >> 4 & 3)) << 2); };  // (d a multiple of 4)
 #pragma unroll
         for (int r = 0; r < NR; r++) {
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -429,51 +461,66 @@ __global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_k
             if (tg == 0) { top_s[warp][g + 8 * r] = m[r]; total_s[warp][g + 8 * r] = l[r]; power_s[warp][g + 8 * r] = power[r]; }
         }
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
-            // (columns 2 tg and 2 tg + 1 of tile i)
+        for (int i = 0; i < NT; i += 4) {
+            // (columns 2 tg and 2 tg + 1 of tiles i .. i + 3)
             const int d0 = C == 64 ? 16 * tg + i : 128 * (i / 16) + 16 * tg + i % 16, d1 = C == 64 ? d0 + 8 : d0 + 64;
-            float *at = so + ((size_t)warp * R + g) * C;
-            if constexpr (TERMS == 2) { at[d0] = o[i][0] + o[i][2]; at[d1] = o[i][1] + o[i][3]; }
-            else { at[d0] = o[i][0]; at[d1] = o[i][1]; at[8 * C + d0] = o[i][2]; at[8 * C + d1] = o[i][3]; }
-        }
-        __syncthreads();
-        if (tid < R) {
-            float top = -INFINITY, total = 0.f;
-#pragma unroll
-            for (int w = 0; w < RW_WARPS; w++) top = fmaxf(top, top_s[w][tid]);
-#pragma unroll
-            for (int w = 0; w < RW_WARPS; w++) {
-                const float f = top_s[w][tid] == -INFINITY ? (total_s[w][tid] == 0.f ? 0.f : 1.0f) : ex2(top_s[w][tid] - top);  // (a sum without a maximum is NaN: it stays)
-                total += total_s[w][tid] * f;
-                fac_s[w][tid] = f * pow2i(power_s[w][tid] - HEAD);
+            float *at = so + (warp * R + g) * ROW;
+            if constexpr (TERMS == 2) {
+                *reinterpret_cast<float4 *>(at + place(d0)) = make_float4(o[i][0] + o[i][2], o[i + 1][0] + o[i + 1][2], o[i + 2][0] + o[i + 2][2], o[i + 3][0] + o[i + 3][2]);
+                *reinterpret_cast<float4 *>(at + place(d1)) = make_float4(o[i][1] + o[i][3], o[i + 1][1] + o[i + 1][3], o[i + 2][1] + o[i + 2][3], o[i + 3][1] + o[i + 3][3]);
+            } else {
+                *reinterpret_cast<float4 *>(at + place(d0)) = make_float4(o[i][0], o[i + 1][0], o[i + 2][0], o[i + 3][0]);
+                *reinterpret_cast<float4 *>(at + place(d1)) = make_float4(o[i][1], o[i + 1][1], o[i + 2][1], o[i + 3][1]);
+                *reinterpret_cast<float4 *>(at + 8 * ROW + place(d0)) = make_float4(o[i][2], o[i + 1][2], o[i + 2][2], o[i + 3][2]);
+                *reinterpret_cast<float4 *>(at + 8 * ROW + place(d1)) = make_float4(o[i][3], o[i + 1][3], o[i + 2][3], o[i + 3][3]);
             }
-            top_s[0][tid] = top;
-            total_s[0][tid] = total;
         }
-        __syncthreads();
-        auto sum_of = [&](int r, int d) {
-            float x = 0.f;
-#pragma unroll
-            for (int w = 0; w < RW_WARPS; w++) x += so[((size_t)w * R + r) * C + d] * fac_s[w][r];
-            return x;
-        };
-        // a row's share of 1 / (sum and sink), for results relative to maximum `top`
+        // the factor that takes a row's results relative to maximum `top` to the row: 1 / (sum and sink)
         auto finish = [&](int r, float top, float total) {
-            const int head = h * group + (row0 + r) % group;
-            const float sink = a.sink ? a.sink[head] * LOG2E : -INFINITY;
+            const float sink = a.sink ? a.sink[h * group + head0 + r - token(r) * group] * LOG2E : -INFINITY;
             const float mm = fmaxf(top, sink);
             const float f = top == -INFINITY ? (total == 0.f ? 0.f : 1.0f) : ex2(top - mm);
             const float sum = total * f + (sink == -INFINITY ? 0.f : ex2(sink - mm));
             return sum == 0.f ? 0.f : f / sum;
         };
-        auto put = [&](int r, int d, float x) {
-            const int i = (row0 + r) / group, head = h * group + (row0 + r) % group;
-            row_put(a.dst, a.type, (int64_t)(q.first + i) * a.dst_stride + (int64_t)head * c.vdim + d, x);
+        const bool whole_block = n_here == sp.units;
+        __syncthreads();
+        if (tid < R) {
+            float top = -INFINITY, total = 0.f;
+#pragma unroll
+            for (int w = 0; w < RW_WARPS; w++) top = fmaxf(top, top_s[w][tid]);
+            float f[RW_WARPS];
+#pragma unroll
+            for (int w = 0; w < RW_WARPS; w++) {
+                f[w] = top_s[w][tid] == -INFINITY ? (total_s[w][tid] == 0.f ? 0.f : 1.0f) : ex2(top_s[w][tid] - top);  // (a sum without a maximum is NaN: it stays)
+                total += total_s[w][tid] * f[w];
+            }
+            const float share = whole_block && tid < n_rows ? finish(tid, top, total) : 1.0f;
+#pragma unroll
+            for (int w = 0; w < RW_WARPS; w++) fac_s[w][tid] = f[w] * pow2i(power_s[w][tid] - HEAD) * share;
+            top_s[0][tid] = top;
+            total_s[0][tid] = total;
+        }
+        __syncthreads();
+        const int quads = c.vdim / 4, quads_shift = 32 - __clz(quads - 1);  // 4 dims a thread; rows 2^quads_shift apart
+        auto sum_of = [&](int r, int d) {
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < RW_WARPS; w++) {
+                const float4 z = *reinterpret_cast<const float4 *>(so + (w * R + r) * ROW + place(d));
+                const float f = fac_s[w][r];
+                y = make_float4(y.x + z.x * f, y.y + z.y * f, y.z + z.z * f, y.w + z.w * f);
+            }
+            return y;
         };
-        if (n_here == sp.units) {
-            for (int i = tid; i < n_rows * c.vdim; i += RW_WARPS * 32) {
-                const int r = i / c.vdim, d = i % c.vdim;
-                put(r, d, sum_of(r, d) * finish(r, top_s[0][r], total_s[0][r]));
+        auto put = [&](int r, int d, float4 y) {
+            const int tok = token(r);
+            row_store4(a.dst, a.type, (int64_t)(q.first + tok0 + tok) * a.dst_stride + (int64_t)(h * group + head0 + r - tok * group) * c.vdim + d, vec, y);
+        };
+        if (whole_block) {
+            for (int i = tid; i < n_rows << quads_shift; i += RW_THREADS) {
+                const int r = i >> quads_shift, d = (i & ((1 << quads_shift) - 1)) * 4;
+                if (d < c.vdim) put(r, d, sum_of(r, d));
             }
         } else {
             // ---- part of a block: what began in an earlier CTA is this one's partial 0, what it begins itself its partial 1
@@ -484,9 +531,9 @@ __global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_k
             auto part_at = [&](int k) { return args.partials + ((size_t)(c0 + k) * 2 + (k == 0 ? 1 : 0)) * PART; };
             float *out = part_at((int)blockIdx.x - c0);
             if (tid < R) { out[tid] = top_s[0][tid]; out[R + tid] = total_s[0][tid]; }
-            for (int i = tid; i < R * c.vdim; i += RW_WARPS * 32) {
-                const int r = i / c.vdim, d = i % c.vdim;
-                out[2 * R + r * C + d] = sum_of(r, d);
+            for (int i = tid; i < R << quads_shift; i += RW_THREADS) {
+                const int r = i >> quads_shift, d = (i & ((1 << quads_shift) - 1)) * 4;
+                if (d < c.vdim) *reinterpret_cast<float4 *>(out + 2 * R + r * C + d) = sum_of(r, d);
             }
             __threadfence();
             __syncthreads();
@@ -497,29 +544,40 @@ __global__ void __launch_bounds__(RW_WARPS * 32, rw_per_sm<C>()) kv8_attn_rows_k
             }
             __syncthreads();
             if (last_s) {
-                float *fac = so;  // [parts][R]
-                for (int r = warp; r < n_rows; r += RW_WARPS) {  // a warp a row: maximum, then the parts' shares
+                // maxima and sums of all parts, then a warp a row: the parts' shares
+                float *fac = so, *tot = so + parts * R;  // [part][R]
+                for (int i = tid; i < parts * R; i += RW_THREADS) {
+                    const float *at = part_at(i / R) + i % R;
+                    fac[i] = __ldcg(at);
+                    tot[i] = __ldcg(at + R);
+                }
+                __syncthreads();
+                for (int r = warp; r < n_rows; r += RW_WARPS) {
                     float top = -INFINITY, total = 0.f;
-                    for (int k = lane; k < parts; k += 32) top = fmaxf(top, __ldcg(part_at(k) + r));
+                    for (int k = lane; k < parts; k += 32) top = fmaxf(top, fac[k * R + r]);
                     top = warp_max(top);
                     for (int k = lane; k < parts; k += 32) {
-                        const float mk = __ldcg(part_at(k) + r), lk = __ldcg(part_at(k) + R + r);
+                        const float mk = fac[k * R + r], lk = tot[k * R + r];
                         const float f = mk == -INFINITY ? (lk == 0.f ? 0.f : 1.0f) : ex2(mk - top);
                         fac[k * R + r] = f;
                         total += lk * f;
                     }
                     total = warp_sum(total);
-                    __syncwarp();
-                    const float f = finish(r, top, total);
-                    for (int k = lane; k < parts; k += 32) fac[k * R + r] *= f;
+                    if (lane == 0) share_s[r] = finish(r, top, total);
                 }
                 __syncthreads();
-                for (int i = tid; i < n_rows * c.vdim; i += RW_WARPS * 32) {
-                    const int r = i / c.vdim, d = i % c.vdim;
-                    float x = 0.f;
-#pragma unroll 4
-                    for (int k = 0; k < parts; k++) x += __ldcg(part_at(k) + 2 * R + r * C + d) * fac[k * R + r];
-                    put(r, d, x);
+                for (int i = tid; i < n_rows << quads_shift; i += RW_THREADS) {
+                    const int r = i >> quads_shift, d = (i & ((1 << quads_shift) - 1)) * 4;
+                    if (d >= c.vdim) continue;
+                    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+                    for (int k = 0; k < parts; k++) {
+                        const float4 z = __ldcg(reinterpret_cast<const float4 *>(part_at(k) + 2 * R + r * C + d));
+                        const float f = fac[k * R + r];
+                        y = make_float4(y.x + z.x * f, y.y + z.y * f, y.z + z.z * f, y.w + z.w * f);
+                    }
+                    const float f = share_s[r];
+                    put(r, d, make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
                 }
             }
         }
@@ -543,15 +601,15 @@ static int rows_grid(const b200_kv8_cache &c) {
 }
 static size_t rows_counter_bytes(int grid) { return ((size_t)grid * 4 + 255) / 256 * 256; }
 template <int C, int TERMS>
-static int launch_rows(const AttnArgs &args, cudaStream_t st) {
+static int launch_rows(const AttnArgs &args, bool vec, cudaStream_t st) {
     static bool done[16] = {};  // cudaFuncSetAttribute is per device
     int dev = 0;
     B200_CUDA_TRY(cudaGetDevice(&dev));
     if (dev >= 16 || !done[dev]) {
-        B200_CUDA_TRY(cudaFuncSetAttribute(kv8_attn_rows_kernel<C, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rw_smem<C>()));
+        B200_CUDA_TRY(cudaFuncSetAttribute(kv8_attn_rows_kernel<C, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, rw_fixed<C>() + 8 * B200_KV8_MAX_SEQ));
         if (dev < 16) done[dev] = true;
     }
-    B200_CUDA_TRY(launch_chained(kv8_attn_rows_kernel<C, TERMS>, (unsigned)rows_grid(args.a.cache), RW_WARPS * 32, rw_smem<C>(), st, args));
+    B200_CUDA_TRY(launch_chained(kv8_attn_rows_kernel<C, TERMS>, (unsigned)rows_grid(args.a.cache), RW_THREADS, (size_t)rw_fixed<C>() + 8 * (size_t)args.a.n_seq, st, args, vec));
     return B200_OK;
 }
 
@@ -610,15 +668,15 @@ int b200_op_kv8_attn(const b200_kv8_attn_args *a, void *workspace, size_t worksp
     args.group_div = (unsigned)(((1ull << 32) + args.group - 1) / args.group);
     const cudaStream_t st = (cudaStream_t)stream;
     const int k = attn_class(c);
+    const bool vec = rows_aligned(a->q, a->q_stride, a->type) && rows_aligned(a->dst, a->dst_stride, a->type);
     const int64_t longest = (int64_t)(a->max_new > 0 && a->max_new < a->n_tokens ? a->max_new : a->n_tokens) * args.group;  // query rows a kv head of one sequence, at most
     if (k <= 128 && longest > ROWS_MOST && (int64_t)a->n_tokens * args.group < (1ll << 30)) {
         args.rows_most = ROWS_MOST;
-        const bool vec = rows_aligned(a->q, a->q_stride, a->type) && rows_aligned(a->dst, a->dst_stride, a->type), one = one_term(a);
-        const int rc2 = launch_prompt(args, vec, k, one, PAIR_WAIT_LIMIT, st);
+        const int rc2 = launch_prompt(args, vec, k, one_term(a), PAIR_WAIT_LIMIT, st);
         if (rc2 != B200_OK) return rc2;
     }
-    if (one_term(a)) return k == 64 ? launch_rows<64, 1>(args, st) : k == 128 ? launch_rows<128, 1>(args, st) : launch_rows<256, 1>(args, st);
-    return k == 64 ? launch_rows<64, 2>(args, st) : k == 128 ? launch_rows<128, 2>(args, st) : launch_rows<256, 2>(args, st);
+    if (one_term(a)) return k == 64 ? launch_rows<64, 1>(args, vec, st) : k == 128 ? launch_rows<128, 1>(args, vec, st) : launch_rows<256, 1>(args, vec, st);
+    return k == 64 ? launch_rows<64, 2>(args, vec, st) : k == 128 ? launch_rows<128, 2>(args, vec, st) : launch_rows<256, 2>(args, vec, st);
 }
 
 }  // extern "C"

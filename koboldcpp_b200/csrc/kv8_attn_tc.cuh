@@ -94,19 +94,6 @@ __device__ __forceinline__ void row_values8(const uint4 (&u)[2], int type, float
         for (int e = 0; e < 8; e++) x[e] = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
     }
 }
-__device__ __forceinline__ void row_store4(void *row, int type, int64_t at, bool vec, float4 y) {
-    if (!vec) {
-        row_put(row, type, at, y.x); row_put(row, type, at + 1, y.y); row_put(row, type, at + 2, y.z); row_put(row, type, at + 3, y.w);
-    } else if (type == B200_TYPE_F32) {
-        *reinterpret_cast<float4 *>(reinterpret_cast<float *>(row) + at) = y;
-    } else if (type == B200_TYPE_F16) {
-        *reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(row) + at) = make_uint2(pack_half(y.x, y.y), pack_half(y.z, y.w));
-    } else {
-        const __nv_bfloat162 a = __floats2bfloat162_rn(y.x, y.y), b = __floats2bfloat162_rn(y.z, y.w);
-        *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(row) + at) = make_uint2(*reinterpret_cast<const unsigned *>(&a), *reinterpret_cast<const unsigned *>(&b));
-    }
-}
-
 template <int C, int GROUPS, int TERMS>
 __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(const __grid_constant__ AttnArgs args, bool vec, long long limit, int *timeout) {
     constexpr int NB = kt_buffers<GROUPS, TERMS>(), PANELS = C / 64, BLOCK = GROUPS * KT_ROWS, SOFTMAX = GROUPS * 4, CONVERT = SOFTMAX + 4;
