@@ -109,6 +109,7 @@ struct AttnArgs {
 // Scales: a key's joins its score; a value's joins its weight, relative to the power of two above the largest one that the row has seen.
 constexpr int RW_WARPS = 4, RW_TILE = 32, RW_UNIT = RW_WARPS * RW_TILE, RW_THREADS = RW_WARPS * 32;
 constexpr int RW_STAGES = 2, RW_PARTS = 128;
+constexpr int RW_BEGIN = 2;  // to begin and end a block costs a CTA about as much as two units: they are counted with each block's
 template <int C> constexpr int rw_stage_bytes() { return RW_TILE * 2 * C + 32; }  // keys, values, 2 scales of each, which pages are there
 template <int C> constexpr int rw_per_sm() { return C == 64 ? 4 : C == 128 ? 3 : 1; }
 template <int C> constexpr int rw_fixed() { return RW_WARPS * RW_STAGES * rw_stage_bytes<C>() + C * 32; }  // stages; q as operands of the first product
@@ -126,13 +127,13 @@ __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kern
     pdl_enter();
     constexpr int R = 16 / TERMS, NR = 2 / TERMS;  // rows of a block; a thread's rows in the MMA's result
     constexpr int NT = C / 8, STAGE = rw_stage_bytes<C>(), ROW = rw_row<C>();
-    static_assert(RW_WARPS == 4 && RW_PARTS * R * 8 <= RW_WARPS * RW_STAGES * STAGE, "parts' maxima and sums too");
+    static_assert(RW_WARPS == 4 && RW_PARTS * R * 4 <= RW_WARPS * RW_STAGES * STAGE, "the parts' shares too");
     static_assert(RW_WARPS * R * ROW * 4 <= RW_WARPS * RW_STAGES * STAGE, "the warps' results lie where the stages were");
     extern __shared__ __align__(16) unsigned char smem[];
     uint4 *q_s = reinterpret_cast<uint4 *>(smem + RW_WARPS * RW_STAGES * STAGE);                 // [step of 16 dims][lane]
     long long *sum_s = reinterpret_cast<long long *>(smem + rw_fixed<C>());                      // units of the sequences up to this one
     __shared__ long long warp_sum_s[RW_WARPS];
-    __shared__ float top_s[RW_WARPS][16], total_s[RW_WARPS][16], fac_s[RW_WARPS][16], share_s[16], scale_s[16];
+    __shared__ float top_s[RW_WARPS][16], total_s[RW_WARPS][16], fac_s[RW_WARPS][16], share_s[16], scale_s[16], sink_s[16];
     __shared__ int power_s[RW_WARPS][16], most_s[RW_WARPS], last_s;
     const b200_kv8_attn_args &a = args.a;
     const b200_kv8_cache &c = a.cache;
@@ -160,8 +161,8 @@ __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kern
         for (int s = s0; s < min(s0 + each, st.n_seq); s++) {
             const Seq q = seq_of(st, info, s);
             const Span sp = span_of(q);
-            mine += (long long)sp.units * sp.blocks * c.n_head_kv;
-            most = max(most, sp.blocks > 0 ? sp.units : 1);
+            mine += (long long)(sp.units + RW_BEGIN) * sp.blocks * c.n_head_kv;
+            most = max(most, sp.blocks > 0 ? sp.units + RW_BEGIN : 1);
             sum_s[s] = mine;
         }
         long long inc = mine;
@@ -190,9 +191,15 @@ __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kern
         }
         const Seq q = seq_of(st, info, s);
         const Span sp = span_of(q);
-        const long long rem = u - (s ? sum_s[s - 1] : 0), item = rem / sp.units;
-        const int unit0 = (int)(rem % sp.units), n_here = (int)min((long long)(sp.units - unit0), u_end - u);
-        const int h = (int)(item / sp.blocks), row0 = (int)(item % sp.blocks) * R, n_rows = min(R, q.count * group - row0);
+        const long long rem = u - (s ? sum_s[s - 1] : 0);
+        const unsigned each = (unsigned)(sp.units + RW_BEGIN);
+        const int item = rem >> 32 ? (int)(rem / each) : (int)((unsigned)rem / each);
+        const int at = (int)(rem - (long long)item * each);  // where in the block this CTA's run of it begins, what RW_BEGIN stands for in front of its units
+        const int unit0 = max(at - RW_BEGIN, 0), n_here = (int)min((long long)sp.units, u_end - u + at - RW_BEGIN) - unit0;
+        const long long begin = u - at, end = begin + each;
+        u = min(end, u_end);
+        if (n_here <= 0) continue;  // (the next CTA begins it)
+        const int h = item / sp.blocks, row0 = (item - h * sp.blocks) * R, n_rows = min(R, q.count * group - row0);
         const int len = q.held + q.count;
         // row r of the block is query head head0 + r - token(r) * group of token tok0 + token(r)
         const int tok0 = row0 / group, head0 = row0 - tok0 * group;
@@ -250,6 +257,7 @@ __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kern
             }
             cp_async_commit();
         };
+        if (tid < n_rows) sink_s[tid] = a.sink ? a.sink[h * group + head0 + tid - token(tid) * group] * LOG2E : -INFINITY;
         static_assert(RW_STAGES == 2, "one tile on its way, one in use");
         int next_pages = fetch(1);
         issue(0, fetch(0));
@@ -477,8 +485,7 @@ __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kern
         }
         // the factor that takes a row's results relative to maximum `top` to the row: 1 / (sum and sink)
         auto finish = [&](int r, float top, float total) {
-            const float sink = a.sink ? a.sink[h * group + head0 + r - token(r) * group] * LOG2E : -INFINITY;
-            const float mm = fmaxf(top, sink);
+            const float sink = sink_s[r], mm = fmaxf(top, sink);
             const float f = top == -INFINITY ? (total == 0.f ? 0.f : 1.0f) : ex2(top - mm);
             const float sum = total * f + (sink == -INFINITY ? 0.f : ex2(sink - mm));
             return sum == 0.f ? 0.f : f / sum;
@@ -524,9 +531,8 @@ __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kern
             }
         } else {
             // ---- part of a block: what began in an earlier CTA is this one's partial 0, what it begins itself its partial 1
-            const long long begin = u - unit0, end = begin + sp.units;
             auto cta_of = [&](long long unit) { return (int)(((unit + 1) * ctas - 1) / all); };
-            const int c0 = cta_of(begin), parts = cta_of(end - 1) - c0 + 1;
+            const int c0 = cta_of(begin + RW_BEGIN), parts = cta_of(end - 1) - c0 + 1;
             constexpr int PART = R * (C + 2);
             auto part_at = [&](int k) { return args.partials + ((size_t)(c0 + k) * 2 + (k == 0 ? 1 : 0)) * PART; };
             float *out = part_at((int)blockIdx.x - c0);
@@ -535,36 +541,40 @@ __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kern
                 const int r = i >> quads_shift, d = (i & ((1 << quads_shift) - 1)) * 4;
                 if (d < c.vdim) *reinterpret_cast<float4 *>(out + 2 * R + r * C + d) = sum_of(r, d);
             }
-            __threadfence();
             __syncthreads();
             if (tid == 0) {
+                __threadfence();  // (what the CTA wrote, the barrier in front)
                 last_s = atomicAdd(&args.counters[c0], 1) == parts - 1;
                 if (last_s) args.counters[c0] = 0;
                 __threadfence();
             }
             __syncthreads();
             if (last_s) {
-                // maxima and sums of all parts, then a warp a row: the parts' shares
-                float *fac = so, *tot = so + parts * R;  // [part][R]
-                for (int i = tid; i < parts * R; i += RW_THREADS) {
-                    const float *at = part_at(i / R) + i % R;
-                    fac[i] = __ldcg(at);
-                    tot[i] = __ldcg(at + R);
+                // maxima and sums of all parts: LANES threads a row
+                float *fac = so;  // [part][R]
+                constexpr int LANES = RW_THREADS / R, EACH = RW_PARTS / LANES;
+                const int r = tid / LANES, j = tid % LANES;
+                float mk[EACH], lk[EACH], top = -INFINITY, total = 0.f;
+#pragma unroll
+                for (int i = 0; i < EACH; i++) {
+                    const int k = j + i * LANES;
+                    mk[i] = -INFINITY;
+                    lk[i] = 0.f;
+                    if (k < parts) { mk[i] = __ldcg(part_at(k) + r); lk[i] = __ldcg(part_at(k) + R + r); }
+                    top = fmaxf(top, mk[i]);
                 }
-                __syncthreads();
-                for (int r = warp; r < n_rows; r += RW_WARPS) {
-                    float top = -INFINITY, total = 0.f;
-                    for (int k = lane; k < parts; k += 32) top = fmaxf(top, fac[k * R + r]);
-                    top = warp_max(top);
-                    for (int k = lane; k < parts; k += 32) {
-                        const float mk = fac[k * R + r], lk = tot[k * R + r];
-                        const float f = mk == -INFINITY ? (lk == 0.f ? 0.f : 1.0f) : ex2(mk - top);
-                        fac[k * R + r] = f;
-                        total += lk * f;
-                    }
-                    total = warp_sum(total);
-                    if (lane == 0) share_s[r] = finish(r, top, total);
+#pragma unroll
+                for (int off = 1; off < LANES; off *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+#pragma unroll
+                for (int i = 0; i < EACH; i++) {
+                    const int k = j + i * LANES;
+                    const float f = mk[i] == -INFINITY ? (lk[i] == 0.f ? 0.f : 1.0f) : ex2(mk[i] - top);
+                    if (k < parts) fac[k * R + r] = f;
+                    total += lk[i] * f;
                 }
+#pragma unroll
+                for (int off = 1; off < LANES; off *= 2) total += __shfl_xor_sync(0xffffffffu, total, off);
+                if (j == 0) share_s[r] = r < n_rows ? finish(r, top, total) : 0.f;
                 __syncthreads();
                 for (int i = tid; i < n_rows << quads_shift; i += RW_THREADS) {
                     const int r = i >> quads_shift, d = (i & ((1 << quads_shift) - 1)) * 4;
@@ -582,7 +592,6 @@ __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kern
             }
         }
         __syncthreads();  // (the stages are free again)
-        u += n_here;
     }
 }
 
