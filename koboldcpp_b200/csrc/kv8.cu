@@ -28,26 +28,32 @@ int check_step(const b200_kv8_cache *c, const int32_t *seq_info, const int32_t *
 }
 
 // ------------------------------------------------------------------------------------------------ store
-// round(x / s) of the exact quotient, ties to even, |x| <= 127.5 s or thereabouts, s normal.  x * (1 / s) is off by two roundings at most, so r is
-// the right integer or a neighbour of it; x - r s is exact in f32 (both are multiples of the finer of their last places, and the difference is below
-// 2^24 of those), as is s / 2, so two comparisons settle it.
-__device__ __forceinline__ float quotient(float x, float s, float inv) {
-    float r = rintf(x * inv);
-    const float d = fmaf(-r, s, x), half = 0.5f * s;
-    const bool odd = ((int)r & 1) != 0;
-    if (d > half || (d == half && odd)) r += 1.0f;
-    else if (d < -half || (d == -half && odd)) r -= 1.0f;
-    return fminf(fmaxf(r, -127.0f), 127.0f);
+// Quotients x / s are rounded exactly (to the nearest integer, ties to even), |x| <= 127 s and a little.  MAGIC + x (1 / s) rounds to an integer in the lowest bits, the right one or
+// its neighbour; x less r s is exact in f32 (both are multiples of the finer of their last places, and the difference is below 2^24 of those; where |x| < s, r is 0 or +-1 and
+// the difference is Sterbenz's), and so is s / 2, so that comparisons tell whether r is the right one.  It hardly ever is not: off() says so, mend() moves it.
+constexpr float MAGIC = 12582912.0f;  // 1.5 2^23
+__device__ __forceinline__ float rest(float x, float t, float s) { return fmaf(-(t - MAGIC), s, x); }
+__device__ __forceinline__ float mend(float t, float d, float below, float above) {  // below: of d - s / 2, above: of d + s / 2, their signs
+    const bool odd = (__float_as_uint(t) & 1u) != 0;
+    if (below > 0.f || (below == 0.f && odd)) return t + 1.0f;
+    if (above < 0.f || (above == 0.f && odd)) return t - 1.0f;
+    return t;
 }
+// lowest bytes of four
 __device__ __forceinline__ unsigned pack4(float a, float b, float c, float d) {
-    return ((unsigned)(int)a & 0xffu) | ((unsigned)(int)b & 0xffu) << 8 | ((unsigned)(int)c & 0xffu) << 16 | (unsigned)(int)d << 24;
+    return prmt(prmt(__float_as_uint(a), __float_as_uint(b), 0x0040), prmt(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
+}
+__device__ __forceinline__ float max_nan(float x, float y, float z) {  // NaN if one is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
 }
 
-// One CTA per (page that gets new tokens, head, keys or values): the largest magnitude of the new values, the scale, what was there before if the
-// scale grew, the new values.  The values wait in registers between the two (KEEP pieces of 16 a thread; a page with more is read twice).
+// One CTA per (page that gets new tokens, head), half of its threads for the keys and half for the values: the largest magnitude of the new values, the scale, what was there
+// before if the scale grew, the new values.  The values wait in registers as they came (KEEP pieces of 16 a thread; of a page with more they are read twice).
 // Item j of the grid is a page of sequence s where first_s / page_size + 2 s <= j: a sequence of n tokens touches n / page_size + 2 pages at most, so
 // the items of the sequences do not overlap and nothing has to be summed up beforehand.
-constexpr int ST_THREADS = 128, ST_KEEP = 4;
+constexpr int ST_THREADS = 128;
 struct StoreArgs {
     b200_kv8_cache cache;
     Step step;
@@ -55,18 +61,19 @@ struct StoreArgs {
     int64_t k_stride, v_stride;
 };
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(ST_THREADS) kv8_store_kernel(const StoreArgs a) {
+__global__ void __launch_bounds__(2 * ST_THREADS, 4) kv8_store_kernel(const StoreArgs a) {
     pdl_enter();
-    __shared__ unsigned top[ST_THREADS / 32];
+    constexpr int KEEP = 16 / sizeof(T) / 2;  // f32: 2, else 4
+    __shared__ float top[2 * ST_THREADS / 32];
     const b200_kv8_cache &c = a.cache;
     const Step &st = a.step;
-    const int j = blockIdx.x, ps = c.page_size, h = blockIdx.y >> 1;
-    const bool is_v = blockIdx.y & 1;
+    const int j = blockIdx.x, ps = c.page_size, ps_shift = 31 - __clz(ps), h = blockIdx.y, tid = threadIdx.x % ST_THREADS;
+    const bool is_v = threadIdx.x >= ST_THREADS;
     const int32_t *info = behind(st.info), *table = behind(st.table);
-    const int s = find_seq(info, st.n_seq, j, [&](int first, int i) { return first / ps + 2 * i; });
-    const Seq q = seq_of(st, info, s);
-    const int at = q.held / ps + (j - (q.first / ps + 2 * s));
-    if (q.count == 0 || at < q.held / ps || (int64_t)at * ps >= (int64_t)q.held + q.count) return;
+    int s;
+    const Seq q = find_seq(st, info, j, s, [&](int first, int i) { return (first >> ps_shift) + 2 * i; });
+    const int at = (q.held >> ps_shift) + (j - ((q.first >> ps_shift) + 2 * s));
+    if (q.count == 0 || at < q.held >> ps_shift || (int64_t)at * ps >= (int64_t)q.held + q.count) return;
     const int page = page_of(st, table, q.row, at);
     if (page < 0) return;
     const int begin = max(q.held, at * ps), used = begin - at * ps, n = (int)min((int64_t)q.held + q.count, (int64_t)(at + 1) * ps) - begin;
@@ -78,41 +85,44 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_store_kernel(const StoreArgs a
     float *scale = reinterpret_cast<float *>(record + scales_at(c)) + (is_v ? c.n_head_kv : 0) + h;
     const float before = used > 0 ? *scale : 0.f;
 
-    float x[ST_KEEP][16];
-    unsigned loud = 0;  // magnitudes compare like their bits; what is not finite is above all others
-    auto value = [&](int i, float (&y)[16]) { load16<T, VEC>(src + (int64_t)(i / pieces) * stride + i % pieces * 16, y); };
-    auto magnitude = [&](const float (&y)[16]) {
+    Raw16<T> x[KEEP];
+    const unsigned per = (65536u + (unsigned)pieces - 1) / (unsigned)pieces;  // i / pieces = i per >> 16 (i < 2048, pieces <= 16)
+    auto fetch = [&](int i, Raw16<T> &y) {
+        const int row = (int)((unsigned)i * per >> 16);
+        load_raw16<T, VEC>(src + (int64_t)row * stride + (i - row * pieces) * 16, y);
+    };
+    float loud = 0.f;  // NaN stays
+    auto magnitude = [&](const Raw16<T> &y) {
 #pragma unroll
-        for (int e = 0; e < 16; e++) loud = max(loud, __float_as_uint(y[e]) & 0x7fffffffu);
+        for (int e = 0; e < 16; e += 2) loud = max_nan(loud, fabsf(raw_value(y, e)), fabsf(raw_value(y, e + 1)));
     };
 #pragma unroll
-    for (int u = 0; u < ST_KEEP; u++) {
-        const int i = threadIdx.x + u * ST_THREADS;
-        if (i < total) { value(i, x[u]); magnitude(x[u]); }
-    }
-    for (int i = threadIdx.x + ST_KEEP * ST_THREADS; i < total; i += ST_THREADS) {
-        float y[16];
-        value(i, y);
+    for (int u = 0; u < KEEP; u++) if (tid + u * ST_THREADS < total) fetch(tid + u * ST_THREADS, x[u]);
+#pragma unroll
+    for (int u = 0; u < KEEP; u++) if (tid + u * ST_THREADS < total) magnitude(x[u]);
+    for (int i = tid + KEEP * ST_THREADS; i < total; i += ST_THREADS) {
+        Raw16<T> y;
+        fetch(i, y);
         magnitude(y);
     }
-    loud = __reduce_max_sync(0xffffffffu, loud);
+    // (magnitudes compare like their bits, NaN above all)
+    loud = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(loud) & 0x7fffffffu));
     if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = loud;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < ST_THREADS / 32; w++) loud = max(loud, top[w]);
-    // (behind the barrier every thread has read the scale: a thread waits there for its own load, whose value it needs below only)
-    float want = __fdiv_rn(__uint_as_float(loud), 127.0f), now;
+    for (int w = 0; w < ST_THREADS / 32; w++) loud = max_nan(loud, top[(is_v ? ST_THREADS / 32 : 0) + w], 0.f);
+    float want = __fdiv_rn(loud, 127.0f), now;
     want = want < FLT_MIN ? 0.f : want;
-    const bool broken = loud >= 0x7f800000u || !(fabsf(before) <= FLT_MAX);
+    const bool broken = !(loud <= FLT_MAX) || !(fabsf(before) <= FLT_MAX);
     if (broken) now = __uint_as_float(0x7fc00000u);
     else if (used == 0) now = want;
     else now = want <= before ? before : fmaxf(want, __fmul_rn(1.25f, before));
-    __syncthreads();
-    if (threadIdx.x == 0) *scale = now;
+    __syncthreads();  // (every thread has read the scale)
+    if (tid == 0) *scale = now;
+    const float inv = now > 0.f ? __fdiv_rn(1.0f, now) : 0.f, half = 0.5f * now;  // (NaN, 0: all values become 0)
 
-    if (used > 0 && !broken && now != before) {  // (f64: ratios of scales; at most a page for each sequence and step)
-        const double ratio_up = (double)before, ratio_down = (double)now;
-        for (int i = threadIdx.x; i < used * pieces; i += ST_THREADS) {
+    if (used > 0 && !broken && now != before) {  // a scale of 0 in front of one that is not: all of them are 0
+        for (int i = tid; i < used * pieces; i += ST_THREADS) {
             uint4 *p = reinterpret_cast<uint4 *>(ints) + i;
             const uint4 u = *p;
             unsigned w[4] = {u.x, u.y, u.z, u.w};
@@ -120,32 +130,39 @@ __global__ void __launch_bounds__(ST_THREADS) kv8_store_kernel(const StoreArgs a
             for (int e = 0; e < 4; e++) {
                 float f[4];
 #pragma unroll
-                for (int b = 0; b < 4; b++) f[b] = (float)rint((double)(signed char)(w[e] >> (8 * b)) * ratio_up / ratio_down);
+                for (int b = 0; b < 4; b++) {
+                    // q before = hi + lo exactly; with d = hi - r now exact, as above, the signs of d + lo -+ now / 2 are those of (d -+ now / 2) + lo
+                    const float qf = (float)(signed char)(w[e] >> (8 * b)), hi = __fmul_rn(qf, before), lo = fmaf(qf, before, -hi);
+                    const float t = fmaf(hi, inv, MAGIC), d = rest(hi, t, now);
+                    f[b] = mend(t, d, (d - half) + lo, (d + half) + lo);
+                }
                 w[e] = pack4(f[0], f[1], f[2], f[3]);
             }
             *p = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
-    const float inv = now > 0.f ? __fdiv_rn(1.0f, now) : 0.f;  // (NaN, 0: all values become 0)
-    auto put = [&](int i, const float (&y)[16]) {
-        unsigned w[4];
+    auto put = [&](int i, const Raw16<T> &y) {
+        float t[16], off = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            float f[4];
-#pragma unroll
-            for (int b = 0; b < 4; b++) f[b] = inv > 0.f ? quotient(y[4 * e + b], now, inv) : 0.f;
-            w[e] = pack4(f[0], f[1], f[2], f[3]);
+        for (int e = 0; e < 16; e++) {
+            const float v = raw_value(y, e);
+            t[e] = fmaf(v, inv, MAGIC);
+            off = fmaxf(off, fabsf(rest(v, t[e], now)));
         }
-        reinterpret_cast<uint4 *>(ints + (size_t)used * size)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        if (!(off < half)) {  // a tie, or beside one (or a scale that is no number: off is 0 or NaN is passed over, half is not above it)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const float d = rest(raw_value(y, e), t[e], now);
+                t[e] = inv > 0.f ? mend(t[e], d, d - half, d + half) : MAGIC;
+            }
+        }
+        reinterpret_cast<uint4 *>(ints + (size_t)used * size)[i] = make_uint4(pack4(t[0], t[1], t[2], t[3]), pack4(t[4], t[5], t[6], t[7]), pack4(t[8], t[9], t[10], t[11]), pack4(t[12], t[13], t[14], t[15]));
     };
 #pragma unroll
-    for (int u = 0; u < ST_KEEP; u++) {
-        const int i = threadIdx.x + u * ST_THREADS;
-        if (i < total) put(i, x[u]);
-    }
-    for (int i = threadIdx.x + ST_KEEP * ST_THREADS; i < total; i += ST_THREADS) {
-        float y[16];
-        value(i, y);
+    for (int u = 0; u < KEEP; u++) if (tid + u * ST_THREADS < total) put(tid + u * ST_THREADS, x[u]);
+    for (int i = tid + KEEP * ST_THREADS; i < total; i += ST_THREADS) {
+        Raw16<T> y;
+        fetch(i, y);
         put(i, y);
     }
 }
@@ -166,8 +183,8 @@ __global__ void __launch_bounds__(LD_THREADS) kv8_load_kernel(const LoadArgs a) 
     const Step &st = a.step;
     const int t = blockIdx.x, ps = c.page_size;
     const int32_t *info = behind(st.info), *table = behind(st.table);
-    const int s = find_seq(info, st.n_seq, t, [](int first, int) { return first; });
-    const Seq q = seq_of(st, info, s);
+    int s;
+    const Seq q = find_seq(st, info, t, s, [](int first, int) { return first; });
     if (t < q.first || t - q.first >= q.count) return;
     const int pos = q.held + t - q.first, page = page_of(st, table, q.row, pos / ps), slot = pos % ps;
     const unsigned char *record = behind(reinterpret_cast<const unsigned char *>(c.pages)) + (size_t)max(page, 0) * record_bytes(c);
@@ -289,14 +306,22 @@ constexpr int GR_EACH = 8;  // neighbouring entries of refs a thread looks at pe
 __global__ void __launch_bounds__(1024) kv8_grow_kernel(const Map m, const int32_t *__restrict__ rows, const int32_t *__restrict__ n_new, int n, int32_t *__restrict__ seq_info, int32_t *refused,
                                                         int32_t *__restrict__ pairs) {
     pdl_enter(rows, n_new, pairs);
-    __shared__ int sh[32], row_s[1024], start_s[1024], first_s[1024], short_s;  // start: pages of the rows before; first: table entry of a row's first page
+    __shared__ __align__(16) int row_s[1024];
+    __shared__ int sh[32], start_s[1024], first_s[1024], short_s;  // start: pages of the rows before; first: table entry of a row's first page
     const int i = threadIdx.x, ps = m.page_size;
     const int row = i < n ? rows[i] : -1, asked = i < n ? n_new[i] : 0;
     row_s[i] = row;
     if (i == 0) short_s = 0;
     __syncthreads();
     bool ok = i < n && row >= 0 && row < m.n_rows && asked >= 0;
-    for (int j = 0; j < i && ok; j++) ok = row_s[j] != row;
+    if (i < n) {
+        bool again = false;
+        for (int j = 0; j < i; j += 4) {
+            const int4 r = *reinterpret_cast<const int4 *>(row_s + j);
+            again |= r.x == row || (r.y == row && j + 1 < i) || (r.z == row && j + 2 < i) || (r.w == row && j + 3 < i);
+        }
+        ok = ok && !again;
+    }
     const int held = ok ? max(m.len[row], 0) : 0;
     ok = ok && (int64_t)held + asked <= min(m.stride * ps, (int64_t)0x7fffffff);
     const int begin = pages_for(held, ps), more = ok ? pages_for(held + asked, ps) - begin : 0;
@@ -311,11 +336,19 @@ __global__ void __launch_bounds__(1024) kv8_grow_kernel(const Map m, const int32
     const int first_token = scan_1024(i < n ? max(asked, 0) : 0, sh, tokens);
     start_s[i] = start;
     first_s[i] = begin - (tail >= 0);
-    for (int base = 0; base < m.n_pages && n_free < total; base += 1024 * GR_EACH) {
-        int mine = 0, all;
+    auto free_pages = [&](int base) {
+        unsigned mask = 0;
 #pragma unroll
-        for (int u = 0; u < GR_EACH; u++) { const int p = base + i * GR_EACH + u; mine += p < m.n_pages && m.refs[p] == 0; }
-        scan_1024(mine, sh, all);
+        for (int u = 0; u < GR_EACH; u++) { const int p = base + i * GR_EACH + u; if (p < m.n_pages && m.refs[p] == 0) mask |= 1u << u; }
+        return mask;
+    };
+    unsigned first_mask = 0;  // of the first round, which is most often the only one: it need not be asked for twice
+    int first_rank = 0, first_all = 0;
+    for (int base = 0; base < m.n_pages && n_free < total; base += 1024 * GR_EACH) {
+        const unsigned mask = free_pages(base);
+        int all;
+        const int rank = scan_1024(__popc(mask), sh, all);
+        if (base == 0) { first_mask = mask; first_rank = rank; first_all = all; }
         n_free += all;
     }
     ok = ok && (need == 0 || start + need <= n_free);
@@ -324,11 +357,12 @@ __global__ void __launch_bounds__(1024) kv8_grow_kernel(const Map m, const int32
     __syncthreads();
     int before = 0;
     for (int base = 0; base < m.n_pages && before < min(total, n_free); base += 1024 * GR_EACH) {
-        unsigned free_mask = 0;
-        int all;
-#pragma unroll
-        for (int u = 0; u < GR_EACH; u++) { const int p = base + i * GR_EACH + u; if (p < m.n_pages && m.refs[p] == 0) free_mask |= 1u << u; }
-        int rank = before + scan_1024(__popc(free_mask), sh, all);
+        unsigned free_mask = first_mask;
+        int all = first_all, rank = first_rank;
+        if (base > 0) {
+            free_mask = free_pages(base);
+            rank = before + scan_1024(__popc(free_mask), sh, all);
+        }
         while (free_mask && rank < total) {
             const int p = base + i * GR_EACH + __ffs(free_mask) - 1;
             free_mask &= free_mask - 1;
@@ -493,7 +527,7 @@ static Map map_of(const b200_kv8_map *m) { return Map{m->table, m->len, m->refs,
 
 template <typename T>
 static int launch_store(const StoreArgs &s, bool vec, dim3 grid, cudaStream_t st) {
-    B200_CUDA_TRY(vec ? launch_chained(kv8_store_kernel<T, true>, grid, ST_THREADS, 0, st, s) : launch_chained(kv8_store_kernel<T, false>, grid, ST_THREADS, 0, st, s));
+    B200_CUDA_TRY(vec ? launch_chained(kv8_store_kernel<T, true>, grid, 2 * ST_THREADS, 0, st, s) : launch_chained(kv8_store_kernel<T, false>, grid, 2 * ST_THREADS, 0, st, s));
     return B200_OK;
 }
 template <typename T>
@@ -528,7 +562,7 @@ int b200_op_kv8_store(const b200_kv8_store_args *a, b200_stream_t stream) {
     OPX_REQUIRE(a->k_stride >= (int64_t)c.n_head_kv * c.dim && a->v_stride >= (int64_t)c.n_head_kv * c.vdim, B200_ERR_INVALID, "%s: rows of k or v overlap (strides %lld, %lld)", who,
                 (long long)a->k_stride, (long long)a->v_stride);
     const StoreArgs s = {c, {a->seq_info, a->table, a->table_stride, a->n_rows, a->n_seq, a->n_tokens, c.n_pages, c.page_size}, a->k, a->v, a->k_stride, a->v_stride};
-    const dim3 grid((unsigned)(a->n_tokens / c.page_size + 2 * a->n_seq), (unsigned)(2 * c.n_head_kv));
+    const dim3 grid((unsigned)(a->n_tokens / c.page_size + 2 * a->n_seq), (unsigned)c.n_head_kv);
     const bool vec = rows_aligned(a->k, a->k_stride, a->type) && rows_aligned(a->v, a->v_stride, a->type);
     const cudaStream_t st = (cudaStream_t)stream;
     return a->type == B200_TYPE_F32 ? launch_store<float>(s, vec, grid, st) : a->type == B200_TYPE_F16 ? launch_store<__half>(s, vec, grid, st) : launch_store<__nv_bfloat16>(s, vec, grid, st);

@@ -31,19 +31,51 @@ __device__ __forceinline__ int page_of(const Step &st, const int32_t *table, int
     const int p = table[(int64_t)row * st.table_stride + at];
     return p >= 0 && p < st.n_pages ? p : -1;
 }
-// The last sequence s with begin(first token of s, s) <= j, by a whole warp (begin does not fall with s; sequence 0 begins at or below j): 32 of them at a time.
+// The last sequence s with begin(its first token, s) <= j, and what is known of it, by a whole warp (begin does not fall with s; sequence 0 begins at or below j): 32 of them at a
+// time, the last 32 with all that a step says of them.
 template <typename F>
-__device__ __forceinline__ int find_seq(const int32_t *first, int n_seq, int j, F begin) {
-    const int lane = threadIdx.x & 31;
+__device__ __forceinline__ Seq find_seq(const Step &st, const int32_t *info, int j, int &s, F begin) {
+    const int lane = threadIdx.x & 31, n_seq = st.n_seq;
     int lo = 0, n = n_seq;  // the answer is in [lo, lo + n)
-    while (n > 1) {
-        const int step = (n + 31) / 32, s = lo + lane * step;
-        const unsigned yes = __ballot_sync(0xffffffffu, lane * step < n && begin(first[min(s, n_seq - 1)], s) <= j);
+    while (n > 32) {
+        const int step = (n + 31) / 32, at = lo + lane * step;
+        const unsigned yes = __ballot_sync(0xffffffffu, lane * step < n && begin(info[min(at, n_seq - 1)], at) <= j);
         const int k = yes ? 31 - __clz(yes) : 0;
         lo += k * step;
         n = min(step, n - k * step);
     }
-    return lo;
+    const int at = min(lo + lane, n_seq - 1);
+    Seq q = seq_of(st, info, at);
+    const int first = info[at];
+    const unsigned yes = __ballot_sync(0xffffffffu, lane < n && begin(first, lo + lane) <= j);
+    const int k = yes ? 31 - __clz(yes) : 0;
+    s = lo + k;
+    return Seq{__shfl_sync(0xffffffffu, q.first, k), __shfl_sync(0xffffffffu, q.count, k), __shfl_sync(0xffffffffu, q.row, k), __shfl_sync(0xffffffffu, q.held, k)};
+}
+
+// 16 consecutive values of a row as they lie there, without a conversion; VEC: the row's pieces of 16 values are 16-byte aligned
+template <typename T> struct Raw16 { uint4 u[sizeof(T)]; };
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_raw16(const T *p, Raw16<T> &r) {
+    if constexpr (VEC) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T); i++) r.u[i] = reinterpret_cast<const uint4 *>(p)[i];
+    } else {
+        __align__(16) T v[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) v[i] = p[i];
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T); i++) r.u[i] = reinterpret_cast<const uint4 *>(v)[i];
+    }
+}
+template <typename T>
+__device__ __forceinline__ float raw_value(const Raw16<T> &r, int i) {  // (i known when compiled)
+    const uint4 u = r.u[i * (int)sizeof(T) / 16];
+    const int word = i * (int)sizeof(T) / 4 % 4;
+    const unsigned w = word == 0 ? u.x : word == 1 ? u.y : word == 2 ? u.z : u.w;
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+    else if constexpr (std::is_same<T, __half>::value) return h2f((unsigned short)(w >> (16 * (i & 1))));
+    else return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
 }
 
 // 16 consecutive values of a row of activations as f32; VEC: the row's pieces of 16 values are 16-byte aligned

@@ -117,8 +117,8 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
     // block j of rows belongs to the sequence s with first_s group / BLOCK + s <= j (long causal walks first, of all heads)
     const int j = (int)((gridDim.x - 1 - blockIdx.x) / (unsigned)c.n_head_kv);
     auto first_block = [&](int first, int s) { return (int)((int64_t)first * group / BLOCK) + s; };
-    const int s = find_seq(info, st.n_seq, j, first_block);
-    const Seq q = seq_of(st, info, s);
+    int s;
+    const Seq q = find_seq(st, info, j, s, first_block);
     const int64_t row0_64 = (int64_t)(j - first_block(q.first, s)) * BLOCK, rows_64 = (int64_t)q.count * group;
     if (rows_64 <= args.rows_most || row0_64 < 0 || row0_64 >= rows_64) return;  // (another kernel's, or no block)
     const int row0 = (int)row0_64, n_rows = (int)min((int64_t)BLOCK, rows_64 - row0_64);
