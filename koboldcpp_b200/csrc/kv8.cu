@@ -142,21 +142,32 @@ __global__ void __launch_bounds__(2 * ST_THREADS, 4) kv8_store_kernel(const Stor
         }
     }
     auto put = [&](int i, const Raw16<T> &y) {
-        float t[16], off = 0.f;
+        unsigned w[4];
+        float off = 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const float v = raw_value(y, e);
-            t[e] = fmaf(v, inv, MAGIC);
-            off = fmaxf(off, fabsf(rest(v, t[e], now)));
+        for (int e = 0; e < 4; e++) {
+            float t[4];
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                const float v = raw_value(y, 4 * e + b);
+                t[b] = fmaf(v, inv, MAGIC);
+                off = fmaxf(off, fabsf(rest(v, t[b], now)));
+            }
+            w[e] = pack4(t[0], t[1], t[2], t[3]);
         }
-        if (!(off < half)) {  // a tie, or beside one (or a scale that is no number: off is 0 or NaN is passed over, half is not above it)
+        if (!(off < half)) {  // a tie, or beside one (or a scale that is 0 or no number)
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const float d = rest(raw_value(y, e), t[e], now);
-                t[e] = inv > 0.f ? mend(t[e], d, d - half, d + half) : MAGIC;
+            for (int e = 0; e < 4; e++) {
+                float t[4];
+#pragma unroll
+                for (int b = 0; b < 4; b++) {
+                    const float v = raw_value(y, 4 * e + b), t0 = fmaf(v, inv, MAGIC), d = rest(v, t0, now);
+                    t[b] = inv > 0.f ? mend(t0, d, d - half, d + half) : MAGIC;
+                }
+                w[e] = pack4(t[0], t[1], t[2], t[3]);
             }
         }
-        reinterpret_cast<uint4 *>(ints + (size_t)used * size)[i] = make_uint4(pack4(t[0], t[1], t[2], t[3]), pack4(t[4], t[5], t[6], t[7]), pack4(t[8], t[9], t[10], t[11]), pack4(t[12], t[13], t[14], t[15]));
+        reinterpret_cast<uint4 *>(ints + (size_t)used * size)[i] = make_uint4(w[0], w[1], w[2], w[3]);
     };
 #pragma unroll
     for (int u = 0; u < KEEP; u++) if (tid + u * ST_THREADS < total) put(tid + u * ST_THREADS, x[u]);
