@@ -153,6 +153,10 @@ enum b200_ext_op {
                                   dst [n, T, 1 or 2]: x, then h (b200_op_norm_chain); op_params: [2] kind1, [3] eps, [4] kind2, [5] y scale (0 reads as 1) */
     B200_EXT_TOKEN_SHIFT = 23, /* src: h [n, T], mu [n, n_mix], seq_info, prev [n, slots]; dst [n, T, n_mix] (b200_op_token_shift) */
     B200_EXT_TIME_MIX_SCAN = 24, /* src: r, k, v, z, w0, u, seq_info, state; op_params: [2] heads, [3] dim (b200_op_time_mix_scan) */
+    B200_EXT_KV8_STORE = 25,   /* src: k, v (f32 rows), seq_info [n_seq, 4], table [entries, rows], pages [record / 4, n_pages] f32 words, [what wrote k and v]; the result is the pages, in place;
+                                  op_params: [2] page_size, [3] kv heads, [4] dim, [5] vdim (b200_op_kv8_store, b200_kv8.h) */
+    B200_EXT_KV8_ATTN = 26,    /* src: q, the store's result, seq_info, table, sink (optional), workspace (zeroed once, for all layers of a stream); op_params: [2] page_size, [3] kv heads,
+                                  [4] dim, [5] vdim, [6] scale, [7] window, [8] keep_first, [9] soft cap, [10] f16 products, [11] most new tokens of a sequence (b200_op_kv8_attn) */
 };
 /* how attention turns scores into weights: SOFTMAX over the visible keys (with the sink in the denominator), or SIGMOID of every score by
  * itself with no normalisation over the keys (a sink has no meaning then) */

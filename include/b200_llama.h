@@ -46,6 +46,8 @@ typedef struct {
     float   embed_scale;             /* the embedding row is multiplied by this (0 reads as 1) */
     float   residual_mult;           /* architectures that scale a sublayer's result before it joins the residual stream (0 reads as 1) */
     float   logit_scale;             /* the logits are multiplied by this (0 reads as 1) */
+    int32_t kv8_page;                /* > 0: softmax attention layers keep keys and values in 8 bits, in pages of so many tokens (16, 32, 64 or 128; include/b200_kv8.h), a
+                                        quarter of the bytes; architectures that cannot refuse it when finalized.  0: f32 rows by cell */
 } b200_llama_params;
 
 enum b200_arch { B200_ARCH_LLAMA = 0, B200_ARCH_GENESUN = 1, B200_ARCH_GALIRAX = 2, B200_ARCH_ZEVOPEL = 3, B200_ARCH_MEDODRA = 4, B200_ARCH_MAFUZEN = 5, B200_ARCH_TUGEZEN = 6 };

@@ -22,6 +22,7 @@ def main(argv=None) -> int:
     g.add_argument("--top-p", type=float, default=1.0)
     g.add_argument("--seed", type=int, default=0)
     g.add_argument("--n-ctx", type=int, default=0, help="cache cells (default: what the prompts need)")
+    g.add_argument("--kv8-page", type=int, default=0, choices=[0, 16, 32, 64, 128], help="keep attention caches in 8 bits, in pages of so many tokens (0: f32 rows)")
     a = ap.parse_args(argv)
 
     from . import build as _build
@@ -31,7 +32,7 @@ def main(argv=None) -> int:
 
     prompts = [[int(t) for t in p.split(",") if t.strip()] for p in a.prompt]
     need = sum(len(p) + a.max_new_tokens for p in prompts)
-    model = load_model(a.model, dtype=a.dtype, n_ctx=a.n_ctx or need, n_seq_max=len(prompts), max_batch=min(max(need, 1), 4096))
+    model = load_model(a.model, dtype=a.dtype, n_ctx=a.n_ctx or need, n_seq_max=len(prompts), max_batch=min(max(need, 1), 4096), kv8_page=a.kv8_page)
     reqs = [Request(p, a.max_new_tokens, Sampler(a.temperature, a.top_k, a.top_p, a.seed + i)) for i, p in enumerate(prompts)]
     for p, out in zip(prompts, Engine(model).generate(reqs)):
         print(json.dumps({"prompt": p, "tokens": out}))

@@ -13,6 +13,7 @@
 
 #include "../../include/b200_ggml_backend.h"
 #include "../../include/b200_ggml_ops.h"
+#include "../../include/b200_kv8.h"
 
 // ---- dry run (B200_DRY_RUN=<n devices>): host-side validation of the drop-in boundary on a machine WITHOUT a GPU.
 // Every CUDA runtime call of the backend glue (buffers, devices, events, streams, copies) is routed through these wrappers; with
@@ -220,6 +221,8 @@ void graph_exec_free(GraphExec *g);
 cudaStream_t graph_exec_stream(GraphExec *g);
 enum ggml_status graph_exec_compute(GraphExec *g, ggml_cgraph *cgraph);
 bool op_supported(int device, const ggml_tensor *op);
+
+int kv8_attn_launches(const b200_kv8_attn_args *a);  // kernels of b200_op_kv8_attn (kv8_attn.cu)
 
 extern bool g_use_graphs, g_use_fusion;
 extern int64_t g_stat_launches, g_stat_replays, g_stat_captures;

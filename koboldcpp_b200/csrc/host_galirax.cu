@@ -4,7 +4,7 @@
 // A Galirax model is a list of layers, run in an order that may repeat a stretch of them (every run has its own cache rows or
 // recurrent state, b200_llama_set_layer_order).  A layer is parallel: h = LayerNorm(x) with weight and bias feeds both the mixer
 // and the feed-forward, and x <- x + (mixer(h) + ff(h)).  Mixers (b200_layer_params):
-//   * attention: heads query heads over kv_heads key / value heads, optional biases and an RMS norm over the whole q / k projection,
+//   * attention (over f32 rows by cell, or with hp.kv8_page over pages in 8 bits): heads query heads over kv_heads key / value heads, optional biases and an RMS norm over the whole q / k projection,
 //     interleaved rotation by a frequency table (band-wise scaled or plain), a per-head sink in the softmax denominator, and an
 //     optional sliding window that keeps the first positions visible;
 //   * lightning: linear attention with silu on q, k, v, a fixed decay per head, an RMS norm over all heads and a sigmoid gate.
@@ -27,6 +27,7 @@ struct GxLayer {
 };
 struct GxRun {
     ggml_tensor *k_cache = nullptr, *v_cache = nullptr;  // attention: [kv_heads * dim, n_ctx], [kv_heads * vdim, n_ctx] f32
+    ggml_tensor *pages = nullptr;                         // or, with hp.kv8_page, pages of keys and values in 8 bits
     ggml_tensor *state = nullptr;                         // lightning: [heads * vdim * dim, n_seq_max] f32
 };
 struct GxData {
@@ -189,7 +190,10 @@ int gx_finalize(b200_llama *m) {
         const b200_layer_params &lp = m->layer_hp[(size_t)m->run_layer[r]];
         GxRun &R = g->runs[r];
         const std::string pre = "run" + std::to_string(r) + ".";
-        if (lp.mixer == B200_MIXER_ATTENTION) {
+        if (lp.mixer == B200_MIXER_ATTENTION && hp.kv8_page > 0) {
+            const int rc = new_kv8_pool(m, (pre + "pages").c_str(), lp, &R.pages);
+            if (rc != B200_OK) return rc;
+        } else if (lp.mixer == B200_MIXER_ATTENTION) {
             R.k_cache = new_device_tensor(m, (pre + "k").c_str(), GGML_TYPE_F32, (int64_t)lp.kv_heads * lp.dim, hp.n_ctx, true);
             R.v_cache = new_device_tensor(m, (pre + "v").c_str(), GGML_TYPE_F32, (int64_t)lp.kv_heads * lp.vdim, hp.n_ctx, true);
             LL_REQUIRE(R.k_cache && R.v_cache, B200_ERR_NOMEM, "b200_llama_finalize: out of device memory for the cache of run %zu", r);
@@ -255,20 +259,33 @@ int gx_build(b200_llama *m, const BatchShape &bs) {
         ggml_tensor *y;  // the mixer's result, [W, T]
         if (lp.mixer == B200_MIXER_ATTENTION) {
             const int64_t G = lp.kv_heads;
-            ggml_tensor *kc_all = b.view_2d(R.k_cache, G * D, hp.n_ctx, R.k_cache->nb[1], 0), *vc_all = b.view_2d(R.v_cache, G * V, hp.n_ctx, R.v_cache->nb[1], 0);
+            const bool paged = hp.kv8_page > 0;  // the normed and rotated rows then stay beside one another, on their way to the pages
+            ggml_tensor *kc_all = paged ? b.alloc_result(GGML_TYPE_F32, G * D, T) : b.view_2d(R.k_cache, G * D, hp.n_ctx, R.k_cache->nb[1], 0);
+            ggml_tensor *vc_all = paged ? b.alloc_result(GGML_TYPE_F32, G * V, T) : b.view_2d(R.v_cache, G * V, hp.n_ctx, R.v_cache->nb[1], 0);
             ggml_tensor *q = part("mix.q");
             ggml_tensor *qo = part("mix.q");  // the store rewrites q in place
-            b.ext(qo, B200_EXT_QKV_STORE, {q, part("mix.k"), part("mix.v"), L.qkvec, pos, L.freqs, cells, kc_all, vc_all});
+            b.ext(qo, B200_EXT_QKV_STORE, {q, part("mix.k"), part("mix.v"), L.qkvec, pos, L.freqs, paged ? input_view(*m->pages.ids, T) : cells, kc_all, vc_all});
             qo->op_params[2] = (int32_t)D; qo->op_params[3] = (int32_t)V; qo->op_params[4] = lp.rope_dims; Builder::set_f(qo, 5, eps);
             qo->op_params[6] = lp.qkv_bias ? 1 : 0; qo->op_params[7] = lp.qk_norm ? 1 : 0;
             ggml_tensor *o = b.alloc_result(GGML_TYPE_F32, H * V, T);
-            b.ext(o, B200_EXT_SINK_ATTN, {qo, b.view_2d(R.k_cache, G * D, bs.n_kv, R.k_cache->nb[1], 0), b.view_2d(R.v_cache, G * V, bs.n_kv, R.v_cache->nb[1], 0), L.sink, tok_seq, pos,
-                                           cell_seq, cell_pos});
-            o->op_params[2] = (int32_t)D; Builder::set_f(o, 3, lp.scale); o->op_params[4] = lp.window; o->op_params[5] = lp.keep_first;
             // bf16 weights: the attention products of a prompt batch may be bf16 as well (B200_ATTN_F32=1 keeps them in f32)
             static const bool attn_f32 = getenv("B200_ATTN_F32") != nullptr;
-            o->op_params[6] = L.proj1->type == GGML_TYPE_BF16 && !attn_f32;
-            o->op_params[7] = (int32_t)V;
+            const bool rounded = L.proj1->type == GGML_TYPE_BF16 && !attn_f32;
+            if (paged) {
+                const int32_t page = m->pages.page_size;
+                ggml_tensor *info = input_view(*m->pages.info, bs.n_seq, 4), *pool = b.view_2d(R.pages, R.pages->ne[0], R.pages->ne[1], R.pages->nb[1], 0);
+                b.ext(pool, B200_EXT_KV8_STORE, {kc_all, vc_all, info, m->pages.table, R.pages, qo});
+                b.ext(o, B200_EXT_KV8_ATTN, {qo, pool, info, m->pages.table, L.sink, m->pages.attn_ws});
+                for (ggml_tensor *t : {pool, o}) { t->op_params[2] = page; t->op_params[3] = (int32_t)G; t->op_params[4] = (int32_t)D; t->op_params[5] = (int32_t)V; }
+                Builder::set_f(o, 6, lp.scale); o->op_params[7] = lp.window; o->op_params[8] = lp.keep_first; Builder::set_f(o, 9, 0.0f);
+                o->op_params[10] = rounded; o->op_params[11] = (int32_t)T - (bs.n_seq - 1);  // (every sequence of a step has a token at least)
+            } else {
+                b.ext(o, B200_EXT_SINK_ATTN, {qo, b.view_2d(R.k_cache, G * D, bs.n_kv, R.k_cache->nb[1], 0), b.view_2d(R.v_cache, G * V, bs.n_kv, R.v_cache->nb[1], 0), L.sink, tok_seq, pos,
+                                               cell_seq, cell_pos});
+                o->op_params[2] = (int32_t)D; Builder::set_f(o, 3, lp.scale); o->op_params[4] = lp.window; o->op_params[5] = lp.keep_first;
+                o->op_params[6] = rounded;
+                o->op_params[7] = (int32_t)V;
+            }
             y = b.mul_mat(L.wo, o);
         } else {
             ggml_tensor *o = b.alloc_result(GGML_TYPE_F32, H * V, T);
@@ -316,7 +333,7 @@ int gx_build(b200_llama *m, const BatchShape &bs) {
     return B200_OK;
 }
 
-const Arch k_galirax = {"galirax", gx_place_tensor, gx_finalize, nullptr, gx_build, nullptr};
+const Arch k_galirax = {"galirax", gx_place_tensor, gx_finalize, nullptr, gx_build, nullptr, true};
 
 }  // namespace
 

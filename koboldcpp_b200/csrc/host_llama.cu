@@ -113,6 +113,22 @@ ggml_tensor *b200::host::new_device_tensor(b200_llama *m, const char *name, int 
     return t;
 }
 
+int b200::host::new_kv8_pool(b200_llama *m, const char *name, const b200_layer_params &lp, ggml_tensor **pool) {
+    b200_llama::Pages &P = m->pages;
+    const size_t record = b200_kv8_page_bytes(P.page_size, lp.kv_heads, lp.dim, lp.vdim);
+    LL_REQUIRE(record > 0, B200_ERR_UNSUPPORTED, "b200_llama_finalize: %s: %d heads of %d and %d values (multiples of 16, at most 256) over pages of %d tokens", name, lp.kv_heads, lp.dim, lp.vdim,
+               P.page_size);
+    *pool = new_device_tensor(m, name, GGML_TYPE_F32, (int64_t)(record / 4), P.n_pages, true);
+    b200_kv8_attn_args a = {};
+    a.cache = {nullptr, P.n_pages, P.page_size, lp.kv_heads, lp.dim, lp.vdim, 0};
+    a.f16_products = 1;  // (wants more room than exact products)
+    const size_t ws = (b200_kv8_attn_workspace_bytes(&a) + 3) / 4;
+    if (*pool && (!P.attn_ws || (size_t)P.attn_ws->ne[0] < ws)) P.attn_ws = new_device_tensor(m, "kv8.attn", GGML_TYPE_F32, (int64_t)ws, 1, true);
+    LL_REQUIRE(*pool && P.attn_ws, B200_ERR_NOMEM, "b200_llama_finalize: out of device memory for %s", name);
+    m->kv_bytes += (int64_t)nbytes(*pool);
+    return B200_OK;
+}
+
 int b200::host::upload_tensor(b200_llama *m, const char *name, int type, int64_t ne0, int64_t ne1, int64_t ne2, const void *data) {
     const TypeTraits tt = type_traits(type);
     LL_REQUIRE(tt.blck > 0 && ne0 > 0 && ne1 > 0 && ne2 > 0 && ne0 % tt.blck == 0, B200_ERR_INVALID, "b200_llama_set_tensor: bad type/shape for %s", name);
@@ -186,14 +202,44 @@ void make_batch_inputs(b200_llama *m, Bump &bp) {
     mk(&m->inp_cell_seq, hp.n_ctx, 1, "inp_cell_seq");
     mk(&m->inp_cell_pos, hp.n_ctx, 1, "inp_cell_pos");
     mk(&m->inp_seq_info, hp.n_seq_max, 4, "inp_seq_info");
+    if (hp.kv8_page > 0) {
+        mk(&m->pages.inp_rows, hp.n_seq_max, 1, "inp_kv8_rows");
+        mk(&m->pages.inp_new, hp.n_seq_max, 1, "inp_kv8_new");
+    }
+}
+
+// What the paged 8-bit cache keeps beside the layers' pools.  Every sequence may leave part of its last page empty, so there is a page more for each than n_ctx
+// tokens fill: as many tokens as there are cells always have room.
+int make_pages(b200_llama *m) {
+    const b200_llama_params &hp = m->hp;
+    b200_llama::Pages &P = m->pages;
+    LL_REQUIRE(hp.kv8_page == 16 || hp.kv8_page == 32 || hp.kv8_page == 64 || hp.kv8_page == 128, B200_ERR_UNSUPPORTED, "b200_llama_finalize: kv8_page %d (16, 32, 64 or 128)", hp.kv8_page);
+    LL_REQUIRE(m->arch->pages, B200_ERR_UNSUPPORTED, "b200_llama_finalize: architecture %s has no paged 8-bit cache", m->arch->name);
+    LL_REQUIRE(hp.n_seq_max <= B200_KV8_MAX_SEQ, B200_ERR_UNSUPPORTED, "b200_llama_finalize: %d sequences over a paged cache, at most %d", hp.n_seq_max, B200_KV8_MAX_SEQ);
+    P.page_size = hp.kv8_page;
+    P.n_pages = hp.n_ctx / hp.kv8_page + hp.n_seq_max;
+    P.table = new_device_tensor(m, "kv8.table", GGML_TYPE_I32, hp.n_ctx / hp.kv8_page, hp.n_seq_max, true);
+    P.len = new_device_tensor(m, "kv8.len", GGML_TYPE_I32, hp.n_seq_max, 1, true);
+    P.refs = new_device_tensor(m, "kv8.refs", GGML_TYPE_I32, P.n_pages, 1, true);
+    P.info = new_device_tensor(m, "kv8.info", GGML_TYPE_I32, hp.n_seq_max, 4, true);
+    P.ids = new_device_tensor(m, "kv8.ids", GGML_TYPE_I32, hp.n_seq_max > m->max_batch ? hp.n_seq_max : m->max_batch, 1, true);
+    P.grow_ws = new_device_tensor(m, "kv8.grow", GGML_TYPE_I32, (int64_t)(b200_kv8_grow_workspace_bytes(hp.n_seq_max) + 3) / 4, 1, true);
+    LL_REQUIRE(P.table && P.len && P.refs && P.info && P.ids && P.grow_ws, B200_ERR_NOMEM, "b200_llama_finalize: out of device memory for the tables of the paged cache");
+    std::vector<int32_t> v((size_t)(P.table->ne[0] * P.table->ne[1]), -1);
+    P.table->buffer->iface.set_tensor(P.table->buffer, P.table, v.data(), 0, nbytes(P.table));
+    v.resize((size_t)P.ids->ne[0]);
+    for (size_t i = 0; i < v.size(); i++) v[i] = (int32_t)i;
+    P.ids->buffer->iface.set_tensor(P.ids->buffer, P.ids, v.data(), 0, nbytes(P.ids));
+    return B200_OK;
 }
 
 int finalize_arch(b200_llama *m, int32_t max_batch) {
     const b200_llama_params &hp = m->hp;
     LL_REQUIRE(hp.n_ctx % KV_PAD == 0, B200_ERR_INVALID, "b200_llama_finalize: n_ctx must be a multiple of %d", KV_PAD);
-    int rc = m->arch->finalize(m);
-    if (rc != B200_OK) return rc;
     m->max_batch = max_batch;
+    int rc = hp.kv8_page > 0 ? make_pages(m) : B200_OK;
+    if (rc == B200_OK) rc = m->arch->finalize(m);
+    if (rc != B200_OK) return rc;
     m->cache.init(hp.n_ctx, hp.n_seq_max);
     // size the regions: build the largest graph over fake addresses and read how far each bump allocator went
     Bump fake;
@@ -223,7 +269,7 @@ int finalize_arch(b200_llama *m, int32_t max_batch) {
     }
     m->graph.n_nodes = 0;
     m->g_shape = {0, 0, 0, 0};
-    const size_t pin_need = 4 * ((size_t)5 * max_batch + 2 * (size_t)hp.n_ctx + 4 * (size_t)hp.n_seq_max) + 256;
+    const size_t pin_need = 4 * ((size_t)5 * max_batch + 2 * (size_t)hp.n_ctx + 6 * (size_t)hp.n_seq_max) + 256;
     LL_REQUIRE(cudaHostAlloc((void **)&m->pin, pin_need, cudaHostAllocDefault) == cudaSuccess, B200_ERR_NOMEM, "b200_llama_finalize: cannot pin %zu bytes of input staging", pin_need);
     m->pin_bytes = pin_need;
     m->finalized = true;
@@ -241,6 +287,11 @@ extern "C" int b200_llama_seq_open(b200_llama *m, int32_t *seq_id) {
 }
 extern "C" int b200_llama_seq_close(b200_llama *m, int32_t seq_id) {
     LL_REQUIRE(m && m->finalized && m->arch && m->cache.is_open(seq_id), B200_ERR_INVALID, "b200_llama_seq_close: sequence %d is not open", seq_id);
+    if (m->hp.kv8_page > 0) {  // its pages are free behind the last step
+        const b200_kv8_map map = m->pages.map();
+        const int rc = b200_op_kv8_cut(&map, (const int32_t *)m->pages.ids->data + seq_id, nullptr, 1, (cudaStream_t)ggml_backend_b200_get_stream(m->be));
+        if (rc != B200_OK) return rc;
+    }
     m->cache.close_seq(seq_id);
     return B200_OK;
 }
@@ -305,14 +356,25 @@ extern "C" int b200_llama_decode_batch(b200_llama *m, const int32_t *tokens, con
     send(&m->inp_cell_seq, kc.cell_seq.data(), (size_t)n_kv);
     send(&m->inp_cell_pos, kc.cell_pos.data(), (size_t)n_kv);
     send(&m->inp_seq_info, info.data(), (size_t)4 * n_seq);
+    if (hp.kv8_page > 0) {
+        send(&m->pages.inp_rows, run_seq.data(), (size_t)n_seq);
+        send(&m->pages.inp_new, run_count.data(), (size_t)n_seq);
+    }
     if (!m->in_ev) LL_REQUIRE(cudaEventCreateWithFlags(&m->in_ev, cudaEventDisableTiming) == cudaSuccess, B200_ERR_CUDA, "b200_llama_decode_batch: cudaEventCreate failed");
     if (cudaEventRecord(m->in_ev, (cudaStream_t)ggml_backend_b200_get_stream(be)) == cudaSuccess) m->in_ev_pending = true;
     else { cudaGetLastError(); cudaStreamSynchronize((cudaStream_t)ggml_backend_b200_get_stream(be)); }
     int64_t l0 = 0, l1 = 0;
+    if (hp.kv8_page > 0) {  // room for the step's tokens; no page is shared, so nothing is copied
+        const b200_llama::Pages &P = m->pages;
+        const b200_kv8_map map = P.map();
+        const int rc = b200_op_kv8_grow(&map, nullptr, 0, (const int32_t *)P.inp_rows.data, (const int32_t *)P.inp_new.data, n_seq, (int32_t *)P.info->data, nullptr, P.grow_ws->data,
+                                        nbytes(P.grow_ws), (cudaStream_t)ggml_backend_b200_get_stream(be));
+        if (rc != B200_OK) return rc;
+    }
     ggml_backend_b200_get_stats(&l0, nullptr, nullptr);
     const ggml_status st = be->iface.graph_compute(be, &m->graph);
     ggml_backend_b200_get_stats(&l1, nullptr, nullptr);
-    m->last_launches = l1 - l0;
+    m->last_launches = l1 - l0 + (hp.kv8_page > 0 ? 1 : 0);
     m->t_calls++;
     LL_REQUIRE(st == GGML_STATUS_SUCCESS, B200_ERR_CUDA, "b200_llama_decode_batch: graph_compute failed (%d)", (int)st);
     if (n_out > 0) be->iface.get_tensor_async(be, m->logits_t, logits, 0, 4 * (size_t)hp.n_vocab * (size_t)n_out);

@@ -258,6 +258,7 @@ struct Arch {
     size_t (*compute_bytes)(b200_llama *m, int32_t max_batch);
     int (*build)(b200_llama *m, const BatchShape &bs);
     void (*release)(b200_llama *m);
+    bool pages = false;  // its softmax attention can keep keys and values in the paged 8-bit cache (hp.kv8_page)
 };
 const Arch *find_arch(int32_t id);
 const Arch *genesun_arch();
@@ -329,6 +330,17 @@ struct b200_llama {
     b200::host::BatchShape g_shape = {0, 0, 0, 0};
     static constexpr int N_REGIONS = 4;      // stacked layer results | layers with even index | odd index | output head
     b200::host::Bump regions[N_REGIONS];
+    // the paged 8-bit cache (hp.kv8_page > 0): which pages a sequence holds, kept on the device by b200_op_kv8_grow / _cut and one for all layers; a step's rows and
+    // counts are inputs, what the step is (seq_info with tokens held) is the grow call's result
+    struct Pages {
+        int32_t n_pages = 0;
+        ggml_tensor *table = nullptr, *len = nullptr, *refs = nullptr, *ids = nullptr, *info = nullptr, *grow_ws = nullptr, *attn_ws = nullptr;
+        ggml_tensor inp_rows, inp_new;
+        b200_kv8_map map() const {
+            return {(int32_t *)table->data, (int64_t)table->ne[0], (int32_t *)len->data, (int32_t *)refs->data, (int32_t)table->ne[1], n_pages, page_size, 0};
+        }
+        int32_t page_size = 0;
+    } pages;
     bool measuring = false;                  // the builder runs over fake addresses to size the regions
     std::vector<int32_t> st_cells, st_pos, st_seq, st_out, st_info;  // host staging of a batch step
 };
@@ -379,6 +391,8 @@ inline ggml_tensor *find_w(b200_llama *m, const std::string &name) {
 int upload_tensor(b200_llama *m, const char *name, int type, int64_t ne0, int64_t ne1, int64_t ne2, const void *data);
 // a zero-initialised device tensor owned by the model (caches, recurrent state)
 ggml_tensor *new_device_tensor(b200_llama *m, const char *name, int type, int64_t ne0, int64_t ne1, bool clear);
+// a layer's pool of pages (hp.kv8_page > 0), and room for the workspace of its attention
+int new_kv8_pool(b200_llama *m, const char *name, const b200_layer_params &lp, ggml_tensor **pool);
 
 }  // namespace host
 }  // namespace b200

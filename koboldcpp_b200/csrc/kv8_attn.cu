@@ -640,6 +640,11 @@ static int check_attn(const b200_kv8_attn_args *a, const char *who) {
 constexpr int ROWS_MOST = 64;
 static bool one_term(const b200_kv8_attn_args *a) { return a->type != B200_TYPE_F32 || a->f16_products != 0; }
 
+// most query rows a kv head of one sequence, and whether that makes some of them the prompt kernel's
+static int64_t longest_rows(const b200_kv8_attn_args *a) { return (int64_t)(a->max_new > 0 && a->max_new < a->n_tokens ? a->max_new : a->n_tokens) * (a->n_head / a->cache.n_head_kv); }
+static bool has_prompts(const b200_kv8_attn_args *a) {
+    return attn_class(a->cache) <= 128 && longest_rows(a) > ROWS_MOST && (int64_t)a->n_tokens * (a->n_head / a->cache.n_head_kv) < (1ll << 30);
+}
 // 256 rows a CTA where that many CTAs fill the device, else 128
 static int launch_prompt(const AttnArgs &args, bool vec, int k, bool one, long long limit, cudaStream_t st) {
     const bool two = (int64_t)args.a.n_tokens * args.group * args.a.cache.n_head_kv >= (int64_t)sm_count() * 2 * KT_ROWS;
@@ -652,6 +657,9 @@ static int launch_prompt(const AttnArgs &args, bool vec, int k, bool one, long l
 }
 
 }  // namespace kv8
+
+int kv8_attn_launches(const b200_kv8_attn_args *a) { return a->n_tokens == 0 || a->n_seq == 0 ? 0 : kv8::has_prompts(a) ? 2 : 1; }
+
 }  // namespace b200
 
 using namespace b200;
@@ -678,8 +686,7 @@ int b200_op_kv8_attn(const b200_kv8_attn_args *a, void *workspace, size_t worksp
     const cudaStream_t st = (cudaStream_t)stream;
     const int k = attn_class(c);
     const bool vec = rows_aligned(a->q, a->q_stride, a->type) && rows_aligned(a->dst, a->dst_stride, a->type);
-    const int64_t longest = (int64_t)(a->max_new > 0 && a->max_new < a->n_tokens ? a->max_new : a->n_tokens) * args.group;  // query rows a kv head of one sequence, at most
-    if (k <= 128 && longest > ROWS_MOST && (int64_t)a->n_tokens * args.group < (1ll << 30)) {
+    if (has_prompts(a)) {
         args.rows_most = ROWS_MOST;
         const int rc2 = launch_prompt(args, vec, k, one_term(a), PAIR_WAIT_LIMIT, st);
         if (rc2 != B200_OK) return rc2;

@@ -82,13 +82,14 @@ def run_order(n_layer: int, loop: dict | None) -> list[int]:
     return list(range(a)) + list(range(a, b)) * k + list(range(b, n_layer))
 
 
-def build(config: dict, tensors, dtype: str = "bfloat16", n_ctx: int = 4096, n_seq_max: int = 16, max_batch: int = 512, device: int = 0) -> SequenceModel:
-    """config: the parsed config.json; tensors: name -> (dtype, shape, raw bytes)."""
+def build(config: dict, tensors, dtype: str = "bfloat16", n_ctx: int = 4096, n_seq_max: int = 16, max_batch: int = 512, device: int = 0,
+          kv8_page: int = 0) -> SequenceModel:
+    """config: the parsed config.json; tensors: name -> (dtype, shape, raw bytes); kv8_page: 0 for f32 caches, or the tokens of a page of the 8-bit cache."""
     if dtype not in ("bfloat16", "float32"):
         raise B200Error(f"dtype {dtype!r}: bfloat16 or float32")
     layers = [layer_params(x) for x in config["layers"]]
     model = SequenceModel(ARCH_GALIRAX, int(config["width"]), int(config["vocab"]), layers, float(config["norm"]["eps"]), n_ctx, n_seq_max, max_batch, device,
-                          logit_softcap=float(config.get("logit_softcap") or 0.0), order=run_order(len(layers), config.get("loop")))
+                          logit_softcap=float(config.get("logit_softcap") or 0.0), order=run_order(len(layers), config.get("loop")), kv8_page=kv8_page)
     matrix_type = BF16 if dtype == "bfloat16" else F32
     for name, (dt, shape, raw) in tensors.items():
         if name.endswith(".mlp.router"):  # the router runs in f32 in both modes

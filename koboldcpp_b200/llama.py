@@ -20,7 +20,7 @@ class LlamaParams(C.Structure):
                 ("rms_eps", C.c_float), ("rope_freq_base", C.c_float), ("rope_freq_scale", C.c_float),
                 ("main_device", C.c_int32), ("n_split_devices", C.c_int32), ("tensor_split", C.c_float * 16),
                 ("tp_rank", C.c_int32), ("tp_world", C.c_int32), ("arch", C.c_int32), ("n_seq_max", C.c_int32), ("logit_softcap", C.c_float),
-                ("embed_scale", C.c_float), ("residual_mult", C.c_float), ("logit_scale", C.c_float)]
+                ("embed_scale", C.c_float), ("residual_mult", C.c_float), ("logit_scale", C.c_float), ("kv8_page", C.c_int32)]
 
 
 class LayerParams(C.Structure):

@@ -190,3 +190,11 @@ def test_reference_pages():
     assert m.refs.tolist() == [2, 0, 1, 1, 1, 0, 0, 0]
     assert m.compact() == (4, [(4, 1)]) and m.table[3, :2].tolist() == [0, 1] and m.table[1, :2].tolist() == [0, 3]
     assert m.grow([0, 0, 1], [70, 1, 400])[1] == 3  # beyond the table; named twice; beyond the table
+
+
+def test_other_architectures_refuse_pages(tmp_path):
+    import json
+    from koboldcpp_b200 import models
+    (tmp_path / "config.json").write_text(json.dumps({"architecture": "Zevopel"}))
+    with pytest.raises(L.B200Error, match="8-bit pages"):
+        models.load_model(tmp_path, kv8_page=16)
