@@ -576,18 +576,29 @@ __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kern
                 for (int off = 1; off < LANES; off *= 2) total += __shfl_xor_sync(0xffffffffu, total, off);
                 if (j == 0) share_s[r] = r < n_rows ? finish(r, top, total) : 0.f;
                 __syncthreads();
-                for (int i = tid; i < n_rows << quads_shift; i += RW_THREADS) {
-                    const int r = i >> quads_shift, d = (i & ((1 << quads_shift) - 1)) * 4;
-                    if (d >= c.vdim) continue;
-                    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-                    for (int k = 0; k < parts; k++) {
-                        const float4 z = __ldcg(reinterpret_cast<const float4 *>(part_at(k) + 2 * R + r * C + d));
-                        const float f = fac[k * R + r];
-                        y = make_float4(y.x + z.x * f, y.y + z.y * f, y.z + z.z * f, y.w + z.w * f);
+                // all of a thread's pieces side by side: a part's loads then take their way to L2 and back once
+                constexpr int PIECES_EACH = (R * C / 4 + RW_THREADS - 1) / RW_THREADS;
+                float4 y[PIECES_EACH];
+#pragma unroll
+                for (int i = 0; i < PIECES_EACH; i++) y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll(PIECES_EACH >= 8 ? 1 : 8 / PIECES_EACH)
+                for (int k = 0; k < parts; k++) {
+                    const float *at = part_at(k) + 2 * R, *f = fac + k * R;
+#pragma unroll
+                    for (int i = 0; i < PIECES_EACH; i++) {
+                        const int e = tid + i * RW_THREADS, row = e >> quads_shift, d = (e & ((1 << quads_shift) - 1)) * 4;
+                        if (row >= n_rows || d >= c.vdim) continue;
+                        const float4 z = __ldcg(reinterpret_cast<const float4 *>(at + row * C + d));
+                        const float w = f[row];
+                        y[i] = make_float4(y[i].x + z.x * w, y[i].y + z.y * w, y[i].z + z.z * w, y[i].w + z.w * w);
                     }
-                    const float f = share_s[r];
-                    put(r, d, make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
+                }
+#pragma unroll
+                for (int i = 0; i < PIECES_EACH; i++) {
+                    const int e = tid + i * RW_THREADS, row = e >> quads_shift, d = (e & ((1 << quads_shift) - 1)) * 4;
+                    if (row >= n_rows || d >= c.vdim) continue;
+                    const float w = share_s[row];
+                    put(row, d, make_float4(y[i].x * w, y[i].y * w, y[i].z * w, y[i].w * w));
                 }
             }
         }
