@@ -1,4 +1,5 @@
 // kv8_attn.cu -- attention over the paged 8-bit cache (include/b200_kv8.h: b200_op_kv8_attn).
+#include <algorithm>
 #include <cfloat>
 #include <type_traits>
 
@@ -95,6 +96,7 @@ struct AttnArgs {
     float *partials;  // two per CTA
     int group;        // query heads per kv head
     unsigned group_div;  // ceil(2^32 / group): __umulhi(x, group_div) = x / group for x < 2^32 / group
+    int splits;       // a prompt's block of rows may be shared by so many CTAs, each with a stretch of its tiles
     int rows_most;    // sequences with more query rows a kv head (tokens times group) are the prompt kernel's; negative: there is none
 };
 
@@ -619,7 +621,8 @@ static int rows_grid(const b200_kv8_cache &c) {
     const int k = attn_class(c);
     return sm_count() * (k == 64 ? rw_per_sm<64>() : k == 128 ? rw_per_sm<128>() : rw_per_sm<256>());
 }
-static size_t rows_counter_bytes(int grid) { return ((size_t)grid * 4 + 255) / 256 * 256; }
+// counters in front of the partial results: as many for heads of all sizes, so that none lies where a call before left partial results
+static size_t rows_counter_bytes() { return ((size_t)sm_count() * rw_per_sm<64>() * 4 + 255) / 256 * 256; }
 template <int C, int TERMS>
 static int launch_rows(const AttnArgs &args, bool vec, cudaStream_t st) {
     static bool done[16] = {};  // cudaFuncSetAttribute is per device
@@ -639,6 +642,7 @@ static int check_attn(const b200_kv8_attn_args *a, const char *who) {
     if (rc != B200_OK) return rc;
     const b200_kv8_cache &c = a->cache;
     OPX_REQUIRE(a->n_head > 0 && a->n_head % c.n_head_kv == 0, B200_ERR_INVALID, "%s: %d query heads over %d kv heads", who, a->n_head, c.n_head_kv);
+    OPX_REQUIRE((int64_t)a->n_tokens * a->n_head <= INT32_MAX, B200_ERR_UNSUPPORTED, "%s: %d tokens of %d query heads", who, a->n_tokens, a->n_head);
     OPX_REQUIRE(a->window >= 0 && a->keep_first >= 0, B200_ERR_INVALID, "%s: window %d, keep_first %d", who, a->window, a->keep_first);
     OPX_REQUIRE(a->scale == a->scale && a->softcap >= 0.0f && a->softcap <= FLT_MAX, B200_ERR_INVALID, "%s: scale or softcap", who);
     if (a->n_tokens == 0 || a->n_seq == 0) return B200_OK;
@@ -647,18 +651,34 @@ static int check_attn(const b200_kv8_attn_args *a, const char *who) {
                 (long long)a->q_stride, (long long)a->dst_stride);
     return B200_OK;
 }
-// Sequences of more query rows a kv head than this go to the tensor cores' kernel, if the heads are of its sizes.
-constexpr int ROWS_MOST = 64;
+// Where a step has PROMPT_ROWS query rows over all heads (rows of two terms count twice), its sequences of more than ROWS_MOST rows a kv head are the prompt kernel's, if the
+// heads are of its sizes.  What a call costs without a past, behind 1000 and behind 8000 tokens, heads of 128 (us, this file's other kernel : the prompt kernel's launches):
+//   bf16, 1 sequence, 32 query heads over 8:   64 tokens  8.6 : 19.5, 22.4 : 28.9,  71 :  47   128 tokens 10 : 21, 32 : 31, 130 :  67   256 tokens 22 : 23, 52 : 35, 246 :  90
+//   f32, the same:                             33 tokens  7.6 : 21.0, 20.4 : 30.0,  67 :  48    64 tokens  9 : 21, 29 : 30, 116 :  53   128 tokens 13 : 22, 44 : 33, 219 :  77
+//   bf16, 4 sequences:                         17 tokens  9.0 : 18.6, 23.3 : 30.2,  88 :  74    33 tokens  9 : 20, 34 : 34, 146 : 102    64 tokens 14 : 19, 49 : 34, 240 : 144
+//   bf16, 16 sequences:                         5 tokens  9.3 : 18.9, 29.7 : 36.8, 136 : 192     9 tokens 10 : 18, 38 : 35, 195 : 183    17 tokens 15 : 18, 56 : 36, 310 : 185
+// (how long the past is, only the device knows; 5 tokens of 4 heads are 20 rows, 9 are 36)
+constexpr int ROWS_MOST = 32, PROMPT_ROWS = 4096;
 static bool one_term(const b200_kv8_attn_args *a) { return a->type != B200_TYPE_F32 || a->f16_products != 0; }
 
-// most query rows a kv head of one sequence, and whether that makes some of them the prompt kernel's
-static int64_t longest_rows(const b200_kv8_attn_args *a) { return (int64_t)(a->max_new > 0 && a->max_new < a->n_tokens ? a->max_new : a->n_tokens) * (a->n_head / a->cache.n_head_kv); }
+// whether some sequences of a step can be the prompt kernel's (which sequences have how many tokens is known on the device only)
 static bool has_prompts(const b200_kv8_attn_args *a) {
-    return attn_class(a->cache) <= 128 && longest_rows(a) > ROWS_MOST && (int64_t)a->n_tokens * (a->n_head / a->cache.n_head_kv) < (1ll << 30);
+    const int64_t group = a->n_head / a->cache.n_head_kv, longest = a->max_new > 0 && a->max_new < a->n_tokens ? a->max_new : a->n_tokens;
+    return attn_class(a->cache) <= 128 && longest * group > ROWS_MOST && (int64_t)a->n_tokens * a->n_head * (one_term(a) ? 1 : 2) >= PROMPT_ROWS;
 }
-// 256 rows a CTA where that many CTAs fill the device, else 128
-static int launch_prompt(const AttnArgs &args, bool vec, int k, bool one, long long limit, cudaStream_t st) {
-    const bool two = (int64_t)args.a.n_tokens * args.group * args.a.cache.n_head_kv >= (int64_t)sm_count() * 2 * KT_ROWS;
+// The prompt kernel's plan.  256 rows a CTA (keys are converted once for all of them) where blocks of 128 would be more than the SMs, sequences being of one length for all that is
+// known here: 32 query heads over 8, bf16, behind 1000: 4 sequences of 256 tokens 67.0 us with 128 rows, 45.0 with 256; of 128 tokens 34.9 and 42.0.  Where blocks are fewer than
+// the SMs, several CTAs share a block's tiles: one sequence of 128 tokens behind 8000 took 129 us with one CTA a block.
+struct PromptPlan { bool two; int splits; };
+static PromptPlan prompt_plan(const b200_kv8_attn_args *a) {
+    const int64_t rows = (int64_t)a->n_tokens * (a->n_head / a->cache.n_head_kv), each = (rows + a->n_seq - 1) / a->n_seq;
+    const int64_t ctas = a->n_seq * ((each + KT_ROWS - 1) / KT_ROWS) * a->cache.n_head_kv;
+    return {ctas > sm_count(), (int)std::max<int64_t>(1, std::min<int64_t>(sm_count() / ctas, KT_SPLITS))};
+}
+static int launch_prompt(AttnArgs &args, bool vec, int k, bool one, long long limit, cudaStream_t st) {
+    const PromptPlan plan = prompt_plan(&args.a);
+    const bool two = plan.two;
+    args.splits = plan.splits;
     if (k == 64) {
         if (two) return one ? launch_tc<64, 2, 1>(args, vec, limit, st) : launch_tc<64, 2, 2>(args, vec, limit, st);
         return one ? launch_tc<64, 1, 1>(args, vec, limit, st) : launch_tc<64, 1, 2>(args, vec, limit, st);
@@ -669,7 +689,10 @@ static int launch_prompt(const AttnArgs &args, bool vec, int k, bool one, long l
 
 }  // namespace kv8
 
-int kv8_attn_launches(const b200_kv8_attn_args *a) { return a->n_tokens == 0 || a->n_seq == 0 ? 0 : kv8::has_prompts(a) ? 2 : 1; }
+int kv8_attn_launches(const b200_kv8_attn_args *a) {
+    if (a->n_tokens == 0 || a->n_seq == 0) return 0;
+    return !kv8::has_prompts(a) ? 1 : kv8::prompt_plan(a).splits > 1 ? 3 : 2;
+}
 
 }  // namespace b200
 
@@ -680,8 +703,10 @@ extern "C" {
 
 size_t b200_kv8_attn_workspace_bytes(const b200_kv8_attn_args *a) {
     if (!a || b200_kv8_page_bytes(a->cache.page_size, a->cache.n_head_kv, a->cache.dim, a->cache.vdim) == 0) return 0;
-    const int grid = rows_grid(a->cache);
-    return rows_counter_bytes(grid) + (size_t)grid * 2 * (one_term(a) ? 16 : 8) * (attn_class(a->cache) + 2) * 4;
+    const int grid = rows_grid(a->cache), k = attn_class(a->cache);
+    // (the two kernels' partial results are not there at the same time; the prompt kernel's grid has room for twice the blocks that its plan counts)
+    const size_t rows = (size_t)grid * 2 * (one_term(a) ? 16 : 8) * (k + 2) * 4, prompts = k <= 128 ? (size_t)2 * sm_count() * KT_ROWS * (k + 2) * 4 : 0;
+    return rows_counter_bytes() + (rows > prompts ? rows : prompts);
 }
 
 int b200_op_kv8_attn(const b200_kv8_attn_args *a, void *workspace, size_t workspace_bytes, b200_stream_t stream) {
@@ -692,7 +717,7 @@ int b200_op_kv8_attn(const b200_kv8_attn_args *a, void *workspace, size_t worksp
                 b200_kv8_attn_workspace_bytes(a));
     const b200_kv8_cache &c = a->cache;
     AttnArgs args = {*a, {a->seq_info, a->table, a->table_stride, a->n_rows, a->n_seq, a->n_tokens, c.n_pages, c.page_size}, (int *)workspace,
-                     (float *)((char *)workspace + rows_counter_bytes(rows_grid(c))), a->n_head / c.n_head_kv, 0, -1};
+                     (float *)((char *)workspace + rows_counter_bytes()), a->n_head / c.n_head_kv, 0, 1, -1};
     args.group_div = (unsigned)(((1ull << 32) + args.group - 1) / args.group);
     const cudaStream_t st = (cudaStream_t)stream;
     const int k = attn_class(c);

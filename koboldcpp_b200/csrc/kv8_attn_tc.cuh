@@ -10,6 +10,7 @@
 // Softmax: four warps a group of 128 rows.  The maximum that the exponent subtracts follows the true one only when that has grown by SLACK, so O is hardly
 // ever rescaled.  A key's scale joins its score, a value's its weight, relative to the power of two above the largest that the row has seen.
 // Every S has two buffers a group: products run while the softmax is busy with the tile before.
+// With few rows behind many keys, several CTAs (of one group) share a block's tiles; kv8_attn_join_kernel adds their results up.
 // Waits have a limit, as in the prompt GEMM: a role that gives up sets `failed`, the others follow, and the status word is set.
 #pragma once
 #include "tcgen05.cuh"
@@ -18,6 +19,7 @@ namespace b200 {
 namespace kv8 {
 
 constexpr int KT_ROWS = 128, KT_KEYS = 64;
+constexpr int KT_SPLITS = 16, KT_SPLIT_TILES = 4;  // CTAs that share a block of rows at most; tiles that each of them has at least
 constexpr int KT_RING = 8;  // scales of so many tiles: a tile's are written when the weights of the tile NB + 2 before it have been used
 constexpr int KT_Q_PANEL = KT_ROWS * 128, KT_PANEL = KT_KEYS * 128;  // panels of 64 values, 128 bytes a row
 template <int GROUPS> constexpr int kt_threads() { return (GROUPS * 4 + 4 + 8) * 32; }  // softmax; products (one warp a group and product); conversion of keys and of values
@@ -27,6 +29,9 @@ template <int C, int GROUPS, int TERMS> constexpr size_t kt_smem() {
 }
 // f16 operands, f32 results, 128 rows
 __device__ __forceinline__ unsigned kt_idesc(int n, bool b_mn) { return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((unsigned)(n >> 3) << 17) | ((unsigned)(KT_ROWS >> 4) << 24); }
+// CTAs that share a block of so many tiles
+__device__ __forceinline__ int kt_splits(int tiles, int most) { return max(1, min(most, tiles / KT_SPLIT_TILES)); }
+template <int C> constexpr size_t kt_part() { return (size_t)KT_ROWS * (C + 2); }  // maxima, sums, rows
 __device__ __forceinline__ float2 mul2(float2 x, float2 y) {
     float2 r;
     asm("{\n.reg .b64 a, b;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 a, a, b;\nmov.b64 {%0, %1}, a;\n}\n" : "=f"(r.x), "=f"(r.y) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
@@ -111,11 +116,11 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
     const b200_kv8_cache &c = a.cache;
     const Step &st = args.step;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    const int group = args.group, ps = c.page_size, h = (int)(blockIdx.x % (unsigned)c.n_head_kv);
+    const int group = args.group, ps = c.page_size, h = (int)(blockIdx.x / (unsigned)args.splits % (unsigned)c.n_head_kv);
     pdl_enter();
     const int32_t *info = behind(st.info), *table = behind(st.table);
     // block j of rows belongs to the sequence s with first_s group / BLOCK + s <= j (long causal walks first, of all heads)
-    const int j = (int)((gridDim.x - 1 - blockIdx.x) / (unsigned)c.n_head_kv);
+    const int j = (int)((gridDim.x - 1 - blockIdx.x) / (unsigned)(args.splits * c.n_head_kv));
     auto first_block = [&](int first, int s) { return (int)((int64_t)first * group / BLOCK) + s; };
     int s;
     const Seq q = find_seq(st, info, j, s, first_block);
@@ -129,8 +134,12 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
     // tiles: those of the kept first tokens, then from the window's on
     const int first_tile = a.window > 0 ? max(0, pos_lo + 1 - a.window) / KT_KEYS : 0;
     const int keep_tiles = a.window > 0 ? min((int)(((int64_t)max(a.keep_first, 0) + KT_KEYS - 1) / KT_KEYS), first_tile) : 0;
-    const int n_tiles = keep_tiles + pos_hi / KT_KEYS + 1 - first_tile;
-    auto key_of = [&](int t) { return (t < keep_tiles ? t : t - keep_tiles + first_tile) * KT_KEYS; };
+    const int all_tiles = keep_tiles + pos_hi / KT_KEYS + 1 - first_tile;
+    // this CTA's stretch of them
+    const int splits = kt_splits(all_tiles, args.splits), z = (int)(blockIdx.x % (unsigned)args.splits);
+    if (z >= splits) return;
+    const int t_begin = (int)((int64_t)all_tiles * z / splits), n_tiles = (int)((int64_t)all_tiles * (z + 1) / splits) - t_begin;
+    auto key_of = [&](int t) { return (t + t_begin < keep_tiles ? t + t_begin : t + t_begin - keep_tiles + first_tile) * KT_KEYS; };
     unsigned char *sq = smem, *sk = sq + GROUPS * TERMS * PANELS * KT_Q_PANEL, *sv = sk + NB * TILE;
 
     if (tid == 0) {
@@ -312,7 +321,11 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
             const float mm = fmaxf(m, sink), f = m == -INFINITY ? (l == 0.f ? 0.f : 1.0f) : ex2(m - mm);
             const float sum = l * f + (sink == -INFINITY ? 0.f : ex2(sink - mm));
             const float inv = sum == 0.f ? 0.f : f / sum, back = pow2i(power - HEAD);
-            const float share = sum == 0.f ? 0.f : inv * back;
+            // (a stretch of the tiles: relative to its own maximum, which goes with its sum to where kv8_attn_join_kernel finds it)
+            const bool whole_block = splits == 1;
+            const float share = !whole_block ? back : sum == 0.f ? 0.f : inv * back;
+            float *part = args.partials + ((size_t)(j * c.n_head_kv + h) * args.splits + z) * kt_part<C>();
+            if (!whole_block && mine) { part[row] = m; part[KT_ROWS + row] = l; }
             // 32 columns at a time through shared memory (where this warp's rows of Q were), so that a row's stores lie side by side
             unsigned char *stage = sq + w * TERMS * PANELS * KT_Q_PANEL + quarter * 4096;
             const int e = lane & 7;
@@ -320,7 +333,8 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 const int rb = w0 + 4 * k + (lane >> 3), tok = token(rb);
-                at[k] = rb < n_rows ? (int64_t)(q.first + tok0 + tok) * a.dst_stride + (int64_t)(h * group + head0 + rb - tok * group) * c.vdim + 4 * e : -1;
+                const int64_t row_at = whole_block ? (int64_t)(q.first + tok0 + tok) * a.dst_stride + (int64_t)(h * group + head0 + rb - tok * group) * c.vdim : 2 * KT_ROWS + (int64_t)rb * C;
+                at[k] = rb < n_rows ? row_at + 4 * e : -1;
             }
 #pragma unroll 1
             for (int ch = 0; ch < c.vdim; ch += 32) {
@@ -338,7 +352,7 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
                     for (int k = 0; k < 8; k++) {
                         const int rr = 4 * k + (lane >> 3);
                         const float4 y = *reinterpret_cast<const float4 *>(stage + rr * 128 + ((e ^ (rr & 7)) << 4));
-                        if (at[k] >= 0) row_store4(a.dst, a.type, at[k] + ch, vec, y);
+                        if (at[k] >= 0) whole_block ? row_store4(a.dst, a.type, at[k] + ch, vec, y) : row_store4(part, B200_TYPE_F32, at[k] + ch, true, y);
                     }
                 }
                 __syncwarp();
@@ -498,6 +512,47 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
     }
 }
 
+// Rows of blocks that several CTAs shared: their stretches' results, in the order of the tiles.  A warp a row.
+constexpr int KJ_ROWS = 16;  // rows of a CTA
+template <int C>
+__global__ void __launch_bounds__(256) kv8_attn_join_kernel(const __grid_constant__ AttnArgs args, bool vec) {
+    pdl_enter();
+    const b200_kv8_attn_args &a = args.a;
+    const b200_kv8_cache &c = a.cache;
+    const Step &st = args.step;
+    const int group = args.group, lane = threadIdx.x & 31, h = (int)(blockIdx.x % (unsigned)c.n_head_kv), j = (int)(blockIdx.x / (unsigned)c.n_head_kv);
+    const int32_t *info = behind(st.info);
+    auto first_block = [&](int first, int s) { return (int)((int64_t)first * group / KT_ROWS) + s; };
+    int s;
+    const Seq q = find_seq(st, info, j, s, first_block);
+    const int64_t row0 = (int64_t)(j - first_block(q.first, s)) * KT_ROWS, rows = (int64_t)q.count * group;
+    if (rows <= args.rows_most || row0 < 0 || row0 >= rows) return;
+    const int n_rows = (int)min((int64_t)KT_ROWS, rows - row0), tok0 = (int)(row0 / group), head0 = (int)(row0 - (int64_t)tok0 * group);
+    const int pos_lo = q.held + tok0, pos_hi = q.held + (int)((row0 + n_rows - 1) / group);
+    const int first_tile = a.window > 0 ? max(0, pos_lo + 1 - a.window) / KT_KEYS : 0;
+    const int keep_tiles = a.window > 0 ? min((int)(((int64_t)max(a.keep_first, 0) + KT_KEYS - 1) / KT_KEYS), first_tile) : 0;
+    const int splits = kt_splits(keep_tiles + pos_hi / KT_KEYS + 1 - first_tile, args.splits);
+    if (splits == 1) return;  // (stored by its one CTA)
+    const float *part = behind(args.partials) + (size_t)(j * c.n_head_kv + h) * args.splits * kt_part<C>();
+    for (int r = blockIdx.y * KJ_ROWS + (threadIdx.x >> 5); r < min((int)(blockIdx.y + 1) * KJ_ROWS, n_rows); r += 8) {
+        const int tok = (head0 + r) / group, head = h * group + head0 + r - tok * group;
+        const float mine = lane < splits ? __ldcg(part + (size_t)lane * kt_part<C>() + r) : -INFINITY, sum_of = lane < splits ? __ldcg(part + (size_t)lane * kt_part<C>() + KT_ROWS + r) : 0.f;
+        const float sink = a.sink ? a.sink[head] * LOG2E : -INFINITY, top = fmaxf(warp_max(mine), sink);
+        const float f = mine == -INFINITY ? (sum_of == 0.f ? 0.f : 1.0f) : ex2(mine - top);
+        const float sum = warp_sum(sum_of * f) + (sink == -INFINITY ? 0.f : ex2(sink - top));
+        const float share = sum == 0.f ? 0.f : f / sum;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int k = 0; k < splits; k++) {
+            const float w = __shfl_sync(0xffffffffu, share, k);
+            if (4 * lane >= c.vdim) continue;
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(part + (size_t)k * kt_part<C>() + 2 * KT_ROWS + (size_t)r * C) + lane);
+            y = make_float4(y.x + v.x * w, y.y + v.y * w, y.z + v.z * w, y.w + v.w * w);
+        }
+        if (4 * lane < c.vdim) row_store4(a.dst, a.type, (int64_t)(q.first + tok0 + tok) * a.dst_stride + (int64_t)head * c.vdim + 4 * lane, vec, y);
+    }
+}
+
 template <int C, int GROUPS, int TERMS>
 static int launch_tc(const AttnArgs &args, bool vec, long long limit, cudaStream_t st) {
     int *status = nullptr;
@@ -510,8 +565,9 @@ static int launch_tc(const AttnArgs &args, bool vec, long long limit, cudaStream
         B200_CUDA_TRY(cudaFuncSetAttribute(kv8_attn_tc_kernel<C, GROUPS, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kt_smem<C, GROUPS, TERMS>()));
         if (dev < 16) done[dev] = true;
     }
-    const unsigned grid = (unsigned)(((int64_t)args.a.n_tokens * args.group / (GROUPS * KT_ROWS) + args.a.n_seq) * args.a.cache.n_head_kv);
-    B200_CUDA_TRY(launch_chained(kv8_attn_tc_kernel<C, GROUPS, TERMS>, grid, kt_threads<GROUPS>(), kt_smem<C, GROUPS, TERMS>(), st, args, vec, limit, status));
+    const unsigned blocks = (unsigned)(((int64_t)args.a.n_tokens * args.group / (GROUPS * KT_ROWS) + args.a.n_seq) * args.a.cache.n_head_kv);
+    B200_CUDA_TRY(launch_chained(kv8_attn_tc_kernel<C, GROUPS, TERMS>, blocks * (unsigned)args.splits, kt_threads<GROUPS>(), kt_smem<C, GROUPS, TERMS>(), st, args, vec, limit, status));
+    if (args.splits > 1) B200_CUDA_TRY(launch_chained(kv8_attn_join_kernel<C>, dim3(blocks, KT_ROWS / KJ_ROWS), 256, 0, st, args, vec));
     return B200_OK;
 }
 

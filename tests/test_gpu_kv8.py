@@ -10,6 +10,10 @@ to bounds made of each case's own numbers.  With E the largest error of a score 
     values, and the products are independent): 2^-18.
   * Weights: exponential and its argument 2^-18 (scores below 64), two f16 2^-22 or one 2^-11, sums in f32 of up to 4096 keys: 2^-24 4096 / 16 (a thread adds every
     16th) = 2^-16.  w = 2^-15 or 2^-11 + 2^-15.
+  * Weights far below the row's largest: f16 has steps of 2^-24 and no finer ones, so a weight as it enters the second product is off by 2^-25 too, however small it
+    is.  It enters as p_j / max p (at least: the sum that divides is 1 or more in this unit) times its scale times 2^6 / 2^power, 2^power being at most twice the
+    largest scale that the row has seen: 2^-25 2^-6 2 = 2^-30 of that scale, times an int8 of at most 127, for each key that is seen.  It shows where a key takes all
+    the weight and its value is 0.
 """
 import ctypes as C
 
@@ -294,7 +298,10 @@ def compare(case, q, name, n_head, scale, got, **opt):
         want, mass, size = case.pool.attend(case.table[r], q[f:f + m], held, np.float64(np.float32(scale)), opt.get("window", 0), opt.get("keep", 0), sink, opt.get("softcap", 0.0))
         x = got[f:f + m]
         assert (np.isnan(x) == np.isnan(want)).all(), (held, m)
-        off, most = np.abs(x - want), bound(name, mass, size, want, opt.get("f16", 0))
+        loud = np.fmax.reduce(case.pool.vs[[p for p in case.table[r] if 0 <= p < case.n_pages]], axis=0, initial=0.0)  # of each kv head
+        keys = np.minimum(held + 1 + np.arange(m), opt["window"] + opt.get("keep", 0) if opt.get("window", 0) else held + m)
+        least = 2.0 ** -30 * 127 * keys[:, None, None] * np.repeat(loud, n_head // case.heads)[None, :, None]
+        off, most = np.abs(x - want), bound(name, mass, size, want, opt.get("f16", 0)) + least
         fine = np.isfinite(want)
         assert (off[fine] <= most[fine]).all(), (held, m, float(np.max(off[fine] / most[fine])), np.argwhere(off > most)[:5].tolist())
         checked += m

@@ -81,7 +81,7 @@ def attn_args(**change):
     return Kv8AttnArgs(*[f[name] for name, _ in Kv8AttnArgs._fields_])
 
 
-@pytest.mark.parametrize("change,code", COMMON + [(dict(q=None), 2), (dict(dst=None), 2), (dict(q_stride=255), 2), (dict(dst_stride=1), 2), (dict(n_head=0), 2), (dict(n_head=5), 2), (dict(window=-1), 2),
+@pytest.mark.parametrize("change,code", COMMON + [(dict(q=None), 2), (dict(dst=None), 2), (dict(q_stride=255), 2), (dict(dst_stride=1), 2), (dict(n_head=0), 2), (dict(n_head=5), 2), (dict(n_tokens=1 << 28, n_head=8, q_stride=512, dst_stride=512), 1), (dict(window=-1), 2),
                                                   (dict(keep_first=-1), 2), (dict(softcap=-1.0), 2), (dict(softcap=float("nan")), 2), (dict(softcap=float("inf")), 2), (dict(scale=float("nan")), 2)])
 def test_attn_refuses(change, code):
     assert lib().b200_op_kv8_attn(C.byref(attn_args(**change)), AT, 1 << 30, None) == code
