@@ -85,7 +85,7 @@ B200_API int b200_op_kv8_load(const b200_kv8_load_args *a, b200_stream_t stream)
  * else they enter as two f16 each, 22 bits.  A query that is not finite gives NaN.
  * max_new: no sequence of the step has more new tokens than that (0: not known).  It only chooses how the work is laid out.
  * n_tokens * n_head below 2^31.  The workspace is zero before its first call and may then go from call to call of one stream, whatever their sizes; the bytes
- * asked for do not depend on lengths.  Kernels of long steps bound their waits: one that gives up makes b200_gemm_status() 1. */
+ * asked for do not depend on lengths.  */
 typedef struct {
     b200_kv8_cache cache;
     const void *q; int64_t q_stride;
@@ -101,6 +101,9 @@ typedef struct {
 } b200_kv8_attn_args;
 B200_API size_t b200_kv8_attn_workspace_bytes(const b200_kv8_attn_args *a);
 B200_API int b200_op_kv8_attn(const b200_kv8_attn_args *a, void *workspace, size_t workspace_bytes, b200_stream_t stream);
+/* The same with the limit of each of the kernel's own waits in clock cycles (b200_op_kv8_attn: about two seconds' worth; 0: it gives up at
+ * once), where many new tokens run on tcgen05 (heads of up to 128).  When one runs out the call ends early: rows of dst are right, NaN or as they were, and b200_gemm_status() becomes 1. */
+B200_API int b200_op_kv8_attn_wait(const b200_kv8_attn_args *a, void *workspace, size_t workspace_bytes, int64_t wait_cycles, b200_stream_t stream);
 
 /* ---- pages: who holds what, on the device (all layers' pools go by one table) -----------------------------------------------------------------
  * refs[p]: how many table entries name page p; len[row]: tokens that the row holds; entries from ceil(len / page_size) on are -1.  A caller

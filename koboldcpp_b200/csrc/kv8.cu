@@ -24,6 +24,7 @@ int check_step(const b200_kv8_cache *c, const int32_t *seq_info, const int32_t *
     OPX_REQUIRE(n_seq <= B200_KV8_MAX_SEQ, B200_ERR_UNSUPPORTED, "%s: %d sequences in a step, at most %d", who, n_seq, B200_KV8_MAX_SEQ);
     OPX_REQUIRE(table_stride <= 0x7fffffff / c->page_size, B200_ERR_UNSUPPORTED, "%s: rows of more than 2^31 tokens", who);
     OPX_REQUIRE(n_tokens == 0 || n_seq == 0 || (seq_info != nullptr && table != nullptr), B200_ERR_INVALID, "%s: NULL seq_info or table", who);
+    OPX_REQUIRE(aligned_to(4, seq_info, table), B200_ERR_INVALID, "%s: seq_info or table at an odd place", who);
     return B200_OK;
 }
 
@@ -572,6 +573,7 @@ int b200_op_kv8_store(const b200_kv8_store_args *a, b200_stream_t stream) {
     OPX_REQUIRE(a->k && a->v, B200_ERR_INVALID, "%s: NULL k or v", who);
     OPX_REQUIRE(a->k_stride >= (int64_t)c.n_head_kv * c.dim && a->v_stride >= (int64_t)c.n_head_kv * c.vdim, B200_ERR_INVALID, "%s: rows of k or v overlap (strides %lld, %lld)", who,
                 (long long)a->k_stride, (long long)a->v_stride);
+    OPX_REQUIRE(aligned_to(type_size(a->type), a->k, a->v), B200_ERR_INVALID, "%s: k or v is not aligned to its type", who);
     const StoreArgs s = {c, {a->seq_info, a->table, a->table_stride, a->n_rows, a->n_seq, a->n_tokens, c.n_pages, c.page_size}, a->k, a->v, a->k_stride, a->v_stride};
     const dim3 grid((unsigned)(a->n_tokens / c.page_size + 2 * a->n_seq), (unsigned)c.n_head_kv);
     const bool vec = rows_aligned(a->k, a->k_stride, a->type) && rows_aligned(a->v, a->v_stride, a->type);
@@ -588,6 +590,7 @@ int b200_op_kv8_load(const b200_kv8_load_args *a, b200_stream_t stream) {
     const b200_kv8_cache &c = a->cache;
     OPX_REQUIRE((!a->k || a->k_stride >= (int64_t)c.n_head_kv * c.dim) && (!a->v || a->v_stride >= (int64_t)c.n_head_kv * c.vdim), B200_ERR_INVALID, "%s: rows of k or v overlap (strides %lld, %lld)",
                 who, (long long)a->k_stride, (long long)a->v_stride);
+    OPX_REQUIRE(aligned_to(type_size(a->type), a->k, a->v), B200_ERR_INVALID, "%s: k or v is not aligned to its type", who);
     const LoadArgs s = {c, {a->seq_info, a->table, a->table_stride, a->n_rows, a->n_seq, a->n_tokens, c.n_pages, c.page_size}, a->k, a->v, a->k_stride, a->v_stride};
     const bool vec = (!a->k || rows_aligned(a->k, a->k_stride, a->type)) && (!a->v || rows_aligned(a->v, a->v_stride, a->type));
     const unsigned grid = (unsigned)a->n_tokens;

@@ -21,8 +21,9 @@ struct Seq { int first, count, row, held; };
 // sequence s as far as it can be: a row that is none, or tokens outside the batch, leave a count of 0
 __device__ __forceinline__ Seq seq_of(const Step &st, const int32_t *info, int s) {
     Seq q = {info[s], info[st.n_seq + s], info[2 * st.n_seq + s], info[3 * st.n_seq + s]};
-    if (q.first < 0 || q.first >= st.n_tokens || q.row < 0 || q.row >= st.n_rows || q.held < 0 || q.count < 0) q.count = 0;
-    q.count = min(q.count, min(st.n_tokens - q.first, 0x7fffffff - q.held));
+    const bool none = q.first < 0 || q.first >= st.n_tokens || q.row < 0 || q.row >= st.n_rows || q.held < 0 || q.count < 0;
+    if (none) q.first = q.held = 0;
+    q.count = none ? 0 : min(q.count, min(st.n_tokens - q.first, 0x7fffffff - q.held));
     return q;
 }
 // page number `at` of a row, or -1
@@ -139,6 +140,8 @@ inline bool type_ok(int t) { return t == B200_TYPE_F32 || t == B200_TYPE_F16 || 
 inline size_t type_size(int t) { return t == B200_TYPE_F32 ? 4 : 2; }
 // rows whose pieces of 16 bytes all begin on 16 bytes
 inline bool rows_aligned(const void *p, int64_t stride, int type) { return (uintptr_t)p % 16 == 0 && stride * (int64_t)type_size(type) % 16 == 0; }
+// pointers to values of so many bytes (NULL too)
+inline bool aligned_to(size_t size, const void *a, const void *b = nullptr, const void *c = nullptr) { return ((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) % size == 0; }
 int check_cache(const b200_kv8_cache *c, const char *who);
 int check_step(const b200_kv8_cache *c, const int32_t *seq_info, const int32_t *table, int64_t table_stride, int32_t n_rows, int32_t n_seq, int32_t n_tokens, int32_t type, const char *who);
 

@@ -96,6 +96,7 @@ struct AttnArgs {
     float *partials;  // two per CTA
     int group;        // query heads per kv head
     unsigned group_div;  // ceil(2^32 / group): __umulhi(x, group_div) = x / group for x < 2^32 / group
+    int table_tokens; // tokens that the table has entries for, at least 1: nobody has to look behind them
     int splits;       // a prompt's block of rows may be shared by so many CTAs, each with a stretch of its tiles
     int rows_most;    // sequences with more query rows a kv head (tokens times group) are the prompt kernel's; negative: there is none
 };
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kern
         Span s;
         s.first = a.window > 0 ? max(0, q.held + 1 - a.window) / RW_UNIT : 0;
         s.keep = a.window > 0 ? min((int)(((int64_t)max(a.keep_first, 0) + RW_UNIT - 1) / RW_UNIT), s.first) : 0;
-        s.units = s.keep + (int)(((int64_t)q.held + q.count + RW_UNIT - 1) / RW_UNIT) - s.first;
+        s.units = s.keep + max((int)((unsigned)(min(q.held + q.count, args.table_tokens) + RW_UNIT - 1) / RW_UNIT) - s.first, 1);
         const int64_t rows = (int64_t)q.count * group;
         s.blocks = args.rows_most >= 0 && rows > args.rows_most ? 0 : (int)((rows + R - 1) / R);
         return s;
@@ -649,6 +650,7 @@ static int check_attn(const b200_kv8_attn_args *a, const char *who) {
     OPX_REQUIRE(a->q && a->dst, B200_ERR_INVALID, "%s: NULL q or dst", who);
     OPX_REQUIRE(a->q_stride >= (int64_t)a->n_head * c.dim && a->dst_stride >= (int64_t)a->n_head * c.vdim, B200_ERR_INVALID, "%s: rows of q or dst overlap (strides %lld, %lld)", who,
                 (long long)a->q_stride, (long long)a->dst_stride);
+    OPX_REQUIRE(aligned_to(type_size(a->type), a->q, a->dst) && aligned_to(4, a->sink), B200_ERR_INVALID, "%s: q, dst or sink is not aligned to its type", who);
     return B200_OK;
 }
 // Where a step has PROMPT_ROWS query rows over all heads (rows of two terms count twice), its sequences of more than ROWS_MOST rows a kv head are the prompt kernel's, if the
@@ -710,21 +712,26 @@ size_t b200_kv8_attn_workspace_bytes(const b200_kv8_attn_args *a) {
 }
 
 int b200_op_kv8_attn(const b200_kv8_attn_args *a, void *workspace, size_t workspace_bytes, b200_stream_t stream) {
+    return b200_op_kv8_attn_wait(a, workspace, workspace_bytes, PAIR_WAIT_LIMIT, stream);
+}
+
+int b200_op_kv8_attn_wait(const b200_kv8_attn_args *a, void *workspace, size_t workspace_bytes, int64_t wait_cycles, b200_stream_t stream) {
     const char *who = "b200_op_kv8_attn";
+    OPX_REQUIRE(wait_cycles >= 0, B200_ERR_INVALID, "%s: limit below zero", who);
     const int rc = check_attn(a, who);
     if (rc != B200_OK || a->n_tokens == 0 || a->n_seq == 0) return rc;
     OPX_REQUIRE(workspace && workspace_bytes >= b200_kv8_attn_workspace_bytes(a) && (uintptr_t)workspace % 16 == 0, B200_ERR_INVALID, "%s: workspace of %zu bytes, 16-byte aligned", who,
                 b200_kv8_attn_workspace_bytes(a));
     const b200_kv8_cache &c = a->cache;
     AttnArgs args = {*a, {a->seq_info, a->table, a->table_stride, a->n_rows, a->n_seq, a->n_tokens, c.n_pages, c.page_size}, (int *)workspace,
-                     (float *)((char *)workspace + rows_counter_bytes()), a->n_head / c.n_head_kv, 0, 1, -1};
+                     (float *)((char *)workspace + rows_counter_bytes()), a->n_head / c.n_head_kv, 0, std::max(1, (int)a->table_stride * c.page_size), 1, -1};
     args.group_div = (unsigned)(((1ull << 32) + args.group - 1) / args.group);
     const cudaStream_t st = (cudaStream_t)stream;
     const int k = attn_class(c);
     const bool vec = rows_aligned(a->q, a->q_stride, a->type) && rows_aligned(a->dst, a->dst_stride, a->type);
     if (has_prompts(a)) {
         args.rows_most = ROWS_MOST;
-        const int rc2 = launch_prompt(args, vec, k, one_term(a), PAIR_WAIT_LIMIT, st);
+        const int rc2 = launch_prompt(args, vec, k, one_term(a), wait_cycles, st);
         if (rc2 != B200_OK) return rc2;
     }
     if (one_term(a)) return k == 64 ? launch_rows<64, 1>(args, vec, st) : k == 128 ? launch_rows<128, 1>(args, vec, st) : launch_rows<256, 1>(args, vec, st);

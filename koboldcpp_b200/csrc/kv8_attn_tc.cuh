@@ -32,6 +32,16 @@ __device__ __forceinline__ unsigned kt_idesc(int n, bool b_mn) { return (1u << 4
 // CTAs that share a block of so many tiles
 __device__ __forceinline__ int kt_splits(int tiles, int most) { return max(1, min(most, tiles / KT_SPLIT_TILES)); }
 template <int C> constexpr size_t kt_part() { return (size_t)KT_ROWS * (C + 2); }  // maxima, sums, rows
+// A block of rows at positions pos_lo .. pos_hi: its tiles are those of the kept first tokens, then from the window's on (of which the table has entries for).
+struct Tiles { int keep, first, all; };
+__device__ __forceinline__ Tiles kt_tiles(const AttnArgs &args, int pos_lo, int pos_hi) {
+    const b200_kv8_attn_args &a = args.a;
+    Tiles t;
+    t.first = a.window > 0 ? max(0, pos_lo + 1 - a.window) / KT_KEYS : 0;
+    t.keep = a.window > 0 ? min((int)(((int64_t)max(a.keep_first, 0) + KT_KEYS - 1) / KT_KEYS), t.first) : 0;
+    t.all = t.keep + max(min(pos_hi, args.table_tokens - 1) / KT_KEYS + 1 - t.first, 1);
+    return t;
+}
 __device__ __forceinline__ float2 mul2(float2 x, float2 y) {
     float2 r;
     asm("{\n.reg .b64 a, b;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 a, a, b;\nmov.b64 {%0, %1}, a;\n}\n" : "=f"(r.x), "=f"(r.y) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
@@ -131,15 +141,12 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
     // local row r is query head head0 + r - token(r) * group of token tok0 + token(r)
     const int tok0 = row0 / group, head0 = row0 - tok0 * group;
     auto token = [&](int r) { return group == 1 ? r : (int)__umulhi((unsigned)(head0 + r), args.group_div); };
-    // tiles: those of the kept first tokens, then from the window's on
-    const int first_tile = a.window > 0 ? max(0, pos_lo + 1 - a.window) / KT_KEYS : 0;
-    const int keep_tiles = a.window > 0 ? min((int)(((int64_t)max(a.keep_first, 0) + KT_KEYS - 1) / KT_KEYS), first_tile) : 0;
-    const int all_tiles = keep_tiles + pos_hi / KT_KEYS + 1 - first_tile;
+    const Tiles tiles_of = kt_tiles(args, pos_lo, pos_hi);
     // this CTA's stretch of them
-    const int splits = kt_splits(all_tiles, args.splits), z = (int)(blockIdx.x % (unsigned)args.splits);
+    const int splits = kt_splits(tiles_of.all, args.splits), z = (int)(blockIdx.x % (unsigned)args.splits);
     if (z >= splits) return;
-    const int t_begin = (int)((int64_t)all_tiles * z / splits), n_tiles = (int)((int64_t)all_tiles * (z + 1) / splits) - t_begin;
-    auto key_of = [&](int t) { return (t + t_begin < keep_tiles ? t + t_begin : t + t_begin - keep_tiles + first_tile) * KT_KEYS; };
+    const int t_begin = (int)((int64_t)tiles_of.all * z / splits), n_tiles = (int)((int64_t)tiles_of.all * (z + 1) / splits) - t_begin;
+    auto key_of = [&](int t) { return (t + t_begin < tiles_of.keep ? t + t_begin : t + t_begin - tiles_of.keep + tiles_of.first) * KT_KEYS; };
     unsigned char *sq = smem, *sk = sq + GROUPS * TERMS * PANELS * KT_Q_PANEL, *sv = sk + NB * TILE;
 
     if (tid == 0) {
@@ -316,6 +323,9 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
         // ===== results
         ok = ok && kt_wait<20>(&o_done[w][(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, &failed, limit);
         tc_fence_after();
+        // (a stretch that was given up: NaN rows rather than what an earlier call left there)
+        float *part = args.partials + ((size_t)(j * c.n_head_kv + h) * args.splits + z) * kt_part<C>();
+        if (!ok && splits > 1 && mine) { part[row] = -INFINITY; part[KT_ROWS + row] = __uint_as_float(0x7fc00000u); }
         if (ok) {
             const float sink = a.sink ? a.sink[head] * LOG2E : -INFINITY;
             const float mm = fmaxf(m, sink), f = m == -INFINITY ? (l == 0.f ? 0.f : 1.0f) : ex2(m - mm);
@@ -324,7 +334,6 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
             // (a stretch of the tiles: relative to its own maximum, which goes with its sum to where kv8_attn_join_kernel finds it)
             const bool whole_block = splits == 1;
             const float share = !whole_block ? back : sum == 0.f ? 0.f : inv * back;
-            float *part = args.partials + ((size_t)(j * c.n_head_kv + h) * args.splits + z) * kt_part<C>();
             if (!whole_block && mine) { part[row] = m; part[KT_ROWS + row] = l; }
             // 32 columns at a time through shared memory (where this warp's rows of Q were), so that a row's stores lie side by side
             unsigned char *stage = sq + w * TERMS * PANELS * KT_Q_PANEL + quarter * 4096;
@@ -444,8 +453,9 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
             asm volatile("bar.sync 2, %0;" ::"n"((SOFTMAX + GROUPS) * 32) : "memory");
             const bool elected = elect_lane();
             const unsigned long long qd = umma_desc_sw128(smem_u32(sq)) + (unsigned)(w * TERMS * PANELS * (KT_Q_PANEL >> 4)), kd0 = umma_desc_sw128(smem_u32(sk));
-            const int steps = c.dim / 16;
-            for (int t = 0; t < n_tiles; t++) {
+            const int steps = c.dim / 16, walk = limit > 0 ? n_tiles : 0;
+            if (limit <= 0) failed = 1;  // (a try of a barrier takes microseconds, longer than any wait of a short call: this warp gives up without one)
+            for (int t = 0; t < walk; t++) {
                 const int b = t & 1, nb = t % NB;
                 if (!kt_wait<40>(&k_full[nb], (t / NB) & 1, &failed, limit)) break;
                 if (t >= 2 && !kt_wait<40>(&o_done[w][b], ((t >> 1) & 1) ^ 1, &failed, limit)) break;  // the weights of tile t - 2 have been used
@@ -529,9 +539,7 @@ __global__ void __launch_bounds__(256) kv8_attn_join_kernel(const __grid_constan
     if (rows <= args.rows_most || row0 < 0 || row0 >= rows) return;
     const int n_rows = (int)min((int64_t)KT_ROWS, rows - row0), tok0 = (int)(row0 / group), head0 = (int)(row0 - (int64_t)tok0 * group);
     const int pos_lo = q.held + tok0, pos_hi = q.held + (int)((row0 + n_rows - 1) / group);
-    const int first_tile = a.window > 0 ? max(0, pos_lo + 1 - a.window) / KT_KEYS : 0;
-    const int keep_tiles = a.window > 0 ? min((int)(((int64_t)max(a.keep_first, 0) + KT_KEYS - 1) / KT_KEYS), first_tile) : 0;
-    const int splits = kt_splits(keep_tiles + pos_hi / KT_KEYS + 1 - first_tile, args.splits);
+    const int splits = kt_splits(kt_tiles(args, pos_lo, pos_hi).all, args.splits);
     if (splits == 1) return;  // (stored by its one CTA)
     const float *part = behind(args.partials) + (size_t)(j * c.n_head_kv + h) * args.splits * kt_part<C>();
     for (int r = blockIdx.y * KJ_ROWS + (threadIdx.x >> 5); r < min((int)(blockIdx.y + 1) * KJ_ROWS, n_rows); r += 8) {

@@ -295,6 +295,7 @@ _KV8_SIGS = {
     "b200_kv8_page_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "b200_op_kv8_store": (C.c_int, [C.POINTER(Kv8StoreArgs), C.c_void_p]),
     "b200_op_kv8_load": (C.c_int, [C.POINTER(Kv8LoadArgs), C.c_void_p]),
+    "b200_op_kv8_attn_wait": (C.c_int, [C.POINTER(Kv8AttnArgs), C.c_void_p, C.c_size_t, C.c_int64, C.c_void_p]),
     "b200_kv8_attn_workspace_bytes": (C.c_size_t, [C.POINTER(Kv8AttnArgs)]),
     "b200_op_kv8_attn": (C.c_int, [C.POINTER(Kv8AttnArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
     "b200_op_kv8_cut": (C.c_int, [C.POINTER(Kv8Map), C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]),

@@ -5,13 +5,16 @@ other kernel's), and workspaces and streams that serve both.
 """
 import copy
 import ctypes as C
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
 import torch
 
 import koboldcpp_b200.lib as L
-from koboldcpp_b200.lib import Kv8AttnArgs, check, lib
+from koboldcpp_b200.lib import Kv8AttnArgs, Kv8LoadArgs, Kv8StoreArgs, check, lib
 from test_gpu_kv8 import Case, attend, dev, rounded
 from test_gpu_kv8 import compare as compare_all
 
@@ -225,3 +228,87 @@ def test_prompts_of_as_many_sequences_as_a_step_may_have():
     q = rounded(case.rng.standard_normal((case.tokens, 8, 64)), "bf16")
     got, _ = attend(case, cache, q, "bf16", 8, 0.125)
     assert compare(case, q, "bf16", 8, 0.125, got) == case.tokens
+
+
+@pytest.mark.parametrize("n_head,heads,name", [(64, 4, "f32"), (80, 80, "bf16"), (8, 2, "f32")])
+def test_steps_that_say_what_cannot_be(n_head, heads, name):
+    """Numbers of a step at the ends of 32 bits: such sequences have nothing in the step, and the others get what is theirs (but where the first tokens no longer ascend)."""
+    case = Case([(300, 30), (0, 0), (40, 40), (77, 9)], 16, heads, 64, 64, seed=35)
+    cache = case.upload()
+    q = rounded(case.rng.standard_normal((case.tokens, n_head, 64)), name)
+    least, most, f = -2 ** 31, 2 ** 31 - 1, case.first[2]
+    fine = copy.copy(case)
+    fine.seqs, fine.new = [(300, 30), (0, 0), (40, 0), (77, 9)], [30, 0, 0, 9]
+    for column, value in ((0, least), (0, most), (1, least), (2, least), (2, most), (3, least), (3, most)):
+        info = case.info().cpu().numpy()
+        info[column, 2] = value
+        case.d_info = dev(info)
+        got, _ = attend(case, cache, q, name, n_head, 0.125)
+        assert (got[f:f + 40] == 3.0).all()
+        if column != 0:
+            compare(fine, q, name, n_head, 0.125, got)
+        k, out = torch.ones(case.tokens, heads * 64, device="cuda"), torch.full((case.tokens, heads * 64), 7.0, device="cuda")
+        a = Kv8StoreArgs(cache, k.data_ptr(), heads * 64, k.data_ptr(), heads * 64, *case.where(), case.tokens, L.F32)
+        check(lib().b200_op_kv8_store(C.byref(a), None))
+        a = Kv8LoadArgs(cache, out.data_ptr(), heads * 64, None, 0, *case.where(), case.tokens, L.F32)
+        check(lib().b200_op_kv8_load(C.byref(a), None))
+        assert (out[f:f + 40] == 7.0).all()
+        if column != 0:
+            others = torch.cat([out[:f], out[f + 40:]])
+            assert (others - 1).abs().max() <= 0.51 * case.pool.ks.max()
+        pages = case.table[case.order[2]]
+        pages = pages[pages >= 0]
+        assert (case.d_pool.cpu().numpy()[pages] == case.pool.records()[pages]).all()
+        case.d_pool.copy_(dev(case.pool.records()))
+    # positions behind the table's last entry: as many tokens as 31 bits have room for, which see nothing through a window
+    info = case.info().cpu().numpy()
+    info[3, 2] = most - 20
+    case.d_info = dev(info)
+    got, _ = attend(case, cache, q, name, n_head, 0.125, window=100)
+    assert (got[f:f + 20] == 0).all() and (got[f + 20:f + 40] == 3.0).all()
+    fine.pool = case.pool
+    compare(fine, q, name, n_head, 0.125, got, window=100)
+
+
+GIVE_UP = """
+import sys
+sys.path[:0] = [{root!r}, {tests!r}]
+import ctypes as C
+import numpy as np
+import torch
+import koboldcpp_b200.lib as L
+from koboldcpp_b200.lib import Kv8AttnArgs, check, lib
+from test_gpu_kv8_prompts import Case, compare, dev, rounded
+seqs, n_head, heads, name = {case!r}
+case = Case(seqs, 16, heads, 128, 128, seed=36)
+cache = case.upload()
+q = rounded(case.rng.standard_normal((case.tokens, n_head, 128)), name)
+tq = dev(q.astype(np.float32))
+tq = tq if name == "f32" else tq.bfloat16()
+out = torch.empty(case.tokens, n_head * 128, dtype=tq.dtype, device="cuda")
+a = Kv8AttnArgs(cache, tq.data_ptr(), n_head * 128, out.data_ptr(), n_head * 128, *case.where(), case.tokens, 0, n_head, L.F32 if name == "f32" else L.BF16, None, 0, 0, 0.1, 0.0, 0)
+ws = torch.zeros(lib().b200_kv8_attn_workspace_bytes(C.byref(a)), dtype=torch.uint8, device="cuda")
+def run(limit):
+    out.fill_(float("nan"))
+    check(lib().b200_op_kv8_attn_wait(C.byref(a), ws.data_ptr(), ws.numel(), limit, None))
+    torch.cuda.synchronize()
+    return out.double().cpu().numpy().reshape(case.tokens, n_head, 128)
+whole = run(4_000_000_000)
+compare(case, q, name, n_head, 0.1, whole)
+assert lib().b200_gemm_status() == 0
+for limit in (100_000, 20_000, 6_000, 2_000, 700, 200, 0):
+    got = run(limit)
+    stored = ~np.isnan(got)
+    print(limit, stored.mean())
+    assert np.array_equal(got[stored], whole[stored]), limit
+assert not stored.all() and lib().b200_gemm_status() == 1
+assert np.array_equal(run(4_000_000_000), whole)
+"""
+
+
+@pytest.mark.parametrize("case", [([(600, 130), (40, 2)], 32, 4, "f32"), ([(600, 130)], 96, 96, "bf16"), ([(100, 130)], 96, 96, "f32"), ([(3000, 130)], 32, 2, "bf16")])
+def test_prompts_whose_waits_run_out(case):
+    """In a process of its own: that a kernel gave up is remembered for the life of a process."""
+    tests = Path(__file__).resolve().parent
+    r = subprocess.run([sys.executable, "-c", GIVE_UP.format(root=str(tests.parent), tests=str(tests), case=case)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]

@@ -59,16 +59,16 @@ def store_args(kind, **change):
 
 COMMON = [(dict(cache=Kv8Cache(None, 4, 16, 2, 64, 64)), 2), (dict(cache=Kv8Cache(AT + 8, 4, 16, 2, 64, 64)), 2), (dict(cache=Kv8Cache(AT, 0, 16, 2, 64, 64)), 2), (dict(seq_info=None), 2),
           (dict(table=None), 2), (dict(n_seq=-1), 2), (dict(n_tokens=-1), 2), (dict(n_rows=-1), 2), (dict(table_stride=-1), 2), (dict(table_stride=1 << 30), 1), (dict(n_seq=1025), 1),
-          (dict(type=L.Q8_0), 1)]
+          (dict(type=L.Q8_0), 1), (dict(seq_info=AT + 2), 2), (dict(table=AT + 1), 2)]
 
 
-@pytest.mark.parametrize("change,code", COMMON + [(dict(k=None), 2), (dict(v=None), 2), (dict(k_stride=127), 2), (dict(v_stride=0), 2)])
+@pytest.mark.parametrize("change,code", COMMON + [(dict(k=None), 2), (dict(v=None), 2), (dict(k_stride=127), 2), (dict(v_stride=0), 2), (dict(k=AT + 2), 2), (dict(v=AT + 1), 2)])
 def test_store_refuses(change, code):
     assert lib().b200_op_kv8_store(C.byref(store_args(Kv8StoreArgs, **change)), None) == code
     assert b"b200_op_kv8_store" in lib().b200_last_error()
 
 
-@pytest.mark.parametrize("change,code", COMMON + [(dict(k_stride=127), 2), (dict(v_stride=0), 2)])
+@pytest.mark.parametrize("change,code", COMMON + [(dict(k_stride=127), 2), (dict(v_stride=0), 2), (dict(k=AT + 1), 2)])
 def test_load_refuses(change, code):
     assert lib().b200_op_kv8_load(C.byref(store_args(Kv8LoadArgs, **change)), None) == code
     assert b"b200_op_kv8_load" in lib().b200_last_error()
@@ -81,7 +81,8 @@ def attn_args(**change):
     return Kv8AttnArgs(*[f[name] for name, _ in Kv8AttnArgs._fields_])
 
 
-@pytest.mark.parametrize("change,code", COMMON + [(dict(q=None), 2), (dict(dst=None), 2), (dict(q_stride=255), 2), (dict(dst_stride=1), 2), (dict(n_head=0), 2), (dict(n_head=5), 2), (dict(n_tokens=1 << 28, n_head=8, q_stride=512, dst_stride=512), 1), (dict(window=-1), 2),
+@pytest.mark.parametrize("change,code", COMMON + [(dict(q=None), 2), (dict(dst=None), 2), (dict(q_stride=255), 2), (dict(dst_stride=1), 2), (dict(n_head=0), 2), (dict(n_head=5), 2), (dict(n_tokens=1 << 28, n_head=8, q_stride=512, dst_stride=512), 1),
+                                                  (dict(q=AT + 2), 2), (dict(dst=AT + 1), 2), (dict(sink=AT + 2), 2), (dict(window=-1), 2),
                                                   (dict(keep_first=-1), 2), (dict(softcap=-1.0), 2), (dict(softcap=float("nan")), 2), (dict(softcap=float("inf")), 2), (dict(scale=float("nan")), 2)])
 def test_attn_refuses(change, code):
     assert lib().b200_op_kv8_attn(C.byref(attn_args(**change)), AT, 1 << 30, None) == code
@@ -94,6 +95,10 @@ def test_attn_refuses_a_workspace_that_is_none():
     assert need > 0
     for ws, size in ((None, need), (AT, need - 1), (AT + 8, need)):
         assert lib().b200_op_kv8_attn(C.byref(a), ws, size, None) == 2
+
+
+def test_attn_refuses_a_limit_below_zero():
+    assert lib().b200_op_kv8_attn_wait(C.byref(attn_args()), AT, 1 << 30, -1, None) == 2
 
 
 def test_calls_without_work_touch_nothing():
