@@ -65,6 +65,62 @@ __device__ __noinline__ void kt_rescale(unsigned o_at, float alpha) {
         tmem_st32(o_at + 32 * ch, x);
     }
 }
+// 4 values of a row that this thread has written
+__device__ __forceinline__ float4 row_load4(const float *p, bool vec) {
+    if (vec) return *reinterpret_cast<const float4 *>(p);
+    return make_float4(p[0], p[1], p[2], p[3]);
+}
+// Every KT_FOLD additions (see CUT) the accumulators go to memory, where f32 additions round: to the rows of dst if they are f32, or to this CTA's share of the partial results.
+// f32, heads of 128, 64 heads, 300 tokens behind 30,000: results were off by 1.5e-4 without the factor and folds, now by 4e-7 (values around a mean) to 1.4e-6 (around 0).  It
+// takes 15% of a prompt's time at 2000 to 16,000 keys (every 256 additions 7%, with twice the error).  Rows of 16 bits that one CTA finishes stay in TMEM: 100,000 keys cost
+// them 2.4e-4 before the factor (one product a key), where half a step of theirs is 2^-12 or 2^-9.
+constexpr int KT_FOLD = 128;
+// A thread's row of accumulators times `unit`, and what lies at base + at times beta (0: nothing does), to base + at (at < 0: no such row).  Eight lanes exchange their rows' pieces of
+// 16 bytes, so that each row's 32 columns are stored side by side (a lane a row took 75% of a prompt's time, 16,000 keys).
+template <int C>
+__device__ __noinline__ void kt_fold(unsigned o_at, float *base, int64_t at, bool vec, int vdim, float unit, float beta) {
+    const int lane = threadIdx.x & 31;
+    int64_t rows[8];
+    float betas[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        rows[j] = __shfl_sync(0xffffffffu, (long long)at, (lane & 24) + j);
+        betas[j] = __shfl_sync(0xffffffffu, beta, (lane & 24) + j);
+    }
+#pragma unroll 1
+    for (int ch = 0; ch < vdim; ch += 32) {
+        float v[32];
+        tmem_ld32(o_at + ch, v);
+#pragma unroll
+        for (int i = 0; i < 32; i++) v[i] *= unit;
+#pragma unroll
+        for (int s = 1; s < 8; s *= 2) {
+            const bool upper = (lane & s) != 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if (i & s) continue;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float &a = v[4 * i + e], &b = v[4 * (i | s) + e];
+                    const float got = __shfl_xor_sync(0xffffffffu, upper ? a : b, s);
+                    a = upper ? got : a;
+                    b = upper ? b : got;
+                }
+            }
+        }
+        // now piece j is number lane % 8 of row lane / 8 * 8 + j
+        const int col = ch + 4 * (lane & 7);
+        if (col >= vdim) continue;
+        float4 z[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) z[j] = rows[j] >= 0 && betas[j] != 0.f ? row_load4(base + rows[j] + col, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (rows[j] >= 0)
+                row_store4(base, B200_TYPE_F32, rows[j] + col, vec,
+                           make_float4(fmaf(z[j].x, betas[j], v[4 * j]), fmaf(z[j].y, betas[j], v[4 * j + 1]), fmaf(z[j].z, betas[j], v[4 * j + 2]), fmaf(z[j].w, betas[j], v[4 * j + 3])));
+    }
+}
 // A thread's registers from here on, by groups of four warps.  A launch has 96 a thread for 20 warps, 61,440 in all: 8 softmax warps of 144, 8 converting ones of 72
 // and 4 of 48 take just those (12 warps of 128 each with one group of rows: 49,152 of its 65,536).
 constexpr int KT_REGS_SOFTMAX = 144, KT_REGS_CONVERT = 72, KT_REGS_PRODUCTS = 48;
@@ -147,6 +203,8 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
     if (z >= splits) return;
     const int t_begin = (int)((int64_t)tiles_of.all * z / splits), n_tiles = (int)((int64_t)tiles_of.all * (z + 1) / splits) - t_begin;
     auto key_of = [&](int t) { return (t + t_begin < tiles_of.keep ? t + t_begin : t + t_begin - tiles_of.keep + tiles_of.first) * KT_KEYS; };
+    // tiles between two folds, a power of two (none: more than there are)
+    const int fold = splits > 1 || a.type == B200_TYPE_F32 ? KT_FOLD / (4 * TERMS) : 0x40000000;
     unsigned char *sq = smem, *sk = sq + GROUPS * TERMS * PANELS * KT_Q_PANEL, *sv = sk + NB * TILE;
 
     if (tid == 0) {
@@ -219,10 +277,26 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
         const int pos_lo_w = w0 < n_rows ? q.held + (row0 + w0) / group : 0, pos_hi_w = w0 < n_rows ? q.held + (row0 + w1) / group : -1;
         const bool all_rows = w0 + 31 < n_rows;
         const unsigned lanes = (unsigned)(quarter * 32) << 16, o_at = tmem_o + (unsigned)(w * C) + lanes;
-        float m = -INFINITY, l = 0.f;
+        float m = -INFINITY, l = 0.f, m_fold = -INFINITY;
         int power = -100;
         bool ok = true;
-        for (int t = 0; t < n_tiles; t++) {
+        const bool whole_block = splits == 1;
+        auto part_at = [&]() { return args.partials + ((size_t)(j * c.n_head_kv + h) * args.splits + z) * kt_part<C>(); };
+        auto fold_rows = [&](float unit, float beta) {
+            const int64_t at = whole_block ? (int64_t)(q.first + i_tok) * a.dst_stride + (int64_t)head * c.vdim : 2 * KT_ROWS + (int64_t)row * C;
+            kt_fold<C>(o_at, whole_block ? reinterpret_cast<float *>(a.dst) : part_at(), mine ? at : -1, vec || !whole_block, c.vdim, unit, beta);
+        };
+#pragma unroll 1
+        for (int t0 = 0; t0 < n_tiles && ok; t0 += min(fold, n_tiles)) {
+        if (t0 > 0) {
+            ok = kt_wait<20>(&o_done[w][1], ((t0 - 1) >> 1) & 1, &failed, limit);
+            if (!ok) break;
+            tc_fence_after();
+            fold_rows(pow2i(power - HEAD) * (1.0f + KT_FOLD * CUT), t0 == fold ? 0.f : m == m_fold ? 1.0f : ex2(m_fold - m));
+            m_fold = m;
+        }
+        const int t1 = t0 + min(fold, n_tiles - t0);
+        for (int t = t0; t < t1; t++) {
             const int b = t & 1, key0 = key_of(t);
             const unsigned s_at = tmem + (unsigned)((w * 2 + b) * KT_KEYS) + lanes;
             ok = kt_wait<0>(&scales_full[t % KT_RING], (t / KT_RING) & 1, &failed, limit);
@@ -287,7 +361,7 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
                     float alpha = grown ? ex2(m - top) : 1.0f;
                     if (grown) { m = top; l *= alpha; }
                     if (now > power) { alpha *= pow2i(max(power - now, -126)); power = now; }
-                    if (t > 0) {
+                    if (t > t0) {
                         ok = kt_wait<20>(&o_done[w][b ^ 1], ((t - 1) >> 1) & 1, &failed, limit);  // (the second product of the tile before may be under way)
                         if (!ok) break;
                         tc_fence_after();
@@ -320,21 +394,28 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[w][b]);
         }
+        }
         // ===== results
         ok = ok && kt_wait<20>(&o_done[w][(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, &failed, limit);
         tc_fence_after();
-        // (a stretch that was given up: NaN rows rather than what an earlier call left there)
-        float *part = args.partials + ((size_t)(j * c.n_head_kv + h) * args.splits + z) * kt_part<C>();
-        if (!ok && splits > 1 && mine) { part[row] = -INFINITY; part[KT_ROWS + row] = __uint_as_float(0x7fc00000u); }
+        const bool folded = n_tiles > fold;
+        float *part = part_at();
+        __syncwarp();
+        if (!ok && mine) {  // given up: NaN rows rather than what an earlier call or this one left there
+            const float nan = __uint_as_float(0x7fc00000u);
+            if (!whole_block) { part[row] = -INFINITY; part[KT_ROWS + row] = nan; }
+            else if (folded) for (int e = 0; e < c.vdim; e++) reinterpret_cast<float *>(a.dst)[(int64_t)(q.first + i_tok) * a.dst_stride + (int64_t)head * c.vdim + e] = nan;
+        }
         if (ok) {
             const float sink = a.sink ? a.sink[head] * LOG2E : -INFINITY;
             const float mm = fmaxf(m, sink), f = m == -INFINITY ? (l == 0.f ? 0.f : 1.0f) : ex2(m - mm);
             const float sum = l * f + (sink == -INFINITY ? 0.f : ex2(sink - mm));
             const float inv = sum == 0.f ? 0.f : f / sum, back = pow2i(power - HEAD);
             // (a stretch of the tiles: relative to its own maximum, which goes with its sum to where kv8_attn_join_kernel finds it)
-            const bool whole_block = splits == 1;
-            const float share = !whole_block ? back : sum == 0.f ? 0.f : inv * back;
+            const float all = whole_block ? inv : 1.0f, share = all * back * (1.0f + (float)(((n_tiles - 1) & (fold - 1)) + 1) * (4 * TERMS * CUT));
+            const float beta = m == m_fold ? all : all * ex2(m_fold - m);
             if (!whole_block && mine) { part[row] = m; part[KT_ROWS + row] = l; }
+            if (folded) fold_rows(share, beta);
             // 32 columns at a time through shared memory (where this warp's rows of Q were), so that a row's stores lie side by side
             unsigned char *stage = sq + w * TERMS * PANELS * KT_Q_PANEL + quarter * 4096;
             const int e = lane & 7;
@@ -346,7 +427,7 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
                 at[k] = rb < n_rows ? row_at + 4 * e : -1;
             }
 #pragma unroll 1
-            for (int ch = 0; ch < c.vdim; ch += 32) {
+            for (int ch = folded ? c.vdim : 0; ch < c.vdim; ch += 32) {
                 float v[32];
                 tmem_ld32(o_at + ch, v);
 #pragma unroll
@@ -465,14 +546,14 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
                     const unsigned long long kd = kd0 + (unsigned)(nb * (TILE >> 4));
                     if (steps == C / 16) {
 #pragma unroll
-                        for (int term = 0; term < TERMS; term++)
+                        for (int term = TERMS - 1; term >= 0; term--)  // (small products first: less is cut off)
 #pragma unroll
                             for (int k = 0; k < C / 16; k++)
-                                tc_mma_bf16(sd, qd + (unsigned)((term * PANELS + k / 4) * (KT_Q_PANEL >> 4) + 2 * (k % 4)), kd + (unsigned)(k / 4 * (KT_PANEL >> 4) + 2 * (k % 4)), kt_idesc(KT_KEYS, false), term + k != 0);
+                                tc_mma_bf16(sd, qd + (unsigned)((term * PANELS + k / 4) * (KT_Q_PANEL >> 4) + 2 * (k % 4)), kd + (unsigned)(k / 4 * (KT_PANEL >> 4) + 2 * (k % 4)), kt_idesc(KT_KEYS, false), term != TERMS - 1 || k != 0);
                     } else {
 #pragma unroll 1
                         for (int i = 0; i < TERMS * steps; i++) {
-                            const int term = i >= steps, k = i - term * steps;
+                            const int term = TERMS - 1 - (i >= steps), k = i >= steps ? i - steps : i;
                             tc_mma_bf16(sd, qd + (unsigned)((term * PANELS + k / 4) * (KT_Q_PANEL >> 4) + 2 * (k % 4)), kd + (unsigned)(k / 4 * (KT_PANEL >> 4) + 2 * (k % 4)), kt_idesc(KT_KEYS, false), i != 0);
                         }
                     }
@@ -499,7 +580,7 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
 #pragma unroll
                     for (int term = 0; term < TERMS; term++)
 #pragma unroll
-                        for (int k = 0; k < KT_KEYS / 16; k++) ft_mma_ts(out, pd + 32 * term + 8 * k, vd + (unsigned)(k * (2048 >> 4)), idesc, t + term + k != 0);
+                        for (int k = 0; k < KT_KEYS / 16; k++) ft_mma_ts(out, pd + 32 * term + 8 * k, vd + (unsigned)(k * (2048 >> 4)), idesc, (t & (fold - 1)) + term + k != 0);
                     tc_commit(&o_done[w][b]);
                     tc_commit(&v_free[nb]);
                 }

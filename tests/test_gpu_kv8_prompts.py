@@ -270,6 +270,21 @@ def test_steps_that_say_what_cannot_be(n_head, heads, name):
     compare(fine, q, name, n_head, 0.125, got, window=100)
 
 
+@pytest.mark.parametrize("extra", [0, 1])
+@pytest.mark.parametrize("n_head,heads,new", [(40, 40, 520), (64, 4, 64)])
+def test_sums_of_many_keys_do_not_drift(n_head, heads, new, extra):
+    """Means of 12,000 values of one sign (q = 0: every weight is 1).  Between two folds there are 128 additions, each off by less than 2^-23 of a sum that grows evenly: 2^-17 of the
+    result, less what the factor gives back.  The sum of the weights takes one rounding for each 64 keys, folding one for each 1024: below 200 2^-24.  Weights: 2^-22."""
+    case = Case([(12000, new)], 64, heads, 16, 64, seed=37)
+    case.pool.put(case.pool.k, np.abs(case.pool.v.astype(np.int16)), case.pool.ks, case.pool.vs)
+    cache = case.upload()
+    got, _ = attend(case, cache, np.zeros((new, n_head, 16)), "f32", n_head, 0.25, extra=extra)
+    v = case.pool.rows(case.table[case.order[0]], 12000 + new, "v")[0]
+    n = np.arange(12001, 12001 + new)
+    want = np.repeat((np.cumsum(v, axis=0)[12000:] / n[:, None, None]), n_head // heads, axis=1)
+    assert (np.abs(got - want) <= (2.0 ** -17 + 200 * 2.0 ** -24 + 2.0 ** -22) * want).all()
+
+
 GIVE_UP = """
 import sys
 sys.path[:0] = [{root!r}, {tests!r}]
