@@ -81,9 +81,9 @@ B200_API int b200_op_kv8_load(const b200_kv8_load_args *a, b200_stream_t stream)
  * window or j < keep_first.  score = scale * q . k, softcap * tanh(score / softcap) where softcap > 0; softmax in f32, whose denominator
  * also holds exp(sink[h]) when sink != NULL.  A token that sees nothing gets zeros.  Rows of dst that belong to no sequence stay as they are.
  * q [n_tokens][n_head * dim], dst [n_tokens][n_head * vdim], of one type.  Sums, maxima and exponentials are f32.  int8 is exact in f16, which
- * the tensor cores take: with rows of 16 bits, and with f16_products != 0, queries and weights are rounded to f16 (relative to the row's largest);
- * else they enter as two f16 each, 22 bits.  Results of f32 are off by 1e-6 or so of
- * their size, whatever the length (rows of 16 bits by 2^-11 and their own rounding).  A query that is not finite gives NaN.
+ * the tensor cores take: with rows of bf16, and with f16_products != 0, queries and weights are rounded to f16 (relative to the row's largest); with rows
+ * of f16 weights enter as two f16, 22 bits, and queries as they are; with rows of f32 both as two.  Results of f32 are off by 1e-6 or so of their size,
+ * whatever the length, those of 16 bits by 2^-11 where weights are rounded and by their own rounding.  A query that is not finite gives NaN.
  * max_new: no sequence of the step has more new tokens than that (0: not known).  It only chooses how the work is laid out.
  * n_tokens * n_head below 2^31.  The workspace is zero before its first call and may then go from call to call of one stream, whatever their sizes; the bytes
  * asked for do not depend on lengths.  */

@@ -130,7 +130,7 @@ __device__ __forceinline__ int rw_piece(int r, int c) {
     else return r * C + (((c & ~7) | ((c & 7) ^ ((r & 1) << 2 | (r >> 1 & 3)))) << 4);
 }
 
-template <int C, int TERMS>
+template <int C, int TERMS, bool REST>
 __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kernel(const __grid_constant__ AttnArgs args, bool vec) {
     pdl_enter();
     constexpr int R = 16 / TERMS, NR = 2 / TERMS;  // rows of a block; a thread's rows in the MMA's result
@@ -410,6 +410,7 @@ __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kern
 #pragma unroll
                 for (int i = 0; i < NT; i++) { o[i][0] *= corr[0]; o[i][1] *= corr[0]; o[i][2] *= corr[NR - 1]; o[i][3] *= corr[NR - 1]; }
             }
+            unsigned rest[2][4];  // REST: what f16 leaves over of them
             unsigned pf[2][4];  // the weights as the second product's first operand, for the two 16s of keys
 #pragma unroll
             for (int r = 0; r < NR; r++) {
@@ -426,6 +427,10 @@ __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kern
                     const unsigned x = pack_half(w[4 * half], w[4 * half + 1]), y = pack_half(w[4 * half + 2], w[4 * half + 3]);
                     pf[half][r] = x;
                     pf[half][2 + r] = y;
+                    if constexpr (REST) {
+                        rest[half][r] = pack_rest(w[4 * half], w[4 * half + 1], x);
+                        rest[half][2 + r] = pack_rest(w[4 * half + 2], w[4 * half + 3], y);
+                    }
                     if constexpr (TERMS == 2) {
                         pf[half][1] = pack_rest(w[4 * half], w[4 * half + 1], x);
                         pf[half][3] = pack_rest(w[4 * half + 2], w[4 * half + 3], y);
@@ -458,7 +463,10 @@ __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kern
                         pairs_to_half(wv[0][w], wv[1][w], b0);
                         pairs_to_half(wv[2][w], wv[3][w], b1);
 #pragma unroll
-                        for (int j = 0; j < 4; j++) mma_f16(o[16 * cb + 4 * w + j], pf[half], b0[j], b1[j]);
+                        for (int j = 0; j < 4; j++) {
+                            if constexpr (REST) mma_f16(o[16 * cb + 4 * w + j], rest[half], b0[j], b1[j]);
+                            mma_f16(o[16 * cb + 4 * w + j], pf[half], b0[j], b1[j]);
+                        }
                     }
                 }
             }
@@ -512,7 +520,7 @@ __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kern
             }
             const float share = whole_block && tid < n_rows ? finish(tid, top, total) : 1.0f;
 #pragma unroll
-            for (int w = 0; w < RW_WARPS; w++) fac_s[w][tid] = f[w] * pow2i(power_s[w][tid] - HEAD) * share * (1.0f + (float)n_here * (RW_TILE / 16 * CUT));
+            for (int w = 0; w < RW_WARPS; w++) fac_s[w][tid] = f[w] * pow2i(power_s[w][tid] - HEAD) * share * (1.0f + (float)n_here * (RW_TILE / 16 * (REST ? 2 : 1) * CUT));
             top_s[0][tid] = top;
             total_s[0][tid] = total;
         }
@@ -629,16 +637,16 @@ static int rows_grid(const b200_kv8_cache &c) {
 }
 // counters in front of the partial results: as many for heads of all sizes, so that none lies where a call before left partial results
 static size_t rows_counter_bytes() { return ((size_t)sm_count() * rw_per_sm<64>() * 4 + 255) / 256 * 256; }
-template <int C, int TERMS>
+template <int C, int TERMS, bool REST>
 static int launch_rows(const AttnArgs &args, bool vec, cudaStream_t st) {
     static bool done[16] = {};  // cudaFuncSetAttribute is per device
     int dev = 0;
     B200_CUDA_TRY(cudaGetDevice(&dev));
     if (dev >= 16 || !done[dev]) {
-        B200_CUDA_TRY(cudaFuncSetAttribute(kv8_attn_rows_kernel<C, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, rw_fixed<C>() + 8 * B200_KV8_MAX_SEQ));
+        B200_CUDA_TRY(cudaFuncSetAttribute(kv8_attn_rows_kernel<C, TERMS, REST>, cudaFuncAttributeMaxDynamicSharedMemorySize, rw_fixed<C>() + 8 * B200_KV8_MAX_SEQ));
         if (dev < 16) done[dev] = true;
     }
-    B200_CUDA_TRY(launch_chained(kv8_attn_rows_kernel<C, TERMS>, (unsigned)rows_grid(args.a.cache), RW_THREADS, (size_t)rw_fixed<C>() + 8 * (size_t)args.a.n_seq, st, args, vec));
+    B200_CUDA_TRY(launch_chained(kv8_attn_rows_kernel<C, TERMS, REST>, (unsigned)rows_grid(args.a.cache), RW_THREADS, (size_t)rw_fixed<C>() + 8 * (size_t)args.a.n_seq, st, args, vec));
     return B200_OK;
 }
 
@@ -666,7 +674,9 @@ static int check_attn(const b200_kv8_attn_args *a, const char *who) {
 //   bf16, 16 sequences:                         5 tokens  9.3 : 18.9, 29.7 : 36.8, 136 : 192     9 tokens 10 : 18, 38 : 35, 195 : 183    17 tokens 15 : 18, 56 : 36, 310 : 185
 // (how long the past is, only the device knows; 5 tokens of 4 heads are 20 rows, 9 are 36)
 constexpr int ROWS_MOST = 32, PROMPT_ROWS = 4096;
+// queries as one f16 (rows of 16 bits: exactly, but for values far below a row's largest), weights as one (no more bits are asked for than bf16 has, or f16_products allows)
 static bool one_term(const b200_kv8_attn_args *a) { return a->type != B200_TYPE_F32 || a->f16_products != 0; }
+static bool one_weight(const b200_kv8_attn_args *a) { return a->type == B200_TYPE_BF16 || a->f16_products != 0; }
 
 // whether some sequences of a step can be the prompt kernel's (which sequences have how many tokens is known on the device only)
 static bool has_prompts(const b200_kv8_attn_args *a) {
@@ -682,16 +692,17 @@ static PromptPlan prompt_plan(const b200_kv8_attn_args *a) {
     const int64_t ctas = a->n_seq * ((each + KT_ROWS - 1) / KT_ROWS) * a->cache.n_head_kv;
     return {ctas > sm_count(), (int)std::max<int64_t>(1, std::min<int64_t>(sm_count() / ctas, KT_SPLITS))};
 }
-static int launch_prompt(AttnArgs &args, bool vec, int k, bool one, long long limit, cudaStream_t st) {
+template <int C, int GROUPS>
+static int launch_prompt_terms(const AttnArgs &args, bool vec, long long limit, cudaStream_t st) {
+    if (!one_term(&args.a)) return launch_tc<C, GROUPS, 2, 2>(args, vec, limit, st);
+    return one_weight(&args.a) ? launch_tc<C, GROUPS, 1, 1>(args, vec, limit, st) : launch_tc<C, GROUPS, 1, 2>(args, vec, limit, st);
+}
+static int launch_prompt(AttnArgs &args, bool vec, int k, long long limit, cudaStream_t st) {
     const PromptPlan plan = prompt_plan(&args.a);
     const bool two = plan.two;
     args.splits = plan.splits;
-    if (k == 64) {
-        if (two) return one ? launch_tc<64, 2, 1>(args, vec, limit, st) : launch_tc<64, 2, 2>(args, vec, limit, st);
-        return one ? launch_tc<64, 1, 1>(args, vec, limit, st) : launch_tc<64, 1, 2>(args, vec, limit, st);
-    }
-    if (two) return one ? launch_tc<128, 2, 1>(args, vec, limit, st) : launch_tc<128, 2, 2>(args, vec, limit, st);
-    return one ? launch_tc<128, 1, 1>(args, vec, limit, st) : launch_tc<128, 1, 2>(args, vec, limit, st);
+    if (k == 64) return two ? launch_prompt_terms<64, 2>(args, vec, limit, st) : launch_prompt_terms<64, 1>(args, vec, limit, st);
+    return two ? launch_prompt_terms<128, 2>(args, vec, limit, st) : launch_prompt_terms<128, 1>(args, vec, limit, st);
 }
 
 }  // namespace kv8
@@ -736,11 +747,12 @@ int b200_op_kv8_attn_wait(const b200_kv8_attn_args *a, void *workspace, size_t w
     const bool vec = rows_aligned(a->q, a->q_stride, a->type) && rows_aligned(a->dst, a->dst_stride, a->type);
     if (has_prompts(a)) {
         args.rows_most = ROWS_MOST;
-        const int rc2 = launch_prompt(args, vec, k, one_term(a), wait_cycles, st);
+        const int rc2 = launch_prompt(args, vec, k, wait_cycles, st);
         if (rc2 != B200_OK) return rc2;
     }
-    if (one_term(a)) return k == 64 ? launch_rows<64, 1>(args, vec, st) : k == 128 ? launch_rows<128, 1>(args, vec, st) : launch_rows<256, 1>(args, vec, st);
-    return k == 64 ? launch_rows<64, 2>(args, vec, st) : k == 128 ? launch_rows<128, 2>(args, vec, st) : launch_rows<256, 2>(args, vec, st);
+    if (!one_term(a)) return k == 64 ? launch_rows<64, 2, false>(args, vec, st) : k == 128 ? launch_rows<128, 2, false>(args, vec, st) : launch_rows<256, 2, false>(args, vec, st);
+    if (one_weight(a)) return k == 64 ? launch_rows<64, 1, false>(args, vec, st) : k == 128 ? launch_rows<128, 1, false>(args, vec, st) : launch_rows<256, 1, false>(args, vec, st);
+    return k == 64 ? launch_rows<64, 1, true>(args, vec, st) : k == 128 ? launch_rows<128, 1, true>(args, vec, st) : launch_rows<256, 1, true>(args, vec, st);
 }
 
 }  // extern "C"

@@ -5,8 +5,8 @@
 //   P = 2^(c S - m)  a thread a row, no exchange between lanes; P goes back to TMEM as f16, in place of S
 //   O += P . V       A = P from TMEM, B = V as it lies in the page (keys are the strided side), O stays in TMEM
 // Eight warps turn int8 keys and values into f16 once for all the CTA's rows: pieces of 16 bytes come from the pages into registers a tile ahead, and leave for
-// shared memory in the 128-byte swizzle that the products read.  int8 is exact in f16, so with TERMS = 2 only Q and P have to be taken apart (upper halves
-// and what those leave over, a second product each) for results as f32 gives them; 64 columns of S are just two times 32 of P.
+// shared memory in the 128-byte swizzle that the products read.  int8 is exact in f16, so only Q (TERMS = 2) and P (WEIGHTS = 2) have to be taken apart (upper
+// halves and what those leave over, a second product each) for results as f32 gives them, rows of f16 only P; 64 columns of S are just two times 32 of P.
 // Softmax: four warps a group of 128 rows.  The maximum that the exponent subtracts follows the true one only when that has grown by SLACK, so O is hardly
 // ever rescaled.  A key's scale joins its score, a value's its weight, relative to the power of two above the largest that the row has seen.
 // Every S has two buffers a group: products run while the softmax is busy with the tile before.
@@ -165,7 +165,7 @@ __device__ __forceinline__ void row_values8(const uint4 (&u)[2], int type, float
         for (int e = 0; e < 8; e++) x[e] = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
     }
 }
-template <int C, int GROUPS, int TERMS>
+template <int C, int GROUPS, int TERMS, int WEIGHTS>
 __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(const __grid_constant__ AttnArgs args, bool vec, long long limit, int *timeout) {
     constexpr int NB = kt_buffers<GROUPS, TERMS>(), PANELS = C / 64, BLOCK = GROUPS * KT_ROWS, SOFTMAX = GROUPS * 4, CONVERT = SOFTMAX + 4;
     constexpr int TILE = PANELS * KT_PANEL;
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
     const int t_begin = (int)((int64_t)tiles_of.all * z / splits), n_tiles = (int)((int64_t)tiles_of.all * (z + 1) / splits) - t_begin;
     auto key_of = [&](int t) { return (t + t_begin < tiles_of.keep ? t + t_begin : t + t_begin - tiles_of.keep + tiles_of.first) * KT_KEYS; };
     // tiles between two folds, a power of two (none: more than there are)
-    const int fold = splits > 1 || a.type == B200_TYPE_F32 ? KT_FOLD / (4 * TERMS) : 0x40000000;
+    const int fold = splits > 1 || a.type == B200_TYPE_F32 ? KT_FOLD / (4 * WEIGHTS) : 0x40000000;
     unsigned char *sq = smem, *sk = sq + GROUPS * TERMS * PANELS * KT_Q_PANEL, *sv = sk + NB * TILE;
 
     if (tid == 0) {
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
 #pragma unroll
                 for (int i = 0; i < 32; i++) x[i] = 0u;
                 tmem_st32(s_at, x);
-                if constexpr (TERMS == 2) tmem_st32(s_at + 32, x);
+                if constexpr (WEIGHTS == 2) tmem_st32(s_at + 32, x);
             } else {
                 float v[64];
                 tmem_ld32_async(s_at, v);
@@ -384,10 +384,10 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
                     const float f = vs[i / 16] * unit;
                     const float2 e = mul2(make_float2(v[i], v[i + 1]), make_float2(f, f));
                     x[i / 2] = pack_half(e.x, e.y);
-                    if constexpr (TERMS == 2) y[i / 2] = pack_rest(e.x, e.y, x[i / 2]);
+                    if constexpr (WEIGHTS == 2) y[i / 2] = pack_rest(e.x, e.y, x[i / 2]);
                 }
                 tmem_st32(s_at, x);  // (over scores that have been read)
-                if constexpr (TERMS == 2) tmem_st32(s_at + 32, y);
+                if constexpr (WEIGHTS == 2) tmem_st32(s_at + 32, y);
             }
             tmem_wait_st();
             tc_fence_before();
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
             const float sum = l * f + (sink == -INFINITY ? 0.f : ex2(sink - mm));
             const float inv = sum == 0.f ? 0.f : f / sum, back = pow2i(power - HEAD);
             // (a stretch of the tiles: relative to its own maximum, which goes with its sum to where kv8_attn_join_kernel finds it)
-            const float all = whole_block ? inv : 1.0f, share = all * back * (1.0f + (float)(((n_tiles - 1) & (fold - 1)) + 1) * (4 * TERMS * CUT));
+            const float all = whole_block ? inv : 1.0f, share = all * back * (1.0f + (float)(((n_tiles - 1) & (fold - 1)) + 1) * (4 * WEIGHTS * CUT));
             const float beta = m == m_fold ? all : all * ex2(m_fold - m);
             if (!whole_block && mine) { part[row] = m; part[KT_ROWS + row] = l; }
             if (folded) fold_rows(share, beta);
@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
                     const unsigned pd = tmem + (unsigned)((w * 2 + b) * KT_KEYS);
                     const unsigned long long vd = vd0 + (unsigned)(nb * (TILE >> 4));
 #pragma unroll
-                    for (int term = 0; term < TERMS; term++)
+                    for (int term = 0; term < WEIGHTS; term++)
 #pragma unroll
                         for (int k = 0; k < KT_KEYS / 16; k++) ft_mma_ts(out, pd + 32 * term + 8 * k, vd + (unsigned)(k * (2048 >> 4)), idesc, (t & (fold - 1)) + term + k != 0);
                     tc_commit(&o_done[w][b]);
@@ -642,7 +642,7 @@ __global__ void __launch_bounds__(256) kv8_attn_join_kernel(const __grid_constan
     }
 }
 
-template <int C, int GROUPS, int TERMS>
+template <int C, int GROUPS, int TERMS, int WEIGHTS>
 static int launch_tc(const AttnArgs &args, bool vec, long long limit, cudaStream_t st) {
     int *status = nullptr;
     const int rc = gemm_status_word(&status);
@@ -651,11 +651,11 @@ static int launch_tc(const AttnArgs &args, bool vec, long long limit, cudaStream
     int dev = 0;
     B200_CUDA_TRY(cudaGetDevice(&dev));
     if (dev >= 16 || !done[dev]) {
-        B200_CUDA_TRY(cudaFuncSetAttribute(kv8_attn_tc_kernel<C, GROUPS, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kt_smem<C, GROUPS, TERMS>()));
+        B200_CUDA_TRY(cudaFuncSetAttribute(kv8_attn_tc_kernel<C, GROUPS, TERMS, WEIGHTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kt_smem<C, GROUPS, TERMS>()));
         if (dev < 16) done[dev] = true;
     }
     const unsigned blocks = (unsigned)(((int64_t)args.a.n_tokens * args.group / (GROUPS * KT_ROWS) + args.a.n_seq) * args.a.cache.n_head_kv);
-    B200_CUDA_TRY(launch_chained(kv8_attn_tc_kernel<C, GROUPS, TERMS>, blocks * (unsigned)args.splits, kt_threads<GROUPS>(), kt_smem<C, GROUPS, TERMS>(), st, args, vec, limit, status));
+    B200_CUDA_TRY(launch_chained(kv8_attn_tc_kernel<C, GROUPS, TERMS, WEIGHTS>, blocks * (unsigned)args.splits, kt_threads<GROUPS>(), kt_smem<C, GROUPS, TERMS>(), st, args, vec, limit, status));
     if (args.splits > 1) B200_CUDA_TRY(launch_chained(kv8_attn_join_kernel<C>, dim3(blocks, KT_ROWS / KJ_ROWS), 256, 0, st, args, vec));
     return B200_OK;
 }
