@@ -54,6 +54,8 @@ __device__ __forceinline__ float max_nan(float x, float y, float z) {  // NaN if
 // before if the scale grew, the new values.  The values wait in registers as they came (KEEP pieces of 16 a thread; of a page with more they are read twice).
 // Item j of the grid is a page of sequence s where first_s / page_size + 2 s <= j: a sequence of n tokens touches n / page_size + 2 pages at most, so
 // the items of the sequences do not overlap and nothing has to be summed up beforehand.
+// Measured: prompts of 3 sequences, 32 heads of 128, bf16, 377 MB in 83 us, 4.5 TB/s (issue 66% of the cycles: 3 rounds of arithmetic a value, of which two check the
+// rounding); one token each of 64 sequences, 8 heads, f32: 10 us, of which two ways to memory (the step, then the page and the rows) and their launch are nearly all.
 constexpr int ST_THREADS = 128;
 struct StoreArgs {
     b200_kv8_cache cache;
@@ -180,7 +182,7 @@ __global__ void __launch_bounds__(2 * ST_THREADS, 4) kv8_store_kernel(const Stor
 }
 
 // ------------------------------------------------------------------------------------------------ load
-// One CTA per token: its page once, then pieces of 16 values of all heads, keys before values.
+// One CTA per token: its page once, then pieces of 16 values of all heads, keys before values.  Bound by memory; meant for looking at a cache, and for carrying it elsewhere.
 constexpr int LD_THREADS = 256;
 struct LoadArgs {
     b200_kv8_cache cache;
@@ -224,7 +226,8 @@ __global__ void __launch_bounds__(LD_THREADS) kv8_load_kernel(const LoadArgs a) 
 // ------------------------------------------------------------------------------------------------ pages
 struct Records { unsigned char *pages[B200_KV8_MAX_CACHES]; unsigned bytes[B200_KV8_MAX_CACHES]; };  // of up to so many caches, as a kernel's argument
 
-// 16 bytes a thread and round, four rounds in flight
+// 16 bytes a thread and round, four rounds in flight.  Copies of pages are bound by memory: in compaction (32 layers, half of the pages live) 526 MB in 88 us of 108, 6 TB/s; the
+// rest are counting and ranking, 10 us each.  16 continuations of 4 prompts that grow, 32 layers: 135 MB in 27 us, 10 of them growing.
 constexpr int CP_THREADS = 256;
 __device__ __forceinline__ void copy_record(unsigned char *base, unsigned bytes, int src, int dst) {
     const uint4 *from = reinterpret_cast<const uint4 *>(base + (size_t)src * bytes);
@@ -314,6 +317,7 @@ __device__ __forceinline__ int scan_1024(int x, int *sh, int &all) {
 
 // One CTA, a thread per row of the list: what each needs, sums before it, then the free pages in ascending order, each to the row whose share
 // it falls in.  The free pages are counted first (as many as are asked for), because a row that does not get all it needs gets nothing.
+// One CTA, because rows are served in order and free pages by number; 48 rows take 9.6 us, all of it latency (8192 entries of refs a round, most often the only one).
 constexpr int GR_EACH = 8;  // neighbouring entries of refs a thread looks at per round
 __global__ void __launch_bounds__(1024) kv8_grow_kernel(const Map m, const int32_t *__restrict__ rows, const int32_t *__restrict__ n_new, int n, int32_t *__restrict__ seq_info, int32_t *refused,
                                                         int32_t *__restrict__ pairs) {
