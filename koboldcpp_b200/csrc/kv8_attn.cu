@@ -4,6 +4,7 @@
 #include <type_traits>
 
 #include "kv8.cuh"
+#include "tcgen05.cuh"
 
 namespace b200 {
 namespace kv8 {
@@ -90,7 +91,7 @@ constexpr int HEAD = 6;
 constexpr float SLACK = 8.0f;
 
 // The tensor cores cut their sums off below the last place instead of rounding them: an addition loses half a last place on average, which is 0.72 2^-24 of a sum whose magnitude
-// is spread evenly over a binade, and half of that of what a sum that grows evenly comes to.  A result of n additions is that much too small (measured, values around a mean: 1.7e-6
+// is spread evenly over a binade, and half of that of what a sum that grows evenly comes to.  A result of n additions of the prompt kernel is that much too small (measured, values around a mean: 1.7e-6
 // after 81 additions, 7.4e-6 after 270, 1.5e-4 after 3800), so it is taken times 1 + n CUT.
 constexpr float CUT = 0.36f / 16777216.0f;
 
@@ -421,10 +422,10 @@ __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kern
                 float w[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float e = ex2(p[r][i] - mb);
-                    l[r] += e;
-                    w[i] = e * (i < 4 ? vs0 : vs1);
+                    p[r][i] = ex2(p[r][i] - mb);
+                    w[i] = p[r][i] * (i < 4 ? vs0 : vs1);
                 }
+                l[r] += ((p[r][0] + p[r][1]) + (p[r][2] + p[r][3])) + ((p[r][4] + p[r][5]) + (p[r][6] + p[r][7]));  // (one rounding of the running sum a tile)
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
                     const unsigned x = pack_half(w[4 * half], w[4 * half + 1]), y = pack_half(w[4 * half + 2], w[4 * half + 3]);
@@ -441,10 +442,14 @@ __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kern
                 }
             }
             // ---- weights times values: thread g brings the dims of its own 8 (C = 64) or 16 bytes (and those 128 further on) of keys 2 tg, 2 tg + 1, 2 tg + 8, 2 tg + 9
+            // The tensor cores cut their sums off instead of rounding them, which a long sum shows as a drift (every addition takes up to 2^-23 of what has been summed up): the products of 16 keys
+            // begin at 0, and what they come to is added to o by f32 additions.  (One-term rows of 128 and more dims: one half's code for both, or registers spill, 63.7 us for 60.9 of a
+            // serving step; the others lose 2 to 3% by that.)
             const unsigned char *sv = stage + RW_TILE * C;
             constexpr int BYTES = C == 64 ? 8 : 16;
-#pragma unroll
+#pragma unroll(C >= 128 && TERMS == 1 && !REST ? 1 : 2)
             for (int half = 0; half < 2; half++) {
+                const unsigned pw[4] = {half ? pf[1][0] : pf[0][0], half ? pf[1][1] : pf[0][1], half ? pf[1][2] : pf[0][2], half ? pf[1][3] : pf[0][3]};
 #pragma unroll
                 for (int cb = 0; cb < (C == 256 ? 2 : 1); cb++) {
                     const int piece = C == 64 ? g >> 1 : (g >> 1 | (g & 1) << 2) + 8 * cb, inside = C == 64 ? (g & 1) * 8 : 0;
@@ -467,8 +472,12 @@ __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kern
                         pairs_to_half(wv[2][w], wv[3][w], b1);
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
-                            if constexpr (REST) mma_f16(o[16 * cb + 4 * w + j], rest[half], b0[j], b1[j]);
-                            mma_f16(o[16 * cb + 4 * w + j], pf[half], b0[j], b1[j]);
+                            float d[4] = {0.f, 0.f, 0.f, 0.f};
+                            if constexpr (REST) mma_f16(d, rest[half], b0[j], b1[j]);
+                            mma_f16(d, pw, b0[j], b1[j]);
+                            float(&to)[4] = o[16 * cb + 4 * w + j];
+                            const float2 x = ft_add2(make_float2(to[0], to[1]), make_float2(d[0], d[1])), y = ft_add2(make_float2(to[2], to[3]), make_float2(d[2], d[3]));
+                            to[0] = x.x; to[1] = x.y; to[2] = y.x; to[3] = y.y;
                         }
                     }
                 }
@@ -523,7 +532,7 @@ __global__ void __launch_bounds__(RW_THREADS, rw_per_sm<C>()) kv8_attn_rows_kern
             }
             const float share = whole_block && tid < n_rows ? finish(tid, top, total) : 1.0f;
 #pragma unroll
-            for (int w = 0; w < RW_WARPS; w++) fac_s[w][tid] = f[w] * pow2i(power_s[w][tid] - HEAD) * share * (1.0f + (float)n_here * (RW_TILE / 16 * (REST ? 2 : 1) * CUT));
+            for (int w = 0; w < RW_WARPS; w++) fac_s[w][tid] = f[w] * pow2i(power_s[w][tid] - HEAD) * share;
             top_s[0][tid] = top;
             total_s[0][tid] = total;
         }
