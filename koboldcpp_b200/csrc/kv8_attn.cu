@@ -90,19 +90,15 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int HEAD = 6;
 constexpr float SLACK = 8.0f;
 
-// The tensor cores cut their sums off below the last place instead of rounding them: an addition loses half a last place on average, which is 0.72 2^-24 of a sum whose magnitude
-// is spread evenly over a binade, and half of that of what a sum that grows evenly comes to.  A result of n additions of the prompt kernel is that much too small (measured, values around a mean: 1.7e-6
-// after 81 additions, 7.4e-6 after 270, 1.5e-4 after 3800), so it is taken times 1 + n CUT.
-constexpr float CUT = 0.36f / 16777216.0f;
-
 struct AttnArgs {
     b200_kv8_attn_args a;
     Step step;
-    int *counters;    // one per CTA, zero between calls
+    int *counters;    // one per CTA, zero between calls (the prompt kernel's: which of its places are taken)
     float *partials;  // two per CTA
     int group;        // query heads per kv head
     unsigned group_div;  // ceil(2^32 / group): __umulhi(x, group_div) = x / group for x < 2^32 / group
     int table_tokens; // tokens that the table has entries for, at least 1: nobody has to look behind them
+    int places;       // for rows that a CTA of the prompt kernel folds (kt_take)
     int splits;       // a prompt's block of rows may be shared by so many CTAs, each with a stretch of its tiles
     int rows_most;    // sequences with more query rows a kv head (tokens times group) are the prompt kernel's; negative: there is none
 };
@@ -734,7 +730,7 @@ extern "C" {
 size_t b200_kv8_attn_workspace_bytes(const b200_kv8_attn_args *a) {
     if (!a || b200_kv8_page_bytes(a->cache.page_size, a->cache.n_head_kv, a->cache.dim, a->cache.vdim) == 0) return 0;
     const int grid = rows_grid(a->cache), k = attn_class(a->cache);
-    // (the two kernels' partial results are not there at the same time; the prompt kernel's grid has room for twice the blocks that its plan counts)
+    // (the two kernels' partial results are not there at the same time; the prompt kernel's are those of twice the blocks that its plan counts, or as many places of up to 256 rows as SMs)
     const size_t rows = (size_t)grid * 2 * (one_term(a) ? 16 : 8) * (k + 2) * 4, prompts = k <= 128 ? (size_t)2 * sm_count() * KT_ROWS * (k + 2) * 4 : 0;
     return rows_counter_bytes() + (rows > prompts ? rows : prompts);
 }
@@ -752,7 +748,7 @@ int b200_op_kv8_attn_wait(const b200_kv8_attn_args *a, void *workspace, size_t w
                 b200_kv8_attn_workspace_bytes(a));
     const b200_kv8_cache &c = a->cache;
     AttnArgs args = {*a, {a->seq_info, a->table, a->table_stride, a->n_rows, a->n_seq, a->n_tokens, c.n_pages, c.page_size}, (int *)workspace,
-                     (float *)((char *)workspace + rows_counter_bytes()), a->n_head / c.n_head_kv, 0, std::max(1, (int)a->table_stride * c.page_size), 1, -1};
+                     (float *)((char *)workspace + rows_counter_bytes()), a->n_head / c.n_head_kv, 0, std::max(1, (int)a->table_stride * c.page_size), sm_count(), 1, -1};
     args.group_div = (unsigned)(((1ull << 32) + args.group - 1) / args.group);
     const cudaStream_t st = (cudaStream_t)stream;
     const int k = attn_class(c);

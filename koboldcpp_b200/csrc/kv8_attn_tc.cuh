@@ -73,11 +73,23 @@ __device__ __forceinline__ float4 row_load4(const float *p, bool vec) {
     if (vec) return *reinterpret_cast<const float4 *>(p);
     return make_float4(p[0], p[1], p[2], p[3]);
 }
-// Every KT_FOLD additions (see CUT) the accumulators go to memory, where f32 additions round: to the rows of dst if they are f32, or to this CTA's share of the partial results.
-// f32, heads of 128, 64 heads, 300 tokens behind 30,000: results were off by 1.5e-4 without the factor and folds, now by 4e-7 (values around a mean) to 1.4e-6 (around 0).  It
-// takes 15% of a prompt's time at 2000 to 16,000 keys (every 256 additions 7%, with twice the error).  Rows of 16 bits that one CTA finishes stay in TMEM: 100,000 keys cost
-// them 2.4e-4 before the factor (one product a key), where half a step of theirs is 2^-12 or 2^-9.
-constexpr int KT_FOLD = 128;
+// The tensor cores cut their sums off below the last place instead of rounding them: an addition takes up to 2^-23 of what has been summed up, half a last place on average, and a sum that is
+// kept in TMEM drifts (values around a mean: 1.7e-6 of the result after 81 additions, 7.4e-6 after 270, 1.5e-4 after 3800).  So after kt_fold_every additions the accumulators go to
+// memory, where f32 additions round, and begin at 0 again: to the rows of dst if they are f32, to this CTA's share of the partial results if several share a block, or to a place
+// that the CTA takes from the workspace for as long as it runs.  Rows of full precision 128 additions: 2.7e-6 of a result that grows evenly at most, 15% of a prompt's time at 2000 to 16,000 keys
+// (64: half of the error, 31%; 256: twice, 6%).  Where queries and weights are one f16, or results have 16 bits, 512: 1.1e-5, where half a step of f16 is 2.4e-4 or more.
+template <int TERMS> constexpr int kt_fold_every() { return TERMS == 2 ? 128 : 512; }
+// A place for GROUPS times 128 rows: there are as many as SMs, which run one CTA each (registers), so one is free.  -1: none was.
+__device__ __forceinline__ int kt_take(int *places, int n) {
+    for (int k = 0; k < 64 * n; k++) {
+        const int i = (int)((blockIdx.x + (unsigned)k) % (unsigned)n);
+        if (atomicCAS(places + i, 0, 1) == 0) {
+            __threadfence();
+            return i;
+        }
+    }
+    return -1;
+}
 // A thread's row of accumulators times `unit`, and what lies at base + at times beta (0: nothing does), to base + at (at < 0: no such row).  Eight lanes exchange their rows' pieces of
 // 16 bytes, so that each row's 32 columns are stored side by side (a lane a row took 75% of a prompt's time, 16,000 keys).
 template <int C>
@@ -122,6 +134,16 @@ __device__ __noinline__ void kt_fold(unsigned o_at, float *base, int64_t at, boo
             if (rows[j] >= 0)
                 row_store4(base, B200_TYPE_F32, rows[j] + col, vec,
                            make_float4(fmaf(z[j].x, betas[j], v[4 * j]), fmaf(z[j].y, betas[j], v[4 * j + 1]), fmaf(z[j].z, betas[j], v[4 * j + 2]), fmaf(z[j].w, betas[j], v[4 * j + 3])));
+    }
+}
+// Rows that kt_fold has put together at base + at go to dst + to in their type; a thread reads what it has written itself.
+__device__ __noinline__ void kt_put(const float *base, int64_t at, void *dst, int type, int64_t to, bool vec, int vdim) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int j = 0; j < 8; j++) {
+        const int64_t from = __shfl_sync(0xffffffffu, (long long)at, (lane & 24) + j), out = __shfl_sync(0xffffffffu, (long long)to, (lane & 24) + j);
+        if (from < 0) continue;
+        for (int col = 4 * (lane & 7); col < vdim; col += 32) row_store4(dst, type, out + col, vec, row_load4(base + from + col, true));
     }
 }
 // A thread's registers from here on, by groups of four warps.  A launch has 96 a thread for 20 warps, 61,440 in all: 8 softmax warps of 144, 8 converting ones of 72
@@ -181,6 +203,7 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
     __shared__ int there_s[KT_RING];                      // bit i: their page is there
     __shared__ __align__(8) unsigned long long scales_full[KT_RING];
     __shared__ volatile int failed;
+    __shared__ int place_s;
     const b200_kv8_attn_args &a = args.a;
     const b200_kv8_cache &c = a.cache;
     const Step &st = args.step;
@@ -206,8 +229,8 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
     if (z >= splits) return;
     const int t_begin = (int)((int64_t)tiles_of.all * z / splits), n_tiles = (int)((int64_t)tiles_of.all * (z + 1) / splits) - t_begin;
     auto key_of = [&](int t) { return (t + t_begin < tiles_of.keep ? t + t_begin : t + t_begin - tiles_of.keep + tiles_of.first) * KT_KEYS; };
-    // tiles between two folds, a power of two (none: more than there are)
-    const int fold = splits > 1 || a.type == B200_TYPE_F32 ? KT_FOLD / (4 * WEIGHTS) : 0x40000000;
+    constexpr int fold = kt_fold_every<TERMS>() / (4 * WEIGHTS);  // tiles between two folds, a power of two
+    const bool whole_block = splits == 1, folded = n_tiles > fold, placed = folded && whole_block && a.type != B200_TYPE_F32;
     unsigned char *sq = smem, *sk = sq + GROUPS * TERMS * PANELS * KT_Q_PANEL, *sv = sk + NB * TILE;
 
     if (tid == 0) {
@@ -215,7 +238,8 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
         for (int i = 0; i < KT_RING; i++) mbar_init(&scales_full[i], 1);
         for (int i = 0; i < 2 * GROUPS; i++) { mbar_init(&s_full[i >> 1][i & 1], 1); mbar_init(&p_full[i >> 1][i & 1], 4); mbar_init(&o_done[i >> 1][i & 1], 1); }
         mbar_fence_init();
-        failed = 0;
+        place_s = placed ? kt_take(args.counters, args.places) : 0;
+        failed = place_s < 0;
     }
     constexpr unsigned TMEM = GROUPS == 2 ? 512 : 256;  // S: two buffers of 64 columns a group; then O
     if (warp == SOFTMAX) tmem_alloc(&tmem_base_s, TMEM);
@@ -282,23 +306,24 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
         const unsigned lanes = (unsigned)(quarter * 32) << 16, o_at = tmem_o + (unsigned)(w * C) + lanes;
         float m = -INFINITY, l = 0.f, m_fold = -INFINITY;
         int power = -100;
-        bool ok = true;
-        const bool whole_block = splits == 1;
+        bool ok = place_s >= 0;
         auto part_at = [&]() { return args.partials + ((size_t)(j * c.n_head_kv + h) * args.splits + z) * kt_part<C>(); };
-        auto fold_rows = [&](float unit, float beta) {
-            const int64_t at = whole_block ? (int64_t)(q.first + i_tok) * a.dst_stride + (int64_t)head * c.vdim : 2 * KT_ROWS + (int64_t)row * C;
-            kt_fold<C>(o_at, whole_block ? reinterpret_cast<float *>(a.dst) : part_at(), mine ? at : -1, vec || !whole_block, c.vdim, unit, beta);
-        };
+        auto row_at = [&]() { return (int64_t)(q.first + i_tok) * a.dst_stride + (int64_t)head * c.vdim; };  // in dst
+        // where rows are folded: dst, this CTA's place or its share of the partial results
+        auto fold_base = [&]() { return placed ? args.partials + (size_t)place_s * (BLOCK * C) : whole_block ? reinterpret_cast<float *>(a.dst) : part_at(); };
+        auto fold_at = [&]() { return !mine ? -1 : placed ? (int64_t)row * C : whole_block ? row_at() : 2 * KT_ROWS + (int64_t)row * C; };
+        auto fold_rows = [&](float unit, float beta) { kt_fold<C>(o_at, fold_base(), fold_at(), vec || placed || !whole_block, c.vdim, unit, beta); };
 #pragma unroll 1
-        for (int t0 = 0; t0 < n_tiles && ok; t0 += min(fold, n_tiles)) {
+        for (int t0 = 0; t0 < n_tiles && ok; t0 += fold) {
         if (t0 > 0) {
             ok = kt_wait<20>(&o_done[w][1], ((t0 - 1) >> 1) & 1, &failed, limit);
             if (!ok) break;
             tc_fence_after();
-            fold_rows(pow2i(power - HEAD) * (1.0f + KT_FOLD * CUT), t0 == fold ? 0.f : m == m_fold ? 1.0f : ex2(m_fold - m));
+            fold_rows(pow2i(power - HEAD), t0 == fold ? 0.f : m == m_fold ? 1.0f : ex2(m_fold - m));
             m_fold = m;
         }
-        const int t1 = t0 + min(fold, n_tiles - t0);
+        const int t1 = min(t0 + fold, n_tiles);
+#pragma unroll 1
         for (int t = t0; t < t1; t++) {
             const int b = t & 1, key0 = key_of(t);
             const unsigned s_at = tmem + (unsigned)((w * 2 + b) * KT_KEYS) + lanes;
@@ -401,13 +426,12 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
         // ===== results
         ok = ok && kt_wait<20>(&o_done[w][(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, &failed, limit);
         tc_fence_after();
-        const bool folded = n_tiles > fold;
         float *part = part_at();
         __syncwarp();
         if (!ok && mine) {  // given up: NaN rows rather than what an earlier call or this one left there
             const float nan = __uint_as_float(0x7fc00000u);
             if (!whole_block) { part[row] = -INFINITY; part[KT_ROWS + row] = nan; }
-            else if (folded) for (int e = 0; e < c.vdim; e++) reinterpret_cast<float *>(a.dst)[(int64_t)(q.first + i_tok) * a.dst_stride + (int64_t)head * c.vdim + e] = nan;
+            else if (folded && !placed) for (int e = 0; e < c.vdim; e++) reinterpret_cast<float *>(a.dst)[(int64_t)(q.first + i_tok) * a.dst_stride + (int64_t)head * c.vdim + e] = nan;
         }
         if (ok) {
             const float sink = a.sink ? a.sink[head] * LOG2E : -INFINITY;
@@ -415,10 +439,11 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
             const float sum = l * f + (sink == -INFINITY ? 0.f : ex2(sink - mm));
             const float inv = sum == 0.f ? 0.f : f / sum, back = pow2i(power - HEAD);
             // (a stretch of the tiles: relative to its own maximum, which goes with its sum to where kv8_attn_join_kernel finds it)
-            const float all = whole_block ? inv : 1.0f, share = all * back * (1.0f + (float)(((n_tiles - 1) & (fold - 1)) + 1) * (4 * WEIGHTS * CUT));
+            const float all = whole_block ? inv : 1.0f, share = all * back;
             const float beta = m == m_fold ? all : all * ex2(m_fold - m);
             if (!whole_block && mine) { part[row] = m; part[KT_ROWS + row] = l; }
             if (folded) fold_rows(share, beta);
+            if (placed) kt_put(fold_base(), fold_at(), a.dst, a.type, row_at(), vec, c.vdim);
             // 32 columns at a time through shared memory (where this warp's rows of Q were), so that a row's stores lie side by side
             unsigned char *stage = sq + w * TERMS * PANELS * KT_Q_PANEL + quarter * 4096;
             const int e = lane & 7;
@@ -600,6 +625,10 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
     }
     tc_fence_before();
     __syncthreads();
+    if (tid == 0 && placed && place_s >= 0) {
+        __threadfence();  // (what the CTA wrote there, the barrier in front)
+        atomicExch(&args.counters[place_s], 0);
+    }
     if (warp == SOFTMAX) {
         tc_fence_after();
         tmem_dealloc(tmem, TMEM);

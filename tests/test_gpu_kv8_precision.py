@@ -95,3 +95,41 @@ def test_long_sums_of_few_rows(kind, n_seq, n, heads, n_head, vdim, f16):
     assert not e.isnan().any()
     many = 0.0 if kind == "first" else 2 * 6 * 2.0 ** -24 * math.sqrt((n / 128 + 8) / 3)
     assert e.abs().max() <= 2.0 ** -21 + 2.0 ** -20 + many, float(e.abs().max())
+
+
+PROMPTS = [  # heads, n_head, new: two groups of rows a CTA; one; several CTAs a block
+    (40, 40, 520), (20, 20, 520), (4, 64, 64)]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,n_head,new", PROMPTS)
+def test_long_sums_of_prompts(kind, heads, n_head, new):
+    """f32 rows.  Between two folds 128 additions, each cutting off less than 2^-23 of the sum so far: 2^-17 of a sum that grows evenly; where all the weight is on key 0 later additions are of
+    nothing.  Folds and the sum of weights are roundings to the nearest, N = n / 64 of them, as above; weights and exponentials as above."""
+    n = 30000
+    r = Rows(kind, 1, n, new, heads, 16, 64, seed=new)
+    got = r.run("f32", n_head)
+    for token in (0, 1, new // 2, new - 1):
+        want, mass = (x.repeat_interleave(n_head // heads, dim=0) for x in r.want(token))
+        e = off(got[0, token], want, mass)
+        many = 0.0 if kind == "first" else 2.0 ** -17 + 6 * 2.0 ** -24 * math.sqrt(n / 64 / 3)
+        assert not e.isnan().any() and e.abs().max() <= 2.0 ** -20 + many, (token, float(e.abs().max()))
+
+
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,n_head,new", PROMPTS)
+def test_long_sums_of_prompts_of_16_bits(name, heads, n_head, new):
+    """100,000 keys.  Sums cut off less than 2^-23 of themselves in each of at most 512 additions between two folds: 2^-15 of sums that grow evenly, far below half a step of f16.  Weights and
+    exponentials 2^-20.  Rounding is monotone: what is off by a share d of itself before it is rounded lies between the roundings of 1 - d and 1 + d times the exact result."""
+    n, dtype = 100000, TYPES[name][1]
+    r = Rows("first", 1, n, new, heads, 16, 64, seed=new)
+    got = r.run(name, n_head)[0]
+    assert (got == (r.v[0].double() * V_SCALE).repeat_interleave(n_head // heads, dim=0)).all()  # ints of 7 bits: both types hold them
+    r = Rows("even", 1, n, new, heads, 16, 64, seed=new)
+    got = r.run(name, n_head)[0]
+    v = r.v.double() * V_SCALE
+    sums = v[:n - new].sum(0) + v[n - new:n].cumsum(0)
+    want = (sums / torch.arange(n - new + 1, n + 1, device="cuda")[:, None, None]).repeat_interleave(n_head // heads, dim=1)
+    d = 2.0 ** -15 + 2.0 ** -20
+    lo, hi = ((want * (1 + x)).to(dtype).double() for x in (-d, d))
+    assert ((got >= lo) & (got <= hi)).all()
