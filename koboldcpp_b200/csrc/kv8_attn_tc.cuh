@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kt_threads<GROUPS>(), 1) kv8_attn_tc_kernel(co
                     if (a.softcap > 0.f) {
                         const float cap_log2 = a.softcap * LOG2E;
 #pragma unroll
-                        for (int i = 0; i < 64; i++) v[i] = cap_log2 * tanh_fast(v[i]);
+                        for (int i = 0; i < 64; i++) v[i] = cap_log2 * cap_tanh<TERMS == 2>(v[i]);
                     }
                     if (!whole) {
                         seen[0] = seen_keys(key0, pos, there, a.window, a.keep_first);

@@ -133,3 +133,31 @@ def test_long_sums_of_prompts_of_16_bits(name, heads, n_head, new):
     d = 2.0 ** -15 + 2.0 ** -20
     lo, hi = ((want * (1 + x)).to(dtype).double() for x in (-d, d))
     assert ((got >= lo) & (got <= hi)).all()
+
+
+@pytest.mark.parametrize("cap", [4.0, 30.0, 50.0])
+@pytest.mark.parametrize("n_seq,new,heads,n_head,dim,vdim", [(4, 1, 8, 32, 64, 64), (1, 7, 8, 24, 128, 80), (2, 4, 1, 4, 192, 256), (1, 520, 40, 40, 64, 64), (3, 129, 4, 40, 128, 128)])
+def test_soft_cap_of_f32_rows(n_seq, new, heads, n_head, dim, vdim, cap):
+    """Every query sees two keys, whose values are v and -v: what comes out is v tanh(d / 2) of the difference d of their scores s.
+    q has 8 bits and keys 8, so products and their sums are exact in f32.  s / cap takes four roundings (2^-22 of it), tanh two units in the last place (2^-22), the way back to a score and its difference
+    from the maximum three roundings (below 2^-22 of the largest score), the exponential 2^-22 of itself, weights, their sum and the quotient 2^-21: with both scores, 2 p (1 - p) <= 1/2,
+    v (|s1| + |s2|) 2^-21 + 2^-20 v."""
+    r = Rows("zero", n_seq, 300 + new, new, heads, dim, vdim, page=32, seed=int(cap))
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    n_pages, page = r.pool.shape[0], r.page
+    sign = torch.where(torch.arange(n_pages * page, device="cuda") % 2 == 0, 1, -1).to(torch.int8)
+    k = torch.randint(-127, 128, (n_pages * page, heads, dim), generator=g, device="cuda").to(torch.int8)
+    v = sign[:, None, None] * torch.randint(60, 128, (1, heads, vdim), generator=g, device="cuda").to(torch.int8)
+    nk, nv = heads * page * dim, heads * page * vdim
+    at = r.table[0].long()
+    r.pool[at, :nk] = k.reshape(n_pages, page, heads, dim).transpose(1, 2).reshape(n_pages, nk).view(torch.uint8)
+    r.pool[at, nk:nk + nv] = v.reshape(n_pages, page, heads, vdim).transpose(1, 2).reshape(n_pages, nv).view(torch.uint8)
+    q = torch.randint(-127, 128, (n_seq, new, n_head, dim), generator=g, device="cuda").float() / 64
+    scale = float(torch.tensor(0.7 / (math.sqrt(dim) * 73 * 1.15), dtype=torch.float32))
+    got = r.run("f32", n_head, q=q.reshape(n_seq * new, -1).contiguous(), scale=scale, window=2, softcap=cap)
+    pos = torch.arange(r.n - new, r.n, device="cuda")
+    s = [cap * torch.tanh((q.double() * k[pos - i].double().repeat_interleave(n_head // heads, dim=1)).sum(-1) * scale / cap) for i in (0, 1)]
+    own = v[pos].double().repeat_interleave(n_head // heads, dim=1) * V_SCALE
+    want = own * torch.tanh((s[0] - s[1]) / 2)[..., None]
+    most = own.abs() * ((s[0].abs() + s[1].abs()) * 2.0 ** -21 + 2.0 ** -20)[..., None]
+    assert ((got - want).abs() <= most).all(), float(((got - want).abs() / most).max())
