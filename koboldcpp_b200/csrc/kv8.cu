@@ -30,11 +30,12 @@ int check_step(const b200_kv8_cache *c, const int32_t *seq_info, const int32_t *
 
 // ------------------------------------------------------------------------------------------------ store
 // Quotients x / s are rounded exactly (to the nearest integer, ties to even), |x| <= 127 s and a little.  MAGIC + x (1 / s) rounds to an integer in the lowest bits, the right one or
-// its neighbour; x less r s is exact in f32 (both are multiples of the finer of their last places, and the difference is below 2^24 of those; where |x| < s, r is 0 or +-1 and
-// the difference is Sterbenz's), and so is s / 2, so that comparisons tell whether r is the right one.  It hardly ever is not: off() says so, mend() moves it.
+// its neighbour; d = x less r s is exact in f32 (both are multiples of the finer of their last places, and the difference is below 2^24 of those; where |x| < s, r is 0 or +-1 and
+// the difference is Sterbenz's), and so is 2 d - s beside a tie: comparisons of 2 d with s tell whether r is the right one (s / 2 is no f32 where s is below 2^-125).  It hardly ever is not: put()
+// asks whether a piece has such a value, mend() moves it.
 constexpr float MAGIC = 12582912.0f;  // 1.5 2^23
 __device__ __forceinline__ float rest(float x, float t, float s) { return fmaf(-(t - MAGIC), s, x); }
-__device__ __forceinline__ float mend(float t, float d, float below, float above) {  // below: of d - s / 2, above: of d + s / 2, their signs
+__device__ __forceinline__ float mend(float t, float d, float below, float above) {  // below: of 2 d - s, above: of 2 d + s, their signs
     const bool odd = (__float_as_uint(t) & 1u) != 0;
     if (below > 0.f || (below == 0.f && odd)) return t + 1.0f;
     if (above < 0.f || (above == 0.f && odd)) return t - 1.0f;
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(2 * ST_THREADS, 4) kv8_store_kernel(const Stor
     else now = want <= before ? before : fmaxf(want, __fmul_rn(1.25f, before));
     __syncthreads();  // (every thread has read the scale)
     if (tid == 0) *scale = now;
-    const float inv = now > 0.f ? __fdiv_rn(1.0f, now) : 0.f, half = 0.5f * now;  // (NaN, 0: all values become 0)
+    const float inv = now > 0.f ? __fdiv_rn(1.0f, now) : 0.f;  // (NaN, 0: all values become 0)
 
     if (used > 0 && !broken && now != before) {  // a scale of 0 in front of one that is not: all of them are 0
         for (int i = tid; i < used * pieces; i += ST_THREADS) {
@@ -134,10 +135,10 @@ __global__ void __launch_bounds__(2 * ST_THREADS, 4) kv8_store_kernel(const Stor
                 float f[4];
 #pragma unroll
                 for (int b = 0; b < 4; b++) {
-                    // q before = hi + lo exactly; with d = hi - r now exact, as above, the signs of d + lo -+ now / 2 are those of (d -+ now / 2) + lo
+                    // q before = hi + lo exactly; with d = hi - r now exact, as above, the signs of 2 (d + lo) -+ now are those of (2 d -+ now) + 2 lo
                     const float qf = (float)(signed char)(w[e] >> (8 * b)), hi = __fmul_rn(qf, before), lo = fmaf(qf, before, -hi);
                     const float t = fmaf(hi, inv, MAGIC), d = rest(hi, t, now);
-                    f[b] = mend(t, d, (d - half) + lo, (d + half) + lo);
+                    f[b] = mend(t, d, fmaf(2.0f, d, -now) + 2.0f * lo, fmaf(2.0f, d, now) + 2.0f * lo);
                 }
                 w[e] = pack4(f[0], f[1], f[2], f[3]);
             }
@@ -158,14 +159,14 @@ __global__ void __launch_bounds__(2 * ST_THREADS, 4) kv8_store_kernel(const Stor
             }
             w[e] = pack4(t[0], t[1], t[2], t[3]);
         }
-        if (!(off < half)) {  // a tie, or beside one (or a scale that is 0 or no number)
+        if (!(off + off < now)) {  // a tie, or beside one (or a scale that is 0 or no number)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 float t[4];
 #pragma unroll
                 for (int b = 0; b < 4; b++) {
                     const float v = raw_value(y, 4 * e + b), t0 = fmaf(v, inv, MAGIC), d = rest(v, t0, now);
-                    t[b] = inv > 0.f ? mend(t0, d, d - half, d + half) : MAGIC;
+                    t[b] = inv > 0.f ? mend(t0, d, fmaf(2.0f, d, -now), fmaf(2.0f, d, now)) : MAGIC;
                 }
                 w[e] = pack4(t[0], t[1], t[2], t[3]);
             }
