@@ -170,7 +170,8 @@ B200_API int b200_llama_seq_length(b200_llama *m, int32_t seq_id);
 
 /* One step over a batch (llama_decode with a llama_batch of several sequences): tokens[i] continues sequence seq_ids[i] at that
  * sequence's next position; the tokens of one sequence are adjacent and in order.  want[i] != 0 asks for the logits at token i;
- * logits receives them in batch order, n_vocab floats each (want == NULL: none).  Synchronous on return. */
+ * logits receives them in batch order, n_vocab floats each (want == NULL: none).  Synchronous on return.  A call that is refused, or that
+ * fails before the device has begun with it, leaves every sequence as it was; sequences of a step that fails on the device can only be closed. */
 B200_API int b200_llama_decode_batch(b200_llama *m, const int32_t *tokens, const int32_t *seq_ids, const int8_t *want, int32_t n_tokens, float *logits);
 
 /* Raw access to KV cells [cell0, cell0+n) of layer il (is_v: 0 = K, 1 = V): rows of n_embd_gqa values in type_k / type_v,

@@ -11,7 +11,7 @@ namespace b200 {
 namespace host {
 
 struct SeqCache {
-    struct Seq { bool open = false; bool fresh = true; int32_t len = 0; };
+    struct Seq { bool open = false; bool fresh = true; bool lost = false; int32_t len = 0; };  // lost: a step with its tokens failed on the device
     std::vector<int32_t> cell_seq, cell_pos;  // per cell: owning sequence (-1: free) and position
     std::vector<Seq> seqs;                    // sequence id == state slot
     int32_t n_used = 0;                       // cells in use
@@ -27,7 +27,7 @@ struct SeqCache {
     int32_t n_cells() const { return (int32_t)cell_seq.size(); }
     int32_t open_seq() {
         for (size_t i = 0; i < seqs.size(); i++) {
-            if (!seqs[i].open) { seqs[i].open = true; seqs[i].fresh = true; seqs[i].len = 0; return (int32_t)i; }
+            if (!seqs[i].open) { seqs[i] = Seq(); seqs[i].open = true; return (int32_t)i; }
         }
         return -1;
     }
@@ -58,6 +58,16 @@ struct SeqCache {
         first_free = c;
         n_used += n;
         return true;
+    }
+    // place() taken back: the n last tokens of sequence id, at these cells (of several sequences of a step: in any order)
+    void unplace(int32_t id, int32_t n, const int32_t *cells) {
+        for (int32_t i = 0; i < n; i++) {
+            cell_seq[(size_t)cells[i]] = -1; cell_pos[(size_t)cells[i]] = -1;
+            if (cells[i] < first_free) first_free = cells[i];
+        }
+        n_used -= n;
+        seqs[(size_t)id].len -= n;
+        while (high > 0 && cell_seq[(size_t)high - 1] < 0) high--;
     }
 };
 

@@ -289,6 +289,7 @@ extern "C" int b200_llama_seq_close(b200_llama *m, int32_t seq_id) {
     LL_REQUIRE(m && m->finalized && m->arch && m->cache.is_open(seq_id), B200_ERR_INVALID, "b200_llama_seq_close: sequence %d is not open", seq_id);
     if (m->hp.kv8_page > 0) {  // its pages are free behind the last step
         const b200_kv8_map map = m->pages.map();
+        LL_REQUIRE(cudaSetDevice(m->hp.main_device) == cudaSuccess, B200_ERR_CUDA, "b200_llama_seq_close: device %d", m->hp.main_device);
         const int rc = b200_op_kv8_cut(&map, (const int32_t *)m->pages.ids->data + seq_id, nullptr, 1, (cudaStream_t)ggml_backend_b200_get_stream(m->be));
         if (rc != B200_OK) return rc;
     }
@@ -310,6 +311,7 @@ extern "C" int b200_llama_decode_batch(b200_llama *m, const int32_t *tokens, con
     for (int i = 0; i < n_tokens; i++) {
         LL_REQUIRE(tokens[i] >= 0 && tokens[i] < hp.n_vocab, B200_ERR_INVALID, "b200_llama_decode_batch: token id out of range");
         LL_REQUIRE(kc.is_open(seq_ids[i]), B200_ERR_INVALID, "b200_llama_decode_batch: sequence %d is not open", seq_ids[i]);
+        LL_REQUIRE(!kc.seqs[(size_t)seq_ids[i]].lost, B200_ERR_INVALID, "b200_llama_decode_batch: sequence %d lost tokens when a step failed: it can only be closed", seq_ids[i]);
         if (i == 0 || seq_ids[i] != seq_ids[i - 1]) {
             for (int32_t s : run_seq) LL_REQUIRE(s != seq_ids[i], B200_ERR_INVALID, "b200_llama_decode_batch: the tokens of sequence %d are not adjacent", seq_ids[i]);
             run_first.push_back(i); run_count.push_back(0); run_seq.push_back(seq_ids[i]);
@@ -318,18 +320,33 @@ extern "C" int b200_llama_decode_batch(b200_llama *m, const int32_t *tokens, con
     }
     LL_REQUIRE(n_tokens <= kc.n_cells() - kc.n_used, B200_ERR_NOMEM, "b200_llama_decode_batch: the cache is full (%d cells, %d in use, %d asked for)", kc.n_cells(), kc.n_used, n_tokens);
     const int32_t n_seq = (int32_t)run_seq.size();
+    m->st_out.clear();
+    for (int i = 0; i < n_tokens; i++) if (want && want[i]) m->st_out.push_back(i);
+    const int32_t n_out = (int32_t)m->st_out.size();
+    LL_REQUIRE(n_out == 0 || logits, B200_ERR_INVALID, "b200_llama_decode_batch: logits wanted but no buffer given");
     m->st_cells.resize((size_t)n_tokens); m->st_pos.resize((size_t)n_tokens); m->st_seq.assign(seq_ids, seq_ids + n_tokens);
     info.assign((size_t)4 * n_seq, 0);
+    // From here to the device's own record of the step (its grown rows, its graph) an error takes the tokens' places back: host and device agree on every sequence's length.
+    struct Placed {
+        SeqCache &kc;
+        const std::vector<int32_t> &seq, &first, &count, &info, &cells;
+        int32_t n = 0;  // sequences placed so far
+        bool kept = false;
+        ~Placed() {
+            for (int32_t r = 0; r < n && !kept; r++) {
+                kc.unplace(seq[(size_t)r], count[(size_t)r], cells.data() + first[(size_t)r]);
+                kc.seqs[(size_t)seq[(size_t)r]].fresh = info[3 * seq.size() + (size_t)r] != 0;
+            }
+        }
+        void lost() { for (int32_t s : seq) kc.seqs[(size_t)s].lost = true; }
+    } placed = {kc, run_seq, run_first, run_count, info, m->st_cells};
     for (int32_t r = 0; r < n_seq; r++) {
         info[(size_t)r] = run_first[(size_t)r]; info[(size_t)n_seq + r] = run_count[(size_t)r]; info[(size_t)2 * n_seq + r] = run_seq[(size_t)r];
         info[(size_t)3 * n_seq + r] = kc.seqs[(size_t)run_seq[(size_t)r]].fresh ? 1 : 0;
         kc.place(run_seq[(size_t)r], run_count[(size_t)r], m->st_cells.data() + run_first[(size_t)r], m->st_pos.data() + run_first[(size_t)r]);
         kc.seqs[(size_t)run_seq[(size_t)r]].fresh = false;
+        placed.n = r + 1;
     }
-    m->st_out.clear();
-    for (int i = 0; i < n_tokens; i++) if (want && want[i]) m->st_out.push_back(i);
-    const int32_t n_out = (int32_t)m->st_out.size();
-    LL_REQUIRE(n_out == 0 || logits, B200_ERR_INVALID, "b200_llama_decode_batch: logits wanted but no buffer given");
     int32_t n_kv = round_up(kc.high, KV_PAD);
     if (n_kv > hp.n_ctx) n_kv = hp.n_ctx;
     const BatchShape bs = {n_tokens, n_kv, n_out, n_seq};
@@ -364,21 +381,27 @@ extern "C" int b200_llama_decode_batch(b200_llama *m, const int32_t *tokens, con
     if (cudaEventRecord(m->in_ev, (cudaStream_t)ggml_backend_b200_get_stream(be)) == cudaSuccess) m->in_ev_pending = true;
     else { cudaGetLastError(); cudaStreamSynchronize((cudaStream_t)ggml_backend_b200_get_stream(be)); }
     int64_t l0 = 0, l1 = 0;
+    int32_t *refused = (int32_t *)(m->pin + m->pin_bytes) - 1;  // (behind what is sent)
+    *refused = 0;
     if (hp.kv8_page > 0) {  // room for the step's tokens; no page is shared, so nothing is copied
         const b200_llama::Pages &P = m->pages;
         const b200_kv8_map map = P.map();
-        const int rc = b200_op_kv8_grow(&map, nullptr, 0, (const int32_t *)P.inp_rows.data, (const int32_t *)P.inp_new.data, n_seq, (int32_t *)P.info->data, nullptr, P.grow_ws->data,
+        const int rc = b200_op_kv8_grow(&map, nullptr, 0, (const int32_t *)P.inp_rows.data, (const int32_t *)P.inp_new.data, n_seq, (int32_t *)P.info->data, refused, P.grow_ws->data,
                                         nbytes(P.grow_ws), (cudaStream_t)ggml_backend_b200_get_stream(be));
         if (rc != B200_OK) return rc;
     }
+    placed.kept = true;
     ggml_backend_b200_get_stats(&l0, nullptr, nullptr);
     const ggml_status st = be->iface.graph_compute(be, &m->graph);
     ggml_backend_b200_get_stats(&l1, nullptr, nullptr);
+    if (st != GGML_STATUS_SUCCESS) placed.lost();
     m->last_launches = l1 - l0 + (hp.kv8_page > 0 ? 1 : 0);
     m->t_calls++;
     LL_REQUIRE(st == GGML_STATUS_SUCCESS, B200_ERR_CUDA, "b200_llama_decode_batch: graph_compute failed (%d)", (int)st);
     if (n_out > 0) be->iface.get_tensor_async(be, m->logits_t, logits, 0, 4 * (size_t)hp.n_vocab * (size_t)n_out);
     be->iface.synchronize(be);
+    if (*(volatile int32_t *)refused != 0) placed.lost();
+    LL_REQUIRE(*(volatile int32_t *)refused == 0, B200_ERR_CUDA, "b200_llama_decode_batch: no pages for %d of the step's sequences: its results are invalid", *refused);
     LL_REQUIRE(b200_gemm_status() == 0, B200_ERR_CUDA, "b200_llama_decode_batch: a product gave up waiting for its operands: the step's results are invalid");
     return B200_OK;
 }
