@@ -223,6 +223,9 @@ enum ggml_status graph_exec_compute(GraphExec *g, ggml_cgraph *cgraph);
 bool op_supported(int device, const ggml_tensor *op);
 
 int kv8_attn_launches(const b200_kv8_attn_args *a);  // kernels of b200_op_kv8_attn (kv8_attn.cu)
+// whether the calls would take these arguments (a status)
+int kv8_attn_check(const b200_kv8_attn_args *a, size_t workspace_bytes);
+int kv8_store_check(const b200_kv8_store_args *a);
 
 extern bool g_use_graphs, g_use_fusion;
 extern int64_t g_stat_launches, g_stat_replays, g_stat_captures;

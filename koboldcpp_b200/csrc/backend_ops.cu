@@ -49,6 +49,44 @@ static bool kv8_pool_ok(const ggml_tensor *pool, const ggml_tensor *n, int at) {
     return pool && (size_t)pool->ne[0] * 4 == b200_kv8_page_bytes(n->op_params[at], n->op_params[at + 1], n->op_params[at + 2], n->op_params[at + 3]);
 }
 
+// the cache that a node's pool of pages [words of a record, pages] is, its sizes in op_params from `at` on
+static b200_kv8_cache kv8_cache_of(const ggml_tensor *pool, const ggml_tensor *n, int at) {
+    return {pool->data, (int32_t)pool->ne[1], n->op_params[at], n->op_params[at + 1], n->op_params[at + 2], n->op_params[at + 3], 0};
+}
+static void fill_kv8_attn_args(const ggml_tensor *n, b200_kv8_attn_args &a) {
+    const ggml_tensor *const *s = n->src;
+    memset(&a, 0, sizeof(a));
+    a.cache = kv8_cache_of(s[1], n, 2);
+    a.q = s[0]->data; a.q_stride = (int64_t)(s[0]->nb[1] / 4); a.dst = n->data; a.dst_stride = (int64_t)(n->nb[1] / 4);
+    a.seq_info = (const int32_t *)s[2]->data; a.n_seq = (int32_t)s[2]->ne[0]; a.n_tokens = (int32_t)s[0]->ne[1];
+    a.table = (const int32_t *)s[3]->data; a.table_stride = (int64_t)(s[3]->nb[1] / 4); a.n_rows = (int32_t)s[3]->ne[1];
+    a.n_head = (int32_t)(s[0]->ne[0] / n->op_params[4]); a.type = B200_TYPE_F32;
+    a.sink = s[4] ? (const float *)s[4]->data : nullptr;
+    a.scale = ext_f(n, 6); a.window = n->op_params[7]; a.keep_first = n->op_params[8]; a.softcap = ext_f(n, 9); a.f16_products = n->op_params[10]; a.max_new = n->op_params[11];
+}
+static void fill_kv8_store_args(const ggml_tensor *n, b200_kv8_store_args &a) {
+    const ggml_tensor *const *s = n->src;
+    memset(&a, 0, sizeof(a));
+    a.cache = kv8_cache_of(s[4], n, 2);
+    a.k = s[0]->data; a.k_stride = (int64_t)(s[0]->nb[1] / 4); a.v = s[1]->data; a.v_stride = (int64_t)(s[1]->nb[1] / 4);
+    a.seq_info = (const int32_t *)s[2]->data; a.n_seq = (int32_t)s[2]->ne[0]; a.n_tokens = (int32_t)s[0]->ne[1];
+    a.table = (const int32_t *)s[3]->data; a.table_stride = (int64_t)(s[3]->nb[1] / 4); a.n_rows = (int32_t)s[3]->ne[1]; a.type = B200_TYPE_F32;
+}
+// whether the calls take what the nodes say; tensors that have no memory yet stand at an address that suits them
+template <typename T> static void somewhere(T *&p) { if (!p) p = (T *)(uintptr_t)4096; }
+static bool kv8_store_takes(const ggml_tensor *n) {
+    b200_kv8_store_args a;
+    fill_kv8_store_args(n, a);
+    somewhere(a.cache.pages); somewhere(a.k); somewhere(a.v); somewhere(a.seq_info); somewhere(a.table);
+    return kv8_store_check(&a) == B200_OK;
+}
+static bool kv8_attn_takes(const ggml_tensor *n) {
+    b200_kv8_attn_args a;
+    fill_kv8_attn_args(n, a);
+    somewhere(a.cache.pages); somewhere(a.q); somewhere(a.dst); somewhere(a.seq_info); somewhere(a.table);
+    return (uintptr_t)n->src[5]->data % 16 == 0 && kv8_attn_check(&a, nbytes(n->src[5])) == B200_OK;
+}
+
 static bool ext_op_supported(const ggml_tensor *op) {
     const ggml_tensor *const *s = op->src;
     switch (op->op_params[1]) {
@@ -134,30 +172,15 @@ static bool ext_op_supported(const ggml_tensor *op) {
         case B200_EXT_KV8_STORE:
             return f32_rows(s[0]) && f32_rows(s[1]) && i32_vec(s[2]) && s[2]->ne[1] == 4 && is_contiguous(s[2]) && i32_vec(s[3]) && f32_vec(s[4]) && kv8_pool_ok(s[4], op, 2) &&
                    s[0]->ne[0] == (int64_t)op->op_params[3] * op->op_params[4] && s[1]->ne[0] == (int64_t)op->op_params[3] * op->op_params[5] && s[0]->ne[1] == s[1]->ne[1] &&
-                   s[2]->ne[0] <= B200_KV8_MAX_SEQ;
+                   s[2]->ne[0] <= B200_KV8_MAX_SEQ && kv8_store_takes(op);
         case B200_EXT_KV8_ATTN:
             return f32_rows(s[0]) && f32_vec(s[1]) && kv8_pool_ok(s[1], op, 2) && i32_vec(s[2]) && s[2]->ne[1] == 4 && is_contiguous(s[2]) && i32_vec(s[3]) && (!s[4] || f32_vec(s[4])) && f32_vec(s[5]) &&
                    f32_rows(op) && op->op_params[4] > 0 && s[0]->ne[0] % ((int64_t)op->op_params[3] * op->op_params[4]) == 0 && s[2]->ne[0] <= B200_KV8_MAX_SEQ &&
-                   op->ne[0] == s[0]->ne[0] / op->op_params[4] * op->op_params[5] && op->ne[1] == s[0]->ne[1] && (!s[4] || s[4]->ne[0] == s[0]->ne[0] / op->op_params[4]);
+                   op->ne[0] == s[0]->ne[0] / op->op_params[4] * op->op_params[5] && op->ne[1] == s[0]->ne[1] && (!s[4] || s[4]->ne[0] == s[0]->ne[0] / op->op_params[4]) &&
+                   kv8_attn_takes(op);
         default:
             return false;
     }
-}
-
-// the cache that a node's pool of pages [words of a record, pages] is, its sizes in op_params from `at` on
-static b200_kv8_cache kv8_cache_of(const ggml_tensor *pool, const ggml_tensor *n, int at) {
-    return {pool->data, (int32_t)pool->ne[1], n->op_params[at], n->op_params[at + 1], n->op_params[at + 2], n->op_params[at + 3], 0};
-}
-static void fill_kv8_attn_args(const ggml_tensor *n, b200_kv8_attn_args &a) {
-    const ggml_tensor *const *s = n->src;
-    memset(&a, 0, sizeof(a));
-    a.cache = kv8_cache_of(s[1], n, 2);
-    a.q = s[0]->data; a.q_stride = (int64_t)(s[0]->nb[1] / 4); a.dst = n->data; a.dst_stride = (int64_t)(n->nb[1] / 4);
-    a.seq_info = (const int32_t *)s[2]->data; a.n_seq = (int32_t)s[2]->ne[0]; a.n_tokens = (int32_t)s[0]->ne[1];
-    a.table = (const int32_t *)s[3]->data; a.table_stride = (int64_t)(s[3]->nb[1] / 4); a.n_rows = (int32_t)s[3]->ne[1];
-    a.n_head = (int32_t)(s[0]->ne[0] / n->op_params[4]); a.type = B200_TYPE_F32;
-    a.sink = s[4] ? (const float *)s[4]->data : nullptr;
-    a.scale = ext_f(n, 6); a.window = n->op_params[7]; a.keep_first = n->op_params[8]; a.softcap = ext_f(n, 9); a.f16_products = n->op_params[10]; a.max_new = n->op_params[11];
 }
 
 static void fill_sink_attn_args(const ggml_tensor *n, b200_sink_attn_args &a) {
@@ -291,11 +314,7 @@ static void run_ext(ExecCtx &x, const ggml_tensor *n) {
         }
         case B200_EXT_KV8_STORE: {
             b200_kv8_store_args a;
-            memset(&a, 0, sizeof(a));
-            a.cache = kv8_cache_of(s[4], n, 2);
-            a.k = s[0]->data; a.k_stride = (int64_t)(s[0]->nb[1] / 4); a.v = s[1]->data; a.v_stride = (int64_t)(s[1]->nb[1] / 4);
-            a.seq_info = (const int32_t *)s[2]->data; a.n_seq = (int32_t)s[2]->ne[0]; a.n_tokens = (int32_t)s[0]->ne[1];
-            a.table = (const int32_t *)s[3]->data; a.table_stride = (int64_t)(s[3]->nb[1] / 4); a.n_rows = (int32_t)s[3]->ne[1]; a.type = B200_TYPE_F32;
+            fill_kv8_store_args(n, a);
             B200_CHECK_RC(b200_op_kv8_store(&a, x.stream));
             break;
         }

@@ -553,7 +553,21 @@ static int launch_load(const LoadArgs &s, bool vec, unsigned grid, cudaStream_t 
     return B200_OK;
 }
 
+static int check_store(const b200_kv8_store_args *a, const char *who) {
+    const int rc = check_step(&a->cache, a->seq_info, a->table, a->table_stride, a->n_rows, a->n_seq, a->n_tokens, a->type, who);
+    if (rc != B200_OK || a->n_tokens == 0 || a->n_seq == 0) return rc;
+    const b200_kv8_cache &c = a->cache;
+    OPX_REQUIRE(a->k && a->v, B200_ERR_INVALID, "%s: NULL k or v", who);
+    OPX_REQUIRE(a->k_stride >= (int64_t)c.n_head_kv * c.dim && a->v_stride >= (int64_t)c.n_head_kv * c.vdim, B200_ERR_INVALID, "%s: rows of k or v overlap (strides %lld, %lld)", who,
+                (long long)a->k_stride, (long long)a->v_stride);
+    OPX_REQUIRE(aligned_to(type_size(a->type), a->k, a->v), B200_ERR_INVALID, "%s: k or v is not aligned to its type", who);
+    return B200_OK;
+}
+
 }  // namespace kv8
+
+int kv8_store_check(const b200_kv8_store_args *a) { return kv8::check_store(a, "b200_op_kv8_store"); }
+
 }  // namespace b200
 
 using namespace b200;
@@ -571,14 +585,9 @@ size_t b200_kv8_page_bytes(int32_t page_size, int32_t n_head_kv, int32_t dim, in
 int b200_op_kv8_store(const b200_kv8_store_args *a, b200_stream_t stream) {
     const char *who = "b200_op_kv8_store";
     OPX_REQUIRE(a, B200_ERR_INVALID, "%s: NULL arguments", who);
-    const int rc = check_step(&a->cache, a->seq_info, a->table, a->table_stride, a->n_rows, a->n_seq, a->n_tokens, a->type, who);
-    if (rc != B200_OK) return rc;
-    if (a->n_tokens == 0 || a->n_seq == 0) return B200_OK;
+    const int rc = check_store(a, who);
+    if (rc != B200_OK || a->n_tokens == 0 || a->n_seq == 0) return rc;
     const b200_kv8_cache &c = a->cache;
-    OPX_REQUIRE(a->k && a->v, B200_ERR_INVALID, "%s: NULL k or v", who);
-    OPX_REQUIRE(a->k_stride >= (int64_t)c.n_head_kv * c.dim && a->v_stride >= (int64_t)c.n_head_kv * c.vdim, B200_ERR_INVALID, "%s: rows of k or v overlap (strides %lld, %lld)", who,
-                (long long)a->k_stride, (long long)a->v_stride);
-    OPX_REQUIRE(aligned_to(type_size(a->type), a->k, a->v), B200_ERR_INVALID, "%s: k or v is not aligned to its type", who);
     const StoreArgs s = {c, {a->seq_info, a->table, a->table_stride, a->n_rows, a->n_seq, a->n_tokens, c.n_pages, c.page_size}, a->k, a->v, a->k_stride, a->v_stride};
     const dim3 grid((unsigned)(a->n_tokens / c.page_size + 2 * a->n_seq), (unsigned)c.n_head_kv);
     const bool vec = rows_aligned(a->k, a->k_stride, a->type) && rows_aligned(a->v, a->v_stride, a->type);

@@ -720,6 +720,12 @@ static int launch_prompt(AttnArgs &args, bool vec, int k, long long limit, cudaS
 
 }  // namespace kv8
 
+int kv8_attn_check(const b200_kv8_attn_args *a, size_t workspace_bytes) {
+    const int rc = kv8::check_attn(a, "b200_op_kv8_attn");
+    if (rc != B200_OK || a->n_tokens == 0 || a->n_seq == 0) return rc;
+    OPX_REQUIRE(workspace_bytes >= b200_kv8_attn_workspace_bytes(a), B200_ERR_INVALID, "b200_op_kv8_attn: workspace of %zu bytes", b200_kv8_attn_workspace_bytes(a));
+    return B200_OK;
+}
 int kv8_attn_launches(const b200_kv8_attn_args *a) {
     if (a->n_tokens == 0 || a->n_seq == 0) return 0;
     return !kv8::has_prompts(a) ? 1 : kv8::prompt_plan(a).splits > 1 ? 3 : 2;
