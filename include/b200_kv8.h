@@ -128,7 +128,7 @@ B200_API int b200_op_kv8_fork(const b200_kv8_map *m, const int32_t *src, const i
  * page that is shared and not full is first replaced by a copy of its own (in all the caches) if n_new[i] > 0.  len grows by n_new[i].  A
  * row that does not fit its table, or for which the pages no longer reach (with those before it in the list, refused ones too), is
  * refused: it stays as it is.  seq_info (optional) [4][n] becomes the step over these rows: tokens in the order of the list, n_new[i] each (negative ones
- * count as 0 and are refused), rows that were refused with a count of 0 in their place. */
+ * count as 0 and are refused), rows that were refused with a count of 0 in their place; a row whose tokens would reach beyond the step's 2^31 - 1st is refused too. */
 B200_API size_t b200_kv8_grow_workspace_bytes(int32_t n);
 B200_API int b200_op_kv8_grow(const b200_kv8_map *m, const b200_kv8_cache *caches, int32_t n_caches, const int32_t *rows, const int32_t *n_new, int32_t n, int32_t *seq_info,
                               int32_t *refused, void *workspace, size_t workspace_bytes, b200_stream_t stream);

@@ -316,6 +316,27 @@ __device__ __forceinline__ int scan_1024(int x, int *sh, int &all) {
     return __shfl_sync(0xffffffffu, w, (warp + 31) & 31) * (warp > 0) + inc - x;
 }
 
+// The same of two values at a time, neither below 0; sums stay at 2^31 - 1 once they come to it.
+__device__ __forceinline__ int add_up(int a, int b) { return (int)min((unsigned)a + (unsigned)b, 0x7fffffffu); }
+__device__ __forceinline__ int2 scan2_1024(int2 x, int2 *sh, int2 &all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    auto up = [](int2 v, int o) { return make_int2(__shfl_up_sync(0xffffffffu, v.x, o), __shfl_up_sync(0xffffffffu, v.y, o)); };
+    auto add = [](int2 a, int2 b) { return make_int2(add_up(a.x, b.x), add_up(a.y, b.y)); };
+    int2 inc = x;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) { const int2 y = up(inc, o); if (lane >= o) inc = add(inc, y); }
+    __syncthreads();
+    if (lane == 31) sh[warp] = inc;
+    __syncthreads();
+    int2 w = sh[lane], before = up(inc, 1);
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) { const int2 y = up(w, o); if (lane >= o) w = add(w, y); }
+    all = make_int2(__shfl_sync(0xffffffffu, w.x, 31), __shfl_sync(0xffffffffu, w.y, 31));
+    const int2 warps = make_int2(__shfl_sync(0xffffffffu, w.x, (warp + 31) & 31), __shfl_sync(0xffffffffu, w.y, (warp + 31) & 31));
+    if (lane == 0) before = make_int2(0, 0);
+    return warp > 0 ? add(before, warps) : before;
+}
+
 // One CTA, a thread per row of the list: what each needs, sums before it, then the free pages in ascending order, each to the row whose share
 // it falls in.  The free pages are counted first (as many as are asked for), because a row that does not get all it needs gets nothing.
 // One CTA, because rows are served in order and free pages by number; 48 rows take 9.6 us, all of it latency (8192 entries of refs a round, most often the only one).
@@ -324,6 +345,7 @@ __global__ void __launch_bounds__(1024) kv8_grow_kernel(const Map m, const int32
                                                         int32_t *__restrict__ pairs) {
     pdl_enter(rows, n_new, pairs);
     __shared__ __align__(16) int row_s[1024];
+    __shared__ int2 sum_sh[32];
     __shared__ int sh[32], start_s[1024], first_s[1024], short_s;  // start: pages of the rows before; first: table entry of a row's first page
     const int i = threadIdx.x, ps = m.page_size;
     const int row = i < n ? rows[i] : -1, asked = i < n ? n_new[i] : 0;
@@ -348,9 +370,11 @@ __global__ void __launch_bounds__(1024) kv8_grow_kernel(const Map m, const int32
         if (p >= 0 && p < m.n_pages && m.refs[p] > 1) tail = p;
     }
     const int need = more + (tail >= 0);
-    int total, n_free = 0, tokens;
-    const int start = scan_1024(need, sh, total);
-    const int first_token = scan_1024(i < n ? max(asked, 0) : 0, sh, tokens);
+    int n_free = 0;
+    int2 sums;
+    const int2 sum = scan2_1024(make_int2(need, i < n ? max(asked, 0) : 0), sum_sh, sums);
+    const int start = sum.x, total = sums.x, first_token = sum.y;
+    ok = ok && (!seq_info || (unsigned)first_token + (unsigned)asked <= 0x7fffffffu);  // (no step has room for it, nor for those behind it)
     start_s[i] = start;
     first_s[i] = begin - (tail >= 0);
     auto free_pages = [&](int base) {
@@ -368,7 +392,7 @@ __global__ void __launch_bounds__(1024) kv8_grow_kernel(const Map m, const int32
         if (base == 0) { first_mask = mask; first_rank = rank; first_all = all; }
         n_free += all;
     }
-    ok = ok && (need == 0 || start + need <= n_free);
+    ok = ok && (need == 0 || (unsigned)start + (unsigned)need <= (unsigned)n_free);
     if (i < n && !ok) atomicAdd(&short_s, 1);
     row_s[i] = ok ? row : -1;
     __syncthreads();
