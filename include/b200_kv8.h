@@ -82,8 +82,11 @@ B200_API int b200_op_kv8_load(const b200_kv8_load_args *a, b200_stream_t stream)
  * also holds exp(sink[h]) when sink != NULL.  A token that sees nothing gets zeros.  Rows of dst that belong to no sequence stay as they are.
  * q [n_tokens][n_head * dim], dst [n_tokens][n_head * vdim], of one type.  Sums, maxima and exponentials are f32.  int8 is exact in f16, which
  * the tensor cores take: with rows of bf16, and with f16_products != 0, queries and weights are rounded to f16 (relative to the row's largest); with rows
- * of f16 weights enter as two f16, 22 bits, and queries as they are; with rows of f32 both as two.  Results of f32 are off by 1e-6 or so of their size,
- * whatever the length, those of 16 bits by 2^-11 where weights are rounded and by their own rounding.  A query that is not finite gives NaN.
+ * of f16 weights enter as two f16, 22 bits, and queries as they are; with rows of f32 both as two.  What a result is off by, as a share of its mass (the sum of
+ * weight times |value|), besides its own rounding: with rows of f32 1e-6 or so (root mean square; in prompts 3e-6 where values are of one sign, 2^-17 at most: the tensor cores
+ * cut sums off, f32 additions take over after 128 of theirs), with rows of f16 in prompts 2^-15 at most (512 of theirs), else 2^-12 of each weight, whatever the length.  Weights count in steps
+ * of 2^-30 of the row's largest, times the largest scale that the values of any page in its sight have: a page 2^20 times as loud as the others leaves them 10 bits,
+ * even where its own tokens have no weight.  A query that is not finite gives NaN.
  * max_new: no sequence of the step has more new tokens than that (0: not known).  It only chooses how the work is laid out.
  * n_tokens * n_head below 2^31.  The workspace is zero before its first call and may then go from call to call of one stream, whatever their sizes; the bytes
  * asked for do not depend on lengths.  */

@@ -55,8 +55,8 @@ __device__ __forceinline__ float max_nan(float x, float y, float z) {  // NaN if
 // before if the scale grew, the new values.  The values wait in registers as they came (KEEP pieces of 16 a thread; of a page with more they are read twice).
 // Item j of the grid is a page of sequence s where first_s / page_size + 2 s <= j: a sequence of n tokens touches n / page_size + 2 pages at most, so
 // the items of the sequences do not overlap and nothing has to be summed up beforehand.
-// Measured: prompts of 3 sequences, 32 heads of 128, bf16, 377 MB in 83 us, 4.5 TB/s (issue 66% of the cycles: 3 rounds of arithmetic a value, of which two check the
-// rounding); one token each of 64 sequences, 8 heads, f32: 10 us, of which two ways to memory (the step, then the page and the rows) and their launch are nearly all.
+// Measured: prompts of 3 sequences, 32 heads of 128, bf16, 377 MB (with reading back) in 83 us, 4.5 TB/s (instructions are issued in 65% of the cycles: 3 rounds of arithmetic a value, of
+// which two check the rounding; warps wait for their rows in the rest); one token each of 64 sequences, 8 heads, f32: 10 us, of which two ways to memory (the step, then the page and the rows) and their launch are nearly all.
 constexpr int ST_THREADS = 128;
 struct StoreArgs {
     b200_kv8_cache cache;

@@ -117,9 +117,9 @@ struct AttnArgs {
 // Warps keep maximum, sum and result of their own and meet in shared memory at the end of a run of units of one block; runs of one block in
 // several CTAs meet in global memory, where the last one to arrive adds them in the order of the CTAs.
 // Scales: a key's joins its score; a value's joins its weight, relative to the power of two above the largest one that the row has seen.
-// Measured (heads of 128, 32 query heads over 8, f32): one token behind 131,000: 268 MB in 70.7 us, 3.8 TB/s; 64 sequences of 129 to 4096 tokens: 280 MB in 75.3 us; behind 511: 9.9 us.
-// What bounds it is the issue of instructions, about 1100 a warp for 32 keys (350 of them turn int8 into f16), at 56% of the cycles with three warps a scheduler; registers
-// (165) allow no fourth, and where blocks are short (drafts: 45 MB in 38.6 us) their beginnings and ends, about 4.5 us each.
+// Measured (heads of 128, 32 query heads over 8, f32): one token behind 131,000: 268 MB in 70.7 us, 3.8 TB/s; 64 sequences of 129 to 4096 tokens: 280 MB in 75.4 us; behind 511: 9.9 us.
+// What it spends its time on is instructions, about 1150 a warp for 32 keys (350 of them turn int8 into f16), issued in 59% of the cycles by three warps a scheduler, which wait for one another's
+// results in the others; registers (168) allow no fourth.  Short blocks (drafts, f16: 45 MB in 40.5 us) are two thirds loop, 3.5 us for 128 keys, 4.5 us beginning and 7 us end.
 constexpr int RW_WARPS = 4, RW_TILE = 32, RW_UNIT = RW_WARPS * RW_TILE, RW_THREADS = RW_WARPS * 32;
 constexpr int RW_STAGES = 2, RW_PARTS = 128;
 constexpr int RW_BEGIN = 2;  // to begin and end a block costs a CTA about as much as two units: they are counted with each block's
@@ -685,9 +685,13 @@ static int check_attn(const b200_kv8_attn_args *a, const char *who) {
 //   f32, the same:                             33 tokens  7.6 : 21.0, 20.4 : 30.0,  67 :  48    64 tokens  9 : 21, 29 : 30, 116 :  53   128 tokens 13 : 22, 44 : 33, 219 :  77
 //   bf16, 4 sequences:                         17 tokens  9.0 : 18.6, 23.3 : 30.2,  88 :  74    33 tokens  9 : 20, 34 : 34, 146 : 102    64 tokens 14 : 19, 49 : 34, 240 : 144
 //   bf16, 16 sequences:                         5 tokens  9.3 : 18.9, 29.7 : 36.8, 136 : 192     9 tokens 10 : 18, 38 : 35, 195 : 183    17 tokens 15 : 18, 56 : 36, 310 : 185
+//   bf16, 1 sequence, 8 query heads over 1:   128 tokens  8.9 : 21.0, 18.0 : 29.1,  44 :  41   256 tokens 14 : 22, 23 : 30,  74 :  45
+//   f32, the same:                             64 tokens  7.4 : 20.0, 15.6 : 27.3,  39 :  37   128 tokens  8 : 22, 20 : 31,  65 :  44   256 tokens 13 : 24, 29 : 32, 119 : 49
+// A border at half of PROMPT_ROWS would win up to 45 us behind 8000 tokens and lose 6 to 14 without a past or behind 1000: steps of a chat begin with little.
 // (how long the past is, only the device knows; 5 tokens of 4 heads are 20 rows, 9 are 36)
 constexpr int ROWS_MOST = 32, PROMPT_ROWS = 4096;
-// queries as one f16 (rows of 16 bits: exactly, but for values far below a row's largest), weights as one (no more bits are asked for than bf16 has, or f16_products allows)
+// queries as one f16 (rows of 16 bits: exactly, but for values far below a row's largest), weights as one (no more bits are asked for than bf16 has, or f16_products allows: 2048 tokens behind
+// 2048 take 154 us with one, 171 with two, and results in bf16 are off by 1.67e-3 and 1.66e-3, root mean square)
 static bool one_term(const b200_kv8_attn_args *a) { return a->type != B200_TYPE_F32 || a->f16_products != 0; }
 static bool one_weight(const b200_kv8_attn_args *a) { return a->type == B200_TYPE_BF16 || a->f16_products != 0; }
 

@@ -10,8 +10,8 @@
 // Softmax: four warps a group of 128 rows.  The maximum that the exponent subtracts follows the true one only when that has grown by SLACK, so O is hardly
 // ever rescaled.  A key's scale joins its score, a value's its weight, relative to the power of two above the largest that the row has seen.
 // Every S has two buffers a group: products run while the softmax is busy with the tile before.
-// Measured (heads of 128, 32 query heads over 8, bf16): 2048 tokens behind 2048 in 153 us, 673 TFLOP/s; 7 ragged prompts of up to 700 tokens, 32 heads with keys of their own, f32,
-// in 96 us.  A tile of 64 keys and 256 rows takes 1.45 us where its products take 0.75 and its exponentials 0.55: the four phases of a softmax warp's tile (scores, maximum,
+// Measured (heads of 128, 32 query heads over 8, bf16): 2048 tokens behind 2048 in 154 us, 668 TFLOP/s; 7 ragged prompts of up to 700 tokens, 32 heads with keys of their own, f32,
+// in 98 us.  A tile of 64 keys and 256 rows takes 1.45 us where its products take 0.75 and its exponentials 0.55: the four phases of a softmax warp's tile (scores, maximum,
 // exponentials, weights) follow one another and two such warps share a scheduler, whose issue is at 54%.  A CTA takes 6.5 us to its first tile and 4.5 after its last.
 // With few rows behind many keys, several CTAs (of one group) share a block's tiles; kv8_attn_join_kernel adds their results up.
 // Waits have a limit, as in the prompt GEMM: a role that gives up sets `failed`, the others follow, and the status word is set.
@@ -76,8 +76,8 @@ __device__ __forceinline__ float4 row_load4(const float *p, bool vec) {
 // The tensor cores cut their sums off below the last place instead of rounding them: an addition takes up to 2^-23 of what has been summed up, half a last place on average, and a sum that is
 // kept in TMEM drifts (values around a mean: 1.7e-6 of the result after 81 additions, 7.4e-6 after 270, 1.5e-4 after 3800).  So after kt_fold_every additions the accumulators go to
 // memory, where f32 additions round, and begin at 0 again: to the rows of dst if they are f32, to this CTA's share of the partial results if several share a block, or to a place
-// that the CTA takes from the workspace for as long as it runs.  Rows of full precision 128 additions: 2.7e-6 of a result that grows evenly at most, 15% of a prompt's time at 2000 to 16,000 keys
-// (64: half of the error, 31%; 256: twice, 6%).  Where queries and weights are one f16, or results have 16 bits, 512: 1.1e-5, where half a step of f16 is 2.4e-4 or more.
+// that the CTA takes from the workspace for as long as it runs.  Rows of full precision 128 additions: 2.8e-6 of a result that grows evenly (measured, 30,000 keys), 2^-17 of any, 15% of a prompt's
+// time at 2000 to 16,000 keys (64: half of the error, 31%; 256: twice, 6%).  Where queries are one f16, or results have 16 bits, 512: 1.1e-5 and 2^-15, where half a step of f16 is 2.4e-4 or more.
 template <int TERMS> constexpr int kt_fold_every() { return TERMS == 2 ? 128 : 512; }
 // A place for GROUPS times 128 rows: there are as many as SMs, which run one CTA each (registers), so one is free.  -1: none was.
 __device__ __forceinline__ int kt_take(int *places, int n) {
@@ -147,7 +147,7 @@ __device__ __noinline__ void kt_put(const float *base, int64_t at, void *dst, in
     }
 }
 // A thread's registers from here on, by groups of four warps.  A launch has 96 a thread for 20 warps, 61,440 in all: 8 softmax warps of 144, 8 converting ones of 72
-// and 4 of 48 take just those (12 warps of 128 each with one group of rows: 49,152 of its 65,536).
+// and 4 of 48 take just those (with one group of rows 16 warps are launched with 128 each, 65,536 in all, of which 4 of 144, 8 of 72 and 4 of 48 take 43,008).
 constexpr int KT_REGS_SOFTMAX = 144, KT_REGS_CONVERT = 72, KT_REGS_PRODUCTS = 48;
 template <int N, bool MORE>
 __device__ __forceinline__ void kt_registers() {

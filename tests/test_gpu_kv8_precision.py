@@ -1,8 +1,9 @@
 """Precision of attention over the paged 8-bit cache (include/b200_kv8.h) where the length of sums shows, against softmax in 64 bits on the GPU.
 
-Keys are made so that scores are exact or hardly matter, values have scales that are powers of two and enter exactly as they are; what is left is how sums are taken.
+Keys are made so that scores are exact or hardly matter, values have scales that are powers of two (but in "inexact") and enter exactly as they are; what is left is how sums are taken.
 Kinds of rows (keys a query sees: key 0 and n others):
-  "even"     all weights are 1, values of one sign: sums grow evenly
+  "even"     all weights are 1, values of one sign: sums grow evenly, and are exact until they pass 24 bits
+  "inexact"  the same under a scale of 22 bits: every addition has bits to lose
   "zero"     all weights are 1, values around zero
   "first"    key 0 takes all the weight (the others e^-30 of it): what comes behind it must not change its value
   "small"    key 0 has most of the weight, each other about 2^-20 of it
@@ -19,8 +20,9 @@ from koboldcpp_b200.lib import Kv8AttnArgs, Kv8Cache, check, lib
 pytestmark = pytest.mark.gpu
 
 TYPES = {"f32": (L.F32, torch.float32), "f16": (L.F16, torch.float16), "bf16": (L.BF16, torch.bfloat16)}
-KINDS = ["even", "zero", "first", "small"]
+KINDS = ["even", "inexact", "zero", "first", "small"]
 V_SCALE = 2.0 ** -7
+INEXACT = 2905413 * 2.0 ** -28  # 0.0108
 
 
 class Rows:
@@ -31,9 +33,10 @@ class Rows:
         self.n_seq, self.n, self.new, self.heads, self.dim, self.vdim, self.page = n_seq, n, new, heads, dim, vdim, page
         n_pages = -(-n // page)
         rand = lambda lo, hi, *s: torch.randint(lo, hi, s, generator=g, device="cuda").to(torch.int8)  # noqa: E731
-        self.v = rand(1, 128, n_pages * page, heads, vdim) if kind == "even" else rand(-127, 128, n_pages * page, heads, vdim)
+        self.v = rand(1, 128, n_pages * page, heads, vdim) if kind in ("even", "inexact") else rand(-127, 128, n_pages * page, heads, vdim)
         self.v[0] = rand(60, 128, heads, vdim)
-        if kind in ("even", "zero"):
+        self.v_scale = INEXACT if kind == "inexact" else V_SCALE
+        if kind in ("even", "inexact", "zero"):
             self.k = torch.zeros(n_pages * page, heads, dim, dtype=torch.int8, device="cuda")
             self.scale = 1.0
         else:  # q = 1: scores are scale times the sum of a key's ints
@@ -44,7 +47,7 @@ class Rows:
         pool = torch.zeros(n_pages, lib().b200_kv8_page_bytes(page, heads, dim, vdim), dtype=torch.uint8, device="cuda")
         pool[:, :nk] = self.k.reshape(n_pages, page, heads, dim).transpose(1, 2).reshape(n_pages, nk).view(torch.uint8)
         pool[:, nk:nk + nv] = self.v.reshape(n_pages, page, heads, vdim).transpose(1, 2).reshape(n_pages, nv).view(torch.uint8)
-        pool[:, nk + nv:nk + nv + 8 * heads] = torch.tensor([1.0] * heads + [V_SCALE] * heads, device="cuda").view(torch.uint8)
+        pool[:, nk + nv:nk + nv + 8 * heads] = torch.tensor([1.0] * heads + [self.v_scale] * heads, device="cuda").view(torch.uint8)
         self.pool = pool
         self.cache = Kv8Cache(pool.data_ptr(), n_pages, page, heads, dim, vdim)
         self.table = torch.randperm(n_pages, generator=torch.Generator().manual_seed(seed)).to("cuda", torch.int32)
@@ -70,7 +73,7 @@ class Rows:
         n = self.n - self.new + token + 1
         s = self.k[:n].double().sum(-1) * float(torch.tensor(self.scale, dtype=torch.float32))
         p = torch.softmax(s, dim=0)
-        v = self.v[:n].double() * V_SCALE
+        v = self.v[:n].double() * self.v_scale
         return torch.einsum("nh,nhd->hd", p, v), torch.einsum("nh,nhd->hd", p, v.abs())
 
 
@@ -87,7 +90,7 @@ def test_long_sums_of_few_rows(kind, n_seq, n, heads, n_head, vdim, f16):
     added in f32, to the nearest: N = n / 128 + 8 roundings of half a last place, 2^-24 of the sum, either way, 6 standard deviations of 2^-24 sqrt(N / 3).  Weights: 2^-22 of two f16 (they are powers of two
     times 1 in "even" and "zero"; with one f16 each of the small ones is off by 2^-12, and their sum by 2^-12 of its share of the mass), exponentials 2^-21; the sum of the weights as
     the tiles' sums.  In "first" additions behind the first tile are of nothing: no term in N."""
-    if kind == "small" and f16:
+    if kind in ("small", "inexact") and f16:
         pytest.skip("weights are rounded to f16 there")
     r = Rows(kind, n_seq, n, 1, heads, 16, vdim, seed=n_head)
     want, mass = (x.repeat_interleave(n_head // heads, dim=0) for x in r.want(0))
