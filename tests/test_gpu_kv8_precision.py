@@ -164,3 +164,17 @@ def test_soft_cap_of_f32_rows(n_seq, new, heads, n_head, dim, vdim, cap):
     want = own * torch.tanh((s[0] - s[1]) / 2)[..., None]
     most = own.abs() * ((s[0].abs() + s[1].abs()) * 2.0 ** -21 + 2.0 ** -20)[..., None]
     assert ((got - want).abs() <= most).all(), float(((got - want).abs() / most).max())
+
+
+@pytest.mark.parametrize("kind", ["even", "zero", "first"])
+@pytest.mark.parametrize("heads,n_head,new", PROMPTS)
+def test_long_sums_of_prompts_with_f16_products(kind, heads, n_head, new):
+    """f32 rows whose queries and weights (powers of two here) are one f16 each: 512 additions between two folds, 2^-15 of a sum that grows evenly; the rest as above."""
+    n = 30000
+    r = Rows(kind, 1, n, new, heads, 16, 64, seed=new)
+    got = r.run("f32", n_head, f16=1)
+    for token in (0, 1, new // 2, new - 1):
+        want, mass = (x.repeat_interleave(n_head // heads, dim=0) for x in r.want(token))
+        e = off(got[0, token], want, mass)
+        many = 0.0 if kind == "first" else 2.0 ** -15 + 6 * 2.0 ** -24 * math.sqrt(n / 64 / 3)
+        assert not e.isnan().any() and e.abs().max() <= 2.0 ** -20 + many, (token, float(e.abs().max()))
