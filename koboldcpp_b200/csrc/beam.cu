@@ -1,0 +1,526 @@
+// beam.cu -- beam search (include/b200_state.h): the best successors over all beams and tokens of a request (b200_op_beam_select), and slots that become what other slots
+// held (b200_op_state_reorder).
+#include <cuda_bf16.h>
+
+#include "../../include/b200_state.h"
+#include "ops_util.cuh"
+
+namespace b200 {
+namespace beam {
+
+// ------------------------------------------------------------------------------------------------ selection
+// Two launches.  The first reads the logits once: of every piece of PIECE tokens of a row (or a power of two of them) it keeps the largest, of every share of a row the sum of exponentials.
+// The second, a CTA a request, knows the logarithms of the sums then, and so every piece's best score.  The n_keep best successors all lie in the n_keep pieces whose best come first
+// (a successor elsewhere comes behind the best of each of these), so it reads those pieces again and nothing else.
+constexpr int PIECE = 512, ROW_WARPS = 8, PICK_THREADS = 512, PICK_WARPS = PICK_THREADS / 32;
+constexpr int MOST_PIECES = 4096;  // of a request: what the second launch looks through
+constexpr int LIST = 512;          // candidates that are ranked by counting; where ties make them more, the best are taken out one after the other
+struct SelectArgs {
+    const void *logits; int64_t logits_stride;
+    const float *score;
+    const int32_t *ended, *slot;
+    float *to_score; int32_t *to_beam, *to_token, *to_slot;
+    int32_t beams, vocab, keep, end_token;
+    // layout: tokens of a piece, pieces of a row, pieces of a share, shares of a row
+    int32_t piece, n_pieces, share, n_shares;
+    float *tops;      // [rows][n_pieces]: the largest logit, -inf where there is none
+    double *sums;     // [rows][n_shares]: a sum of exponentials ..
+    int32_t *refs;    // .. and what it refers to (see Ref)
+};
+constexpr float NEG_INF = -INFINITY;
+
+// log2 e in two parts, so that a logit's product with it is off by the last rounding only
+constexpr float LOG2E_HI = 1.4426950408889634f, LOG2E_LO = (float)(1.4426950408889634074 - (double)LOG2E_HI);
+constexpr double LN2 = 0.69314718055994530942;
+__device__ __forceinline__ float ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+
+// Sums of exponentials refer to their largest logit m.  Where |m| < 2^29 the reference is a whole number e not below m log2 e, and what is summed up are 2^(x log2 e - e): it follows a
+// larger reference by a power of two, exactly.  Logits beyond that (masks of a type's lowest value, +inf) lie 32 apart at least, so there only those count that are m itself: the
+// reference is m, as the number that its bits make.  The references' order is that of the logits: -0x7f800000 (-inf: none so far) .. -0x4e000000, -2^30 .. 2^30, 0x4e000000 .. 0x7f800000 (+inf).
+constexpr int NO_REF = -0x7f800000;
+__device__ __forceinline__ bool ref_is_exponent(int r) { return r >= -0x40000000 && r <= 0x40000000; }
+__device__ __forceinline__ int ref_of(float m) {
+    if (fabsf(m) < 536870912.0f) return (int)ceilf(m * LOG2E_HI);
+    const int bits = (int)(__float_as_uint(m) & 0x7fffffffu);
+    return m < 0.f ? -bits : bits;
+}
+__device__ __forceinline__ float ref_logit(int r) { return r < 0 ? -__uint_as_float((unsigned)-r) : __uint_as_float((unsigned)r); }
+// a sum's share of one that refers to the larger `to`
+__device__ __forceinline__ double follow(double sum, int from, int to) {
+    if (from == to) return sum;
+    return ref_is_exponent(from) && ref_is_exponent(to) && to - from <= 1000 ? scalbn(sum, from - to) : 0.0;
+}
+
+// a logit as it counts: NaN is none
+__device__ __forceinline__ float counted(float x) { return x != x ? NEG_INF : x; }
+template <typename T> __device__ __forceinline__ float value_at(const T *p) {
+    if constexpr (sizeof(T) == 4) return counted(*p);
+    else if constexpr (std::is_same<T, __half>::value) return counted(__half2float(*p));
+    else return counted(__bfloat162float(*p));
+}
+// the two values of a word of 16-bit logits
+template <typename T> __device__ __forceinline__ float2 both(unsigned w) {
+    if constexpr (std::is_same<T, __half>::value) return make_float2(counted(h2f((unsigned short)w)), counted(h2f((unsigned short)(w >> 16))));
+    else return make_float2(counted(__uint_as_float(w << 16)), counted(__uint_as_float(w & 0xffff0000u)));
+}
+
+// PIECE tokens of a row from token t0 on, 16 a lane, those behind the vocabulary -inf.  Which token a lane gets does not depend on where the row lies (WIDE is the same for all rows of
+// a call): rows with the same logits have the same sums, bit by bit.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load_piece(const T *row, int t0, int vocab, int lane, float (&x)[16]) {
+    if constexpr (sizeof(T) == 4) {
+        if (WIDE && t0 + PIECE <= vocab) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float4 v = *reinterpret_cast<const float4 *>(row + t0 + 128 * i + 4 * lane);
+                x[4 * i] = counted(v.x); x[4 * i + 1] = counted(v.y); x[4 * i + 2] = counted(v.z); x[4 * i + 3] = counted(v.w);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int t = WIDE ? t0 + 128 * (i / 4) + 4 * lane + i % 4 : t0 + 32 * i + lane;
+                x[i] = t < vocab ? value_at(row + t) : NEG_INF;
+            }
+        }
+    } else if (WIDE && t0 + PIECE <= vocab) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(row + t0 + 256 * i + 8 * lane);
+            const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float2 f = both<T>(w[j]);
+                x[8 * i + 2 * j] = f.x; x[8 * i + 2 * j + 1] = f.y;
+            }
+        }
+    } else if (!WIDE && t0 + PIECE + 2 <= vocab) {
+        // words; where the row begins in the middle of one, a lane's tokens are the upper half of its word and the lower half of the next lane's
+        const bool odd = ((uintptr_t)row & 2) != 0;
+        const unsigned *w = reinterpret_cast<const unsigned *>(row + t0 - odd);
+        unsigned v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = t0 - odd + 64 * i + 2 * lane >= 0 ? w[32 * i + lane] : (unsigned)*reinterpret_cast<const unsigned short *>(row) << 16;
+        const unsigned last = odd ? w[256] : 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            unsigned z = v[i];
+            if (odd) {
+                const unsigned up = __shfl_down_sync(0xffffffffu, z, 1), next = __shfl_sync(0xffffffffu, i < 7 ? v[i < 7 ? i + 1 : 7] : last, 0);
+                z = __funnelshift_r(z, lane == 31 ? next : up, 16);
+            }
+            const float2 f = both<T>(z);
+            x[2 * i] = f.x; x[2 * i + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int t = WIDE ? t0 + 256 * (i / 8) + 8 * lane + i % 8 : t0 + 64 * (i / 2) + 2 * lane + i % 2;
+            x[i] = t < vocab ? value_at(row + t) : NEG_INF;
+        }
+    }
+}
+
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(32 * ROW_WARPS) beam_rows_kernel(const SelectArgs a) {
+    __shared__ double s_sum[ROW_WARPS];
+    __shared__ int s_ref[ROW_WARPS];
+    pdl_enter();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t r = blockIdx.y;
+    const T *row = (const T *)a.logits + r * a.logits_stride;
+    const int p0 = blockIdx.x * a.share, p1 = min(a.n_pieces, p0 + a.share);
+    // beams that nobody asks for the successors of
+    if ((a.ended && a.ended[r]) || !(a.score[r] > NEG_INF)) return;
+    double sum = 0.0;
+    int ref = NO_REF;
+    for (int p = p0 + warp; p < p1; p += ROW_WARPS) {
+        float top = NEG_INF;
+        for (int t0 = p * a.piece; t0 < min(a.vocab, (p + 1) * a.piece); t0 += PIECE) {
+            float x[16];
+            load_piece<T, WIDE>(row, t0, a.vocab, lane, x);
+            float m = x[0];
+#pragma unroll
+            for (int i = 1; i < 16; i++) m = fmaxf(m, x[i]);
+            m = warp_max(m);
+            if (m == NEG_INF) continue;
+            top = fmaxf(top, m);
+            const int now = max(ref, ref_of(m));
+            sum = follow(sum, ref, now);
+            ref = now;
+            float part = 0.f;
+            if (ref_is_exponent(ref)) {
+                const float e = (float)ref;
+#pragma unroll
+                for (int i = 0; i < 16; i++) part += ex2(fmaf(x[i], LOG2E_LO, fmaf(x[i], LOG2E_HI, -e)));
+            } else {
+                const float big = ref_logit(ref);
+#pragma unroll
+                for (int i = 0; i < 16; i++) part += x[i] == big ? 1.f : 0.f;
+            }
+            sum += part;
+        }
+        if (lane == 0) a.tops[r * a.n_pieces + p] = top;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) { s_sum[warp] = sum; s_ref[warp] = ref; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 0; w < ROW_WARPS; w++) ref = max(ref, s_ref[w]);
+        double all = 0.0;
+        for (int w = 0; w < ROW_WARPS; w++) all += follow(s_sum[w], s_ref[w], ref);
+        a.sums[r * a.n_shares + blockIdx.x] = all;
+        a.refs[r * a.n_shares + blockIdx.x] = ref;
+    }
+}
+
+// A successor: its score and its place beam * vocab + token in the request.  Whether x comes before y:
+struct Cand { double score; int64_t at; };
+__device__ __forceinline__ bool before(const Cand &x, const Cand &y) { return x.score > y.score || (x.score == y.score && x.at < y.at); }
+__device__ __forceinline__ Cand shuffled(const Cand &x, int off) { return {__shfl_xor_sync(0xffffffffu, x.score, off), __shfl_xor_sync(0xffffffffu, x.at, off)}; }
+// numbers whose order as unsigned ones is that of the floats; 0 is behind all of them
+__device__ __forceinline__ unsigned ordered(float f) {
+    const unsigned u = __float_as_uint(f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(unsigned u) { return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
+
+struct PickShared {
+    double base[B200_BEAM_MAX];     // a beam's score; -inf: no successors
+    double ref[B200_BEAM_MAX], norm[B200_BEAM_MAX];  // what is taken off its logits, one after the other
+    int ended[B200_BEAM_MAX];
+    Cand list[LIST];
+    Cand best[B200_BEAM_KEEP];      // first the pieces, then the successors
+    Cand warps[PICK_WARPS];
+    int n, overflow;
+};
+
+// The score of a logit of beam b.  With a reference of +inf the tokens of +inf share evenly, the others have none.
+__device__ __forceinline__ double score_of(const PickShared &sh, int b, float x) {
+    if (x == NEG_INF || sh.base[b] == -(double)INFINITY) return -(double)INFINITY;
+    if (x == INFINITY) return sh.base[b] - sh.norm[b];
+    return sh.base[b] + (((double)x - sh.ref[b]) - sh.norm[b]);
+}
+
+// The `keep` first of the candidates that each(thread's function) names, in order, to sh.best; returns how many there are.  each(f) calls f(candidate) for all candidates of the calling
+// thread, whatever their order, and always for the same ones; `floor`: candidates with smaller scores can be left aside (at least `keep` have a score of that or more, or it is -inf).
+template <typename F>
+__device__ int first_of(PickShared &sh, int keep, double floor, F each) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+    each([&](const Cand &c) {
+        if (c.score == -(double)INFINITY || c.score < floor) return;
+        const int i = atomicAdd(&sh.n, 1);
+        if (i < LIST) sh.list[i] = c;
+    });
+    __syncthreads();
+    const int n = sh.n;
+    if (n <= LIST) {
+        // a candidate's rank is the number of those before it: the list's own order, which is that of arrival, does not matter
+        for (int i = tid; i < n; i += PICK_THREADS) {
+            const Cand c = sh.list[i];
+            int rank = 0;
+            for (int j = 0; j < n; j++) rank += before(sh.list[j], c);
+            if (rank < keep) sh.best[rank] = c;
+        }
+        __syncthreads();
+        return min(n, keep);
+    }
+    // one after the other: the first of those behind the last one found
+    Cand last = {INFINITY, -1};
+    for (int k = 0; k < keep; k++) {
+        Cand mine = {-(double)INFINITY, 0x7fffffffffffffffLL};
+        each([&](const Cand &c) { if (c.score >= floor && before(last, c) && before(c, mine)) mine = c; });
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const Cand other = shuffled(mine, o);
+            if (before(other, mine)) mine = other;
+        }
+        if (lane == 0) sh.warps[warp] = mine;
+        __syncthreads();
+        mine = sh.warps[0];
+        for (int w = 1; w < PICK_WARPS; w++) if (before(sh.warps[w], mine)) mine = sh.warps[w];
+        if (tid == 0) sh.best[k] = mine;
+        last = mine;
+        __syncthreads();
+    }
+    return keep;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(PICK_THREADS) beam_pick_kernel(const SelectArgs a) {
+    __shared__ PickShared sh;
+    pdl_enter();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t r0 = (int64_t)blockIdx.x * a.beams;
+    // ===== the logarithms of the sums, a warp a beam
+    for (int b = warp; b < a.beams; b += PICK_WARPS) {
+        const double *sums = a.sums + (r0 + b) * a.n_shares;
+        const int *refs = a.refs + (r0 + b) * a.n_shares;
+        int ref = NO_REF;
+        for (int i = lane; i < a.n_shares; i += 32) ref = max(ref, refs[i]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ref = max(ref, __shfl_xor_sync(0xffffffffu, ref, o));
+        double all = 0.0;
+        for (int i = lane; i < a.n_shares; i += 32) all += follow(sums[i], refs[i], ref);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        if (lane == 0) {
+            const float s = a.score[r0 + b];
+            sh.base[b] = s != s || (ref == NO_REF && !(a.ended && a.ended[r0 + b])) ? -(double)INFINITY : (double)s;
+            sh.ref[b] = ref_is_exponent(ref) ? 0.0 : (double)ref_logit(ref);
+            sh.norm[b] = ref_is_exponent(ref) ? (double)ref * LN2 + log(all) : log(all);
+            sh.ended[b] = a.ended ? a.ended[r0 + b] != 0 : 0;
+        }
+    }
+    __syncthreads();
+    // ===== the pieces: candidates are their best scores, at beam * n_pieces + piece.  An ended beam is one piece of one successor
+    const float *tops = a.tops + r0 * a.n_pieces;
+    const int total = a.beams * a.n_pieces;
+    auto pieces = [&](auto &&f) {
+        for (int i = tid; i < total; i += PICK_THREADS) {
+            const int b = i / a.n_pieces;
+            if (sh.ended[b]) {
+                if (i == b * a.n_pieces) f(Cand{sh.base[b], i});
+            } else {
+                f(Cand{score_of(sh, b, tops[i]), i});
+            }
+        }
+    };
+    // a score that `keep` threads' best reach at least, from above by halving: what lies below can be left aside
+    float top = NEG_INF;
+    pieces([&](const Cand &c) { top = fmaxf(top, __double2float_rd(c.score)); });
+    const unsigned key = top == NEG_INF ? 0 : ordered(top);
+    unsigned low = 0;
+    if (total > LIST) {
+        for (int bit = 31; bit >= 12; bit--) {
+            const unsigned at = low | 1u << bit;
+            if (__syncthreads_count(key >= at) >= a.keep) low = at;
+        }
+    }
+    const int n_best = first_of(sh, a.keep, low == 0 ? -(double)INFINITY : (double)unordered(low), pieces);
+    // ===== the successors in those pieces, a warp a piece
+    int at_piece[B200_BEAM_KEEP / PICK_WARPS];
+#pragma unroll
+    for (int k = 0; k < B200_BEAM_KEEP / PICK_WARPS; k++) at_piece[k] = warp + k * PICK_WARPS < n_best ? (int)sh.best[warp + k * PICK_WARPS].at : -1;
+    const double floor = n_best == a.keep ? sh.best[a.keep - 1].score : -(double)INFINITY;
+    __syncthreads();
+    auto successors = [&](auto &&f) {
+#pragma unroll
+        for (int k = 0; k < B200_BEAM_KEEP / PICK_WARPS; k++) {
+            if (at_piece[k] < 0) break;
+            const int b = at_piece[k] / a.n_pieces, t0 = (at_piece[k] - b * a.n_pieces) * a.piece;
+            if (sh.ended[b]) {
+                if (lane == 0) f(Cand{sh.base[b], (int64_t)b * a.vocab + a.end_token});
+                continue;
+            }
+            const T *row = (const T *)a.logits + (r0 + b) * a.logits_stride;
+#pragma unroll 4
+            for (int t = t0 + lane; t < min(a.vocab, t0 + a.piece); t += 32) f(Cand{score_of(sh, b, value_at(row + t)), (int64_t)b * a.vocab + t});
+        }
+    };
+    const int n = first_of(sh, a.keep, floor, successors);
+    for (int i = tid; i < a.keep; i += PICK_THREADS) {
+        const int64_t to = (int64_t)blockIdx.x * a.keep + i;
+        const bool there = i < n;
+        const int b = there ? (int)(sh.best[i].at / a.vocab) : -1;
+        a.to_score[to] = there ? (float)sh.best[i].score : NEG_INF;
+        a.to_beam[to] = b;
+        a.to_token[to] = there ? (int)(sh.best[i].at - (int64_t)b * a.vocab) : -1;
+        if (a.to_slot) a.to_slot[to] = there && a.slot ? a.slot[r0 + b] : -1;
+    }
+}
+
+struct SelectPlan { int piece, n_pieces, share, n_shares; };
+static SelectPlan select_plan(const b200_beam_select_args *a) {
+    SelectPlan p;
+    p.piece = PIECE;
+    while ((int64_t)a->n_beams * ((a->n_vocab + p.piece - 1) / p.piece) > MOST_PIECES) p.piece *= 2;
+    p.n_pieces = (a->n_vocab + p.piece - 1) / p.piece;
+    // a piece a warp until every SM has its CTAs, then up to four: fewer and longer ones
+    const int64_t rows = (int64_t)a->n_requests * a->n_beams, ctas = rows * ((p.n_pieces + ROW_WARPS - 1) / ROW_WARPS);
+    p.share = ROW_WARPS * (ctas >= 32 * (int64_t)sm_count() ? 4 : ctas >= 16 * (int64_t)sm_count() ? 2 : 1);
+    p.n_shares = (p.n_pieces + p.share - 1) / p.share;
+    return p;
+}
+static size_t select_room(const b200_beam_select_args *a, const SelectPlan &p) {
+    const size_t rows = (size_t)a->n_requests * a->n_beams;
+    return rows * ((size_t)p.n_shares * 12 + (size_t)p.n_pieces * 4);
+}
+static int check_select_sizes(const b200_beam_select_args *a, const char *who) {
+    OPX_REQUIRE(a, B200_ERR_INVALID, "%s: NULL arguments", who);
+    OPX_REQUIRE(a->type == B200_TYPE_F32 || a->type == B200_TYPE_F16 || a->type == B200_TYPE_BF16, B200_ERR_UNSUPPORTED, "%s: logits of type %d", who, a->type);
+    OPX_REQUIRE(a->n_requests >= 0 && a->n_beams > 0 && a->n_vocab > 0 && a->n_keep > 0, B200_ERR_INVALID, "%s: %d requests of %d beams, %d tokens, %d to keep", who, a->n_requests, a->n_beams, a->n_vocab,
+                a->n_keep);
+    OPX_REQUIRE(a->n_beams <= B200_BEAM_MAX && a->n_keep <= B200_BEAM_KEEP && a->n_vocab <= 0x7fff0000, B200_ERR_UNSUPPORTED, "%s: %d beams (%d at most), %d to keep (%d)", who, a->n_beams, B200_BEAM_MAX,
+                a->n_keep, B200_BEAM_KEEP);
+    OPX_REQUIRE((int64_t)a->n_requests * a->n_beams <= 65535 && (int64_t)a->n_requests * a->n_keep <= 0x7fffffff, B200_ERR_UNSUPPORTED, "%s: %d requests of %d beams, 65535 rows at most", who,
+                a->n_requests, a->n_beams);
+    return B200_OK;
+}
+
+template <typename T>
+static int launch_select(const SelectArgs &a, int rows, bool wide, cudaStream_t st) {
+    const dim3 grid((unsigned)a.n_shares, (unsigned)rows);
+    B200_CUDA_TRY(launch_chained(wide ? beam_rows_kernel<T, true> : beam_rows_kernel<T, false>, grid, 32 * ROW_WARPS, 0, st, a));
+    B200_CUDA_TRY(launch_chained(beam_pick_kernel<T>, (unsigned)(rows / a.beams), PICK_THREADS, 0, st, a));
+    return B200_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ reordering
+// A CTA takes the same bytes of all slots that move, a column: it reads them all into shared memory before it writes any, so nothing is overwritten that is still wanted, whatever cycles
+// the moves make.  Columns do not touch one another.
+constexpr int REORDER_THREADS = 256, REORDER_STATES = 128, COLUMNS_BYTES = 32 * 1024;
+constexpr int REORDER_MOST = COLUMNS_BYTES + 4 * (B200_STATE_MAX_SLOTS + 2 * B200_STATE_MAX_MOVES);
+struct ReorderArgs {
+    char *base[REORDER_STATES];
+    int64_t stride[REORDER_STATES], bytes[REORDER_STATES];
+    int32_t first[REORDER_STATES + 1];  // number of a state's first column
+    int32_t n_states, n, n_slots, width;  // width: bytes of a column
+    const int32_t *src, *dst;
+    int32_t *refused;
+};
+template <int UNIT>  // bytes of an access: 16 or 4
+__global__ void __launch_bounds__(REORDER_THREADS) state_reorder_kernel(const ReorderArgs a) {
+    extern __shared__ __align__(16) unsigned char column[];  // [n][width], then the moves
+    int *claim = (int *)(column + (size_t)a.n * a.width), *from = claim + a.n_slots, *to = from + a.n;
+    __shared__ int n_moves, n_refused;
+    pdl_enter();
+    const int tid = threadIdx.x;
+    if (tid == 0) n_moves = n_refused = 0;
+    for (int i = tid; i < a.n_slots; i += REORDER_THREADS) claim[i] = 0x7fffffff;
+    __syncthreads();
+    for (int i = tid; i < a.n; i += REORDER_THREADS) {
+        const int s = a.src[i], d = a.dst[i];
+        if (s >= 0 && s < a.n_slots && d >= 0 && d < a.n_slots) atomicMin(&claim[d], i);
+    }
+    __syncthreads();
+    for (int i = tid; i < a.n; i += REORDER_THREADS) {
+        const int s = a.src[i], d = a.dst[i];
+        if (s < 0 || s >= a.n_slots || d < 0 || d >= a.n_slots || claim[d] != i) {
+            atomicAdd(&n_refused, 1);
+        } else if (s != d) {
+            const int k = atomicAdd(&n_moves, 1);
+            from[k] = s;
+            to[k] = d;
+        }
+    }
+    __syncthreads();
+    if (a.refused && blockIdx.x == 0 && tid == 0 && n_refused) *a.refused += n_refused;
+    const int n = n_moves, units = a.width / UNIT;
+    if (n == 0) return;
+    for (int item = blockIdx.x; item < a.first[a.n_states]; item += gridDim.x) {
+        int lo = 0, hi = a.n_states - 1;  // the last state whose first column is not behind this one
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (a.first[mid] <= item) lo = mid;
+            else hi = mid - 1;
+        }
+        const int64_t at = (int64_t)(item - a.first[lo]) * a.width, stride = a.stride[lo];
+        char *base = a.base[lo] + at;
+        const int here = (int)min((int64_t)a.width, a.bytes[lo] - at) / UNIT;
+        for (int i = tid; i < n * units; i += REORDER_THREADS) {
+            const int k = i / units, u = i - k * units;
+            if (u < here) {
+                if constexpr (UNIT == 16) cp_async16(column + (size_t)k * a.width + u * UNIT, base + from[k] * stride + u * UNIT);
+                else cp_async4(column + (size_t)k * a.width + u * UNIT, base + from[k] * stride + u * UNIT);
+            }
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        __syncthreads();
+        for (int i = tid; i < n * units; i += REORDER_THREADS) {
+            const int k = i / units, u = i - k * units;
+            if (u < here) {
+                if constexpr (UNIT == 16) *reinterpret_cast<uint4 *>(base + to[k] * stride + u * UNIT) = *reinterpret_cast<const uint4 *>(column + (size_t)k * a.width + u * UNIT);
+                else *reinterpret_cast<unsigned *>(base + to[k] * stride + u * UNIT) = *reinterpret_cast<const unsigned *>(column + (size_t)k * a.width + u * UNIT);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+}  // namespace beam
+}  // namespace b200
+
+using namespace b200;
+using namespace b200::beam;
+
+extern "C" {
+
+size_t b200_beam_select_workspace_bytes(const b200_beam_select_args *a) {
+    if (check_select_sizes(a, "b200_beam_select_workspace_bytes") != B200_OK) return 0;
+    return select_room(a, select_plan(a));
+}
+
+int b200_op_beam_select(const b200_beam_select_args *a, void *workspace, size_t workspace_bytes, b200_stream_t stream) {
+    const char *who = "b200_op_beam_select";
+    const int rc = check_select_sizes(a, who);
+    if (rc != B200_OK || a->n_requests == 0) return rc;
+    OPX_REQUIRE(a->logits && a->score && a->to_score && a->to_beam && a->to_token, B200_ERR_INVALID, "%s: NULL argument", who);
+    OPX_REQUIRE(!a->to_slot || a->slot, B200_ERR_INVALID, "%s: to_slot without slot", who);
+    OPX_REQUIRE(a->logits_stride >= a->n_vocab, B200_ERR_INVALID, "%s: rows overlap (stride %lld, %d tokens)", who, (long long)a->logits_stride, a->n_vocab);
+    OPX_REQUIRE(!a->ended || (a->end_token >= 0 && a->end_token < a->n_vocab), B200_ERR_INVALID, "%s: end token %d of %d", who, a->end_token, a->n_vocab);
+    const size_t size = a->type == B200_TYPE_F32 ? 4 : 2;
+    OPX_REQUIRE((uintptr_t)a->logits % size == 0 && (((uintptr_t)a->score | (uintptr_t)a->ended | (uintptr_t)a->slot | (uintptr_t)a->to_score | (uintptr_t)a->to_beam | (uintptr_t)a->to_token |
+                (uintptr_t)a->to_slot) & 3) == 0, B200_ERR_INVALID, "%s: a pointer is not aligned to its type", who);
+    OPX_REQUIRE((const void *)a->to_score != a->score && (!a->slot || a->to_slot != a->slot), B200_ERR_INVALID, "%s: not in place", who);
+    const SelectPlan p = select_plan(a);
+    const size_t need = select_room(a, p), rows = (size_t)a->n_requests * a->n_beams;
+    OPX_REQUIRE(workspace && workspace_bytes >= need && (uintptr_t)workspace % 8 == 0, B200_ERR_INVALID, "%s: workspace of %zu bytes, 8-byte aligned", who, need);
+    double *sums = (double *)workspace;
+    int32_t *refs = (int32_t *)(sums + rows * p.n_shares);
+    const SelectArgs s = {a->logits, a->logits_stride, a->score, a->ended, a->slot, a->to_score, a->to_beam, a->to_token, a->to_slot, a->n_beams, a->n_vocab, a->n_keep, a->end_token,
+                          p.piece, p.n_pieces, p.share, p.n_shares, (float *)(refs + rows * p.n_shares), sums, refs};
+    const bool wide = (uintptr_t)a->logits % 16 == 0 && a->logits_stride * (int64_t)size % 16 == 0;
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (a->type == B200_TYPE_F32) return launch_select<float>(s, (int)rows, wide, st);
+    if (a->type == B200_TYPE_F16) return launch_select<__half>(s, (int)rows, wide, st);
+    return launch_select<__nv_bfloat16>(s, (int)rows, wide, st);
+}
+
+int b200_op_state_reorder(const b200_slot_state *states, int32_t n_states, const int32_t *src, const int32_t *dst, int32_t n, int32_t n_slots, int32_t *refused, b200_stream_t stream) {
+    const char *who = "b200_op_state_reorder";
+    OPX_REQUIRE(n_states >= 0 && n >= 0 && n_slots >= 0, B200_ERR_INVALID, "%s: %d states, %d moves, %d slots", who, n_states, n, n_slots);
+    OPX_REQUIRE(n <= B200_STATE_MAX_MOVES && n_slots <= B200_STATE_MAX_SLOTS, B200_ERR_UNSUPPORTED, "%s: %d moves (%d at most), %d slots (%d)", who, n, B200_STATE_MAX_MOVES, n_slots, B200_STATE_MAX_SLOTS);
+    if (n == 0) return B200_OK;
+    OPX_REQUIRE(src && dst && (states || n_states == 0), B200_ERR_INVALID, "%s: NULL argument", who);
+    OPX_REQUIRE((((uintptr_t)src | (uintptr_t)dst | (uintptr_t)refused) & 3) == 0, B200_ERR_INVALID, "%s: a list at an odd place", who);
+    bool wide = true;
+    for (int i = 0; i < n_states; i++) {
+        const b200_slot_state &s = states[i];
+        OPX_REQUIRE(s.bytes >= 0 && s.stride >= s.bytes && (s.base || s.bytes == 0), B200_ERR_INVALID, "%s: state %d: %lld bytes of a slot every %lld", who, i, (long long)s.bytes, (long long)s.stride);
+        OPX_REQUIRE((((uintptr_t)s.base | (uint64_t)s.stride | (uint64_t)s.bytes) & 3) == 0, B200_ERR_INVALID, "%s: state %d is not a multiple of 4 bytes", who, i);
+        wide = wide && (((uintptr_t)s.base | (uint64_t)s.stride | (uint64_t)s.bytes) & 15) == 0;
+    }
+    // as wide a column as the moves leave room for
+    int width = COLUMNS_BYTES / n / 16 * 16;
+    width = width > 2048 ? 2048 : width < 32 ? 32 : width;
+    const size_t smem = (size_t)n * width + 4 * ((size_t)n_slots + 2 * n);
+    const auto kern = wide ? state_reorder_kernel<16> : state_reorder_kernel<4>;
+    if (smem > 48 * 1024) B200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, REORDER_MOST));  // (the same for all calls: they may be in several threads)
+    int at = 0;
+    do {  // (without states too: refused moves are counted)
+        ReorderArgs r = {};
+        int64_t columns = 0;
+        while (at < n_states && r.n_states < REORDER_STATES && columns + (states[at].bytes + width - 1) / width <= 0x7fffffff) {
+            const b200_slot_state &s = states[at++];
+            r.base[r.n_states] = (char *)s.base;
+            r.stride[r.n_states] = s.stride;
+            r.bytes[r.n_states] = s.bytes;
+            r.first[r.n_states++] = (int32_t)columns;
+            columns += (s.bytes + width - 1) / width;
+        }
+        OPX_REQUIRE(r.n_states > 0 || n_states == 0, B200_ERR_UNSUPPORTED, "%s: a state of %lld bytes a slot", who, (long long)states[at].bytes);
+        r.first[r.n_states] = (int32_t)columns;
+        r.n = n; r.n_slots = n_slots; r.width = width; r.src = src; r.dst = dst;
+        r.refused = at >= n_states ? refused : nullptr;
+        const int64_t most = 6 * (int64_t)sm_count();
+        const unsigned grid = (unsigned)(columns < 1 ? 1 : columns < most ? columns : most);
+        B200_CUDA_TRY(launch_chained(kern, grid, REORDER_THREADS, smem, (cudaStream_t)stream, r));
+    } while (at < n_states);
+    return B200_OK;
+}
+
+}  // extern "C"

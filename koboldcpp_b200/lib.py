@@ -184,6 +184,34 @@ class Kv8Map(C.Structure):
                 ("_pad", C.c_int32)]
 
 
+class SsmConvArgs(C.Structure):
+    """b200_ssm_conv_args (include/b200_state.h); strides in values."""
+    _fields_ = [("x", C.c_void_p), ("x_stride", C.c_int64), ("w", C.c_void_p), ("bias", C.c_void_p), ("seq_info", C.c_void_p), ("tail", C.c_void_p), ("slot_stride", C.c_int64),
+                ("dst", C.c_void_p), ("dst_stride", C.c_int64), ("n_seq", C.c_int32), ("n_slots", C.c_int32), ("n_tokens", C.c_int32), ("max_new", C.c_int32),
+                ("channels", C.c_int32), ("taps", C.c_int32), ("silu", C.c_int32), ("type", C.c_int32)]
+
+
+class SsmScanArgs(C.Structure):
+    """b200_ssm_scan_args (include/b200_state.h); strides in values."""
+    _fields_ = [("x", C.c_void_p), ("dt", C.c_void_p), ("x_stride", C.c_int64), ("dt_stride", C.c_int64), ("b", C.c_void_p), ("c", C.c_void_p), ("b_stride", C.c_int64),
+                ("c_stride", C.c_int64), ("z", C.c_void_p), ("z_stride", C.c_int64), ("a", C.c_void_p), ("dt_bias", C.c_void_p), ("d", C.c_void_p), ("seq_info", C.c_void_p),
+                ("state", C.c_void_p), ("slot_stride", C.c_int64), ("from", C.c_void_p), ("from_stride", C.c_int64), ("dst", C.c_void_p), ("dst_stride", C.c_int64), ("n_seq", C.c_int32),
+                ("n_slots", C.c_int32), ("n_tokens", C.c_int32), ("max_new", C.c_int32), ("channels", C.c_int32), ("d_state", C.c_int32), ("groups", C.c_int32), ("softplus", C.c_int32),
+                ("type", C.c_int32)]
+
+
+class BeamSelectArgs(C.Structure):
+    """b200_beam_select_args (include/b200_state.h); stride in values."""
+    _fields_ = [("logits", C.c_void_p), ("logits_stride", C.c_int64), ("score", C.c_void_p), ("ended", C.c_void_p), ("slot", C.c_void_p), ("to_score", C.c_void_p), ("to_beam", C.c_void_p),
+                ("to_token", C.c_void_p), ("to_slot", C.c_void_p), ("n_requests", C.c_int32), ("n_beams", C.c_int32), ("n_vocab", C.c_int32), ("n_keep", C.c_int32),
+                ("end_token", C.c_int32), ("type", C.c_int32)]
+
+
+class SlotState(C.Structure):
+    """b200_slot_state (include/b200_state.h): one kind of state of one layer; bytes."""
+    _fields_ = [("base", C.c_void_p), ("stride", C.c_int64), ("bytes", C.c_int64)]
+
+
 _SIGS = {
     # name: (restype, argtypes)
     "b200_last_error": (C.c_char_p, []),
@@ -307,6 +335,16 @@ _KV8_SIGS = {
     "b200_op_kv8_copy_pages": (C.c_int, [C.POINTER(Kv8Cache), C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]),
 }
 
+# include/b200_state.h
+_STATE_SIGS = {
+    "b200_op_ssm_conv": (C.c_int, [C.POINTER(SsmConvArgs), C.c_void_p]),
+    "b200_ssm_scan_workspace_bytes": (C.c_size_t, [C.POINTER(SsmScanArgs)]),
+    "b200_op_ssm_scan": (C.c_int, [C.POINTER(SsmScanArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "b200_beam_select_workspace_bytes": (C.c_size_t, [C.POINTER(BeamSelectArgs)]),
+    "b200_op_beam_select": (C.c_int, [C.POINTER(BeamSelectArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "b200_op_state_reorder": (C.c_int, [C.POINTER(SlotState), C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]),
+}
+
 _lib = None
 
 
@@ -320,7 +358,7 @@ def load(path: Path | None = None):
     if not p.exists():
         raise B200Error(f"{p} not found: build it with `python -m koboldcpp_b200.build` (nvcc, sm_100a)")
     L = C.CDLL(str(p))
-    for name, (res, args) in list(_SIGS.items()) + list(_OPS_SIGS.items()) + list(_KV8_SIGS.items()):
+    for name, (res, args) in list(_SIGS.items()) + list(_OPS_SIGS.items()) + list(_KV8_SIGS.items()) + list(_STATE_SIGS.items()):
         f = getattr(L, name)  # AttributeError if the library does not export a declared symbol
         f.restype = res
         f.argtypes = args
