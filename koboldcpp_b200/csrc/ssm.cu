@@ -37,41 +37,71 @@ template <typename T> __device__ __forceinline__ T narrow(float x) {
     else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(x);
     else return __float2bfloat16_rn(x);
 }
+// two values at once
+template <typename T> __device__ __forceinline__ void narrow2(T *to, float lo, float hi) {
+    if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<__half2 *>(to) = __floats2half2_rn(lo, hi);
+    else if constexpr (sizeof(T) == 2) *reinterpret_cast<__nv_bfloat162 *>(to) = __floats2bfloat162_rn(lo, hi);
+    else { to[0] = lo; to[1] = hi; }
+}
 // V consecutive values, in one access where they lie on a boundary of their size
 template <typename T, int V> struct __align__(sizeof(T) * V) Pack { T v[V]; };
 
-// y * sigmoid(y); one exponential and one reciprocal of the special function unit (2^-22 each)
-__device__ __forceinline__ float silu(float y) { return __fdividef(y, 1.0f + __expf(-y)); }
+constexpr float LOG2E = 1.4426950408889634f;
+// 2^x and 1 / x of the special function unit, off by 2^-22 and 2^-23; numbers below 2^-126 are zeros
+__device__ __forceinline__ float ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+__device__ __forceinline__ float rcp(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+// y * sigmoid(y) (where e^-y is more than f32 holds, -0)
+__device__ __forceinline__ float silu(float y) { return y * rcp(1.0f + ex2(-LOG2E * y)); }
+
+// two floats that are worked on by one instruction
+using Two = unsigned long long;
+__device__ __forceinline__ Two two(float lo, float hi) { Two r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi)); return r; }
+__device__ __forceinline__ float2 each(Two x) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x)); return r; }
+__device__ __forceinline__ Two fma2(Two x, Two y, Two z) { Two r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z)); return r; }
+__device__ __forceinline__ Two mul2(Two x, Two y) { Two r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y)); return r; }
 
 // ------------------------------------------------------------------------------------------------ short convolution
-// A thread takes V channels of CONV_ROWS rows of one sequence and keeps the last K - 1 inputs in registers.  The CTAs that hold a sequence's first rows read its tail, and they alone
-// write it (each channel by one thread), so that nobody reads what another has rewritten.  K: taps, or the next of 8 and 16, whose products of taps that are not there are left out.
-constexpr int CONV_ROWS = 16, CONV_AHEAD = 8, CONV_THREADS = 128;
+// A thread takes V channels of `rows` rows of one sequence and keeps the last K - 1 inputs in registers; rows travel in groups, asynchronously to a ring in shared memory.  The CTAs that hold a
+// sequence's first rows read its tail, and they alone write it (each channel by one thread), so that nobody reads what another has rewritten.  K: taps, or the next of 8 and 16, whose products of
+// taps that are not there are left out.  Weights and biases do not depend on the sequence: they are asked for before it is known.
+constexpr int CONV_THREADS = 128, CONV_GROUP = 4, CONV_GROUPS = 4, CONV_ROWS_MIN = 16, CONV_ROWS_MAX = 64;
 struct ConvArgs {
     Step step;
     const void *x; int64_t x_stride;
     const float *w, *bias;
     float *tail; int64_t slot_stride;
     void *dst; int64_t dst_stride;
-    int32_t channels, taps, silu;
+    int32_t channels, taps, silu, rows;
 };
-template <typename T, int K, int V, bool EXACT>
+template <typename T, int K, int V, bool EXACT, bool RING>
 __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_kernel(const ConvArgs a) {
     pdl_enter();
-    const int c = (blockIdx.x * CONV_THREADS + threadIdx.x) * V, t0 = blockIdx.y * CONV_ROWS;
+    const int c = (blockIdx.x * CONV_THREADS + threadIdx.x) * V, t0 = blockIdx.y * a.rows;
+    const int skip = EXACT ? 0 : K - a.taps;  // taps that are not there
+    if (c >= a.channels) return;
+    float w[K][V], bias[V], win[K][V];  // win[K - 1]: the newest input
+    const float *pw = a.w + (int64_t)c * a.taps;
+    if (K == 4 && EXACT && ((uintptr_t)a.w & 15) == 0) {
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            const float4 v = reinterpret_cast<const float4 *>(pw)[e];
+            w[0][e] = v.x; w[1 % K][e] = v.y; w[2 % K][e] = v.z; w[3 % K][e] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+#pragma unroll
+            for (int j = 0; j < K; j++) w[j][e] = EXACT || j >= skip ? pw[e * a.taps + j - skip] : 0.f;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < V; e++) bias[e] = a.bias ? a.bias[c + e] : 0.f;
     const Seq q = seq_of(a.step, blockIdx.z);
-    if (c >= a.channels || t0 >= q.count) return;
-    const int nt = min(CONV_ROWS, q.count - t0), skip = EXACT ? 0 : K - a.taps;  // taps that are not there
+    if (t0 >= q.count) return;
+    const int nt = min(a.rows, q.count - t0);
     const T *x = (const T *)a.x + (int64_t)q.first * a.x_stride + c;
     float *tail = a.tail + (int64_t)q.slot * a.slot_stride + c;
     using P = Pack<T, V>;
-    float w[K][V], bias[V], win[K][V];  // win[K - 1]: the newest input
-#pragma unroll
-    for (int e = 0; e < V; e++) {
-        bias[e] = a.bias ? a.bias[c + e] : 0.f;
-#pragma unroll
-        for (int j = 0; j < K; j++) w[j][e] = EXACT || j >= skip ? a.w[(int64_t)(c + e) * a.taps + j - skip] : 0.f;
-    }
 #pragma unroll
     for (int j = 1; j < K; j++) {  // win[j]: the input of row t0 - K + j
         const int i = t0 - K + j;
@@ -86,38 +116,85 @@ __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_kernel(const ConvArgs a
         }
     }
     T *dst = (T *)a.dst + (int64_t)(q.first + t0) * a.dst_stride + c;
-    x += (int64_t)t0 * a.x_stride;
-    for (int b = 0; b < nt; b += CONV_AHEAD) {
-        P in[CONV_AHEAD];
+    const T *in_row = x + (int64_t)t0 * a.x_stride;
+    auto turn = [&](const P &in) {  // the next row
+        P out;
 #pragma unroll
-        for (int u = 0; u < CONV_AHEAD; u++) {
-            if (b + u < nt) in[u] = *reinterpret_cast<const P *>(x + (int64_t)(b + u) * a.x_stride);
+        for (int e = 0; e < V; e++) {
+#pragma unroll
+            for (int j = 0; j < K - 1; j++) win[j][e] = win[j + 1][e];
+            win[K - 1][e] = wide(in.v[e]);
         }
 #pragma unroll
-        for (int u = 0; u < CONV_AHEAD; u++) {
-            if (b + u >= nt) break;
-            P out;
+        for (int e = 0; e < V; e += 2) {
+            float y[2];
+            if constexpr (V >= 2) {
+                Two s = two(bias[e], bias[e + 1]);
 #pragma unroll
-            for (int e = 0; e < V; e++) {
+                for (int j = 0; j < K; j++) if (EXACT || j >= skip) s = fma2(two(w[j][e], w[j][e + 1]), two(win[j][e], win[j][e + 1]), s);
+                y[0] = each(s).x; y[1] = each(s).y;
+            } else {
+                y[0] = bias[e];
 #pragma unroll
-                for (int j = 0; j < K - 1; j++) win[j][e] = win[j + 1][e];
-                win[K - 1][e] = wide(in[u].v[e]);
-                float y = bias[e];
-#pragma unroll
-                for (int j = 0; j < K; j++) if (EXACT || j >= skip) y = fmaf(w[j][e], win[j][e], y);
-                out.v[e] = narrow<T>(a.silu ? silu(y) : y);
+                for (int j = 0; j < K; j++) if (EXACT || j >= skip) y[0] = fmaf(w[j][e], win[j][e], y[0]);
             }
-            *reinterpret_cast<P *>(dst + (int64_t)(b + u) * a.dst_stride) = out;
+            if (a.silu) {
+                y[0] = silu(y[0]);
+                if (V >= 2) y[1] = silu(y[1]);
+            }
+            if constexpr (V >= 2) narrow2<T>(out.v + e, y[0], y[1]);
+            else out.v[e] = narrow<T>(y[0]);
+        }
+        *reinterpret_cast<P *>(dst) = out;
+        dst += a.dst_stride;
+    };
+    if constexpr (RING) {
+        // (of the ring every thread reads only what it has asked for)
+        __shared__ __align__(16) P ring[CONV_GROUPS][CONV_GROUP][CONV_THREADS];
+        auto fetch = [&](int g) {
+#pragma unroll
+            for (int u = 0; u < CONV_GROUP; u++) {
+                if (g * CONV_GROUP + u < nt) {
+                    if constexpr (sizeof(P) == 16) cp_async16(&ring[g % CONV_GROUPS][u][threadIdx.x], in_row);
+                    else cp_async8(&ring[g % CONV_GROUPS][u][threadIdx.x], in_row);
+                }
+                in_row += a.x_stride;
+            }
+            cp_async_commit();
+        };
+#pragma unroll
+        for (int g = 0; g < CONV_GROUPS - 1; g++) fetch(g);
+        for (int g = 0; g * CONV_GROUP < nt; g++) {
+            cp_async_wait<CONV_GROUPS - 2>();
+#pragma unroll
+            for (int u = 0; u < CONV_GROUP; u++) {
+                if (g * CONV_GROUP + u < nt) turn(ring[g % CONV_GROUPS][u][threadIdx.x]);
+            }
+            fetch(g + CONV_GROUPS - 1);
+        }
+        cp_async_wait<0>();
+    } else {
+        for (int b = 0; b < nt; b += CONV_GROUP) {
+            P in[CONV_GROUP];
+#pragma unroll
+            for (int u = 0; u < CONV_GROUP; u++) {
+                if (b + u < nt) in[u] = *reinterpret_cast<const P *>(in_row);
+                in_row += a.x_stride;
+            }
+#pragma unroll
+            for (int u = 0; u < CONV_GROUP; u++) {
+                if (b + u < nt) turn(in[u]);
+            }
         }
     }
     if (t0 == 0) {
-        // entry j of the new tail is the input of row count - taps + 1 + j: all of them are in the window, or behind the rows of this CTA
+        // entry j of the new tail is the input of row count - taps + 1 + j: all of them are in the window, or among x's rows
 #pragma unroll
         for (int j = 1; j < K; j++) {
             if (!EXACT && j <= skip) continue;
             const int i = q.count - K + j;
             float *to = tail + (int64_t)(j - 1 - skip) * a.channels;
-            if (q.count <= CONV_ROWS) {
+            if (q.count <= a.rows) {
 #pragma unroll
                 for (int e = 0; e < V; e++) to[e] = win[j][e];
             } else {
@@ -128,13 +205,18 @@ __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_kernel(const ConvArgs a
         }
     }
 }
-static_assert(CONV_ROWS >= 15, "a sequence of more rows than a CTA takes has all the new tail's inputs among its rows");
+static_assert(CONV_ROWS_MIN >= 15, "a sequence of more rows than a CTA takes has all the new tail's inputs among its rows");
 
 template <typename T, int K, int V, bool EXACT>
-static int launch_conv(const ConvArgs &a, cudaStream_t st) {
-    const int each = CONV_THREADS * V;
-    const dim3 grid((unsigned)((a.channels + each - 1) / each), (unsigned)((a.step.max_new + CONV_ROWS - 1) / CONV_ROWS), (unsigned)a.step.n_seq);
-    B200_CUDA_TRY(launch_chained(ssm_conv_kernel<T, K, V, EXACT>, grid, CONV_THREADS, 0, st, a));
+static int launch_conv(ConvArgs a, cudaStream_t st) {
+    // rows of a CTA: as many as leave every SM eight of them (each one reads its weights and the taps - 1 rows in front)
+    const unsigned across = (unsigned)((a.channels + CONV_THREADS * V - 1) / (CONV_THREADS * V));
+    a.rows = CONV_ROWS_MAX;
+    while (a.rows > CONV_ROWS_MIN && (int64_t)across * ((a.step.n_tokens + a.rows - 1) / a.rows) < 8 * (int64_t)sm_count()) a.rows /= 2;
+    const dim3 grid(across, (unsigned)((a.step.max_new + a.rows - 1) / a.rows), (unsigned)a.step.n_seq);
+    // the ring pays where there is something to wait for: 64 sequences of one row, f32: 4.5 us with it, 3.8 without; 5330 rows, bf16: 40 and 46 us
+    const bool ring = V * sizeof(T) >= 8 && a.step.max_new > 2 * CONV_GROUP;
+    B200_CUDA_TRY(launch_chained(ring ? ssm_conv_kernel<T, K, V, EXACT, (V * sizeof(T) >= 8)> : ssm_conv_kernel<T, K, V, EXACT, false>, grid, CONV_THREADS, 0, st, a));
     return B200_OK;
 }
 template <typename T, int V>
@@ -144,7 +226,7 @@ static int launch_conv_taps(const ConvArgs &a, cudaStream_t st) {
         case 2: return launch_conv<T, 2, V, true>(a, st);
         case 3: return launch_conv<T, 3, V, true>(a, st);
         case 4: return launch_conv<T, 4, V, true>(a, st);
-        default: return a.taps <= 8 ? launch_conv<T, 8, V < 4 ? V : 4, false>(a, st) : launch_conv<T, 16, V < 2 ? V : 2, false>(a, st);
+        default: return a.taps <= 8 ? launch_conv<T, 8, V, false>(a, st) : launch_conv<T, 16, V, false>(a, st);
     }
 }
 
@@ -157,16 +239,28 @@ struct ScanArgs {
     const float *from; int64_t from_stride;
     float *state; int64_t slot_stride;
     void *dst; int64_t dst_stride;
-    int32_t channels, d_state, per_group, softplus;
+    int32_t channels, d_state, per_group, softplus, bc_pieces;  // bc_pieces: b and c can be read four numbers at a time
     // stretches: rows of one, how many a sequence may have; where their end states and sums of d wait
     int32_t stretch, n_stretch;
     float *ends, *sums;
 };
 
-constexpr float LOG2E = 1.4426950408889634f;
-__device__ __forceinline__ float ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
-// ln(1 + e^x) without overflow for large x and without cancellation for very negative x
-__device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.f) + log1pf(__expf(-fabsf(x))); }
+// ln(1 + e^x) = max(x, 0) + ln(1 + e^-|x|), and ln(1 + e) = e P(e) on [0, 1] with a polynomial whose relative error is smallest at its largest (fitted by weighted least squares on
+// Chebyshev points; 1.8e-7 with the roundings of f32): one exponential on the special function unit and nothing else there, no overflow, no cancellation.
+__device__ __forceinline__ float2 softplus2(float2 x) {
+    const Two e = two(ex2(-LOG2E * fabsf(x.x)), ex2(-LOG2E * fabsf(x.y)));
+    auto both = [](float v) { return two(v, v); };
+    Two p = both(0.0052326764f);
+    p = fma2(p, e, both(-0.0295051672f));
+    p = fma2(p, e, both(0.0782258362f));
+    p = fma2(p, e, both(-0.136632353f));
+    p = fma2(p, e, both(0.191060022f));
+    p = fma2(p, e, both(-0.248429805f));
+    p = fma2(p, e, both(0.333190978f));
+    p = fma2(p, e, both(-0.499994934f));
+    return each(fma2(fma2(p, e, both(1.0f)), e, two(fmaxf(x.x, 0.f), fmaxf(x.y, 0.f))));
+}
+__device__ __forceinline__ float softplus(float x) { return softplus2(make_float2(x, x)).x; }
 
 // Four neighbouring states of a channel; numbers behind d_state count as zeros
 template <bool VEC>
@@ -269,6 +363,9 @@ __global__ void __launch_bounds__(32 * STEP_WARPS) ssm_step_kernel(const ScanArg
 }
 
 // ===== several rows a sequence
+// A CTA takes CB channels.  L lanes share CI of them, a lane four states of each: the loads of b and c serve CI channels, and a warp's chains are 4 CI exponentials and multiply-adds a lane
+// wide.  Rows come in chunks of TC.  While the warps walk chunk k, chunk k + 1 is made ready (d and d x), the results of chunk k - 1 go out and chunk k + 2 travels: one barrier a chunk.  Every thread
+// stages, and later sends off, the same pieces of a chunk, so what lies in memory's form between its arrival and the end is nobody else's.
 constexpr int SCAN_WARPS = 4, SCAN_THREADS = 32 * SCAN_WARPS;
 // the three things that a CTA can be there for: a whole sequence; the state at the end of a stretch as if it began from nothing (the first one: from the sequence's state), and the sum of
 // its d; a stretch's rows, from the states and sums of those before it
@@ -279,16 +376,17 @@ struct ScanSizes {
     static constexpr int TC = CB >= 64 ? 16 : 1024 / CB;          // rows of a chunk
     static constexpr int PIECES = TC * CB / 4 / SCAN_THREADS;     // pieces of four channels of one row that a thread stages
     static constexpr int RAW = TC * CB * (int)sizeof(T), RAW_BC = TC * NP * (int)sizeof(T);
-    static constexpr int BUF = 3 * RAW + 2 * RAW_BC;              // x, dt, z, b, c as they lie in memory
-    static constexpr int SMEM = 2 * BUF + 4 * (2 * TC * CB + 2 * TC * NP);
-    static_assert(PIECES >= 1 && TC % 4 == 0, "every thread stages the same number of pieces");
+    static constexpr int BUF = 3 * RAW + 2 * RAW_BC;              // x, dt, z, b, c as they lie in memory: three chunks
+    static constexpr int READY = 4 * (2 * TC * CB + 2 * TC * NP); // d (later y), d x, b, c in f32: two chunks
+    static constexpr int SMEM = 3 * BUF + 2 * READY;
+    static_assert(PIECES >= 1 && TC % 4 == 0 && SCAN_THREADS % (CB / 4) == 0 && 2 * TC * L % SCAN_THREADS == 0, "every thread stages the same number of pieces, of one place in the rows");
 };
 template <typename T, int L, int CI, bool VEC, int PASS>
 __global__ void __launch_bounds__(SCAN_THREADS) ssm_scan_kernel(const ScanArgs a) {
     using Z = ScanSizes<T, L, CI>;
-    constexpr int G = Z::G, CB = Z::CB, NP = Z::NP, TC = Z::TC, C4 = CB / 4;
+    constexpr int G = Z::G, CB = Z::CB, NP = Z::NP, TC = Z::TC, C4 = CB / 4, TB = CI == 2 ? 16 : 8;
     extern __shared__ __align__(16) unsigned char ssm_shared[];
-    pdl_enter();
+    pdl_wait();  // (the kernel behind is let in at the end: CTAs of it that wait would take places in an order that leaves SMs unequal, 520 -> 610 us for four long prompts)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, p = lane % L, g = lane / L;
     const Seq q = seq_of(a.step, blockIdx.z);
     const int N = a.d_state, blocks = (a.per_group + CB - 1) / CB, group = blockIdx.x / blocks, in_group = (blockIdx.x - group * blocks) * CB;
@@ -296,45 +394,152 @@ __global__ void __launch_bounds__(SCAN_THREADS) ssm_scan_kernel(const ScanArgs a
     const int stretch = PASS == WHOLE ? 0 : blockIdx.y, begin = PASS == WHOLE ? 0 : stretch * a.stretch, end = PASS == WHOLE ? q.count : min(q.count, begin + a.stretch);
     if (begin >= end) return;
     if (PASS == ENDS && end == q.count && stretch > 0) return;  // nobody asks for the last one's
-    unsigned char *raw = ssm_shared;
-    float *sd = (float *)(ssm_shared + 2 * Z::BUF), *sx = sd + TC * CB, *sb = sx + TC * CB, *sc = sb + TC * NP;
     const int64_t first = q.first + begin;
     const T *px = (const T *)a.x + first * a.x_stride + c0, *pdt = (const T *)a.dt + first * a.dt_stride + c0, *pz = a.z ? (const T *)a.z + first * a.z_stride + c0 : nullptr;
     const T *pb = (const T *)a.b + first * a.b_stride + (int64_t)group * N, *pc = (const T *)a.c + first * a.c_stride + (int64_t)group * N;
     T *pd = (T *)a.dst + first * a.dst_stride + c0;
     const int rows = end - begin, chunks = (rows + TC - 1) / TC;
-    auto copy4 = [&](T *to, const T *row, int c) {  // (four channels; those behind the CTA's last are nobody's)
+    // chunk k as it lies in memory, and made ready
+    auto raw = [&](int k) { return (T *)(ssm_shared + k % 3 * Z::BUF); };                  // x, dt, z [TC][CB], b, c [TC][NP]
+    auto ready = [&](int k) { return (float *)(ssm_shared + 3 * Z::BUF + (k & 1) * Z::READY); };  // d, d x [TC][CB], b, c [TC][NP]
+    // the thread's pieces: four channels from ch on of the rows t1, t1 + TR, ..; four of the numbers of b or c
+    constexpr int TR = SCAN_THREADS / C4, BC = 2 * TC * L / SCAN_THREADS;
+    const int ch = tid % C4 * 4, t1 = tid / C4;
+    const bool mine = ch < nc;
+    float bias[4], skip[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        bias[e] = a.dt_bias && ch + e < nc ? a.dt_bias[c0 + ch + e] : 0.f;
+        skip[e] = PASS != ENDS && a.d && ch + e < nc ? a.d[c0 + ch + e] : 0.f;
+    }
+    px += t1 * a.x_stride + ch;
+    pdt += t1 * a.dt_stride + ch;
+    pd += t1 * a.dst_stride + ch;
+    if (pz) pz += t1 * a.z_stride + ch;
+    auto copy4 = [&](T *to, const T *row) {  // (four channels; those behind the CTA's last are nobody's)
         if constexpr (VEC) {
-            if constexpr (sizeof(T) == 4) cp_async16(to, row + c);
-            else cp_async8(to, row + c);
+            if constexpr (sizeof(T) == 4) cp_async16(to, row);
+            else cp_async8(to, row);
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++) to[e] = c + e < nc ? row[c + e] : narrow<T>(0.f);
+            for (int e = 0; e < 4; e++) to[e] = ch + e < nc ? row[e] : narrow<T>(0.f);
         }
     };
-    auto fetch = [&](int chunk) {
-        T *x = (T *)(raw + (chunk & 1) * Z::BUF), *dt = x + TC * CB, *z = dt + TC * CB, *b = z + TC * CB, *c = b + TC * NP;
-        const int r0 = chunk * TC, nt = min(TC, rows - r0);
+    auto fetch = [&](int k) {  // called for 0, 1, 2, ..
+        if (k < chunks) {
+            T *x = raw(k) + t1 * CB + ch;
+            const int nt = min(TC, rows - k * TC);
+            if (mine) {
 #pragma unroll
-        for (int k = 0; k < Z::PIECES; k++) {
-            const int i = tid + k * SCAN_THREADS, t = i / C4, ch = i % C4 * 4;
-            if (t < nt && ch < nc) {
-                copy4(x + t * CB + ch, px + (r0 + t) * a.x_stride, ch);
-                copy4(dt + t * CB + ch, pdt + (r0 + t) * a.dt_stride, ch);
-                if (PASS != ENDS && pz) copy4(z + t * CB + ch, pz + (r0 + t) * a.z_stride, ch);
+                for (int j = 0; j < Z::PIECES; j++) {
+                    if (t1 + j * TR < nt) {
+                        copy4(x + j * TR * CB, px + j * TR * a.x_stride);
+                        copy4(x + (TC + j * TR) * CB, pdt + j * TR * a.dt_stride);
+                        if (PASS != ENDS && pz) copy4(x + (2 * TC + j * TR) * CB, pz + j * TR * a.z_stride);
+                    }
+                }
             }
-        }
-        for (int i = tid; i < nt * N; i += SCAN_THREADS) {
-            const int t = i / N, n = i - t * N;
-            b[t * NP + n] = pb[(r0 + t) * a.b_stride + n];
-            if (PASS != ENDS) c[t * NP + n] = pc[(r0 + t) * a.c_stride + n];
+            px += TC * a.x_stride;
+            pdt += TC * a.dt_stride;
+            if (pz) pz += TC * a.z_stride;
+            T *b = raw(k) + 3 * TC * CB;
+#pragma unroll
+            for (int j = 0; j < BC; j++) {
+                const int i = tid + j * SCAN_THREADS, r = i / L, n = i % L * 4, t = r % TC;
+                if (t < nt && n < N && (PASS != ENDS || r < TC)) {
+                    const T *row = (r < TC ? pb + (k * TC + t) * a.b_stride : pc + (k * TC + t) * a.c_stride) + n;
+                    if (a.bc_pieces) {
+                        if constexpr (sizeof(T) == 4) cp_async16(b + 4 * i, row);
+                        else cp_async8(b + 4 * i, row);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) b[4 * i + e] = n + e < N ? row[e] : narrow<T>(0.f);
+                    }
+                }
+            }
         }
         cp_async_commit();
     };
+    // d and d x, b and c.  Rows behind the last and channels behind the CTA's leave states as they are
+    auto stage = [&](int k) {
+        if (k >= chunks) return;
+        const T *x = raw(k) + t1 * CB + ch, *b = raw(k) + 3 * TC * CB;
+        float *sd = ready(k) + t1 * CB + ch, *sb = ready(k) + 2 * TC * CB;
+        const int nt = min(TC, rows - k * TC);
+#pragma unroll
+        for (int j = 0; j < Z::PIECES; j++) {
+            float4 d = make_float4(0.f, 0.f, 0.f, 0.f), dx = d;
+            if (mine && t1 + j * TR < nt) {
+                const Pack<T, 4> x4 = *reinterpret_cast<const Pack<T, 4> *>(x + j * TR * CB), dt4 = *reinterpret_cast<const Pack<T, 4> *>(x + (TC + j * TR) * CB);
+                float2 lo = make_float2(wide(dt4.v[0]) + bias[0], wide(dt4.v[1]) + bias[1]), hi = make_float2(wide(dt4.v[2]) + bias[2], wide(dt4.v[3]) + bias[3]);
+                if (a.softplus) {
+                    lo = softplus2(lo);
+                    hi = softplus2(hi);
+                }
+                d = make_float4(lo.x, lo.y, hi.x, hi.y);
+                if (!VEC) {
+                    if (ch + 1 >= nc) d.y = 0.f;
+                    if (ch + 2 >= nc) d.z = 0.f;
+                    if (ch + 3 >= nc) d.w = 0.f;
+                }
+                dx = make_float4(d.x * wide(x4.v[0]), d.y * wide(x4.v[1]), d.z * wide(x4.v[2]), d.w * wide(x4.v[3]));
+            }
+            *reinterpret_cast<float4 *>(sd + j * TR * CB) = d;
+            *reinterpret_cast<float4 *>(sd + (TC + j * TR) * CB) = dx;
+        }
+#pragma unroll
+        for (int j = 0; j < BC; j++) {
+            const int i = tid + j * SCAN_THREADS, r = i / L, n = i % L * 4, t = r % TC;
+            if (PASS == ENDS && r >= TC) break;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (t < nt && n < N) {
+                const Pack<T, 4> b4 = *reinterpret_cast<const Pack<T, 4> *>(b + 4 * i);
+                v = make_float4(wide(b4.v[0]), wide(b4.v[1]), wide(b4.v[2]), wide(b4.v[3]));
+            }
+            *reinterpret_cast<float4 *>(sb + 4 * i) = v;
+        }
+    };
+    // the rows of chunk k that have been walked: skip, gate, out
+    auto send = [&](int k) {  // called for 0, 1, 2, ..
+        const T *x = raw(k) + t1 * CB + ch;
+        const float *sd = ready(k) + t1 * CB + ch;
+        const int nt = min(TC, rows - k * TC);
+        if (mine) {
+#pragma unroll
+            for (int j = 0; j < Z::PIECES; j++) {
+                if (t1 + j * TR >= nt) break;
+                const float4 y4 = *reinterpret_cast<const float4 *>(sd + j * TR * CB);
+                float y[4] = {y4.x, y4.y, y4.z, y4.w};
+                if (a.d) {
+                    const Pack<T, 4> x4 = *reinterpret_cast<const Pack<T, 4> *>(x + j * TR * CB);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) if (VEC || ch + e < nc) y[e] = fmaf(skip[e], wide(x4.v[e]), y[e]);
+                }
+                if (pz) {
+                    const Pack<T, 4> z4 = *reinterpret_cast<const Pack<T, 4> *>(x + (2 * TC + j * TR) * CB);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) y[e] *= silu(wide(z4.v[e]));
+                }
+                T *to = pd + j * TR * a.dst_stride;
+                if constexpr (VEC) {
+                    Pack<T, 4> out;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) out.v[e] = narrow<T>(y[e]);
+                    *reinterpret_cast<Pack<T, 4> *>(to) = out;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) if (ch + e < nc) to[e] = narrow<T>(y[e]);
+                }
+            }
+        }
+        pd += TC * a.dst_stride;
+    };
     fetch(0);
+    fetch(1);
     // ===== the states
     const int cl = warp * Z::WC + g * CI;  // the lane's channels, counted from c0
-    float h[CI][4], rate[CI][4], total[CI];
+    Two h[CI][2], rate[CI][2];
+    float total[CI];
     const bool pieces = (N & 3) == 0 && ((a.slot_stride | a.from_stride) & 3) == 0 && (((uintptr_t)a.state | (uintptr_t)a.from | (uintptr_t)a.a) & 15) == 0;
     const int64_t ends_row = (int64_t)a.channels * N;  // floats of a stretch's end states; the stretch in front of a sequence's first is its state
     float *ends = a.ends + ((int64_t)blockIdx.z * (a.n_stretch + 1) + 1) * ends_row, *sums = a.sums + (int64_t)blockIdx.z * a.n_stretch * a.channels;
@@ -364,130 +569,89 @@ __global__ void __launch_bounds__(SCAN_THREADS) ssm_scan_kernel(const ScanArgs a
                 }
             }
         }
-        rate[ci][0] = r.x; rate[ci][1] = r.y; rate[ci][2] = r.z; rate[ci][3] = r.w;
-        h[ci][0] = s.x; h[ci][1] = s.y; h[ci][2] = s.z; h[ci][3] = s.w;
+        rate[ci][0] = two(r.x, r.y); rate[ci][1] = two(r.z, r.w);
+        h[ci][0] = two(s.x, s.y); h[ci][1] = two(s.z, s.w);
     }
-    for (int i = tid; i < TC * NP; i += SCAN_THREADS) {  // (numbers behind d_state stay zeros)
-        sb[i] = 0.f;
-        sc[i] = 0.f;
-    }
-    for (int chunk = 0; chunk < chunks; chunk++) {
-        const int r0 = chunk * TC, nt = min(TC, rows - r0);
-        const T *x = (const T *)(raw + (chunk & 1) * Z::BUF), *dt = x + TC * CB, *z = dt + TC * CB, *b = z + TC * CB, *c = b + TC * NP;
-        cp_async_wait<0>();
-        __syncthreads();
-        if (chunk + 1 < chunks) fetch(chunk + 1);
-        // ===== d and d x.  Rows behind the last and channels behind the CTA's leave states as they are
-#pragma unroll
-        for (int k = 0; k < Z::PIECES; k++) {
-            const int i = tid + k * SCAN_THREADS, t = i / C4, ch = i % C4 * 4;
-            float4 d4 = make_float4(0.f, 0.f, 0.f, 0.f), x4 = d4;
-            if (t < nt && ch < nc) {
-                const Pack<T, 4> pdt4 = *reinterpret_cast<const Pack<T, 4> *>(dt + t * CB + ch), px4 = *reinterpret_cast<const Pack<T, 4> *>(x + t * CB + ch);
-                float dv[4], xv[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const bool there = VEC || ch + e < nc;
-                    float d = there ? wide(pdt4.v[e]) + (a.dt_bias ? a.dt_bias[c0 + ch + e] : 0.f) : 0.f;
-                    if (a.softplus && there) d = softplus(d);
-                    dv[e] = d;
-                    xv[e] = there ? d * wide(px4.v[e]) : 0.f;
-                }
-                d4 = make_float4(dv[0], dv[1], dv[2], dv[3]);
-                x4 = make_float4(xv[0], xv[1], xv[2], xv[3]);
-            }
-            *reinterpret_cast<float4 *>(sd + t * CB + ch) = d4;
-            *reinterpret_cast<float4 *>(sx + t * CB + ch) = x4;
-        }
-        for (int i = tid; i < nt * N; i += SCAN_THREADS) {
-            const int t = i / N, n = i - t * N;
-            sb[t * NP + n] = wide(b[t * NP + n]);
-            if (PASS != ENDS) sc[t * NP + n] = wide(c[t * NP + n]);
-        }
-        __syncthreads();
-        // ===== the rows, four at a time
+    // ===== chunk k's rows, all of them (those behind the last change nothing), in blocks of up to 16 whose loads can go ahead of the chains: results are written behind the block
+    auto walk = [&](int k) {
+        float *sd = ready(k);
+        const float *sx = sd + TC * CB, *sb = sx + TC * CB, *sc = sb + TC * NP;
 #pragma unroll 1
-        for (int t0 = 0; t0 < nt; t0 += 4) {
-            float y[4][CI];
+        for (int tb = 0; tb < TC; tb += TB) {
+            float v[TB / 4][CI];
+            const bool hi = (p & (L / 2)) != 0, odd = (p & (L / 4)) != 0;
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int t = t0 + u;
-                const float4 b4 = *reinterpret_cast<const float4 *>(sb + t * NP + 4 * p);
-                const float4 c4 = PASS == ENDS ? b4 : *reinterpret_cast<const float4 *>(sc + t * NP + 4 * p);
-                const Pack<float, CI> d = *reinterpret_cast<const Pack<float, CI> *>(sd + t * CB + cl), dx = *reinterpret_cast<const Pack<float, CI> *>(sx + t * CB + cl);
-                const float bv[4] = {b4.x, b4.y, b4.z, b4.w}, cv[4] = {c4.x, c4.y, c4.z, c4.w};
+            for (int t0 = 0; t0 < TB; t0 += 4) {
+                float y[4][CI];
 #pragma unroll
-                for (int ci = 0; ci < CI; ci++) {
-                    if (PASS == ENDS) total[ci] += d.v[ci];
+                for (int u = 0; u < 4; u++) {
+                    const int t = tb + t0 + u;
+                    const ulonglong2 b2 = *reinterpret_cast<const ulonglong2 *>(sb + t * NP + 4 * p);
+                    const ulonglong2 c2 = PASS == ENDS ? b2 : *reinterpret_cast<const ulonglong2 *>(sc + t * NP + 4 * p);
+                    const Pack<float, CI> d = *reinterpret_cast<const Pack<float, CI> *>(sd + t * CB + cl), dx = *reinterpret_cast<const Pack<float, CI> *>(sx + t * CB + cl);
 #pragma unroll
-                    for (int n = 0; n < 4; n++) {
-                        h[ci][n] = fmaf(ex2(d.v[ci] * rate[ci][n]), h[ci][n], dx.v[ci] * bv[n]);
-                        if (PASS != ENDS) y[u][ci] = n == 0 ? cv[0] * h[ci][0] : fmaf(cv[n], h[ci][n], y[u][ci]);
+                    for (int ci = 0; ci < CI; ci++) {
+                        if (PASS == ENDS) total[ci] += d.v[ci];
+                        const Two dd = two(d.v[ci], d.v[ci]), xx = two(dx.v[ci], dx.v[ci]);
+                        const float2 e0 = each(mul2(dd, rate[ci][0])), e1 = each(mul2(dd, rate[ci][1]));
+                        h[ci][0] = fma2(two(ex2(e0.x), ex2(e0.y)), h[ci][0], mul2(xx, b2.x));
+                        h[ci][1] = fma2(two(ex2(e1.x), ex2(e1.y)), h[ci][1], mul2(xx, b2.y));
+                        if (PASS != ENDS) {
+                            const float2 s = each(fma2(c2.y, h[ci][1], mul2(c2.x, h[ci][0])));
+                            y[u][ci] = s.x + s.y;
+                        }
+                    }
+                }
+                if (PASS != ENDS) {
+                    // sums over the channel's lanes: those of one half keep rows 2 and 3, then a quarter one row each
+#pragma unroll
+                    for (int ci = 0; ci < CI; ci++) {
+                        const float s0 = hi ? y[0][ci] : y[2][ci], s1 = hi ? y[1][ci] : y[3][ci], k0 = hi ? y[2][ci] : y[0][ci], k1 = hi ? y[3][ci] : y[1][ci];
+                        const float w0 = k0 + __shfl_xor_sync(0xffffffffu, s0, L / 2), w1 = k1 + __shfl_xor_sync(0xffffffffu, s1, L / 2);
+                        const float s = odd ? w0 : w1, kk = odd ? w1 : w0;
+                        v[t0 / 4][ci] = kk + __shfl_xor_sync(0xffffffffu, s, L / 4);
+                    }
+#pragma unroll
+                    for (int n = L / 8; n >= 1; n /= 2) {
+#pragma unroll
+                        for (int ci = 0; ci < CI; ci++) v[t0 / 4][ci] += __shfl_xor_sync(0xffffffffu, v[t0 / 4][ci], n);
                     }
                 }
             }
             if (PASS != ENDS) {
-                // sums over the channel's lanes: those of one half keep rows 2 and 3, then a quarter one row each
-                const bool hi = (p & (L / 2)) != 0, odd = (p & (L / 4)) != 0;
-                float v[CI];
-#pragma unroll
-                for (int ci = 0; ci < CI; ci++) {
-                    const float s0 = hi ? y[0][ci] : y[2][ci], s1 = hi ? y[1][ci] : y[3][ci], k0 = hi ? y[2][ci] : y[0][ci], k1 = hi ? y[3][ci] : y[1][ci];
-                    const float w0 = k0 + __shfl_xor_sync(0xffffffffu, s0, L / 2), w1 = k1 + __shfl_xor_sync(0xffffffffu, s1, L / 2);
-                    const float s = odd ? w0 : w1, k = odd ? w1 : w0;
-                    v[ci] = k + __shfl_xor_sync(0xffffffffu, s, L / 4);
-                }
-#pragma unroll
-                for (int n = L / 8; n >= 1; n /= 2) {
-#pragma unroll
-                    for (int ci = 0; ci < CI; ci++) v[ci] += __shfl_xor_sync(0xffffffffu, v[ci], n);
-                }
                 __syncwarp();  // the warp has read these rows of its channels in sd: their results take the place
                 if ((p & (L / 4 - 1)) == 0) {
-                    Pack<float, CI> out;
 #pragma unroll
-                    for (int ci = 0; ci < CI; ci++) out.v[ci] = v[ci];
-                    *reinterpret_cast<Pack<float, CI> *>(sd + (t0 + 2 * hi + odd) * CB + cl) = out;
+                    for (int i = 0; i < TB / 4; i++) {
+                        Pack<float, CI> out;
+#pragma unroll
+                        for (int ci = 0; ci < CI; ci++) out.v[ci] = v[i][ci];
+                        *reinterpret_cast<Pack<float, CI> *>(sd + (tb + 4 * i + 2 * hi + odd) * CB + cl) = out;
+                    }
                 }
             }
         }
-        if (PASS == ENDS) continue;
+    };
+    cp_async_wait<1>();
+    stage(0);
+    __syncthreads();
+    for (int k = 0; k < chunks; k++) {
+        if (PASS != ENDS && k > 0) send(k - 1);
+        fetch(k + 2);
+        cp_async_wait<1>();
+        stage(k + 1);
+        walk(k);
         __syncthreads();
-#pragma unroll
-        for (int k = 0; k < Z::PIECES; k++) {
-            const int i = tid + k * SCAN_THREADS, t = i / C4, ch = i % C4 * 4;
-            if (t < nt && ch < nc) {
-                const float4 y4 = *reinterpret_cast<const float4 *>(sd + t * CB + ch);
-                float y[4] = {y4.x, y4.y, y4.z, y4.w};
-                if (a.d) {
-                    const Pack<T, 4> px4 = *reinterpret_cast<const Pack<T, 4> *>(x + t * CB + ch);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) if (VEC || ch + e < nc) y[e] = fmaf(a.d[c0 + ch + e], wide(px4.v[e]), y[e]);
-                }
-                if (a.z) {
-                    const Pack<T, 4> pz4 = *reinterpret_cast<const Pack<T, 4> *>(z + t * CB + ch);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) y[e] *= silu(wide(pz4.v[e]));
-                }
-                T *to = pd + (r0 + t) * a.dst_stride + ch;
-                if constexpr (VEC) {
-                    Pack<T, 4> out;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) out.v[e] = narrow<T>(y[e]);
-                    *reinterpret_cast<Pack<T, 4> *>(to) = out;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) if (ch + e < nc) to[e] = narrow<T>(y[e]);
-                }
-            }
-        }
     }
+    pdl_trigger();
+    if (PASS != ENDS) send(chunks - 1);
     // ===== where the states go: the stretch's place, or the slot
 #pragma unroll
     for (int ci = 0; ci < CI; ci++) {
         if (cl + ci >= nc) continue;
         const int c = c0 + cl + ci;
-        const float4 s = make_float4(h[ci][0], h[ci][1], h[ci][2], h[ci][3]);
+        const float2 s0 = each(h[ci][0]), s1 = each(h[ci][1]);
+        const float4 s = make_float4(s0.x, s0.y, s1.x, s1.y);
         if (PASS == ENDS) {
             store_states<false>(ends + stretch * ends_row + (int64_t)c * N, 4 * p, N, s);
             if (p == 0) sums[(int64_t)stretch * a.channels + c] = total[ci];
@@ -519,7 +683,7 @@ static ScanPlan plan_of(const b200_ssm_scan_args *a) {
     const int longest = a->seq_info ? max_new_of(a) : (a->n_seq > 0 ? a->n_tokens / a->n_seq : 0);
     p.lanes = a->d_state <= 16 ? 4 : a->d_state <= 32 ? 8 : a->d_state <= 64 ? 16 : 32;
     p.step = longest <= 1;
-    p.per_lane = 4;
+    p.per_lane = p.lanes == 4 ? 2 : p.lanes == 32 ? 4 : 4;
     p.n_stretch = 1;
     const int block = SCAN_WARPS * 32 / p.lanes * p.per_lane, per_group = a->channels / a->groups;
     const int64_t ctas = (int64_t)((per_group + block - 1) / block) * a->groups * a->n_seq;
@@ -543,8 +707,9 @@ static size_t scan_room(const b200_ssm_scan_args *a, const ScanPlan &p) {
 
 template <typename T, int L, bool VEC, int PASS>
 static int launch_scan(const ScanArgs &a, cudaStream_t st) {
-    using Z = ScanSizes<T, L, 4>;
-    const auto kern = ssm_scan_kernel<T, L, 4, VEC, PASS>;
+    constexpr int CI = L == 4 ? 2 : 4;
+    using Z = ScanSizes<T, L, CI>;
+    const auto kern = ssm_scan_kernel<T, L, CI, VEC, PASS>;
     if (Z::SMEM > 48 * 1024) {
         static bool attr_set_dev[16] = {};  // cudaFuncSetAttribute is per device
         int dev = 0;
@@ -631,14 +796,14 @@ int b200_op_ssm_conv(const b200_ssm_conv_args *a, b200_stream_t stream) {
     OPX_REQUIRE(on(type_size(a->type), {a->x, a->dst}) && on(4, {a->w, a->bias, a->tail}), B200_ERR_INVALID, "%s: a pointer is not aligned to its type", who);
     OPX_REQUIRE(a->x != a->dst, B200_ERR_INVALID, "%s: not in place", who);
     const int each = a->seq_info ? a->n_tokens : a->n_tokens / a->n_seq, longest = a->max_new > 0 && a->max_new < each ? a->max_new : each;
-    OPX_REQUIRE((longest + CONV_ROWS - 1) / CONV_ROWS <= 65535, B200_ERR_UNSUPPORTED, "%s: at most %d rows of a sequence", who, 65535 * CONV_ROWS);
-    const ConvArgs c = {{a->seq_info, a->n_seq, a->n_slots, a->n_tokens, longest}, a->x, a->x_stride, a->w, a->bias, a->tail, a->slot_stride, a->dst, a->dst_stride, a->channels, a->taps, a->silu};
+    OPX_REQUIRE((longest + CONV_ROWS_MIN - 1) / CONV_ROWS_MIN <= 65535, B200_ERR_UNSUPPORTED, "%s: at most %d rows of a sequence", who, 65535 * CONV_ROWS_MIN);
+    const ConvArgs c = {{a->seq_info, a->n_seq, a->n_slots, a->n_tokens, longest}, a->x, a->x_stride, a->w, a->bias, a->tail, a->slot_stride, a->dst, a->dst_stride, a->channels, a->taps, a->silu, 0};
     const cudaStream_t st = (cudaStream_t)stream;
-    const int v = a->type == B200_TYPE_F32 ? 4 : 8;
-    const bool vec = on(16, {a->x, a->dst}) && ((a->x_stride | a->dst_stride | a->channels) & (v - 1)) == 0;
-    if (a->type == B200_TYPE_F32) return vec ? launch_conv_taps<float, 4>(c, st) : launch_conv_taps<float, 1>(c, st);
-    if (a->type == B200_TYPE_F16) return vec ? launch_conv_taps<__half, 8>(c, st) : launch_conv_taps<__half, 1>(c, st);
-    return vec ? launch_conv_taps<__nv_bfloat16, 8>(c, st) : launch_conv_taps<__nv_bfloat16, 1>(c, st);
+    constexpr int CV = 4;
+    const bool vec = on(CV * type_size(a->type), {a->x, a->dst}) && ((a->x_stride | a->dst_stride | a->channels) & (CV - 1)) == 0;
+    if (a->type == B200_TYPE_F32) return vec ? launch_conv_taps<float, CV>(c, st) : launch_conv_taps<float, 1>(c, st);
+    if (a->type == B200_TYPE_F16) return vec ? launch_conv_taps<__half, CV>(c, st) : launch_conv_taps<__half, 1>(c, st);
+    return vec ? launch_conv_taps<__nv_bfloat16, CV>(c, st) : launch_conv_taps<__nv_bfloat16, 1>(c, st);
 }
 
 size_t b200_ssm_scan_workspace_bytes(const b200_ssm_scan_args *a) {
@@ -655,10 +820,11 @@ int b200_op_ssm_scan(const b200_ssm_scan_args *a, void *workspace, size_t worksp
     OPX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0), B200_ERR_INVALID, "%s: workspace of %zu bytes, 16-byte aligned", who, need);
     const int per_group = a->channels / a->groups, each = a->seq_info ? a->n_tokens : a->n_tokens / a->n_seq, longest = a->max_new > 0 && a->max_new < each ? a->max_new : each;
     float *ends = (float *)workspace;
-    const ScanArgs s = {{a->seq_info, a->n_seq, a->n_slots, a->n_tokens, longest}, a->x, a->dt, a->b, a->c, a->z, a->x_stride, a->dt_stride, a->b_stride, a->c_stride, a->z_stride, a->a, a->dt_bias, a->d,
-                        a->from ? a->from : a->state, a->from ? a->from_stride : a->slot_stride, a->state, a->slot_stride, a->dst, a->dst_stride, a->channels, a->d_state, per_group, a->softplus,
-                        p.stretch, p.n_stretch, ends, ends ? ends + (size_t)a->n_seq * (p.n_stretch + 1) * a->channels * a->d_state : nullptr};
     const size_t four = 4 * type_size(a->type);
+    const bool bc_pieces = on(four, {a->b, a->c}) && ((a->b_stride | a->c_stride | a->d_state) & 3) == 0;
+    const ScanArgs s = {{a->seq_info, a->n_seq, a->n_slots, a->n_tokens, longest}, a->x, a->dt, a->b, a->c, a->z, a->x_stride, a->dt_stride, a->b_stride, a->c_stride, a->z_stride, a->a, a->dt_bias, a->d,
+                        a->from ? a->from : a->state, a->from ? a->from_stride : a->slot_stride, a->state, a->slot_stride, a->dst, a->dst_stride, a->channels, a->d_state, per_group, a->softplus, bc_pieces,
+                        p.stretch, p.n_stretch, ends, ends ? ends + (size_t)a->n_seq * (p.n_stretch + 1) * a->channels * a->d_state : nullptr};
     const bool vec = per_group % 4 == 0 && on(four, {a->x, a->dt, a->z, a->dst}) && ((a->x_stride | a->dt_stride | a->dst_stride | (a->z ? a->z_stride : 0)) & 3) == 0;
     const bool states16 = (a->d_state & 3) == 0 && ((s.slot_stride | s.from_stride) & 3) == 0 && on(16, {s.state, s.from, a->a});
     const cudaStream_t st = (cudaStream_t)stream;
