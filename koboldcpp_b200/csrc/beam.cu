@@ -12,7 +12,8 @@ namespace beam {
 // Two launches.  The first reads the logits once: of every piece of PIECE tokens of a row (or a power of two of them) it keeps the largest, of every share of a row the sum of exponentials.
 // The second, a CTA a request, knows the logarithms of the sums then, and so every piece's best score.  The n_keep best successors all lie in the n_keep pieces whose best come first
 // (a successor elsewhere comes behind the best of each of these), so it reads those pieces again and nothing else.
-constexpr int PIECE = 512, ROW_WARPS = 8, PICK_THREADS = 512, PICK_WARPS = PICK_THREADS / 32;
+// What bounds it: the first launch memory (six instructions a token beside the loads), the second the way from one result to the next.
+constexpr int PIECE = 512, ROW_WARPS = 8, PICK_THREADS = 256, PICK_WARPS = PICK_THREADS / 32;
 constexpr int MOST_PIECES = 4096;  // of a request: what the second launch looks through
 constexpr int LIST = 512;          // candidates that are ranked by counting; where ties make them more, the best are taken out one after the other
 struct SelectArgs {
@@ -23,107 +24,119 @@ struct SelectArgs {
     int32_t beams, vocab, keep, end_token;
     // layout: tokens of a piece, pieces of a row, pieces of a share, shares of a row
     int32_t piece, n_pieces, share, n_shares;
-    float *tops;      // [rows][n_pieces]: the largest logit, -inf where there is none
-    double *sums;     // [rows][n_shares]: a sum of exponentials ..
-    int32_t *refs;    // .. and what it refers to (see Ref)
+    unsigned by_pieces;  // ceil(2^32 / n_pieces): i / n_pieces is the upper half of its product with i < MOST_PIECES (n_pieces > 1)
+    float *tops;         // [rows][n_pieces]: the largest logit, -inf where there is none
+    double *sums;        // [rows][n_shares]: sum of exp(logit - ref) ..
+    float *refs;         // .. and its ref: the largest logit, rounded up to a whole number
 };
 constexpr float NEG_INF = -INFINITY;
-
-// log2 e in two parts, so that a logit's product with it is off by the last rounding only
-constexpr float LOG2E_HI = 1.4426950408889634f, LOG2E_LO = (float)(1.4426950408889634074 - (double)LOG2E_HI);
-constexpr double LN2 = 0.69314718055994530942;
+constexpr float LOG2E = 1.4426950408889634f;
 __device__ __forceinline__ float ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+using Two = unsigned long long;
+__device__ __forceinline__ Two two(float lo, float hi) { Two r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi)); return r; }
+__device__ __forceinline__ float2 each(Two x) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x)); return r; }
+__device__ __forceinline__ Two add2(Two x, Two y) { Two r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y)); return r; }
+__device__ __forceinline__ Two mul2(Two x, Two y) { Two r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y)); return r; }
 
-// Sums of exponentials refer to their largest logit m.  Where |m| < 2^29 the reference is a whole number e not below m log2 e, and what is summed up are 2^(x log2 e - e): it follows a
-// larger reference by a power of two, exactly.  Logits beyond that (masks of a type's lowest value, +inf) lie 32 apart at least, so there only those count that are m itself: the
-// reference is m, as the number that its bits make.  The references' order is that of the logits: -0x7f800000 (-inf: none so far) .. -0x4e000000, -2^30 .. 2^30, 0x4e000000 .. 0x7f800000 (+inf).
-constexpr int NO_REF = -0x7f800000;
-__device__ __forceinline__ bool ref_is_exponent(int r) { return r >= -0x40000000 && r <= 0x40000000; }
-__device__ __forceinline__ int ref_of(float m) {
-    if (fabsf(m) < 536870912.0f) return (int)ceilf(m * LOG2E_HI);
-    const int bits = (int)(__float_as_uint(m) & 0x7fffffffu);
-    return m < 0.f ? -bits : bits;
-}
-__device__ __forceinline__ float ref_logit(int r) { return r < 0 ? -__uint_as_float((unsigned)-r) : __uint_as_float((unsigned)r); }
-// a sum's share of one that refers to the larger `to`
-__device__ __forceinline__ double follow(double sum, int from, int to) {
-    if (from == to) return sum;
-    return ref_is_exponent(from) && ref_is_exponent(to) && to - from <= 1000 ? scalbn(sum, from - to) : 0.0;
-}
+// A sum of exponentials that refers to `from` as one that refers to the larger `to`.  References are whole numbers where f32 has a choice, so that few larger logits move them, and the
+// largest logits' exponents are small numbers, whose product with log2 e is off by little.
+__device__ __noinline__ double less(double sum, double by) { return sum * exp(-by); }  // (once in the code: it is seldom wanted, and a short kernel waits for every line that it fetches)
+__device__ __forceinline__ double follow(double sum, float from, float to) { return from == to ? sum : from == NEG_INF ? 0.0 : less(sum, (double)to - (double)from); }
+// the largest of a warp's, NaN apart; -inf where all are NaN
+__device__ __forceinline__ float largest(float x) { float r; asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x)); return r != r ? NEG_INF : r; }
 
 // a logit as it counts: NaN is none
 __device__ __forceinline__ float counted(float x) { return x != x ? NEG_INF : x; }
 template <typename T> __device__ __forceinline__ float value_at(const T *p) {
-    if constexpr (sizeof(T) == 4) return counted(*p);
-    else if constexpr (std::is_same<T, __half>::value) return counted(__half2float(*p));
-    else return counted(__bfloat162float(*p));
+    if constexpr (sizeof(T) == 4) return *p;
+    else if constexpr (std::is_same<T, __half>::value) return __half2float(*p);
+    else return __bfloat162float(*p);
 }
 // the two values of a word of 16-bit logits
 template <typename T> __device__ __forceinline__ float2 both(unsigned w) {
-    if constexpr (std::is_same<T, __half>::value) return make_float2(counted(h2f((unsigned short)w)), counted(h2f((unsigned short)(w >> 16))));
-    else return make_float2(counted(__uint_as_float(w << 16)), counted(__uint_as_float(w & 0xffff0000u)));
+    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
 // PIECE tokens of a row from token t0 on, 16 a lane, those behind the vocabulary -inf.  Which token a lane gets does not depend on where the row lies (WIDE is the same for all rows of
 // a call): rows with the same logits have the same sums, bit by bit.
 template <typename T, bool WIDE>
-__device__ __forceinline__ void load_piece(const T *row, int t0, int vocab, int lane, float (&x)[16]) {
-    if constexpr (sizeof(T) == 4) {
-        if (WIDE && t0 + PIECE <= vocab) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float4 v = *reinterpret_cast<const float4 *>(row + t0 + 128 * i + 4 * lane);
-                x[4 * i] = counted(v.x); x[4 * i + 1] = counted(v.y); x[4 * i + 2] = counted(v.z); x[4 * i + 3] = counted(v.w);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const int t = WIDE ? t0 + 128 * (i / 4) + 4 * lane + i % 4 : t0 + 32 * i + lane;
-                x[i] = t < vocab ? value_at(row + t) : NEG_INF;
-            }
-        }
-    } else if (WIDE && t0 + PIECE <= vocab) {
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(row + t0 + 256 * i + 8 * lane);
-            const unsigned w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float2 f = both<T>(w[j]);
-                x[8 * i + 2 * j] = f.x; x[8 * i + 2 * j + 1] = f.y;
-            }
-        }
-    } else if (!WIDE && t0 + PIECE + 2 <= vocab) {
-        // words; where the row begins in the middle of one, a lane's tokens are the upper half of its word and the lower half of the next lane's
-        const bool odd = ((uintptr_t)row & 2) != 0;
-        const unsigned *w = reinterpret_cast<const unsigned *>(row + t0 - odd);
-        unsigned v[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = t0 - odd + 64 * i + 2 * lane >= 0 ? w[32 * i + lane] : (unsigned)*reinterpret_cast<const unsigned short *>(row) << 16;
-        const unsigned last = odd ? w[256] : 0;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            unsigned z = v[i];
-            if (odd) {
-                const unsigned up = __shfl_down_sync(0xffffffffu, z, 1), next = __shfl_sync(0xffffffffu, i < 7 ? v[i < 7 ? i + 1 : 7] : last, 0);
-                z = __funnelshift_r(z, lane == 31 ? next : up, 16);
-            }
-            const float2 f = both<T>(z);
-            x[2 * i] = f.x; x[2 * i + 1] = f.y;
-        }
-    } else {
+__device__ __forceinline__ int token_of(int i, int lane) {  // number i of a lane, counted from t0
+    if constexpr (sizeof(T) == 4) return WIDE ? 128 * (i / 4) + 4 * lane + i % 4 : 32 * i + lane;
+    else return WIDE ? 256 * (i / 8) + 8 * lane + i % 8 : 64 * (i / 2) + 2 * lane + i % 2;
+}
+// .. as they lie in memory: words of one or two logits
+template <typename T>
+struct Raw {
+    static constexpr int N = 4 * (int)sizeof(T);  // 16 or 8
+    unsigned v[N + 1];
+    bool odd;  // 16 bits: the row begins in the middle of a word, so a lane's tokens are the upper half of its word and the lower half of the next lane's
+};
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load_raw(const T *row, int t0, int vocab, int lane, Raw<T> &r) {
+    r.odd = false;
+    if (t0 + PIECE + 2 > vocab) {
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            const int t = WIDE ? t0 + 256 * (i / 8) + 8 * lane + i % 8 : t0 + 64 * (i / 2) + 2 * lane + i % 2;
-            x[i] = t < vocab ? value_at(row + t) : NEG_INF;
+            const int t = t0 + token_of<T, WIDE>(i, lane);
+            if constexpr (sizeof(T) == 4) {
+                r.v[i] = t < vocab ? __float_as_uint(row[t]) : __float_as_uint(NEG_INF);
+            } else {
+                const unsigned none = std::is_same<T, __half>::value ? 0xfc00u : 0xff80u, h = t < vocab ? reinterpret_cast<const unsigned short *>(row)[t] : none;
+                r.v[i / 2] = i & 1 ? r.v[i / 2] | h << 16 : h;
+            }
+        }
+    } else if constexpr (WIDE) {
+#pragma unroll
+        for (int i = 0; i < Raw<T>::N / 4; i++) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(row + t0 + token_of<T, true>(4 * i * (4 / (int)sizeof(T)), lane));
+            r.v[4 * i] = v.x; r.v[4 * i + 1] = v.y; r.v[4 * i + 2] = v.z; r.v[4 * i + 3] = v.w;
+        }
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) r.v[i] = __float_as_uint(row[t0 + 32 * i + lane]);
+    } else {
+        r.odd = ((uintptr_t)row & 2) != 0;
+        const unsigned *w = reinterpret_cast<const unsigned *>(row + t0 - r.odd);
+        r.v[0] = t0 > 0 || !r.odd || lane > 0 ? w[lane] : (unsigned)*reinterpret_cast<const unsigned short *>(row) << 16;  // (nothing in front of the row is read)
+#pragma unroll
+        for (int i = 1; i < 8; i++) r.v[i] = w[32 * i + lane];
+        r.v[8] = r.odd && lane == 0 ? w[256] : 0;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void values_of(Raw<T> &r, int lane, float (&x)[16]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) x[i] = __uint_as_float(r.v[i]);
+    } else {
+        if (r.odd) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) r.v[i] = __funnelshift_r(r.v[i], __shfl_sync(0xffffffffu, lane == 0 ? r.v[i + 1] : r.v[i], lane + 1), 16);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float2 f = both<T>(r.v[i]);
+            x[2 * i] = f.x; x[2 * i + 1] = f.y;
         }
     }
+}
+
+// the sum over a lane's 16 logits of exp(x - ref)
+__device__ __forceinline__ float sum_of(const float (&x)[16], float ref) {
+    Two s = 0;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+        const float2 e = each(mul2(add2(two(x[i], x[i + 1]), two(-ref, -ref)), two(LOG2E, LOG2E)));
+        s = add2(s, two(ex2(e.x), ex2(e.y)));
+    }
+    return each(s).x + each(s).y;
 }
 
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(32 * ROW_WARPS) beam_rows_kernel(const SelectArgs a) {
     __shared__ double s_sum[ROW_WARPS];
-    __shared__ int s_ref[ROW_WARPS];
+    __shared__ float s_ref[ROW_WARPS];
     pdl_enter();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t r = blockIdx.y;
@@ -132,45 +145,62 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) beam_rows_kernel(const SelectA
     // beams that nobody asks for the successors of
     if ((a.ended && a.ended[r]) || !(a.score[r] > NEG_INF)) return;
     double sum = 0.0;
-    int ref = NO_REF;
-    for (int p = p0 + warp; p < p1; p += ROW_WARPS) {
+    float ref = NEG_INF;
+    // (the next PIECE tokens travel while these are added up)
+    Raw<T> next;
+    int p = p0 + warp, t0 = p * a.piece;
+    if (p < p1) load_raw<T, WIDE>(row, t0, a.vocab, lane, next);
+    while (p < p1) {
         float top = NEG_INF;
-        for (int t0 = p * a.piece; t0 < min(a.vocab, (p + 1) * a.piece); t0 += PIECE) {
+        for (const int end = min(a.vocab, (p + 1) * a.piece); t0 < end;) {
+            Raw<T> now_here = next;
+            t0 += PIECE;
+            const int ahead = t0 < end ? t0 : (p + ROW_WARPS) * a.piece;
+            if (t0 < end || p + ROW_WARPS < p1) load_raw<T, WIDE>(row, ahead, a.vocab, lane, next);
             float x[16];
-            load_piece<T, WIDE>(row, t0, a.vocab, lane, x);
+            values_of<T>(now_here, lane, x);
             float m = x[0];
 #pragma unroll
-            for (int i = 1; i < 16; i++) m = fmaxf(m, x[i]);
-            m = warp_max(m);
+            for (int i = 1; i < 16; i++) m = fmaxf(m, x[i]);  // (a NaN loses)
+            m = largest(m);
             if (m == NEG_INF) continue;
             top = fmaxf(top, m);
-            const int now = max(ref, ref_of(m));
-            sum = follow(sum, ref, now);
-            ref = now;
+            const float now = fmaxf(ref, ceilf(m));
+            if (now != ref) {
+                sum = follow(sum, ref, now);
+                ref = now;
+            }
             float part = 0.f;
-            if (ref_is_exponent(ref)) {
-                const float e = (float)ref;
+            if (ref < INFINITY) {
+                part = sum_of(x, ref);
+                if (__any_sync(0xffffffffu, part != part)) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) part += ex2(fmaf(x[i], LOG2E_LO, fmaf(x[i], LOG2E_HI, -e)));
+                    for (int i = 0; i < 16; i++) x[i] = counted(x[i]);
+                    part = sum_of(x, ref);
+                }
             } else {
-                const float big = ref_logit(ref);
 #pragma unroll
-                for (int i = 0; i < 16; i++) part += x[i] == big ? 1.f : 0.f;
+                for (int i = 0; i < 16; i++) part += x[i] == INFINITY ? 1.f : 0.f;
             }
             sum += part;
         }
         if (lane == 0) a.tops[r * a.n_pieces + p] = top;
+        p += ROW_WARPS;
+        t0 = p * a.piece;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) { s_sum[warp] = sum; s_ref[warp] = ref; }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 0; w < ROW_WARPS; w++) ref = max(ref, s_ref[w]);
-        double all = 0.0;
-        for (int w = 0; w < ROW_WARPS; w++) all += follow(s_sum[w], s_ref[w], ref);
-        a.sums[r * a.n_shares + blockIdx.x] = all;
-        a.refs[r * a.n_shares + blockIdx.x] = ref;
+    if (warp == 0) {
+        ref = warp_max(lane < ROW_WARPS ? s_ref[lane] : NEG_INF);
+        sum = lane < ROW_WARPS ? follow(s_sum[lane], s_ref[lane], ref) : 0.0;
+#pragma unroll
+        for (int o = ROW_WARPS / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) {
+            a.sums[r * a.n_shares + blockIdx.x] = sum;
+            a.refs[r * a.n_shares + blockIdx.x] = ref;
+        }
     }
 }
 
@@ -192,7 +222,9 @@ struct PickShared {
     Cand list[LIST];
     Cand best[B200_BEAM_KEEP];      // first the pieces, then the successors
     Cand warps[PICK_WARPS];
-    int n, overflow;
+    unsigned low[PICK_WARPS], high[PICK_WARPS];
+    int piece[B200_BEAM_KEEP];      // where the successors are looked for
+    int n;
 };
 
 // The score of a logit of beam b.  With a reference of +inf the tokens of +inf share evenly, the others have none.
@@ -204,11 +236,10 @@ __device__ __forceinline__ double score_of(const PickShared &sh, int b, float x)
 
 // The `keep` first of the candidates that each(thread's function) names, in order, to sh.best; returns how many there are.  each(f) calls f(candidate) for all candidates of the calling
 // thread, whatever their order, and always for the same ones; `floor`: candidates with smaller scores can be left aside (at least `keep` have a score of that or more, or it is -inf).
+// (sh.n is 0 and everybody knows.)
 template <typename F>
-__device__ int first_of(PickShared &sh, int keep, double floor, F each) {
+__device__ __forceinline__ int first_of(PickShared &sh, int keep, double floor, F each) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid == 0) sh.n = 0;
-    __syncthreads();
     each([&](const Cand &c) {
         if (c.score == -(double)INFINITY || c.score < floor) return;
         const int i = atomicAdd(&sh.n, 1);
@@ -221,103 +252,129 @@ __device__ int first_of(PickShared &sh, int keep, double floor, F each) {
         for (int i = tid; i < n; i += PICK_THREADS) {
             const Cand c = sh.list[i];
             int rank = 0;
+#pragma unroll 8
             for (int j = 0; j < n; j++) rank += before(sh.list[j], c);
             if (rank < keep) sh.best[rank] = c;
         }
-        __syncthreads();
-        return min(n, keep);
-    }
-    // one after the other: the first of those behind the last one found
-    Cand last = {INFINITY, -1};
-    for (int k = 0; k < keep; k++) {
-        Cand mine = {-(double)INFINITY, 0x7fffffffffffffffLL};
-        each([&](const Cand &c) { if (c.score >= floor && before(last, c) && before(c, mine)) mine = c; });
+    } else {
+        // one after the other: the first of those behind the last one found
+        Cand last = {INFINITY, -1};
+        for (int k = 0; k < keep; k++) {
+            Cand mine = {-(double)INFINITY, 0x7fffffffffffffffLL};
+            each([&](const Cand &c) { if (c.score >= floor && before(last, c) && before(c, mine)) mine = c; });
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const Cand other = shuffled(mine, o);
-            if (before(other, mine)) mine = other;
+            for (int o = 16; o > 0; o >>= 1) {
+                const Cand other = shuffled(mine, o);
+                if (before(other, mine)) mine = other;
+            }
+            if (lane == 0) sh.warps[warp] = mine;
+            __syncthreads();
+            mine = sh.warps[0];
+            for (int w = 1; w < PICK_WARPS; w++) if (before(sh.warps[w], mine)) mine = sh.warps[w];
+            if (tid == 0) sh.best[k] = mine;
+            last = mine;
+            __syncthreads();
         }
-        if (lane == 0) sh.warps[warp] = mine;
-        __syncthreads();
-        mine = sh.warps[0];
-        for (int w = 1; w < PICK_WARPS; w++) if (before(sh.warps[w], mine)) mine = sh.warps[w];
-        if (tid == 0) sh.best[k] = mine;
-        last = mine;
-        __syncthreads();
     }
-    return keep;
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+    return min(n, keep);
 }
 
-template <typename T>
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(PICK_THREADS) beam_pick_kernel(const SelectArgs a) {
     __shared__ PickShared sh;
+    __shared__ float tops[MOST_PIECES];
     pdl_enter();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t r0 = (int64_t)blockIdx.x * a.beams;
+    const int total = a.beams * a.n_pieces;
+    for (int i = tid; i < total; i += PICK_THREADS) cp_async4(&tops[i], a.tops + r0 * a.n_pieces + i);
+    cp_async_commit();
     // ===== the logarithms of the sums, a warp a beam
+    if (tid == 0) sh.n = 0;
     for (int b = warp; b < a.beams; b += PICK_WARPS) {
         const double *sums = a.sums + (r0 + b) * a.n_shares;
-        const int *refs = a.refs + (r0 + b) * a.n_shares;
-        int ref = NO_REF;
-        for (int i = lane; i < a.n_shares; i += 32) ref = max(ref, refs[i]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ref = max(ref, __shfl_xor_sync(0xffffffffu, ref, o));
+        const float *refs = a.refs + (r0 + b) * a.n_shares;
+        const float s = a.score[r0 + b];
+        const bool ended = a.ended && a.ended[r0 + b];
+        float ref = NEG_INF;
+        for (int i = lane; i < a.n_shares; i += 32) ref = fmaxf(ref, refs[i]);
+        ref = warp_max(ref);
         double all = 0.0;
         for (int i = lane; i < a.n_shares; i += 32) all += follow(sums[i], refs[i], ref);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
         if (lane == 0) {
-            const float s = a.score[r0 + b];
-            sh.base[b] = s != s || (ref == NO_REF && !(a.ended && a.ended[r0 + b])) ? -(double)INFINITY : (double)s;
-            sh.ref[b] = ref_is_exponent(ref) ? 0.0 : (double)ref_logit(ref);
-            sh.norm[b] = ref_is_exponent(ref) ? (double)ref * LN2 + log(all) : log(all);
-            sh.ended[b] = a.ended ? a.ended[r0 + b] != 0 : 0;
+            sh.base[b] = s != s || (!ended && ref == NEG_INF) ? -(double)INFINITY : (double)s;  // (of a beam whose row was not read ref and sum are anything, and its score -inf)
+            sh.ref[b] = (double)ref;
+            sh.norm[b] = log(all);
+            sh.ended[b] = ended;
         }
     }
+    cp_async_wait<0>();
     __syncthreads();
     // ===== the pieces: candidates are their best scores, at beam * n_pieces + piece.  An ended beam is one piece of one successor
-    const float *tops = a.tops + r0 * a.n_pieces;
-    const int total = a.beams * a.n_pieces;
+    auto beam_of = [&](int i) { return a.n_pieces == 1 ? i : (int)__umulhi((unsigned)i, a.by_pieces); };
     auto pieces = [&](auto &&f) {
+#pragma unroll 4
         for (int i = tid; i < total; i += PICK_THREADS) {
-            const int b = i / a.n_pieces;
-            if (sh.ended[b]) {
-                if (i == b * a.n_pieces) f(Cand{sh.base[b], i});
-            } else {
-                f(Cand{score_of(sh, b, tops[i]), i});
-            }
+            const int b = beam_of(i);
+            const double s = sh.ended[b] ? (i == b * a.n_pieces ? sh.base[b] : -(double)INFINITY) : score_of(sh, b, tops[i]);
+            f(Cand{s, i});
         }
     };
-    // a score that `keep` threads' best reach at least, from above by halving: what lies below can be left aside
-    float top = NEG_INF;
-    pieces([&](const Cand &c) { top = fmaxf(top, __double2float_rd(c.score)); });
-    const unsigned key = top == NEG_INF ? 0 : ordered(top);
-    unsigned low = 0;
-    if (total > LIST) {
-        for (int bit = 31; bit >= 12; bit--) {
-            const unsigned at = low | 1u << bit;
-            if (__syncthreads_count(key >= at) >= a.keep) low = at;
+    // a score that `keep` threads' best reach at least, by halving between the smallest and the largest of these: what lies below can be left aside
+    double floor = -(double)INFINITY;
+    if (total > 64) {
+        float top = NEG_INF;
+        pieces([&](const Cand &c) { top = fmaxf(top, __double2float_rd(c.score)); });
+        const unsigned key = top == NEG_INF ? 0 : ordered(top);
+        const unsigned lo = __reduce_min_sync(0xffffffffu, key ? key : 0xffffffffu), hi = __reduce_max_sync(0xffffffffu, key);
+        if (lane == 0) { sh.low[warp] = lo; sh.high[warp] = hi; }
+        const int n_there = __syncthreads_count(key != 0);
+        if (n_there >= a.keep) {
+            unsigned low = sh.low[0], high = sh.high[0];
+            for (int w = 1; w < PICK_WARPS; w++) {
+                low = min(low, sh.low[w]);
+                high = max(high, sh.high[w]);
+            }
+            for (int k = 0; k < 12 && low < high; k++) {
+                const unsigned at = low + (high - low + 1) / 2;
+                if (__syncthreads_count(key >= at) >= a.keep) low = at;
+                else high = at - 1;
+            }
+            floor = (double)unordered(low);
         }
     }
-    const int n_best = first_of(sh, a.keep, low == 0 ? -(double)INFINITY : (double)unordered(low), pieces);
+    const int n_best = first_of(sh, a.keep, floor, pieces);
     // ===== the successors in those pieces, a warp a piece
-    int at_piece[B200_BEAM_KEEP / PICK_WARPS];
-#pragma unroll
-    for (int k = 0; k < B200_BEAM_KEEP / PICK_WARPS; k++) at_piece[k] = warp + k * PICK_WARPS < n_best ? (int)sh.best[warp + k * PICK_WARPS].at : -1;
-    const double floor = n_best == a.keep ? sh.best[a.keep - 1].score : -(double)INFINITY;
+    for (int k = tid; k < n_best; k += PICK_THREADS) sh.piece[k] = (int)sh.best[k].at;
+    floor = n_best == a.keep ? sh.best[a.keep - 1].score : -(double)INFINITY;
     __syncthreads();
     auto successors = [&](auto &&f) {
-#pragma unroll
-        for (int k = 0; k < B200_BEAM_KEEP / PICK_WARPS; k++) {
-            if (at_piece[k] < 0) break;
-            const int b = at_piece[k] / a.n_pieces, t0 = (at_piece[k] - b * a.n_pieces) * a.piece;
+#pragma unroll 1
+        for (int k = warp; k < n_best; k += PICK_WARPS) {
+            const int piece = sh.piece[k], b = beam_of(piece), t1 = (piece - b * a.n_pieces) * a.piece;
             if (sh.ended[b]) {
                 if (lane == 0) f(Cand{sh.base[b], (int64_t)b * a.vocab + a.end_token});
                 continue;
             }
             const T *row = (const T *)a.logits + (r0 + b) * a.logits_stride;
-#pragma unroll 4
-            for (int t = t0 + lane; t < min(a.vocab, t0 + a.piece); t += 32) f(Cand{score_of(sh, b, value_at(row + t)), (int64_t)b * a.vocab + t});
+            // (a logit below this has a score below the floor: 2^-20 of what its terms may be is more than their roundings)
+            const double at = (floor - sh.base[b]) + sh.norm[b] + sh.ref[b];
+            const float least = __double2float_rd(at - 0x1p-20 * (fabs(floor) + fabs(sh.base[b]) + fabs(sh.norm[b]) + fabs(sh.ref[b])));
+#pragma unroll 1
+            for (int t0 = t1; t0 < min(a.vocab, t1 + a.piece); t0 += PIECE) {
+                Raw<T> raw;
+                float x[16];
+                load_raw<T, WIDE>(row, t0, a.vocab, lane, raw);
+                values_of<T>(raw, lane, x);
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    if (!(x[i] < least) && x[i] > NEG_INF) f(Cand{score_of(sh, b, x[i]), (int64_t)b * a.vocab + t0 + token_of<T, WIDE>(i, lane)});
+                }
+            }
         }
     };
     const int n = first_of(sh, a.keep, floor, successors);
@@ -340,7 +397,7 @@ static SelectPlan select_plan(const b200_beam_select_args *a) {
     p.n_pieces = (a->n_vocab + p.piece - 1) / p.piece;
     // a piece a warp until every SM has its CTAs, then up to four: fewer and longer ones
     const int64_t rows = (int64_t)a->n_requests * a->n_beams, ctas = rows * ((p.n_pieces + ROW_WARPS - 1) / ROW_WARPS);
-    p.share = ROW_WARPS * (ctas >= 32 * (int64_t)sm_count() ? 4 : ctas >= 16 * (int64_t)sm_count() ? 2 : 1);
+    p.share = ROW_WARPS * (ctas >= 64 * (int64_t)sm_count() ? 8 : ctas >= 32 * (int64_t)sm_count() ? 4 : ctas >= 16 * (int64_t)sm_count() ? 2 : 1);
     p.n_shares = (p.n_pieces + p.share - 1) / p.share;
     return p;
 }
@@ -364,7 +421,7 @@ template <typename T>
 static int launch_select(const SelectArgs &a, int rows, bool wide, cudaStream_t st) {
     const dim3 grid((unsigned)a.n_shares, (unsigned)rows);
     B200_CUDA_TRY(launch_chained(wide ? beam_rows_kernel<T, true> : beam_rows_kernel<T, false>, grid, 32 * ROW_WARPS, 0, st, a));
-    B200_CUDA_TRY(launch_chained(beam_pick_kernel<T>, (unsigned)(rows / a.beams), PICK_THREADS, 0, st, a));
+    B200_CUDA_TRY(launch_chained(wide ? beam_pick_kernel<T, true> : beam_pick_kernel<T, false>, (unsigned)(rows / a.beams), PICK_THREADS, 0, st, a));
     return B200_OK;
 }
 
@@ -470,9 +527,9 @@ int b200_op_beam_select(const b200_beam_select_args *a, void *workspace, size_t 
     const size_t need = select_room(a, p), rows = (size_t)a->n_requests * a->n_beams;
     OPX_REQUIRE(workspace && workspace_bytes >= need && (uintptr_t)workspace % 8 == 0, B200_ERR_INVALID, "%s: workspace of %zu bytes, 8-byte aligned", who, need);
     double *sums = (double *)workspace;
-    int32_t *refs = (int32_t *)(sums + rows * p.n_shares);
+    float *refs = (float *)(sums + rows * p.n_shares);
     const SelectArgs s = {a->logits, a->logits_stride, a->score, a->ended, a->slot, a->to_score, a->to_beam, a->to_token, a->to_slot, a->n_beams, a->n_vocab, a->n_keep, a->end_token,
-                          p.piece, p.n_pieces, p.share, p.n_shares, (float *)(refs + rows * p.n_shares), sums, refs};
+                          p.piece, p.n_pieces, p.share, p.n_shares, (unsigned)(((1ull << 32) + p.n_pieces - 1) / p.n_pieces), refs + rows * p.n_shares, sums, refs};
     const bool wide = (uintptr_t)a->logits % 16 == 0 && a->logits_stride * (int64_t)size % 16 == 0;
     const cudaStream_t st = (cudaStream_t)stream;
     if (a->type == B200_TYPE_F32) return launch_select<float>(s, (int)rows, wide, st);

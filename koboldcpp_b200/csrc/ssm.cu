@@ -363,304 +363,258 @@ __global__ void __launch_bounds__(32 * STEP_WARPS) ssm_step_kernel(const ScanArg
 }
 
 // ===== several rows a sequence
-// A CTA takes CB channels.  L lanes share CI of them, a lane four states of each: the loads of b and c serve CI channels, and a warp's chains are 4 CI exponentials and multiply-adds a lane
-// wide.  Rows come in chunks of TC.  While the warps walk chunk k, chunk k + 1 is made ready (d and d x), the results of chunk k - 1 go out and chunk k + 2 travels: one barrier a chunk.  Every thread
-// stages, and later sends off, the same pieces of a chunk, so what lies in memory's form between its arrival and the end is nobody else's.
-constexpr int SCAN_WARPS = 4, SCAN_THREADS = 32 * SCAN_WARPS;
+// A channel is L lanes, NS of its states each: with 16 states a lane is a channel.  What belongs to a channel alone (dt, x, z, the result) then never leaves the lane's registers, and the 16 exponentials
+// and multiply-adds of a row are chains that run side by side.  b and c of a chunk of rows wait in shared memory, where all lanes read the same words.  Rows go in groups of TG; lane p of a channel makes d and d x of the group's rows p, p + L, ..,
+// and sends off their results; the next group's rows are loaded meanwhile.
+// What bounds it: exponentials, d_state + 3 for each row and channel at 16 a cycle and SM (four prompts of 2048 rows x 8192 channels: 283 us), and that 1024 warps make two on some schedulers and one
+// on others: 474 us; the unit is busy 64 % of the time on average.  Some of the exponentials made by multiply-adds (two or four of 16 as polynomials) gave nothing: the other instructions, 90 a row, fill up what that leaves.
+constexpr int SCAN_WARPS = 4, SCAN_THREADS = 32 * SCAN_WARPS, TG = 8;
 // the three things that a CTA can be there for: a whole sequence; the state at the end of a stretch as if it began from nothing (the first one: from the sequence's state), and the sum of
 // its d; a stretch's rows, from the states and sums of those before it
 enum Pass { WHOLE, ENDS, ROWS };
-template <typename T, int L, int CI>
+template <int L, int NS>
 struct ScanSizes {
-    static constexpr int G = 32 / L, WC = G * CI, CB = SCAN_WARPS * WC, NP = 4 * L;
-    static constexpr int TC = CB >= 64 ? 16 : 1024 / CB;          // rows of a chunk
-    static constexpr int PIECES = TC * CB / 4 / SCAN_THREADS;     // pieces of four channels of one row that a thread stages
-    static constexpr int RAW = TC * CB * (int)sizeof(T), RAW_BC = TC * NP * (int)sizeof(T);
-    static constexpr int BUF = 3 * RAW + 2 * RAW_BC;              // x, dt, z, b, c as they lie in memory: three chunks
-    static constexpr int READY = 4 * (2 * TC * CB + 2 * TC * NP); // d (later y), d x, b, c in f32: two chunks
-    static constexpr int SMEM = 3 * BUF + 2 * READY;
-    static_assert(PIECES >= 1 && TC % 4 == 0 && SCAN_THREADS % (CB / 4) == 0 && 2 * TC * L % SCAN_THREADS == 0, "every thread stages the same number of pieces, of one place in the rows");
+    static constexpr int CB = SCAN_THREADS / L, NP = NS * L;       // channels of a CTA; states of a channel, those behind d_state included
+    static constexpr int TC = NP <= 16 ? 32 : 16;                  // rows of a chunk
+    static constexpr int PIECES = (2 * TC * NP / 4 + SCAN_THREADS - 1) / SCAN_THREADS;  // pieces of four numbers of b or c that a thread fetches
 };
-template <typename T, int L, int CI, bool VEC, int PASS>
-__global__ void __launch_bounds__(SCAN_THREADS) ssm_scan_kernel(const ScanArgs a) {
-    using Z = ScanSizes<T, L, CI>;
-    constexpr int G = Z::G, CB = Z::CB, NP = Z::NP, TC = Z::TC, C4 = CB / 4, TB = CI == 2 ? 16 : 8;
-    extern __shared__ __align__(16) unsigned char ssm_shared[];
+// CTAs that an SM is to hold: with 16 states a lane and nothing to exchange the compiler's own order of loads and exponentials, which wants 168 registers, is worth more than a fourth one (four
+// long prompts 474 us, 629 with 128 registers); with exchanges between lanes it is not (64 states: 300 us, 189)
+constexpr int scan_ctas(int lanes) { return lanes == 1 ? 3 : 4; }
+template <typename T, int L, int NS, int PASS>
+__global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L)) ssm_scan_kernel(const ScanArgs a) {
+    using Z = ScanSizes<L, NS>;
+    constexpr int CB = Z::CB, NP = Z::NP, TC = Z::TC, NQ = NS / 4, MT = TG / L;  // MT: rows of a group that a lane makes ready
+    __shared__ __align__(16) float sbc[2][2][TC][NP];  // [chunk & 1][b, c]
     pdl_wait();  // (the kernel behind is let in at the end: CTAs of it that wait would take places in an order that leaves SMs unequal, 520 -> 610 us for four long prompts)
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, p = lane % L, g = lane / L;
+    const int tid = threadIdx.x, lane = tid & 31, p = lane % L;
     const Seq q = seq_of(a.step, blockIdx.z);
-    const int N = a.d_state, blocks = (a.per_group + CB - 1) / CB, group = blockIdx.x / blocks, in_group = (blockIdx.x - group * blocks) * CB;
-    const int c0 = group * a.per_group + in_group, nc = min(CB, a.per_group - in_group);  // channels of the CTA
+    const int N = a.d_state, blocks = (a.per_group + CB - 1) / CB, group = blockIdx.x / blocks, in_group = (blockIdx.x - group * blocks) * CB + tid / L;
+    const bool mine = in_group < a.per_group;
+    const int c = group * a.per_group + min(in_group, a.per_group - 1);  // the lane's channel (those behind the group's last walk along with it and leave nothing)
     const int stretch = PASS == WHOLE ? 0 : blockIdx.y, begin = PASS == WHOLE ? 0 : stretch * a.stretch, end = PASS == WHOLE ? q.count : min(q.count, begin + a.stretch);
     if (begin >= end) return;
-    if (PASS == ENDS && end == q.count && stretch > 0) return;  // nobody asks for the last one's
+    const bool last = end == q.count;  // (of the ends nobody asks for the last one's)
+    if (PASS == ENDS && last && stretch > 0) return;
     const int64_t first = q.first + begin;
-    const T *px = (const T *)a.x + first * a.x_stride + c0, *pdt = (const T *)a.dt + first * a.dt_stride + c0, *pz = a.z ? (const T *)a.z + first * a.z_stride + c0 : nullptr;
+    const int rows = end - begin;
     const T *pb = (const T *)a.b + first * a.b_stride + (int64_t)group * N, *pc = (const T *)a.c + first * a.c_stride + (int64_t)group * N;
-    T *pd = (T *)a.dst + first * a.dst_stride + c0;
-    const int rows = end - begin, chunks = (rows + TC - 1) / TC;
-    // chunk k as it lies in memory, and made ready
-    auto raw = [&](int k) { return (T *)(ssm_shared + k % 3 * Z::BUF); };                  // x, dt, z [TC][CB], b, c [TC][NP]
-    auto ready = [&](int k) { return (float *)(ssm_shared + 3 * Z::BUF + (k & 1) * Z::READY); };  // d, d x [TC][CB], b, c [TC][NP]
-    // the thread's pieces: four channels from ch on of the rows t1, t1 + TR, ..; four of the numbers of b or c
-    constexpr int TR = SCAN_THREADS / C4, BC = 2 * TC * L / SCAN_THREADS;
-    const int ch = tid % C4 * 4, t1 = tid / C4;
-    const bool mine = ch < nc;
-    float bias[4], skip[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        bias[e] = a.dt_bias && ch + e < nc ? a.dt_bias[c0 + ch + e] : 0.f;
-        skip[e] = PASS != ENDS && a.d && ch + e < nc ? a.d[c0 + ch + e] : 0.f;
-    }
-    px += t1 * a.x_stride + ch;
-    pdt += t1 * a.dt_stride + ch;
-    pd += t1 * a.dst_stride + ch;
-    if (pz) pz += t1 * a.z_stride + ch;
-    auto copy4 = [&](T *to, const T *row) {  // (four channels; those behind the CTA's last are nobody's)
-        if constexpr (VEC) {
-            if constexpr (sizeof(T) == 4) cp_async16(to, row);
-            else cp_async8(to, row);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++) to[e] = ch + e < nc ? row[e] : narrow<T>(0.f);
-        }
-    };
-    auto fetch = [&](int k) {  // called for 0, 1, 2, ..
-        if (k < chunks) {
-            T *x = raw(k) + t1 * CB + ch;
-            const int nt = min(TC, rows - k * TC);
-            if (mine) {
-#pragma unroll
-                for (int j = 0; j < Z::PIECES; j++) {
-                    if (t1 + j * TR < nt) {
-                        copy4(x + j * TR * CB, px + j * TR * a.x_stride);
-                        copy4(x + (TC + j * TR) * CB, pdt + j * TR * a.dt_stride);
-                        if (PASS != ENDS && pz) copy4(x + (2 * TC + j * TR) * CB, pz + j * TR * a.z_stride);
-                    }
-                }
-            }
-            px += TC * a.x_stride;
-            pdt += TC * a.dt_stride;
-            if (pz) pz += TC * a.z_stride;
-            T *b = raw(k) + 3 * TC * CB;
-#pragma unroll
-            for (int j = 0; j < BC; j++) {
-                const int i = tid + j * SCAN_THREADS, r = i / L, n = i % L * 4, t = r % TC;
-                if (t < nt && n < N && (PASS != ENDS || r < TC)) {
-                    const T *row = (r < TC ? pb + (k * TC + t) * a.b_stride : pc + (k * TC + t) * a.c_stride) + n;
-                    if (a.bc_pieces) {
-                        if constexpr (sizeof(T) == 4) cp_async16(b + 4 * i, row);
-                        else cp_async8(b + 4 * i, row);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) b[4 * i + e] = n + e < N ? row[e] : narrow<T>(0.f);
-                    }
-                }
-            }
-        }
-        cp_async_commit();
-    };
-    // d and d x, b and c.  Rows behind the last and channels behind the CTA's leave states as they are
-    auto stage = [&](int k) {
-        if (k >= chunks) return;
-        const T *x = raw(k) + t1 * CB + ch, *b = raw(k) + 3 * TC * CB;
-        float *sd = ready(k) + t1 * CB + ch, *sb = ready(k) + 2 * TC * CB;
-        const int nt = min(TC, rows - k * TC);
+    // ===== b and c of a chunk: to registers, then to shared memory, zeros behind d_state and behind the last row
+    Pack<T, 4> held[Z::PIECES];
+    auto fetch = [&](int r0) {
 #pragma unroll
         for (int j = 0; j < Z::PIECES; j++) {
-            float4 d = make_float4(0.f, 0.f, 0.f, 0.f), dx = d;
-            if (mine && t1 + j * TR < nt) {
-                const Pack<T, 4> x4 = *reinterpret_cast<const Pack<T, 4> *>(x + j * TR * CB), dt4 = *reinterpret_cast<const Pack<T, 4> *>(x + (TC + j * TR) * CB);
-                float2 lo = make_float2(wide(dt4.v[0]) + bias[0], wide(dt4.v[1]) + bias[1]), hi = make_float2(wide(dt4.v[2]) + bias[2], wide(dt4.v[3]) + bias[3]);
-                if (a.softplus) {
-                    lo = softplus2(lo);
-                    hi = softplus2(hi);
-                }
-                d = make_float4(lo.x, lo.y, hi.x, hi.y);
-                if (!VEC) {
-                    if (ch + 1 >= nc) d.y = 0.f;
-                    if (ch + 2 >= nc) d.z = 0.f;
-                    if (ch + 3 >= nc) d.w = 0.f;
-                }
-                dx = make_float4(d.x * wide(x4.v[0]), d.y * wide(x4.v[1]), d.z * wide(x4.v[2]), d.w * wide(x4.v[3]));
-            }
-            *reinterpret_cast<float4 *>(sd + j * TR * CB) = d;
-            *reinterpret_cast<float4 *>(sd + (TC + j * TR) * CB) = dx;
-        }
+            const int i = tid + j * SCAN_THREADS, r = i / (NP / 4), n = i % (NP / 4) * 4, t = r % TC;
+            if (r >= (PASS == ENDS ? TC : 2 * TC) || r0 + t >= rows) continue;
+            const T *row = (r < TC ? pb + (r0 + t) * a.b_stride : pc + (r0 + t) * a.c_stride) + n;
+            if (a.bc_pieces) {
+                if (n < N) held[j] = *reinterpret_cast<const Pack<T, 4> *>(row);
+            } else {
 #pragma unroll
-        for (int j = 0; j < BC; j++) {
-            const int i = tid + j * SCAN_THREADS, r = i / L, n = i % L * 4, t = r % TC;
-            if (PASS == ENDS && r >= TC) break;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (t < nt && n < N) {
-                const Pack<T, 4> b4 = *reinterpret_cast<const Pack<T, 4> *>(b + 4 * i);
-                v = make_float4(wide(b4.v[0]), wide(b4.v[1]), wide(b4.v[2]), wide(b4.v[3]));
+                for (int e = 0; e < 4; e++) held[j].v[e] = n + e < N ? row[e] : narrow<T>(0.f);
             }
-            *reinterpret_cast<float4 *>(sb + 4 * i) = v;
         }
     };
-    // the rows of chunk k that have been walked: skip, gate, out
-    auto send = [&](int k) {  // called for 0, 1, 2, ..
-        const T *x = raw(k) + t1 * CB + ch;
-        const float *sd = ready(k) + t1 * CB + ch;
-        const int nt = min(TC, rows - k * TC);
-        if (mine) {
+    auto keep = [&](int r0, int buf) {
 #pragma unroll
-            for (int j = 0; j < Z::PIECES; j++) {
-                if (t1 + j * TR >= nt) break;
-                const float4 y4 = *reinterpret_cast<const float4 *>(sd + j * TR * CB);
-                float y[4] = {y4.x, y4.y, y4.z, y4.w};
-                if (a.d) {
-                    const Pack<T, 4> x4 = *reinterpret_cast<const Pack<T, 4> *>(x + j * TR * CB);
+        for (int j = 0; j < Z::PIECES; j++) {
+            const int i = tid + j * SCAN_THREADS, r = i / (NP / 4), n = i % (NP / 4) * 4, t = r % TC;
+            if (r >= (PASS == ENDS ? TC : 2 * TC)) continue;
+            const bool there = r0 + t < rows && n < N;
+            *reinterpret_cast<float4 *>(&sbc[buf][0][0][0] + 4 * i) =
+                there ? make_float4(wide(held[j].v[0]), wide(held[j].v[1]), wide(held[j].v[2]), wide(held[j].v[3])) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    };
+    // ===== the channel's rows: lane p has rows p, p + L, .. of a group
+    const T *px = (const T *)a.x + (first + p) * a.x_stride + c, *pdt = (const T *)a.dt + (first + p) * a.dt_stride + c, *pz = a.z ? (const T *)a.z + (first + p) * a.z_stride + c : nullptr;
+    T *pd = (T *)a.dst + (first + p) * a.dst_stride + c;
+    const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, skip = PASS != ENDS && a.d ? a.d[c] : 0.f;
+    T nx[MT], ndt[MT], nz[MT];
+    auto load = [&](int r0) {
+        if (r0 + TG <= rows) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) if (VEC || ch + e < nc) y[e] = fmaf(skip[e], wide(x4.v[e]), y[e]);
-                }
-                if (pz) {
-                    const Pack<T, 4> z4 = *reinterpret_cast<const Pack<T, 4> *>(x + (2 * TC + j * TR) * CB);
+            for (int j = 0; j < MT; j++) {
+                nx[j] = px[j * L * a.x_stride];
+                ndt[j] = pdt[j * L * a.dt_stride];
+                if (PASS != ENDS && pz) nz[j] = pz[j * L * a.z_stride];
+            }
+        } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) y[e] *= silu(wide(z4.v[e]));
-                }
-                T *to = pd + j * TR * a.dst_stride;
-                if constexpr (VEC) {
-                    Pack<T, 4> out;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) out.v[e] = narrow<T>(y[e]);
-                    *reinterpret_cast<Pack<T, 4> *>(to) = out;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) if (ch + e < nc) to[e] = narrow<T>(y[e]);
-                }
+            for (int j = 0; j < MT; j++) {
+                const bool there = r0 + j * L + p < rows;
+                nx[j] = there ? px[j * L * a.x_stride] : narrow<T>(0.f);
+                ndt[j] = there ? pdt[j * L * a.dt_stride] : narrow<T>(0.f);
+                if (PASS != ENDS && pz) nz[j] = there ? pz[j * L * a.z_stride] : narrow<T>(0.f);
             }
         }
-        pd += TC * a.dst_stride;
+        px += TG * a.x_stride;
+        pdt += TG * a.dt_stride;
+        if (pz) pz += TG * a.z_stride;
     };
     fetch(0);
-    fetch(1);
+    load(0);
     // ===== the states
-    const int cl = warp * Z::WC + g * CI;  // the lane's channels, counted from c0
-    Two h[CI][2], rate[CI][2];
-    float total[CI];
+    Two h[NS / 2], rate[NS / 2];
+    float total = 0.f;
     const bool pieces = (N & 3) == 0 && ((a.slot_stride | a.from_stride) & 3) == 0 && (((uintptr_t)a.state | (uintptr_t)a.from | (uintptr_t)a.a) & 15) == 0;
-    const int64_t ends_row = (int64_t)a.channels * N;  // floats of a stretch's end states; the stretch in front of a sequence's first is its state
-    float *ends = a.ends + ((int64_t)blockIdx.z * (a.n_stretch + 1) + 1) * ends_row, *sums = a.sums + (int64_t)blockIdx.z * a.n_stretch * a.channels;
-#pragma unroll
-    for (int ci = 0; ci < CI; ci++) {
-        const int c = c0 + cl + ci;
-        float4 r = make_float4(0.f, 0.f, 0.f, 0.f), s = r;
-        total[ci] = 0.f;
-        if (cl + ci < nc) {
-            const float *pa = a.a + (int64_t)c * N;
-            r = pieces ? load_states<true>(pa, 4 * p, N) : load_states<false>(pa, 4 * p, N);
-            if (PASS != ROWS && stretch == 0 && !q.begins) {
-                const float *from = a.from + (int64_t)q.slot * a.from_stride + (int64_t)c * N;
-                s = pieces ? load_states<true>(from, 4 * p, N) : load_states<false>(from, 4 * p, N);
-            }
-            if (PASS == ENDS && stretch == 0) store_states<false>(ends - ends_row + (int64_t)c * N, 4 * p, N, s);
-            r.x *= LOG2E; r.y *= LOG2E; r.z *= LOG2E; r.w *= LOG2E;
-            if (PASS == ROWS) {
-                s = load_states<false>(ends + (stretch > 0 ? 0 : -ends_row) + (int64_t)c * N, 4 * p, N);
-                for (int j = 1; j < stretch; j++) {
-                    const float4 e = load_states<false>(ends + j * ends_row + (int64_t)c * N, 4 * p, N);
-                    const float d = sums[(int64_t)j * a.channels + c];
-                    s.x = fmaf(ex2(d * r.x), s.x, e.x);
-                    s.y = fmaf(ex2(d * r.y), s.y, e.y);
-                    s.z = fmaf(ex2(d * r.z), s.z, e.z);
-                    s.w = fmaf(ex2(d * r.w), s.w, e.w);
-                }
-            }
-        }
-        rate[ci][0] = two(r.x, r.y); rate[ci][1] = two(r.z, r.w);
-        h[ci][0] = two(s.x, s.y); h[ci][1] = two(s.z, s.w);
-    }
-    // ===== chunk k's rows, all of them (those behind the last change nothing), in blocks of up to 16 whose loads can go ahead of the chains: results are written behind the block
-    auto walk = [&](int k) {
-        float *sd = ready(k);
-        const float *sx = sd + TC * CB, *sb = sx + TC * CB, *sc = sb + TC * NP;
-#pragma unroll 1
-        for (int tb = 0; tb < TC; tb += TB) {
-            float v[TB / 4][CI];
-            const bool hi = (p & (L / 2)) != 0, odd = (p & (L / 4)) != 0;
-#pragma unroll
-            for (int t0 = 0; t0 < TB; t0 += 4) {
-                float y[4][CI];
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const int t = tb + t0 + u;
-                    const ulonglong2 b2 = *reinterpret_cast<const ulonglong2 *>(sb + t * NP + 4 * p);
-                    const ulonglong2 c2 = PASS == ENDS ? b2 : *reinterpret_cast<const ulonglong2 *>(sc + t * NP + 4 * p);
-                    const Pack<float, CI> d = *reinterpret_cast<const Pack<float, CI> *>(sd + t * CB + cl), dx = *reinterpret_cast<const Pack<float, CI> *>(sx + t * CB + cl);
-#pragma unroll
-                    for (int ci = 0; ci < CI; ci++) {
-                        if (PASS == ENDS) total[ci] += d.v[ci];
-                        const Two dd = two(d.v[ci], d.v[ci]), xx = two(dx.v[ci], dx.v[ci]);
-                        const float2 e0 = each(mul2(dd, rate[ci][0])), e1 = each(mul2(dd, rate[ci][1]));
-                        h[ci][0] = fma2(two(ex2(e0.x), ex2(e0.y)), h[ci][0], mul2(xx, b2.x));
-                        h[ci][1] = fma2(two(ex2(e1.x), ex2(e1.y)), h[ci][1], mul2(xx, b2.y));
-                        if (PASS != ENDS) {
-                            const float2 s = each(fma2(c2.y, h[ci][1], mul2(c2.x, h[ci][0])));
-                            y[u][ci] = s.x + s.y;
-                        }
-                    }
-                }
-                if (PASS != ENDS) {
-                    // sums over the channel's lanes: those of one half keep rows 2 and 3, then a quarter one row each
-#pragma unroll
-                    for (int ci = 0; ci < CI; ci++) {
-                        const float s0 = hi ? y[0][ci] : y[2][ci], s1 = hi ? y[1][ci] : y[3][ci], k0 = hi ? y[2][ci] : y[0][ci], k1 = hi ? y[3][ci] : y[1][ci];
-                        const float w0 = k0 + __shfl_xor_sync(0xffffffffu, s0, L / 2), w1 = k1 + __shfl_xor_sync(0xffffffffu, s1, L / 2);
-                        const float s = odd ? w0 : w1, kk = odd ? w1 : w0;
-                        v[t0 / 4][ci] = kk + __shfl_xor_sync(0xffffffffu, s, L / 4);
-                    }
-#pragma unroll
-                    for (int n = L / 8; n >= 1; n /= 2) {
-#pragma unroll
-                        for (int ci = 0; ci < CI; ci++) v[t0 / 4][ci] += __shfl_xor_sync(0xffffffffu, v[t0 / 4][ci], n);
-                    }
-                }
-            }
-            if (PASS != ENDS) {
-                __syncwarp();  // the warp has read these rows of its channels in sd: their results take the place
-                if ((p & (L / 4 - 1)) == 0) {
-#pragma unroll
-                    for (int i = 0; i < TB / 4; i++) {
-                        Pack<float, CI> out;
-#pragma unroll
-                        for (int ci = 0; ci < CI; ci++) out.v[ci] = v[i][ci];
-                        *reinterpret_cast<Pack<float, CI> *>(sd + (tb + 4 * i + 2 * hi + odd) * CB + cl) = out;
-                    }
-                }
-            }
-        }
+    // end states of a stretch lie as [d_state][channels], so that neighbouring lanes read neighbouring words; the stretch in front of a sequence's first is its state
+    const int64_t ends_row = (int64_t)a.channels * N;
+    auto load_end = [&](const float *from, int n) {
+        const float *q4 = from + (int64_t)n * a.channels;
+        return make_float4(n < N ? q4[0] : 0.f, n + 1 < N ? q4[a.channels] : 0.f, n + 2 < N ? q4[2 * (int64_t)a.channels] : 0.f, n + 3 < N ? q4[3 * (int64_t)a.channels] : 0.f);
     };
-    cp_async_wait<1>();
-    stage(0);
+    auto store_end = [&](float *to, int n, float4 v) {
+        float *q4 = to + (int64_t)n * a.channels;
+        if (n < N) q4[0] = v.x;
+        if (n + 1 < N) q4[a.channels] = v.y;
+        if (n + 2 < N) q4[2 * (int64_t)a.channels] = v.z;
+        if (n + 3 < N) q4[3 * (int64_t)a.channels] = v.w;
+    };
+    float *ends = a.ends + ((int64_t)blockIdx.z * (a.n_stretch + 1) + 1) * ends_row + c, *sums = a.sums + (int64_t)blockIdx.z * a.n_stretch * a.channels + c;
+#pragma unroll
+    for (int i = 0; i < NQ; i++) {
+        const int n = 4 * (i * L + p);  // (the channel's lanes side by side: their loads of b and c too)
+        const float *pa = a.a + (int64_t)c * N;
+        float4 r = pieces ? load_states<true>(pa, n, N) : load_states<false>(pa, n, N), s = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (PASS != ROWS && stretch == 0 && !q.begins) {
+            const float *from = a.from + (int64_t)q.slot * a.from_stride + (int64_t)c * N;
+            s = pieces ? load_states<true>(from, n, N) : load_states<false>(from, n, N);
+        }
+        if (PASS == ENDS && stretch == 0 && mine) store_end(ends - ends_row, n, s);
+        r.x *= LOG2E; r.y *= LOG2E; r.z *= LOG2E; r.w *= LOG2E;
+        if (PASS == ROWS) {
+            s = load_end(ends - (stretch > 0 ? 0 : ends_row), n);
+#pragma unroll 4
+            for (int j = 1; j < stretch; j++) {
+                const float4 e = load_end(ends + j * ends_row, n);
+                const float d = sums[(int64_t)j * a.channels];
+                s.x = fmaf(ex2(d * r.x), s.x, e.x);
+                s.y = fmaf(ex2(d * r.y), s.y, e.y);
+                s.z = fmaf(ex2(d * r.z), s.z, e.z);
+                s.w = fmaf(ex2(d * r.w), s.w, e.w);
+            }
+        }
+        rate[2 * i] = two(r.x, r.y); rate[2 * i + 1] = two(r.z, r.w);
+        h[2 * i] = two(s.x, s.y); h[2 * i + 1] = two(s.z, s.w);
+    }
+    if (PASS == ENDS && last) return;  // (a sequence of one stretch: its state is all that is wanted)
+    keep(0, 0);
     __syncthreads();
-    for (int k = 0; k < chunks; k++) {
-        if (PASS != ENDS && k > 0) send(k - 1);
-        fetch(k + 2);
-        cp_async_wait<1>();
-        stage(k + 1);
-        walk(k);
-        __syncthreads();
+    for (int r0 = 0, buf = 0; r0 < rows; r0 += TC, buf ^= 1) {
+        if (r0 + TC < rows) fetch(r0 + TC);
+#pragma unroll 1
+        for (int tg = 0; tg < TC && r0 + tg < rows; tg += TG) {
+            float d[MT], x[MT], dx[MT], z[MT];
+#pragma unroll
+            for (int j = 0; j < MT; j++) {
+                x[j] = wide(nx[j]);
+                if (PASS != ENDS) z[j] = wide(nz[j]);
+                d[j] = wide(ndt[j]) + bias;
+            }
+            if (a.softplus) {
+                if constexpr (MT == 1) {
+                    d[0] = softplus(d[0]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < MT; j += 2) {
+                        const float2 s = softplus2(make_float2(d[j], d[j + 1]));
+                        d[j] = s.x; d[j + 1] = s.y;
+                    }
+                }
+            }
+            const bool full = r0 + tg + TG <= rows;
+            if (!full) {  // rows behind the last leave the states as they are
+#pragma unroll
+                for (int j = 0; j < MT; j++) if (r0 + tg + j * L + p >= rows) d[j] = 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < MT; j++) {
+                dx[j] = d[j] * x[j];
+                if (PASS == ENDS) total += d[j];
+            }
+            load(r0 + tg + TG);
+            float ds[TG], dxs[TG];  // of all the group's rows
+#pragma unroll
+            for (int t = 0; t < TG; t++) {
+                ds[t] = L == 1 ? d[t / L] : __shfl_sync(0xffffffffu, d[t / L], lane - p + t % L);
+                dxs[t] = L == 1 ? dx[t / L] : __shfl_sync(0xffffffffu, dx[t / L], lane - p + t % L);
+            }
+            float y[TG];
+#pragma unroll
+            for (int t = 0; t < TG; t++) {
+                const ulonglong2 *b2 = reinterpret_cast<const ulonglong2 *>(&sbc[buf][0][tg + t][4 * p]), *c2 = reinterpret_cast<const ulonglong2 *>(&sbc[buf][1][tg + t][4 * p]);
+                const Two dd = two(ds[t], ds[t]), xx = two(dxs[t], dxs[t]);
+                Two sum = 0;
+#pragma unroll
+                for (int i = 0; i < NQ; i++) {
+                    const ulonglong2 bv = b2[i * L];
+                    const float2 e0 = each(mul2(dd, rate[2 * i])), e1 = each(mul2(dd, rate[2 * i + 1]));
+                    h[2 * i] = fma2(two(ex2(e0.x), ex2(e0.y)), h[2 * i], mul2(xx, bv.x));
+                    h[2 * i + 1] = fma2(two(ex2(e1.x), ex2(e1.y)), h[2 * i + 1], mul2(xx, bv.y));
+                    if (PASS != ENDS) {
+                        const ulonglong2 cv = c2[i * L];
+                        sum = i == 0 ? mul2(cv.x, h[0]) : fma2(cv.x, h[2 * i], sum);
+                        sum = fma2(cv.y, h[2 * i + 1], sum);
+                    }
+                }
+                const float2 s = each(sum);
+                y[t] = s.x + s.y;
+            }
+            if (PASS == ENDS) continue;
+            // sums over the channel's lanes: lane p ends up with the rows p, p + L, ..
+#pragma unroll
+            for (int n = L / 2; n >= 1; n /= 2) {
+#pragma unroll
+                for (int t = 0; t < TG; t++) {
+                    if ((t & n) || (t & (L - 1)) >= 2 * n) continue;  // (rows that are still there: t < 2 n modulo L)
+                    const float send = p & n ? y[t] : y[t + n], kept = p & n ? y[t + n] : y[t];
+                    y[t] = kept + __shfl_xor_sync(0xffffffffu, send, n);
+                }
+            }
+            // (0 times an x that is not finite would be no number: no skip is no product)
+            if (a.d) {
+#pragma unroll
+                for (int j = 0; j < MT; j++) y[j * L] = fmaf(skip, x[j], y[j * L]);
+            }
+            if (pz) {
+#pragma unroll
+                for (int j = 0; j < MT; j++) y[j * L] *= silu(z[j]);
+            }
+            if (mine && full) {
+#pragma unroll
+                for (int j = 0; j < MT; j++) pd[j * L * a.dst_stride] = narrow<T>(y[j * L]);
+            } else if (mine) {
+#pragma unroll
+                for (int j = 0; j < MT; j++) if (r0 + tg + j * L + p < rows) pd[j * L * a.dst_stride] = narrow<T>(y[j * L]);
+            }
+            pd += TG * a.dst_stride;
+        }
+        if (r0 + TC < rows) {
+            keep(r0 + TC, buf ^ 1);
+            __syncthreads();
+        }
     }
     pdl_trigger();
-    if (PASS != ENDS) send(chunks - 1);
     // ===== where the states go: the stretch's place, or the slot
+    if constexpr (PASS == ENDS && L > 1) {
 #pragma unroll
-    for (int ci = 0; ci < CI; ci++) {
-        if (cl + ci >= nc) continue;
-        const int c = c0 + cl + ci;
-        const float2 s0 = each(h[ci][0]), s1 = each(h[ci][1]);
+        for (int n = L / 2; n >= 1; n /= 2) total += __shfl_xor_sync(0xffffffffu, total, n);
+    }
+    if (!mine) return;
+#pragma unroll
+    for (int i = 0; i < NQ; i++) {
+        const int n = 4 * (i * L + p);
+        const float2 s0 = each(h[2 * i]), s1 = each(h[2 * i + 1]);
         const float4 s = make_float4(s0.x, s0.y, s1.x, s1.y);
         if (PASS == ENDS) {
-            store_states<false>(ends + stretch * ends_row + (int64_t)c * N, 4 * p, N, s);
-            if (p == 0) sums[(int64_t)stretch * a.channels + c] = total[ci];
-        } else if (end == q.count) {
+            store_end(ends + stretch * ends_row, n, s);
+        } else if (last) {
             float *to = a.state + (int64_t)q.slot * a.slot_stride + (int64_t)c * N;
-            if (pieces) store_states<true>(to, 4 * p, N, s);
-            else store_states<false>(to, 4 * p, N, s);
+            if (pieces) store_states<true>(to, n, N, s);
+            else store_states<false>(to, n, N, s);
         }
     }
+    if (PASS == ENDS && p == 0) sums[(int64_t)stretch * a.channels] = total;
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -673,30 +627,26 @@ static inline bool on(size_t size, std::initializer_list<const void *> ps) {
 
 // How a call's work is laid out.
 struct ScanPlan {
-    int lanes, per_lane;          // lanes of a channel, channels of a lane
-    int stretch, n_stretch;       // 0, 1: no stretches
+    int stretch, n_stretch;       // rows of a stretch, stretches of the longest sequence; n_stretch 1: no stretches
     bool step;                    // one row a sequence
 };
-static int max_new_of(const b200_ssm_scan_args *a) { return a->max_new > 0 && a->max_new < a->n_tokens ? a->max_new : a->n_tokens; }
+static int max_new_of(const b200_ssm_scan_args *a) {
+    const int each = a->seq_info || a->n_seq <= 0 ? a->n_tokens : a->n_tokens / a->n_seq;
+    return a->max_new > 0 && a->max_new < each ? a->max_new : each;
+}
+static int lanes_of(int d_state) { return d_state <= 16 ? 1 : d_state <= 32 ? 2 : d_state <= 64 ? 4 : 8; }
 static ScanPlan plan_of(const b200_ssm_scan_args *a) {
-    ScanPlan p = {};
-    const int longest = a->seq_info ? max_new_of(a) : (a->n_seq > 0 ? a->n_tokens / a->n_seq : 0);
-    p.lanes = a->d_state <= 16 ? 4 : a->d_state <= 32 ? 8 : a->d_state <= 64 ? 16 : 32;
+    ScanPlan p = {0, 1, false};
+    const int longest = max_new_of(a), block = SCAN_THREADS / lanes_of(a->d_state), per_group = a->channels / a->groups;
     p.step = longest <= 1;
-    p.per_lane = p.lanes == 4 ? 2 : p.lanes == 32 ? 4 : 4;
-    p.n_stretch = 1;
-    const int block = SCAN_WARPS * 32 / p.lanes * p.per_lane, per_group = a->channels / a->groups;
-    const int64_t ctas = (int64_t)((per_group + block - 1) / block) * a->groups * a->n_seq;
-    const int want = 3 * sm_count();
-    if (!p.step && ctas < want / 2 && longest >= 128) {
-        int n = (int)(want / ctas);
-        if (n > 32) n = 32;
-        if (n > longest / 64) n = longest / 64;
-        if (n > 1) {
-            p.stretch = ((longest + n - 1) / n + 31) / 32 * 32;
-            p.n_stretch = (longest + p.stretch - 1) / p.stretch;
-            if (p.n_stretch < 2) p.n_stretch = 1;
-        }
+    if (p.step) return p;
+    // CTAs that are there on average while the longest sequence lasts
+    const double ctas = (double)((per_group + block - 1) / block) * a->groups * a->n_tokens / longest;
+    if (ctas < 1.25 * sm_count() && longest >= 128) {
+        const double n = (double)scan_ctas(lanes_of(a->d_state)) * sm_count() / ctas;  // as many as are there at once
+        const int rows = (int)(longest / (n < 32 ? n : 32));
+        p.stretch = ((rows < 64 ? 64 : rows) + 7) / 8 * 8;
+        p.n_stretch = (longest + p.stretch - 1) / p.stretch;
     }
     return p;
 }
@@ -705,45 +655,35 @@ static size_t scan_room(const b200_ssm_scan_args *a, const ScanPlan &p) {
     return 4 * (size_t)a->n_seq * ((size_t)(p.n_stretch + 1) * a->channels * a->d_state + (size_t)p.n_stretch * a->channels);
 }
 
-template <typename T, int L, bool VEC, int PASS>
+template <typename T, int L, int NS, int PASS>
 static int launch_scan(const ScanArgs &a, cudaStream_t st) {
-    constexpr int CI = L == 4 ? 2 : 4;
-    using Z = ScanSizes<T, L, CI>;
-    const auto kern = ssm_scan_kernel<T, L, CI, VEC, PASS>;
-    if (Z::SMEM > 48 * 1024) {
-        static bool attr_set_dev[16] = {};  // cudaFuncSetAttribute is per device
-        int dev = 0;
-        B200_CUDA_TRY(cudaGetDevice(&dev));
-        if (dev > 15 || !attr_set_dev[dev]) {
-            B200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::SMEM));
-            if (dev <= 15) attr_set_dev[dev] = true;
-        }
-    }
-    const int groups = a.channels / a.per_group;
-    const dim3 grid((unsigned)((a.per_group + Z::CB - 1) / Z::CB * groups), (unsigned)(PASS == WHOLE ? 1 : a.n_stretch), (unsigned)a.step.n_seq);
-    B200_CUDA_TRY(launch_chained(kern, grid, SCAN_THREADS, Z::SMEM, st, a));
+    constexpr int CB = ScanSizes<L, NS>::CB;
+    const dim3 grid((unsigned)((a.per_group + CB - 1) / CB * (a.channels / a.per_group)), (unsigned)(PASS == WHOLE ? 1 : a.n_stretch), (unsigned)a.step.n_seq);
+    B200_CUDA_TRY(launch_chained(ssm_scan_kernel<T, L, NS, PASS>, grid, SCAN_THREADS, 0, st, a));
     return B200_OK;
 }
+template <typename T, int L, int NS>
+static int launch_scan_rows(const ScanArgs &a, const ScanPlan &p, cudaStream_t st) {
+    if (p.n_stretch < 2) return launch_scan<T, L, NS, WHOLE>(a, st);
+    const int rc = launch_scan<T, L, NS, ENDS>(a, st);
+    return rc != B200_OK ? rc : launch_scan<T, L, NS, ROWS>(a, st);
+}
 template <typename T, int L>
-static int launch_scan_lanes(const ScanArgs &a, const ScanPlan &p, bool vec, bool states16, cudaStream_t st) {
-    if (p.step) {
-        const dim3 grid((unsigned)((a.channels + 32 * STEP_WARPS - 1) / (32 * STEP_WARPS)), (unsigned)a.step.n_seq);
-        B200_CUDA_TRY(launch_chained(states16 ? ssm_step_kernel<T, L, true> : ssm_step_kernel<T, L, false>, grid, 32 * STEP_WARPS, 0, st, a));
-        return B200_OK;
-    }
-    if (p.n_stretch < 2) return vec ? launch_scan<T, L, true, WHOLE>(a, st) : launch_scan<T, L, false, WHOLE>(a, st);
-    const int rc = vec ? launch_scan<T, L, true, ENDS>(a, st) : launch_scan<T, L, false, ENDS>(a, st);
-    if (rc != B200_OK) return rc;
-    return vec ? launch_scan<T, L, true, ROWS>(a, st) : launch_scan<T, L, false, ROWS>(a, st);
+static int launch_step(const ScanArgs &a, bool states16, cudaStream_t st) {
+    const dim3 grid((unsigned)((a.channels + 32 * STEP_WARPS - 1) / (32 * STEP_WARPS)), (unsigned)a.step.n_seq);
+    B200_CUDA_TRY(launch_chained(states16 ? ssm_step_kernel<T, L, true> : ssm_step_kernel<T, L, false>, grid, 32 * STEP_WARPS, 0, st, a));
+    return B200_OK;
 }
 template <typename T>
-static int launch_scan_type(const ScanArgs &a, const ScanPlan &p, bool vec, bool states16, cudaStream_t st) {
-    switch (p.lanes) {
-        case 4: return launch_scan_lanes<T, 4>(a, p, vec, states16, st);
-        case 8: return launch_scan_lanes<T, 8>(a, p, vec, states16, st);
-        case 16: return launch_scan_lanes<T, 16>(a, p, vec, states16, st);
-        default: return launch_scan_lanes<T, 32>(a, p, vec, states16, st);
-    }
+static int launch_scan_type(const ScanArgs &a, const ScanPlan &p, bool states16, cudaStream_t st) {
+    const int n = a.d_state;
+    if (p.step) return n <= 16 ? launch_step<T, 4>(a, states16, st) : n <= 32 ? launch_step<T, 8>(a, states16, st) : n <= 64 ? launch_step<T, 16>(a, states16, st) : launch_step<T, 32>(a, states16, st);
+    if (n <= 4) return launch_scan_rows<T, 1, 4>(a, p, st);
+    if (n <= 8) return launch_scan_rows<T, 1, 8>(a, p, st);
+    if (n <= 16) return launch_scan_rows<T, 1, 16>(a, p, st);
+    if (n <= 32) return launch_scan_rows<T, 2, 16>(a, p, st);
+    if (n <= 64) return launch_scan_rows<T, 4, 16>(a, p, st);
+    return launch_scan_rows<T, 8, 16>(a, p, st);
 }
 
 static int check_step(const int32_t *seq_info, int32_t n_seq, int32_t n_slots, int32_t n_tokens, int32_t max_new, int32_t type, const char *who) {
@@ -825,12 +765,11 @@ int b200_op_ssm_scan(const b200_ssm_scan_args *a, void *workspace, size_t worksp
     const ScanArgs s = {{a->seq_info, a->n_seq, a->n_slots, a->n_tokens, longest}, a->x, a->dt, a->b, a->c, a->z, a->x_stride, a->dt_stride, a->b_stride, a->c_stride, a->z_stride, a->a, a->dt_bias, a->d,
                         a->from ? a->from : a->state, a->from ? a->from_stride : a->slot_stride, a->state, a->slot_stride, a->dst, a->dst_stride, a->channels, a->d_state, per_group, a->softplus, bc_pieces,
                         p.stretch, p.n_stretch, ends, ends ? ends + (size_t)a->n_seq * (p.n_stretch + 1) * a->channels * a->d_state : nullptr};
-    const bool vec = per_group % 4 == 0 && on(four, {a->x, a->dt, a->z, a->dst}) && ((a->x_stride | a->dt_stride | a->dst_stride | (a->z ? a->z_stride : 0)) & 3) == 0;
     const bool states16 = (a->d_state & 3) == 0 && ((s.slot_stride | s.from_stride) & 3) == 0 && on(16, {s.state, s.from, a->a});
     const cudaStream_t st = (cudaStream_t)stream;
-    if (a->type == B200_TYPE_F32) return launch_scan_type<float>(s, p, vec, states16, st);
-    if (a->type == B200_TYPE_F16) return launch_scan_type<__half>(s, p, vec, states16, st);
-    return launch_scan_type<__nv_bfloat16>(s, p, vec, states16, st);
+    if (a->type == B200_TYPE_F32) return launch_scan_type<float>(s, p, states16, st);
+    if (a->type == B200_TYPE_F16) return launch_scan_type<__half>(s, p, states16, st);
+    return launch_scan_type<__nv_bfloat16>(s, p, states16, st);
 }
 
 }  // extern "C"
