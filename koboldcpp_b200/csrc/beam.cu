@@ -434,7 +434,7 @@ struct ReorderArgs {
     char *base[REORDER_STATES];
     int64_t stride[REORDER_STATES], bytes[REORDER_STATES];
     int32_t first[REORDER_STATES + 1];  // number of a state's first column
-    int32_t n_states, n, n_slots, width;  // width: bytes of a column
+    int32_t n_states, n, n_slots, width, width_log2;  // width: bytes of a column
     const int32_t *src, *dst;
     int32_t *refused;
 };
@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(REORDER_THREADS) state_reorder_kernel(const Re
     }
     __syncthreads();
     if (a.refused && blockIdx.x == 0 && tid == 0 && n_refused) *a.refused += n_refused;
-    const int n = n_moves, units = a.width / UNIT;
+    const int n = n_moves, shift = a.width_log2 - (UNIT == 16 ? 4 : 2), units = 1 << shift;
     if (n == 0) return;
     for (int item = blockIdx.x; item < a.first[a.n_states]; item += gridDim.x) {
         int lo = 0, hi = a.n_states - 1;  // the last state whose first column is not behind this one
@@ -477,8 +477,9 @@ __global__ void __launch_bounds__(REORDER_THREADS) state_reorder_kernel(const Re
         const int64_t at = (int64_t)(item - a.first[lo]) * a.width, stride = a.stride[lo];
         char *base = a.base[lo] + at;
         const int here = (int)min((int64_t)a.width, a.bytes[lo] - at) / UNIT;
+#pragma unroll 4
         for (int i = tid; i < n * units; i += REORDER_THREADS) {
-            const int k = i / units, u = i - k * units;
+            const int k = i >> shift, u = i & (units - 1);
             if (u < here) {
                 if constexpr (UNIT == 16) cp_async16(column + (size_t)k * a.width + u * UNIT, base + from[k] * stride + u * UNIT);
                 else cp_async4(column + (size_t)k * a.width + u * UNIT, base + from[k] * stride + u * UNIT);
@@ -487,8 +488,9 @@ __global__ void __launch_bounds__(REORDER_THREADS) state_reorder_kernel(const Re
         cp_async_commit();
         cp_async_wait<0>();
         __syncthreads();
+#pragma unroll 4
         for (int i = tid; i < n * units; i += REORDER_THREADS) {
-            const int k = i / units, u = i - k * units;
+            const int k = i >> shift, u = i & (units - 1);
             if (u < here) {
                 if constexpr (UNIT == 16) *reinterpret_cast<uint4 *>(base + to[k] * stride + u * UNIT) = *reinterpret_cast<const uint4 *>(column + (size_t)k * a.width + u * UNIT);
                 else *reinterpret_cast<unsigned *>(base + to[k] * stride + u * UNIT) = *reinterpret_cast<const unsigned *>(column + (size_t)k * a.width + u * UNIT);
@@ -552,8 +554,9 @@ int b200_op_state_reorder(const b200_slot_state *states, int32_t n_states, const
         wide = wide && (((uintptr_t)s.base | (uint64_t)s.stride | (uint64_t)s.bytes) & 15) == 0;
     }
     // as wide a column as the moves leave room for
-    int width = COLUMNS_BYTES / n / 16 * 16;
-    width = width > 2048 ? 2048 : width < 32 ? 32 : width;
+    int log2 = 5;  // (COLUMNS_BYTES / B200_STATE_MAX_MOVES)
+    while (log2 < 11 && n << (log2 + 1) <= COLUMNS_BYTES) log2++;
+    const int width = 1 << log2;
     const size_t smem = (size_t)n * width + 4 * ((size_t)n_slots + 2 * n);
     const auto kern = wide ? state_reorder_kernel<16> : state_reorder_kernel<4>;
     if (smem > 48 * 1024) B200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, REORDER_MOST));  // (the same for all calls: they may be in several threads)
@@ -571,7 +574,7 @@ int b200_op_state_reorder(const b200_slot_state *states, int32_t n_states, const
         }
         OPX_REQUIRE(r.n_states > 0 || n_states == 0, B200_ERR_UNSUPPORTED, "%s: a state of %lld bytes a slot", who, (long long)states[at].bytes);
         r.first[r.n_states] = (int32_t)columns;
-        r.n = n; r.n_slots = n_slots; r.width = width; r.src = src; r.dst = dst;
+        r.n = n; r.n_slots = n_slots; r.width = width; r.width_log2 = log2; r.src = src; r.dst = dst;
         r.refused = at >= n_states ? refused : nullptr;
         const int64_t most = 6 * (int64_t)sm_count();
         const unsigned grid = (unsigned)(columns < 1 ? 1 : columns < most ? columns : most);

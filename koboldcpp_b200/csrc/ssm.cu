@@ -285,7 +285,12 @@ __device__ __forceinline__ void store_states(float *row, int n0, int d_state, fl
     }
 }
 template <typename T>
-__device__ __forceinline__ float4 load_row4(const T *row, int n0, int d_state) {
+__device__ __forceinline__ float4 load_row4(const T *row, int n0, int d_state, bool pieces) {
+    if (pieces) {
+        if (n0 >= d_state) return make_float4(0.f, 0.f, 0.f, 0.f);
+        const Pack<T, 4> v = *reinterpret_cast<const Pack<T, 4> *>(row + n0);
+        return make_float4(wide(v.v[0]), wide(v.v[1]), wide(v.v[2]), wide(v.v[3]));
+    }
     float4 r;
     r.x = n0 < d_state ? wide(row[n0]) : 0.f;
     r.y = n0 + 1 < d_state ? wide(row[n0 + 1]) : 0.f;
@@ -295,54 +300,72 @@ __device__ __forceinline__ float4 load_row4(const T *row, int n0, int d_state) {
 }
 
 // ===== one row a sequence.  A warp takes 32 channels; L lanes share a channel, a lane four of its states, so that a load of the warp is 512 consecutive bytes of the state.  What a channel
-// needs by itself (d, d x, z) is made by one lane and handed to the other L - 1; the sums of L channels are exchanged so that each lane ends up with one of them.
+// needs by itself (d, d x, z) is made by one lane and handed to the other L - 1; the sums of L channels are exchanged so that each lane ends up with one of them.  What takes longest is asked for
+// first.  What bounds it is instructions as much as memory (96 sequences of 8192 channels, 16 states: 4 TB/s); sequences one after the other in a warp, whose rates would stay, are 45 us instead of 26.
 constexpr int STEP_WARPS = 2;
 template <typename T, int L, bool VEC>
 __global__ void __launch_bounds__(32 * STEP_WARPS) ssm_step_kernel(const ScanArgs a) {
-    constexpr int G = 32 / L, U = L < 4 ? L : 4;  // channels of a round; rounds whose loads travel together
+    constexpr int G = 32 / L, U = 4;  // channels of a round; rounds whose loads travel together
     pdl_enter();
     const int lane = threadIdx.x & 31, p = lane % L, g = lane / L;
-    const int c0 = (blockIdx.x * STEP_WARPS + (threadIdx.x >> 5)) * 32;
+    const int c0 = (blockIdx.x * STEP_WARPS + (threadIdx.x >> 5)) * 32, left = a.channels - c0;  // (left > 31: no channel has to be asked for)
     const Seq q = seq_of(a.step, blockIdx.y);
-    if (c0 >= a.channels || q.count == 0) return;
+    if (left <= 0 || q.count == 0) return;
     const int64_t row = q.first;
+    // the lane's first piece of the states and rates, and how far the next channel's is
+    const int64_t at = (int64_t)(c0 + g) * a.d_state;
+    const int step = G * a.d_state;
+    const float *from = a.from + (int64_t)q.slot * a.from_stride + at, *rates = a.a + at;
+    float *state = a.state + (int64_t)q.slot * a.slot_stride + at;
+    float4 h[U], rate[U];
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            h[u] = rate[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (left > 31 || G * (i0 + u) + g < left) {
+                if (!q.begins) h[u] = load_states<VEC>(from + (i0 + u) * step, 4 * p, a.d_state);
+                rate[u] = load_states<VEC>(rates + (i0 + u) * step, 4 * p, a.d_state);
+            }
+        }
+    };
+    load(0);
+    // b and c of the warp's channels, which are of one group as a rule
+    const bool groups = a.per_group < a.channels;
+    const int group0 = groups ? c0 / a.per_group : 0;
+    const bool one_group = !groups || min(c0 + 31, a.channels - 1) < (group0 + 1) * a.per_group;
+    const T *pb = (const T *)a.b + row * a.b_stride, *pc = (const T *)a.c + row * a.c_stride;
+    float4 b = load_row4(pb + (int64_t)group0 * a.d_state, 4 * p, a.d_state, a.bc_pieces), cc = load_row4(pc + (int64_t)group0 * a.d_state, 4 * p, a.d_state, a.bc_pieces);
     const int mine = c0 + G * p + g;  // the channel that is this lane's by itself
     const bool ok = mine < a.channels;
-    float d = 0.f, x = 0.f;
+    float d = 0.f, x = 0.f, z = 0.f, skip = 0.f;
     if (ok) {
+        if (a.z) z = wide(((const T *)a.z)[row * a.z_stride + mine]);
+        if (a.d) skip = a.d[mine];
         d = wide(((const T *)a.dt)[row * a.dt_stride + mine]) + (a.dt_bias ? a.dt_bias[mine] : 0.f);
         x = wide(((const T *)a.x)[row * a.x_stride + mine]);
         if (a.softplus) d = softplus(d);
     }
     const float dx = d * x;
-    const float *from = a.from + (int64_t)q.slot * a.from_stride;
-    float *state = a.state + (int64_t)q.slot * a.slot_stride;
+    d *= LOG2E;
     float sum[L];
 #pragma unroll
     for (int i0 = 0; i0 < L; i0 += U) {
-        float4 h[U], rate[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int c = c0 + G * (i0 + u) + g;
-            h[u] = rate[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (c < a.channels) {
-                rate[u] = load_states<VEC>(a.a + (int64_t)c * a.d_state, 4 * p, a.d_state);
-                if (!q.begins) h[u] = load_states<VEC>(from + (int64_t)c * a.d_state, 4 * p, a.d_state);
+            if (!one_group) {
+                const int64_t of = (int64_t)(min(c0 + G * (i0 + u) + g, a.channels - 1) / a.per_group) * a.d_state;
+                b = load_row4(pb + of, 4 * p, a.d_state, a.bc_pieces);
+                cc = load_row4(pc + of, 4 * p, a.d_state, a.bc_pieces);
             }
+            const float dc = __shfl_sync(0xffffffffu, d, g * L + i0 + u), dxc = __shfl_sync(0xffffffffu, dx, g * L + i0 + u);
+            const Two dd = two(dc, dc), xx = two(dxc, dxc);
+            const float2 e0 = each(mul2(dd, two(rate[u].x, rate[u].y))), e1 = each(mul2(dd, two(rate[u].z, rate[u].w)));
+            const Two s0 = fma2(two(ex2(e0.x), ex2(e0.y)), two(h[u].x, h[u].y), mul2(xx, two(b.x, b.y))), s1 = fma2(two(ex2(e1.x), ex2(e1.y)), two(h[u].z, h[u].w), mul2(xx, two(b.z, b.w)));
+            const float2 v0 = each(s0), v1 = each(s1), y = each(fma2(two(cc.x, cc.y), s0, mul2(two(cc.z, cc.w), s1)));
+            if (left > 31 || G * (i0 + u) + g < left) store_states<VEC>(state + (i0 + u) * step, 4 * p, a.d_state, make_float4(v0.x, v0.y, v1.x, v1.y));
+            sum[i0 + u] = y.x + y.y;
         }
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int c = c0 + G * (i0 + u) + g, at = min(c, a.channels - 1) / a.per_group * a.d_state;
-            const float4 b = load_row4((const T *)a.b + row * a.b_stride + at, 4 * p, a.d_state), cc = load_row4((const T *)a.c + row * a.c_stride + at, 4 * p, a.d_state);
-            const float dc = LOG2E * __shfl_sync(0xffffffffu, d, g * L + i0 + u), dxc = __shfl_sync(0xffffffffu, dx, g * L + i0 + u);
-            float4 s = h[u];
-            s.x = fmaf(ex2(dc * rate[u].x), s.x, dxc * b.x);
-            s.y = fmaf(ex2(dc * rate[u].y), s.y, dxc * b.y);
-            s.z = fmaf(ex2(dc * rate[u].z), s.z, dxc * b.z);
-            s.w = fmaf(ex2(dc * rate[u].w), s.w, dxc * b.w);
-            if (c < a.channels) store_states<VEC>(state + (int64_t)c * a.d_state, 4 * p, a.d_state, s);
-            sum[i0 + u] = fmaf(cc.x, s.x, fmaf(cc.y, s.y, fmaf(cc.z, s.z, cc.w * s.w)));
-        }
+        if (i0 + U < L) load(i0 + U);
     }
     // sum i of the lanes of a channel ends up in lane i of them
 #pragma unroll
@@ -356,8 +379,8 @@ __global__ void __launch_bounds__(32 * STEP_WARPS) ssm_step_kernel(const ScanArg
     }
     if (ok) {
         float y = sum[0];
-        if (a.d) y = fmaf(a.d[mine], x, y);
-        if (a.z) y *= silu(wide(((const T *)a.z)[row * a.z_stride + mine]));
+        if (a.d) y = fmaf(skip, x, y);
+        if (a.z) y *= silu(z);
         ((T *)a.dst)[row * a.dst_stride + mine] = narrow<T>(y);
     }
 }
