@@ -69,7 +69,7 @@ enum ggml_type {
 
 enum ggml_prec { GGML_PREC_DEFAULT = 0, GGML_PREC_F32 = 1 }; /* include/ggml.h:401-404 */
 
-/* enum ggml_op, include/ggml.h:426-518 -- positional values of the ops in a llama / mixtral graph */
+/* enum ggml_op, include/ggml.h:426-518 -- positional values of the ops in a llama / mixtral / mamba graph */
 enum ggml_op {
     GGML_OP_NONE           = 0,
     GGML_OP_DUP            = 1,
@@ -80,6 +80,7 @@ enum ggml_op {
     GGML_OP_SQR            = 8,
     GGML_OP_SUM_ROWS       = 14,
     GGML_OP_ARGMAX         = 16,
+    GGML_OP_CONCAT         = 20,
     GGML_OP_RMS_NORM       = 23,
     GGML_OP_MUL_MAT        = 26,
     GGML_OP_MUL_MAT_ID     = 27,
@@ -96,6 +97,8 @@ enum ggml_op {
     GGML_OP_CLAMP          = 46,
     GGML_OP_ARGSORT        = 58,
     GGML_OP_FLASH_ATTN_EXT = 60,
+    GGML_OP_SSM_CONV       = 62,
+    GGML_OP_SSM_SCAN       = 63,
     GGML_OP_UNARY          = 69,
     GGML_OP_MAP_CUSTOM1    = 75, /* carries the tensor-parallel collectives (b200_comm.h); llama.cpp never emits it */
     GGML_OP_COUNT          = 81,

@@ -94,6 +94,19 @@ B200_API int b200_op_moe_router(const float *logits, int64_t ld_logits, float *p
                                 float *wsum, float *w_out, int32_t n_expert, int32_t n_used, int64_t n_tok, b200_stream_t stream);
 B200_API int b200_op_argsort(const b200_tensor *x, const b200_tensor *dst, int order, b200_stream_t stream);
 
+/* The three nodes of a state space layer (src/llama.cpp llm_build_mamba), f32; replaces nothing in ggml-cuda, which leaves them to the CPU.
+ * CONCAT: dst is a, then b, along dimension dim (any strides); semantics ggml_compute_forward_concat_f32, ggml.c.
+ * SSM_CONV: sx [taps - 1 + T, channels, n_seq], c [taps, channels], dst [channels, T, n_seq]: dst[c, t, s] = sum_j c[j, c] * sx[t + j, c, s]; sx with nb[0] == 4, c and dst contiguous, taps
+ * <= 16; semantics ggml_compute_forward_ssm_conv_f32, ggml.c.
+ * SSM_SCAN: s [d_state, channels, n_seq], x, dt [channels, T, n_seq], a [d_state, channels], b, c [d_state, T, n_seq]; dst, one run of floats: y [channels, T, n_seq], then the states
+ * behind the last row as s has them.  h = exp(d a) h + d x b with d = ln(1 + e^dt), y = sum c h; all contiguous but b and c, whose rows (nb[0] == 4) follow one another at one stride.  A workspace of
+ * b200_op_ssm_scan_nodes_workspace_bytes (16-byte aligned, 0: none); semantics ggml_compute_forward_ssm_scan_f32, ggml.c.  (For states in slots, and other types: b200_state.h.) */
+B200_API int b200_op_concat(const b200_tensor *a, const b200_tensor *b, const b200_tensor *dst, int dim, b200_stream_t stream);
+B200_API int b200_op_ssm_conv_nodes(const b200_tensor *sx, const b200_tensor *c, const b200_tensor *dst, b200_stream_t stream);
+B200_API size_t b200_op_ssm_scan_nodes_workspace_bytes(const b200_tensor *s, const b200_tensor *x);
+B200_API int b200_op_ssm_scan_nodes(const b200_tensor *s, const b200_tensor *x, const b200_tensor *dt, const b200_tensor *a, const b200_tensor *b, const b200_tensor *c, const b200_tensor *dst,
+                                    void *workspace, size_t workspace_bytes, b200_stream_t stream);
+
 /* SUM_ROWS: dst[row] = sum over ne0.  replaces k_sum_rows_f32, ggml-cuda/sumrows.cu:3-30 */
 B200_API int b200_op_sum_rows(const b200_tensor *x, const b200_tensor *dst, b200_stream_t stream);
 

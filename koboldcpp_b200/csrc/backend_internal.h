@@ -226,6 +226,9 @@ int kv8_attn_launches(const b200_kv8_attn_args *a);  // kernels of b200_op_kv8_a
 // whether the calls would take these arguments (a status)
 int kv8_attn_check(const b200_kv8_attn_args *a, size_t workspace_bytes);
 int kv8_store_check(const b200_kv8_store_args *a);
+// b200_op_ssm_conv_nodes and b200_op_ssm_scan_nodes: whether they take tensors of these types and shapes
+bool ssm_conv_nodes_ok(const b200_tensor *sx, const b200_tensor *c, const b200_tensor *dst);
+bool ssm_scan_nodes_ok(const b200_tensor *s, const b200_tensor *x, const b200_tensor *dt, const b200_tensor *a, const b200_tensor *b, const b200_tensor *c, const b200_tensor *dst);
 
 extern bool g_use_graphs, g_use_fusion;
 extern int64_t g_stat_launches, g_stat_replays, g_stat_captures;

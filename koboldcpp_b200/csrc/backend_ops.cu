@@ -502,6 +502,24 @@ bool op_supported(int /*device*/, const ggml_tensor *op) {
     switch (op->op) {
         case GGML_OP_NONE: case GGML_OP_RESHAPE: case GGML_OP_VIEW: case GGML_OP_PERMUTE: case GGML_OP_TRANSPOSE:
             return true;
+        case GGML_OP_CONCAT: {
+            if (!s0 || !s1 || s0->type != GGML_TYPE_F32 || s1->type != GGML_TYPE_F32 || op->type != GGML_TYPE_F32 || op->op_params[0] < 0 || op->op_params[0] > 3) return false;
+            for (int i = 0; i < 4; i++) if (i == op->op_params[0] ? op->ne[i] != s0->ne[i] + s1->ne[i] : (op->ne[i] != s0->ne[i] || op->ne[i] != s1->ne[i])) return false;
+            return true;
+        }
+        case GGML_OP_SSM_CONV: {
+            if (!s0 || !s1) return false;
+            const b200_tensor sx = as_b200(s0), c = as_b200(s1), d = as_b200(op);
+            return ssm_conv_nodes_ok(&sx, &c, &d);
+        }
+        case GGML_OP_SSM_SCAN: {
+            b200_tensor t[6], d = as_b200(op);
+            for (int i = 0; i < 6; i++) {
+                if (!op->src[i]) return false;
+                t[i] = as_b200(op->src[i]);
+            }
+            return ssm_scan_nodes_ok(t, t + 1, t + 2, t + 3, t + 4, t + 5, &d);
+        }
         case GGML_OP_MAP_CUSTOM1:  // an extension op (b200_ggml_ops.h) or a collective of the tensor-parallel decoder (b200_comm.h)
             if ((uint32_t)op->op_params[0] == B200_EXT_TAG) return ext_op_supported(op);
             if (!s0 || (uint32_t)op->op_params[0] != B200_COLLECTIVE_TAG || b200_comm_world() < 1) return false;
@@ -817,6 +835,10 @@ static bool bf16_gemm_ok(const ggml_tensor *n) {
 }
 
 size_t node_scratch_bytes(const ggml_tensor *n) {
+    if (n->op == GGML_OP_SSM_SCAN) {
+        const b200_tensor s = as_b200(n->src[0]), x = as_b200(n->src[1]);
+        return b200_op_ssm_scan_nodes_workspace_bytes(&s, &x);
+    }
     if (bf16_gemm_ok(n)) {
         const ggml_tensor *w = n->src[0], *a = n->src[1];
         const size_t one = b200_mul_mat_q_workspace_bytes(w->type, w->ne[0], w->ne[1], a->ne[1]);
@@ -946,6 +968,28 @@ void run_node(ExecCtx &x, const ggml_tensor *n, void *const *dst_slot) {
         case GGML_OP_SUM_ROWS: {
             b200_tensor a = as_b200(s0), d = as_b200(n);
             B200_CHECK_RC(b200_op_sum_rows(&a, &d, x.stream));
+            break;
+        }
+        case GGML_OP_CONCAT: {
+            b200_tensor a = as_b200(s0), b = as_b200(s1), d = as_b200(n);
+            B200_CHECK_RC(b200_op_concat(&a, &b, &d, n->op_params[0], x.stream));
+            x.launches++;
+            break;
+        }
+        case GGML_OP_SSM_CONV: {
+            b200_tensor a = as_b200(s0), b = as_b200(s1), d = as_b200(n);
+            B200_CHECK_RC(b200_op_ssm_conv_nodes(&a, &b, &d, x.stream));
+            break;
+        }
+        case GGML_OP_SSM_SCAN: {
+            b200_tensor t[6], d = as_b200(n);
+            for (int i = 0; i < 6; i++) t[i] = as_b200(n->src[i]);
+            const size_t need = b200_op_ssm_scan_nodes_workspace_bytes(t, t + 1);
+            if (need > 0) {
+                x.xb_src = nullptr;  // the scratch no longer holds a product's converted activations
+                x.launches++;
+            }
+            B200_CHECK_RC(b200_op_ssm_scan_nodes(t, t + 1, t + 2, t + 3, t + 4, t + 5, &d, x.scratch, x.scratch_bytes, x.stream));
             break;
         }
         default:

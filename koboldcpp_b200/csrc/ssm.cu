@@ -640,6 +640,34 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L)) ssm_scan_kernel(co
     if (PASS == ENDS && p == 0) sums[(int64_t)stretch * a.channels] = total;
 }
 
+// ------------------------------------------------------------------------------------------------ convolution as a graph node has it
+// The inputs of a channel lie side by side (the last ones of the sequence in front, made so by a CONCAT), the results channel by channel: a CTA turns a tile of NODE_CHANNELS channels and
+// NODE_ROWS rows over in shared memory.
+constexpr int NODE_CHANNELS = 32, NODE_ROWS = 64, NODE_WARPS = 8, NODE_TAPS = 16;
+__global__ void __launch_bounds__(32 * NODE_WARPS) ssm_conv_nodes_kernel(const char *sx, int64_t nb1, int64_t nb2, const float *w, float *dst, int channels, int rows, int taps) {
+    __shared__ float in[NODE_CHANNELS][NODE_ROWS + NODE_TAPS + 1];  // (a stride without common factors with the banks)
+    pdl_enter();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.x * NODE_CHANNELS, t0 = blockIdx.y * NODE_ROWS;
+    const int nt = min(NODE_ROWS, rows - t0), nc = min(NODE_CHANNELS, channels - c0);
+    sx += blockIdx.z * nb2;
+    dst += (int64_t)blockIdx.z * rows * channels;
+    for (int c = warp; c < nc; c += NODE_WARPS) {
+        const float *row = (const float *)(sx + (c0 + c) * nb1) + t0;
+        for (int t = lane; t < nt + taps - 1; t += 32) in[c][t] = row[t];
+    }
+    __syncthreads();
+    if (lane >= nc) return;
+    float k[NODE_TAPS];
+#pragma unroll
+    for (int j = 0; j < NODE_TAPS; j++) k[j] = j < taps ? w[(int64_t)(c0 + lane) * taps + j] : 0.f;
+    for (int t = warp; t < nt; t += NODE_WARPS) {
+        float y = 0.f;
+#pragma unroll
+        for (int j = 0; j < NODE_TAPS; j++) if (j < taps) y = fmaf(k[j], in[lane][t + j], y);
+        dst[(int64_t)(t0 + t) * channels + c0 + lane] = y;
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ host side
 static inline bool type_ok(int t) { return t == B200_TYPE_F32 || t == B200_TYPE_F16 || t == B200_TYPE_BF16; }
 static inline size_t type_size(int t) { return t == B200_TYPE_F32 ? 4 : 2; }
@@ -738,6 +766,43 @@ int ssm_scan_check(const b200_ssm_scan_args *a) {
 }
 
 }  // namespace ssm
+
+// whether the calls take tensors of these shapes (their memory apart): what supports_op asks
+static bool dense(const b200_tensor *t) {
+    int64_t nb = 4;
+    for (int i = 0; i < 4; i++) {
+        if (t->ne[i] != 1 && (int64_t)t->nb[i] != nb) return false;
+        nb *= t->ne[i];
+    }
+    return t->type == B200_TYPE_F32;
+}
+bool ssm_conv_nodes_ok(const b200_tensor *sx, const b200_tensor *c, const b200_tensor *dst) {
+    return sx && c && dst && sx->type == B200_TYPE_F32 && sx->nb[0] == 4 && sx->nb[1] % 4 == 0 && sx->nb[2] % 4 == 0 && dense(c) && dense(dst) && c->ne[0] >= 1 && c->ne[0] <= ssm::NODE_TAPS &&
+           c->ne[2] == 1 && c->ne[3] == 1 && sx->ne[3] == 1 && dst->ne[3] == 1 && sx->ne[0] == dst->ne[1] + c->ne[0] - 1 && sx->ne[1] == dst->ne[0] && c->ne[1] == dst->ne[0] &&
+           sx->ne[2] == dst->ne[2] && dst->ne[0] <= 0x7fffffff && dst->ne[1] <= 65535 * (int64_t)ssm::NODE_ROWS && dst->ne[2] <= 65535;
+}
+bool ssm_scan_nodes_ok(const b200_tensor *s, const b200_tensor *x, const b200_tensor *dt, const b200_tensor *a, const b200_tensor *b, const b200_tensor *c, const b200_tensor *dst) {
+    if (!s || !x || !dt || !a || !b || !c || !dst || !dense(s) || !dense(x) || !dense(dt) || !dense(a) || !dense(dst)) return false;
+    const int64_t n = s->ne[0], ch = s->ne[1], seqs = s->ne[2], rows = x->ne[1];
+    for (const b200_tensor *t : {b, c}) {
+        if (t->type != B200_TYPE_F32 || t->nb[0] != 4 || t->nb[1] % 4 || t->ne[0] != n || t->ne[1] != rows || t->ne[2] != seqs || t->ne[3] != 1) return false;
+        if ((rows > 1 || seqs > 1) && t->nb[1] < 4 * (size_t)n) return false;
+        if (seqs > 1 && t->nb[2] != t->nb[1] * (size_t)rows) return false;
+    }
+    return n >= 1 && n <= 128 && ch >= 1 && seqs >= 1 && seqs <= 65535 && rows >= 1 && s->ne[3] == 1 && x->ne[0] == ch && x->ne[2] == seqs && x->ne[3] == 1 && a->ne[0] == n && a->ne[1] == ch &&
+           a->ne[2] == 1 && a->ne[3] == 1 && dt->ne[0] == ch && dt->ne[1] == rows && dt->ne[2] == seqs && dt->ne[3] == 1 && rows * seqs <= 0x7fffffff && ch <= 0x7fffffff &&
+           opx::nelements(dst) == opx::nelements(x) + opx::nelements(s);
+}
+namespace ssm {
+static void scan_node_sizes(const b200_tensor *s, const b200_tensor *x, b200_ssm_scan_args *a) {
+    a->d_state = (int32_t)s->ne[0];
+    a->channels = (int32_t)s->ne[1];
+    a->n_seq = a->n_slots = (int32_t)s->ne[2];
+    a->n_tokens = (int32_t)(x->ne[1] * s->ne[2]);
+    a->groups = 1;
+    a->type = B200_TYPE_F32;
+}
+}  // namespace ssm
 }  // namespace b200
 
 using namespace b200;
@@ -793,6 +858,60 @@ int b200_op_ssm_scan(const b200_ssm_scan_args *a, void *workspace, size_t worksp
     if (a->type == B200_TYPE_F32) return launch_scan_type<float>(s, p, states16, st);
     if (a->type == B200_TYPE_F16) return launch_scan_type<__half>(s, p, states16, st);
     return launch_scan_type<__nv_bfloat16>(s, p, states16, st);
+}
+
+int b200_op_concat(const b200_tensor *a, const b200_tensor *b, const b200_tensor *dst, int dim, b200_stream_t stream) {
+    const char *who = "b200_op_concat";
+    OPX_REQUIRE(a && b && dst && dim >= 0 && dim < 4, B200_ERR_INVALID, "%s: NULL argument or no such dimension", who);
+    OPX_REQUIRE(a->type == B200_TYPE_F32 && b->type == B200_TYPE_F32 && dst->type == B200_TYPE_F32, B200_ERR_UNSUPPORTED, "%s: f32 only", who);
+    for (int i = 0; i < 4; i++) {
+        OPX_REQUIRE(i == dim ? dst->ne[i] == a->ne[i] + b->ne[i] : dst->ne[i] == a->ne[i] && dst->ne[i] == b->ne[i], B200_ERR_INVALID, "%s: shapes do not fit", who);
+    }
+    b200_tensor part = *dst;
+    for (const b200_tensor *s : {a, b}) {
+        part.ne[dim] = s->ne[dim];
+        const int rc = opx::nelements(s) > 0 ? b200_op_cpy(s, &part, stream) : B200_OK;
+        if (rc != B200_OK) return rc;
+        part.data = (char *)part.data + s->ne[dim] * dst->nb[dim];
+    }
+    return B200_OK;
+}
+
+int b200_op_ssm_conv_nodes(const b200_tensor *sx, const b200_tensor *c, const b200_tensor *dst, b200_stream_t stream) {
+    const char *who = "b200_op_ssm_conv_nodes";
+    OPX_REQUIRE(ssm_conv_nodes_ok(sx, c, dst), B200_ERR_UNSUPPORTED, "%s: f32, one row in front for every tap but one, at most %d taps", who, NODE_TAPS);
+    if (opx::nelements(dst) == 0) return B200_OK;
+    OPX_REQUIRE(sx->data && c->data && dst->data, B200_ERR_INVALID, "%s: NULL argument", who);
+    const int channels = (int)dst->ne[0], rows = (int)dst->ne[1];
+    const dim3 grid((unsigned)((channels + NODE_CHANNELS - 1) / NODE_CHANNELS), (unsigned)((rows + NODE_ROWS - 1) / NODE_ROWS), (unsigned)dst->ne[2]);
+    B200_CUDA_TRY(launch_chained(ssm_conv_nodes_kernel, grid, 32 * NODE_WARPS, 0, (cudaStream_t)stream, (const char *)sx->data, (int64_t)sx->nb[1], (int64_t)sx->nb[2], (const float *)c->data,
+                                 (float *)dst->data, channels, rows, (int)c->ne[0]));
+    return B200_OK;
+}
+
+size_t b200_op_ssm_scan_nodes_workspace_bytes(const b200_tensor *s, const b200_tensor *x) {
+    b200_ssm_scan_args a = {};
+    if (!s || !x) return 0;
+    scan_node_sizes(s, x, &a);
+    return b200_ssm_scan_workspace_bytes(&a);
+}
+
+int b200_op_ssm_scan_nodes(const b200_tensor *s, const b200_tensor *x, const b200_tensor *dt, const b200_tensor *a, const b200_tensor *b, const b200_tensor *c, const b200_tensor *dst,
+                           void *workspace, size_t workspace_bytes, b200_stream_t stream) {
+    const char *who = "b200_op_ssm_scan_nodes";
+    OPX_REQUIRE(ssm_scan_nodes_ok(s, x, dt, a, b, c, dst), B200_ERR_UNSUPPORTED, "%s: f32, contiguous but for b and c, at most 128 states", who);
+    b200_ssm_scan_args n = {};
+    scan_node_sizes(s, x, &n);
+    n.x = x->data; n.dt = dt->data; n.x_stride = n.dt_stride = n.dst_stride = n.channels;
+    n.b = b->data; n.b_stride = (int64_t)(b->nb[1] / 4);
+    n.c = c->data; n.c_stride = (int64_t)(c->nb[1] / 4);
+    n.a = (const float *)a->data;
+    n.from = (const float *)s->data;
+    n.dst = dst->data;
+    n.state = (float *)dst->data + (int64_t)n.n_tokens * n.channels;
+    n.slot_stride = n.from_stride = (int64_t)n.channels * n.d_state;
+    n.softplus = 1;
+    return b200_op_ssm_scan(&n, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"
