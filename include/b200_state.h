@@ -39,7 +39,7 @@ B200_API int b200_op_ssm_conv(const b200_ssm_conv_args *a, b200_stream_t stream)
  *   d = dt[t][c] + dt_bias[c], softplus != 0: d = ln(1 + e^d);   h[c][n] <- exp(d * a[c][n]) * h[c][n] + d * x[t][c] * b[t][g][n];
  *   y = sum_n c[t][g][n] * h[c][n] + skip[c] * x[t][c];   dst[t][c] = y, or y * silu(z[t][c]) with z,
  * where channel c belongs to group g = c / (channels / groups).  Everything between the rows is f32.  `from` (optional): states are read there, in slots of from_stride, instead of
- * from `state`.  Few channels and a long sequence: the rows are shared out in stretches, whose states meet in the workspace (b200_ssm_scan_workspace_bytes bytes, 16-byte
+ * from `state` (other memory than that).  Few channels and a long sequence: the rows are shared out in stretches, whose states meet in the workspace (b200_ssm_scan_workspace_bytes bytes, 16-byte
  * aligned, 0: none). */
 typedef struct {
     const void *x, *dt; int64_t x_stride, dt_stride;         /* [n_tokens][channels] */
@@ -50,7 +50,7 @@ typedef struct {
     const int32_t *seq_info;
     float *state; int64_t slot_stride;                       /* [channels][d_state] per slot */
     const float *from; int64_t from_stride;
-    void *dst; int64_t dst_stride;                           /* [n_tokens][channels]; may be x, dt or z */
+    void *dst; int64_t dst_stride;                           /* [n_tokens][channels]; may be x, dt or z at its stride */
     int32_t n_seq, n_slots, n_tokens, max_new;
     int32_t channels, d_state, groups;                       /* d_state <= 128; groups divides channels */
     int32_t softplus, type;                                  /* type: of x, dt, b, c, z and dst */
@@ -66,6 +66,7 @@ B200_API int b200_op_ssm_scan(const b200_ssm_scan_args *a, void *workspace, size
  * Where there are fewer than n_keep successors, the rest are score -inf, beam -1, token -1, slot -1.  With logits of +inf those tokens share their row evenly. */
 #define B200_BEAM_MAX 64     /* beams of a request */
 #define B200_BEAM_KEEP 128   /* successors that are kept */
+#define B200_BEAM_VOCAB (1 << 30)
 typedef struct {
     const void *logits; int64_t logits_stride;               /* [n_requests * n_beams][n_vocab] */
     const float *score;                                      /* [n_requests * n_beams] */

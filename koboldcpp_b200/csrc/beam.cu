@@ -410,8 +410,8 @@ static int check_select_sizes(const b200_beam_select_args *a, const char *who) {
     OPX_REQUIRE(a->type == B200_TYPE_F32 || a->type == B200_TYPE_F16 || a->type == B200_TYPE_BF16, B200_ERR_UNSUPPORTED, "%s: logits of type %d", who, a->type);
     OPX_REQUIRE(a->n_requests >= 0 && a->n_beams > 0 && a->n_vocab > 0 && a->n_keep > 0, B200_ERR_INVALID, "%s: %d requests of %d beams, %d tokens, %d to keep", who, a->n_requests, a->n_beams, a->n_vocab,
                 a->n_keep);
-    OPX_REQUIRE(a->n_beams <= B200_BEAM_MAX && a->n_keep <= B200_BEAM_KEEP && a->n_vocab <= 0x7fff0000, B200_ERR_UNSUPPORTED, "%s: %d beams (%d at most), %d to keep (%d)", who, a->n_beams, B200_BEAM_MAX,
-                a->n_keep, B200_BEAM_KEEP);
+    OPX_REQUIRE(a->n_beams <= B200_BEAM_MAX && a->n_keep <= B200_BEAM_KEEP && a->n_vocab <= B200_BEAM_VOCAB, B200_ERR_UNSUPPORTED, "%s: %d beams (%d at most), %d to keep (%d), %d tokens (%d)", who, a->n_beams,
+                B200_BEAM_MAX, a->n_keep, B200_BEAM_KEEP, a->n_vocab, B200_BEAM_VOCAB);
     OPX_REQUIRE((int64_t)a->n_requests * a->n_beams <= 65535 && (int64_t)a->n_requests * a->n_keep <= 0x7fffffff, B200_ERR_UNSUPPORTED, "%s: %d requests of %d beams, 65535 rows at most", who,
                 a->n_requests, a->n_beams);
     return B200_OK;

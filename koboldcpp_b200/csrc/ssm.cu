@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L)) ssm_scan_kernel(co
     load(0);
     // ===== the states
     Two h[NS / 2], rate[NS / 2];
-    float total = 0.f;
+    double total = 0.0;  // (a stretch may be long: terms of one size would all be rounded the same way)
     const bool pieces = (N & 3) == 0 && ((a.slot_stride | a.from_stride) & 3) == 0 && (((uintptr_t)a.state | (uintptr_t)a.from | (uintptr_t)a.a) & 15) == 0;
     // end states of a stretch lie as [d_state][channels], so that neighbouring lanes read neighbouring words; the stretch in front of a sequence's first is its state
     const int64_t ends_row = (int64_t)a.channels * N;
@@ -553,7 +553,12 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L)) ssm_scan_kernel(co
 #pragma unroll
             for (int j = 0; j < MT; j++) {
                 dx[j] = d[j] * x[j];
-                if (PASS == ENDS) total += d[j];
+            }
+            if (PASS == ENDS) {
+                float some = d[0];
+#pragma unroll
+                for (int j = 1; j < MT; j++) some += d[j];
+                total += some;
             }
             load(r0 + tg + TG);
             float ds[TG], dxs[TG];  // of all the group's rows
@@ -637,7 +642,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L)) ssm_scan_kernel(co
             else store_states<false>(to, n, N, s);
         }
     }
-    if (PASS == ENDS && p == 0) sums[(int64_t)stretch * a.channels] = total;
+    if (PASS == ENDS && p == 0) sums[(int64_t)stretch * a.channels] = (float)total;
 }
 
 // ------------------------------------------------------------------------------------------------ convolution as a graph node has it
@@ -762,6 +767,9 @@ int ssm_scan_check(const b200_ssm_scan_args *a) {
     OPX_REQUIRE(a->slot_stride >= states && (!a->from || a->from_stride >= states), B200_ERR_INVALID, "%s: slots overlap", who);
     OPX_REQUIRE(on(type_size(a->type), {a->x, a->dt, a->b, a->c, a->z, a->dst}) && on(4, {a->a, a->dt_bias, a->d, a->state, a->from}), B200_ERR_INVALID, "%s: a pointer is not aligned to its type", who);
     OPX_REQUIRE(a->dst != a->b && a->dst != a->c, B200_ERR_INVALID, "%s: dst is b or c, which other channels read", who);
+    OPX_REQUIRE((a->dst != a->x || a->dst_stride == a->x_stride) && (a->dst != a->dt || a->dst_stride == a->dt_stride) && (a->dst != a->z || a->dst_stride == a->z_stride), B200_ERR_INVALID,
+                "%s: dst is an input at another stride", who);
+    OPX_REQUIRE(a->from != a->state || a->from_stride == a->slot_stride, B200_ERR_INVALID, "%s: from is state at another stride", who);
     return B200_OK;
 }
 

@@ -66,7 +66,9 @@ def scan_args(**change):
     (dict(channels=0), INVALID), (dict(d_state=0), INVALID), (dict(groups=0), INVALID), (dict(groups=3), INVALID), (dict(d_state=129, slot_stride=9999, b_stride=999, c_stride=999), UNSUPPORTED),
     (dict(x_stride=7), INVALID), (dict(dt_stride=7), INVALID), (dict(z_stride=7), INVALID), (dict(dst_stride=7), INVALID), (dict(b_stride=31), INVALID), (dict(c_stride=31), INVALID),
     (dict(slot_stride=127), INVALID), ({"from": AT, "from_stride": 127}, INVALID), (dict(x=AT + 2), INVALID), (dict(z=AT + 1, type=L.BF16), INVALID), (dict(a=AT + 2), INVALID), (dict(state=AT + 2), INVALID),
-    (dict(dst=AT), INVALID), (dict(seq_info=AT + 2), INVALID), (dict(seq_info=None, n_seq=2), INVALID), (dict(seq_info=None, n_seq=3), INVALID)])
+    (dict(dst=AT), INVALID), (dict(seq_info=AT + 2), INVALID), (dict(seq_info=None, n_seq=2), INVALID), (dict(seq_info=None, n_seq=3), INVALID),
+    (dict(dst=3 * AT, x=3 * AT, dst_stride=9), INVALID), (dict(dst=3 * AT, dt=3 * AT, dst_stride=9), INVALID), (dict(dst=3 * AT, z=3 * AT, dst_stride=9), INVALID),
+    ({"from": AT, "from_stride": 132}, INVALID)])
 def test_scans_that_are_refused(change, status):
     assert lib().b200_op_ssm_scan(C.byref(scan_args(**change)), AT, 1 << 30, None) == status
     assert lib().b200_last_error()
@@ -104,7 +106,7 @@ def select_args(**change):
 @pytest.mark.parametrize("change,status", [
     (dict(logits=None), INVALID), (dict(score=None), INVALID), (dict(to_score=None), INVALID), (dict(to_beam=None), INVALID), (dict(to_token=None), INVALID), (dict(slot=None), INVALID),
     (dict(type=L.Q4_0), UNSUPPORTED), (dict(n_requests=-1), INVALID), (dict(n_beams=0), INVALID), (dict(n_vocab=0), INVALID), (dict(n_keep=0), INVALID), (dict(n_beams=65), UNSUPPORTED),
-    (dict(n_keep=129), UNSUPPORTED), (dict(n_requests=16384), UNSUPPORTED), (dict(logits_stride=99), INVALID), (dict(end_token=100), INVALID), (dict(end_token=-1), INVALID), (dict(logits=AT + 2), INVALID),
+    (dict(n_keep=129), UNSUPPORTED), (dict(n_requests=16384), UNSUPPORTED), (dict(n_vocab=(1 << 30) + 1, logits_stride=1 << 31), UNSUPPORTED), (dict(logits_stride=99), INVALID), (dict(end_token=100), INVALID), (dict(end_token=-1), INVALID), (dict(logits=AT + 2), INVALID),
     (dict(logits=AT + 1, type=L.F16), INVALID), (dict(score=AT + 2), INVALID), (dict(to_token=AT + 2), INVALID), (dict(to_score=AT), INVALID), (dict(to_slot=AT), INVALID)])
 def test_selections_that_are_refused(change, status):
     assert lib().b200_op_beam_select(C.byref(select_args(**change)), AT, 1 << 30, None) == status
