@@ -142,14 +142,14 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) beam_rows_kernel(const SelectA
     const int64_t r = blockIdx.y;
     const T *row = (const T *)a.logits + r * a.logits_stride;
     const int p0 = blockIdx.x * a.share, p1 = min(a.n_pieces, p0 + a.share);
-    // beams that nobody asks for the successors of
-    if ((a.ended && a.ended[r]) || !(a.score[r] > NEG_INF)) return;
+    const bool unwanted = (a.ended && a.ended[r]) || !(a.score[r] > NEG_INF);  // a beam that nobody asks for the successors of
     double sum = 0.0;
     float ref = NEG_INF;
-    // (the next PIECE tokens travel while these are added up)
+    // (the next PIECE tokens travel while these are added up; the first ones before it is known whether they are wanted)
     Raw<T> next;
     int p = p0 + warp, t0 = p * a.piece;
     if (p < p1) load_raw<T, WIDE>(row, t0, a.vocab, lane, next);
+    if (unwanted) return;
     while (p < p1) {
         float top = NEG_INF;
         for (const int end = min(a.vocab, (p + 1) * a.piece); t0 < end;) {
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(PICK_THREADS) beam_pick_kernel(const SelectArg
                 low = min(low, sh.low[w]);
                 high = max(high, sh.high[w]);
             }
-            for (int k = 0; k < 12 && low < high; k++) {
+            for (int k = 0; k < 9 && low < high; k++) {
                 const unsigned at = low + (high - low + 1) / 2;
                 if (__syncthreads_count(key >= at) >= a.keep) low = at;
                 else high = at - 1;
@@ -555,7 +555,7 @@ int b200_op_state_reorder(const b200_slot_state *states, int32_t n_states, const
     }
     // as wide a column as the moves leave room for
     int log2 = 5;  // (COLUMNS_BYTES / B200_STATE_MAX_MOVES)
-    while (log2 < 11 && n << (log2 + 1) <= COLUMNS_BYTES) log2++;
+    while (log2 < 12 && n << (log2 + 1) <= COLUMNS_BYTES) log2++;
     const int width = 1 << log2;
     const size_t smem = (size_t)n * width + 4 * ((size_t)n_slots + 2 * n);
     const auto kern = wide ? state_reorder_kernel<16> : state_reorder_kernel<4>;
@@ -576,7 +576,7 @@ int b200_op_state_reorder(const b200_slot_state *states, int32_t n_states, const
         r.first[r.n_states] = (int32_t)columns;
         r.n = n; r.n_slots = n_slots; r.width = width; r.width_log2 = log2; r.src = src; r.dst = dst;
         r.refused = at >= n_states ? refused : nullptr;
-        const int64_t most = 6 * (int64_t)sm_count();
+        const int64_t most = (int64_t)(smem < 27 * 1024 ? 8 : smem < 36 * 1024 ? 6 : 4) * sm_count();  // as many as an SM holds, by threads or by shared memory
         const unsigned grid = (unsigned)(columns < 1 ? 1 : columns < most ? columns : most);
         B200_CUDA_TRY(launch_chained(kern, grid, REORDER_THREADS, smem, (cudaStream_t)stream, r));
     } while (at < n_states);

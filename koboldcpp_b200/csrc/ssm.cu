@@ -152,23 +152,28 @@ __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_kernel(const ConvArgs a
         // (of the ring every thread reads only what it has asked for)
         __shared__ __align__(16) P ring[CONV_GROUPS][CONV_GROUP][CONV_THREADS];
         auto fetch = [&](int g) {
+            const int left = nt - g * CONV_GROUP;
+            P *to = &ring[g % CONV_GROUPS][0][threadIdx.x];
 #pragma unroll
             for (int u = 0; u < CONV_GROUP; u++) {
-                if (g * CONV_GROUP + u < nt) {
-                    if constexpr (sizeof(P) == 16) cp_async16(&ring[g % CONV_GROUPS][u][threadIdx.x], in_row);
-                    else cp_async8(&ring[g % CONV_GROUPS][u][threadIdx.x], in_row);
+                if (u < left) {
+                    if constexpr (sizeof(P) == 16) cp_async16(to + u * CONV_THREADS, in_row + u * a.x_stride);
+                    else cp_async8(to + u * CONV_THREADS, in_row + u * a.x_stride);
                 }
-                in_row += a.x_stride;
             }
+            in_row += CONV_GROUP * a.x_stride;
             cp_async_commit();
         };
 #pragma unroll
         for (int g = 0; g < CONV_GROUPS - 1; g++) fetch(g);
         for (int g = 0; g * CONV_GROUP < nt; g++) {
             cp_async_wait<CONV_GROUPS - 2>();
+            const P *from = &ring[g % CONV_GROUPS][0][threadIdx.x];
+            if ((g + 1) * CONV_GROUP <= nt) {
 #pragma unroll
-            for (int u = 0; u < CONV_GROUP; u++) {
-                if (g * CONV_GROUP + u < nt) turn(ring[g % CONV_GROUPS][u][threadIdx.x]);
+                for (int u = 0; u < CONV_GROUP; u++) turn(from[u * CONV_THREADS]);
+            } else {
+                for (int u = 0; g * CONV_GROUP + u < nt; u++) turn(from[u * CONV_THREADS]);
             }
             fetch(g + CONV_GROUPS - 1);
         }
