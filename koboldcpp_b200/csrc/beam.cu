@@ -434,16 +434,46 @@ struct ReorderArgs {
     char *base[REORDER_STATES];
     int64_t stride[REORDER_STATES], bytes[REORDER_STATES];
     int32_t first[REORDER_STATES + 1];  // number of a state's first column
+    uint8_t unit_log2[REORDER_STATES];  // bytes of an access: 16, 8 or 4
     int32_t n_states, n, n_slots, width, width_log2;  // width: bytes of a column
     const int32_t *src, *dst;
     int32_t *refused;
 };
-template <int UNIT>  // bytes of an access: 16 or 4
-__global__ void __launch_bounds__(REORDER_THREADS) state_reorder_kernel(const ReorderArgs a) {
+template <int LOG2>
+__device__ __forceinline__ void move_column(unsigned char *column, char *base, int64_t stride, const int *from, const int *to, int n, int width_log2, int bytes) {
+    const int shift = width_log2 - LOG2, last = bytes >> LOG2;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n << shift; i += REORDER_THREADS) {
+        const int k = i >> shift, u = i & ((1 << shift) - 1);
+        if (u < last) {
+            void *in = column + ((size_t)i << LOG2);
+            const char *out = base + from[k] * stride + (u << LOG2);
+            if constexpr (LOG2 == 4) cp_async16(in, out);
+            else if constexpr (LOG2 == 3) cp_async8(in, out);
+            else cp_async4(in, out);
+        }
+    }
+    cp_async_commit();
+    cp_async_wait<0>();
+    __syncthreads();
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n << shift; i += REORDER_THREADS) {
+        const int k = i >> shift, u = i & ((1 << shift) - 1);
+        if (u < last) {
+            const unsigned char *in = column + ((size_t)i << LOG2);
+            char *out = base + to[k] * stride + (u << LOG2);
+            if constexpr (LOG2 == 4) *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<const uint4 *>(in);
+            else if constexpr (LOG2 == 3) *reinterpret_cast<uint2 *>(out) = *reinterpret_cast<const uint2 *>(in);
+            else *reinterpret_cast<unsigned *>(out) = *reinterpret_cast<const unsigned *>(in);
+        }
+    }
+    __syncthreads();
+}
+__global__ void __launch_bounds__(REORDER_THREADS, 8) state_reorder_kernel(const ReorderArgs a) {
     extern __shared__ __align__(16) unsigned char column[];  // [n][width], then the moves
     int *claim = (int *)(column + (size_t)a.n * a.width), *from = claim + a.n_slots, *to = from + a.n;
     __shared__ int n_moves, n_refused;
-    pdl_enter();
+    pdl_wait();  // (the kernel behind is let in by CTAs that are done: one that took places early would leave SMs unequal)
     const int tid = threadIdx.x;
     if (tid == 0) n_moves = n_refused = 0;
     for (int i = tid; i < a.n_slots; i += REORDER_THREADS) claim[i] = 0x7fffffff;
@@ -465,7 +495,7 @@ __global__ void __launch_bounds__(REORDER_THREADS) state_reorder_kernel(const Re
     }
     __syncthreads();
     if (a.refused && blockIdx.x == 0 && tid == 0 && n_refused) *a.refused += n_refused;
-    const int n = n_moves, shift = a.width_log2 - (UNIT == 16 ? 4 : 2), units = 1 << shift;
+    const int n = n_moves;
     if (n == 0) return;
     for (int item = blockIdx.x; item < a.first[a.n_states]; item += gridDim.x) {
         int lo = 0, hi = a.n_states - 1;  // the last state whose first column is not behind this one
@@ -476,27 +506,10 @@ __global__ void __launch_bounds__(REORDER_THREADS) state_reorder_kernel(const Re
         }
         const int64_t at = (int64_t)(item - a.first[lo]) * a.width, stride = a.stride[lo];
         char *base = a.base[lo] + at;
-        const int here = (int)min((int64_t)a.width, a.bytes[lo] - at) / UNIT;
-#pragma unroll 4
-        for (int i = tid; i < n * units; i += REORDER_THREADS) {
-            const int k = i >> shift, u = i & (units - 1);
-            if (u < here) {
-                if constexpr (UNIT == 16) cp_async16(column + (size_t)k * a.width + u * UNIT, base + from[k] * stride + u * UNIT);
-                else cp_async4(column + (size_t)k * a.width + u * UNIT, base + from[k] * stride + u * UNIT);
-            }
-        }
-        cp_async_commit();
-        cp_async_wait<0>();
-        __syncthreads();
-#pragma unroll 4
-        for (int i = tid; i < n * units; i += REORDER_THREADS) {
-            const int k = i >> shift, u = i & (units - 1);
-            if (u < here) {
-                if constexpr (UNIT == 16) *reinterpret_cast<uint4 *>(base + to[k] * stride + u * UNIT) = *reinterpret_cast<const uint4 *>(column + (size_t)k * a.width + u * UNIT);
-                else *reinterpret_cast<unsigned *>(base + to[k] * stride + u * UNIT) = *reinterpret_cast<const unsigned *>(column + (size_t)k * a.width + u * UNIT);
-            }
-        }
-        __syncthreads();
+        const int here = (int)min((int64_t)a.width, a.bytes[lo] - at);
+        if (a.unit_log2[lo] == 4) move_column<4>(column, base, stride, from, to, n, a.width_log2, here);
+        else if (a.unit_log2[lo] == 3) move_column<3>(column, base, stride, from, to, n, a.width_log2, here);
+        else move_column<2>(column, base, stride, from, to, n, a.width_log2, here);
     }
 }
 
@@ -546,20 +559,17 @@ int b200_op_state_reorder(const b200_slot_state *states, int32_t n_states, const
     if (n == 0) return B200_OK;
     OPX_REQUIRE(src && dst && (states || n_states == 0), B200_ERR_INVALID, "%s: NULL argument", who);
     OPX_REQUIRE((((uintptr_t)src | (uintptr_t)dst | (uintptr_t)refused) & 3) == 0, B200_ERR_INVALID, "%s: a list at an odd place", who);
-    bool wide = true;
     for (int i = 0; i < n_states; i++) {
         const b200_slot_state &s = states[i];
         OPX_REQUIRE(s.bytes >= 0 && s.stride >= s.bytes && (s.base || s.bytes == 0), B200_ERR_INVALID, "%s: state %d: %lld bytes of a slot every %lld", who, i, (long long)s.bytes, (long long)s.stride);
         OPX_REQUIRE((((uintptr_t)s.base | (uint64_t)s.stride | (uint64_t)s.bytes) & 3) == 0, B200_ERR_INVALID, "%s: state %d is not a multiple of 4 bytes", who, i);
-        wide = wide && (((uintptr_t)s.base | (uint64_t)s.stride | (uint64_t)s.bytes) & 15) == 0;
     }
     // as wide a column as the moves leave room for
     int log2 = 5;  // (COLUMNS_BYTES / B200_STATE_MAX_MOVES)
     while (log2 < 12 && n << (log2 + 1) <= COLUMNS_BYTES) log2++;
     const int width = 1 << log2;
     const size_t smem = (size_t)n * width + 4 * ((size_t)n_slots + 2 * n);
-    const auto kern = wide ? state_reorder_kernel<16> : state_reorder_kernel<4>;
-    if (smem > 48 * 1024) B200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, REORDER_MOST));  // (the same for all calls: they may be in several threads)
+    if (smem > 48 * 1024) B200_CUDA_TRY(cudaFuncSetAttribute(state_reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, REORDER_MOST));  // (the same for all calls: they may be in several threads)
     int at = 0;
     do {  // (without states too: refused moves are counted)
         ReorderArgs r = {};
@@ -569,6 +579,8 @@ int b200_op_state_reorder(const b200_slot_state *states, int32_t n_states, const
             r.base[r.n_states] = (char *)s.base;
             r.stride[r.n_states] = s.stride;
             r.bytes[r.n_states] = s.bytes;
+            const uint64_t all = (uintptr_t)s.base | (uint64_t)s.stride | (uint64_t)s.bytes;
+            r.unit_log2[r.n_states] = all % 16 == 0 ? 4 : all % 8 == 0 ? 3 : 2;
             r.first[r.n_states++] = (int32_t)columns;
             columns += (s.bytes + width - 1) / width;
         }
@@ -578,7 +590,7 @@ int b200_op_state_reorder(const b200_slot_state *states, int32_t n_states, const
         r.refused = at >= n_states ? refused : nullptr;
         const int64_t most = (int64_t)(smem < 27 * 1024 ? 8 : smem < 36 * 1024 ? 6 : 4) * sm_count();  // as many as an SM holds, by threads or by shared memory
         const unsigned grid = (unsigned)(columns < 1 ? 1 : columns < most ? columns : most);
-        B200_CUDA_TRY(launch_chained(kern, grid, REORDER_THREADS, smem, (cudaStream_t)stream, r));
+        B200_CUDA_TRY(launch_chained(state_reorder_kernel, grid, REORDER_THREADS, smem, (cudaStream_t)stream, r));
     } while (at < n_states);
     return B200_OK;
 }
