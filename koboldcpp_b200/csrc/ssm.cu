@@ -395,8 +395,8 @@ __global__ void __launch_bounds__(32 * STEP_WARPS) ssm_step_kernel(const ScanArg
 // and multiply-adds of a row are chains that run side by side.  b and c of a chunk of rows wait in shared memory, where all lanes read the same words.  Rows go in groups of TG; lane p of a channel makes d and d x of the group's rows p, p + L, ..,
 // and sends off their results; the next group's rows are loaded meanwhile.
 // What bounds it: exponentials, d_state + 3 for each row and channel at 16 a cycle and SM (four prompts of 2048 rows x 8192 channels: 283 us), and that 1024 warps make two on some schedulers and one
-// on others: 474 us; the unit is busy 64 % of the time on average.  Some of the exponentials made by multiply-adds (two or four of 16 as polynomials) gave nothing: the other instructions, 90 a row, fill up what that leaves.
-constexpr int SCAN_WARPS = 4, SCAN_THREADS = 32 * SCAN_WARPS, TG = 8;
+// on others, where a row takes 370 cycles: 447 us.  Some of the exponentials made by multiply-adds (two or four of 16 as polynomials) gave nothing: the other instructions, 90 a row, fill up what that leaves.
+constexpr int SCAN_WARPS = 4, SCAN_THREADS = 32 * SCAN_WARPS;
 // the three things that a CTA can be there for: a whole sequence; the state at the end of a stretch as if it began from nothing (the first one: from the sequence's state), and the sum of
 // its d; a stretch's rows, from the states and sums of those before it
 enum Pass { WHOLE, ENDS, ROWS };
@@ -406,13 +406,14 @@ struct ScanSizes {
     static constexpr int TC = NP <= 16 ? 32 : 16;                  // rows of a chunk
     static constexpr int PIECES = (2 * TC * NP / 4 + SCAN_THREADS - 1) / SCAN_THREADS;  // pieces of four numbers of b or c that a thread fetches
 };
-// CTAs that an SM is to hold: with 16 states a lane and nothing to exchange the compiler's own order of loads and exponentials, which wants 168 registers, is worth more than a fourth one (four
-// long prompts 474 us, 629 with 128 registers); with exchanges between lanes it is not (64 states: 300 us, 189)
-constexpr int scan_ctas(int lanes) { return lanes == 1 ? 3 : 4; }
+// Rows of a group, and CTAs that an SM is to hold.  Where nothing is exchanged, long groups in the order that the compiler gives them with 255 registers are worth more than more CTAs (four long prompts: 16 rows
+// 447 us with two CTAs and 626 with three, 8 rows 460, 473 and 629 with four); with exchanges between lanes they are not (64 states: 8 rows 300 us with three CTAs, 188 with four).
+constexpr int scan_rows(int lanes) { return lanes == 1 ? 16 : 8; }
+constexpr int scan_ctas(int lanes) { return lanes == 1 ? 2 : 4; }
 template <typename T, int L, int NS, int PASS>
 __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L)) ssm_scan_kernel(const ScanArgs a) {
     using Z = ScanSizes<L, NS>;
-    constexpr int CB = Z::CB, NP = Z::NP, TC = Z::TC, NQ = NS / 4, MT = TG / L;  // MT: rows of a group that a lane makes ready
+    constexpr int CB = Z::CB, NP = Z::NP, TC = Z::TC, NQ = NS / 4, TG = scan_rows(L), MT = TG / L;  // TG: rows of a group; MT: those that a lane makes ready
     __shared__ __align__(16) float sbc[2][2][TC][NP];  // [chunk & 1][b, c]
     pdl_wait();  // (the kernel behind is let in at the end: CTAs of it that wait would take places in an order that leaves SMs unequal, 520 -> 610 us for four long prompts)
     const int tid = threadIdx.x, lane = tid & 31, p = lane % L;
@@ -704,7 +705,9 @@ static ScanPlan plan_of(const b200_ssm_scan_args *a) {
     // CTAs that are there on average while the longest sequence lasts
     const double ctas = (double)((per_group + block - 1) / block) * a->groups * a->n_tokens / longest;
     if (ctas < 1.25 * sm_count() && longest >= 128) {
-        const double n = (double)scan_ctas(lanes_of(a->d_state)) * sm_count() / ctas;  // as many as are there at once
+        // One sequence: as many CTAs as are there at once (4096 rows of 2048 channels: 96 us; twice as many: 120).  Several, whose ends come at different times: more than that (six of 37 to 1501 rows of
+        // 5120 channels: 265 us with four an SM, 298 with two).
+        const double n = (double)(a->n_seq > 1 ? 4 : scan_ctas(lanes_of(a->d_state))) * sm_count() / ctas;
         const int rows = (int)(longest / (n < 32 ? n : 32));
         p.stretch = ((rows < 64 ? 64 : rows) + 7) / 8 * 8;
         p.n_stretch = (longest + p.stretch - 1) / p.stretch;
