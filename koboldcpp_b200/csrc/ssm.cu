@@ -397,23 +397,26 @@ __global__ void __launch_bounds__(32 * STEP_WARPS) ssm_step_kernel(const ScanArg
 // What bounds it: exponentials, d_state + 3 for each row and channel at 16 a cycle and SM (four prompts of 2048 rows x 8192 channels: 283 us), and that 1024 warps make two on some schedulers and one
 // on others, where a row takes 370 cycles: 447 us.  Some of the exponentials made by multiply-adds (two or four of 16 as polynomials) gave nothing: the other instructions, 90 a row, fill up what that leaves.
 constexpr int SCAN_WARPS = 4, SCAN_THREADS = 32 * SCAN_WARPS;
-// the three things that a CTA can be there for: a whole sequence; the state at the end of a stretch as if it began from nothing (the first one: from the sequence's state), and the sum of
+// the things that a CTA can be there for: a whole sequence, with few CTAs or with many; the state at the end of a stretch as if it began from nothing (the first one: from the sequence's state), and the sum of
 // its d; a stretch's rows, from the states and sums of those before it
-enum Pass { WHOLE, ENDS, ROWS };
+enum Pass { WHOLE, MANY, ENDS, ROWS };
 template <int L, int NS>
 struct ScanSizes {
     static constexpr int CB = SCAN_THREADS / L, NP = NS * L;       // channels of a CTA; states of a channel, those behind d_state included
     static constexpr int TC = NP <= 16 ? 32 : 16;                  // rows of a chunk
     static constexpr int PIECES = (2 * TC * NP / 4 + SCAN_THREADS - 1) / SCAN_THREADS;  // pieces of four numbers of b or c that a thread fetches
 };
-// Rows of a group, and CTAs that an SM is to hold.  Where nothing is exchanged, long groups in the order that the compiler gives them with 255 registers are worth more than more CTAs (four long prompts: 16 rows
-// 447 us with two CTAs and 626 with three, 8 rows 460, 473 and 629 with four); with exchanges between lanes they are not (64 states: 8 rows 300 us with three CTAs, 188 with four).
-constexpr int scan_rows(int lanes) { return lanes == 1 ? 16 : 8; }
-constexpr int scan_ctas(int lanes) { return lanes == 1 ? 2 : 4; }
+// Rows of a group, and CTAs that an SM is to hold.  A lane that is a channel, in few CTAs: long groups in the order that the compiler gives them with 255 registers (four long prompts, 1.7 CTAs
+// an SM: 16 rows 447 us; 8 rows 460, with 168 registers 473, with 128 629).  Where there are CTAs for every place that an SM has, more places are worth more: short groups, four CTAs (128 sequences of
+// 48 rows, 8192 channels: 285 us, 351 the other way; of 5 rows, where a long group would also walk what is not there, 81 and 186).  Stretches stay with the first (one prompt of 4096 rows of 2048
+// channels: 96 us, 107 the other way; of 8192 channels: 398 and 373).  With exchanges between lanes: four CTAs (64 states: 188 us, with three 300).
+constexpr int SCAN_SHORT = 32;  // rows up to which sequences take the second way whatever the number of CTAs
+constexpr int scan_rows(int lanes, int pass) { return lanes > 1 ? 8 : pass == MANY ? 4 : 16; }
+constexpr int scan_ctas(int lanes, int pass) { return lanes > 1 || pass == MANY ? 4 : 2; }
 template <typename T, int L, int NS, int PASS>
-__global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L)) ssm_scan_kernel(const ScanArgs a) {
+__global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L, PASS)) ssm_scan_kernel(const ScanArgs a) {
     using Z = ScanSizes<L, NS>;
-    constexpr int CB = Z::CB, NP = Z::NP, TC = Z::TC, NQ = NS / 4, TG = scan_rows(L), MT = TG / L;  // TG: rows of a group; MT: those that a lane makes ready
+    constexpr int CB = Z::CB, NP = Z::NP, TC = Z::TC, NQ = NS / 4, TG = scan_rows(L, PASS), MT = TG / L;  // TG: rows of a group; MT: those that a lane makes ready
     __shared__ __align__(16) float sbc[2][2][TC][NP];  // [chunk & 1][b, c]
     pdl_wait();  // (the kernel behind is let in at the end: CTAs of it that wait would take places in an order that leaves SMs unequal, 520 -> 610 us for four long prompts)
     const int tid = threadIdx.x, lane = tid & 31, p = lane % L;
@@ -421,7 +424,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L)) ssm_scan_kernel(co
     const int N = a.d_state, blocks = (a.per_group + CB - 1) / CB, group = blockIdx.x / blocks, in_group = (blockIdx.x - group * blocks) * CB + tid / L;
     const bool mine = in_group < a.per_group;
     const int c = group * a.per_group + min(in_group, a.per_group - 1);  // the lane's channel (those behind the group's last walk along with it and leave nothing)
-    const int stretch = PASS == WHOLE ? 0 : blockIdx.y, begin = PASS == WHOLE ? 0 : stretch * a.stretch, end = PASS == WHOLE ? q.count : min(q.count, begin + a.stretch);
+    constexpr bool ALL = PASS == WHOLE || PASS == MANY;
+    const int stretch = ALL ? 0 : blockIdx.y, begin = ALL ? 0 : stretch * a.stretch, end = ALL ? q.count : min(q.count, begin + a.stretch);
     if (begin >= end) return;
     const bool last = end == q.count;  // (of the ends nobody asks for the last one's)
     if (PASS == ENDS && last && stretch > 0) return;
@@ -691,6 +695,7 @@ static inline bool on(size_t size, std::initializer_list<const void *> ps) {
 struct ScanPlan {
     int stretch, n_stretch;       // rows of a stretch, stretches of the longest sequence; n_stretch 1: no stretches
     bool step;                    // one row a sequence
+    bool many;                    // whole sequences in many CTAs, or short ones
 };
 static int max_new_of(const b200_ssm_scan_args *a) {
     const int each = a->seq_info || a->n_seq <= 0 ? a->n_tokens : a->n_tokens / a->n_seq;
@@ -698,16 +703,17 @@ static int max_new_of(const b200_ssm_scan_args *a) {
 }
 static int lanes_of(int d_state) { return d_state <= 16 ? 1 : d_state <= 32 ? 2 : d_state <= 64 ? 4 : 8; }
 static ScanPlan plan_of(const b200_ssm_scan_args *a) {
-    ScanPlan p = {0, 1, false};
+    ScanPlan p = {0, 1, false, false};
     const int longest = max_new_of(a), block = SCAN_THREADS / lanes_of(a->d_state), per_group = a->channels / a->groups;
     p.step = longest <= 1;
     if (p.step) return p;
     // CTAs that are there on average while the longest sequence lasts
     const double ctas = (double)((per_group + block - 1) / block) * a->groups * a->n_tokens / longest;
+    p.many = longest <= SCAN_SHORT || ctas >= 3.0 * sm_count();
     if (ctas < 1.25 * sm_count() && longest >= 128) {
         // One sequence: as many CTAs as are there at once (4096 rows of 2048 channels: 96 us; twice as many: 120).  Several, whose ends come at different times: more than that (six of 37 to 1501 rows of
         // 5120 channels: 265 us with four an SM, 298 with two).
-        const double n = (double)(a->n_seq > 1 ? 4 : scan_ctas(lanes_of(a->d_state))) * sm_count() / ctas;
+        const double n = (double)(a->n_seq > 1 ? 4 : scan_ctas(lanes_of(a->d_state), ENDS)) * sm_count() / ctas;
         const int rows = (int)(longest / (n < 32 ? n : 32));
         p.stretch = ((rows < 64 ? 64 : rows) + 7) / 8 * 8;
         p.n_stretch = (longest + p.stretch - 1) / p.stretch;
@@ -722,13 +728,13 @@ static size_t scan_room(const b200_ssm_scan_args *a, const ScanPlan &p) {
 template <typename T, int L, int NS, int PASS>
 static int launch_scan(const ScanArgs &a, cudaStream_t st) {
     constexpr int CB = ScanSizes<L, NS>::CB;
-    const dim3 grid((unsigned)((a.per_group + CB - 1) / CB * (a.channels / a.per_group)), (unsigned)(PASS == WHOLE ? 1 : a.n_stretch), (unsigned)a.step.n_seq);
+    const dim3 grid((unsigned)((a.per_group + CB - 1) / CB * (a.channels / a.per_group)), (unsigned)(PASS == WHOLE || PASS == MANY ? 1 : a.n_stretch), (unsigned)a.step.n_seq);
     B200_CUDA_TRY(launch_chained(ssm_scan_kernel<T, L, NS, PASS>, grid, SCAN_THREADS, 0, st, a));
     return B200_OK;
 }
 template <typename T, int L, int NS>
 static int launch_scan_rows(const ScanArgs &a, const ScanPlan &p, cudaStream_t st) {
-    if (p.n_stretch < 2) return launch_scan<T, L, NS, WHOLE>(a, st);
+    if (p.n_stretch < 2) return L == 1 && p.many ? launch_scan<T, L, NS, L == 1 ? MANY : WHOLE>(a, st) : launch_scan<T, L, NS, WHOLE>(a, st);
     const int rc = launch_scan<T, L, NS, ENDS>(a, st);
     return rc != B200_OK ? rc : launch_scan<T, L, NS, ROWS>(a, st);
 }

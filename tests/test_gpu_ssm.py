@@ -258,6 +258,28 @@ def test_rows_and_slots_at_any_place(kind, shift, gap, slot_gap, count):
         s.verify()
 
 
+@pytest.mark.parametrize("kind,n,groups", [("f32", 16, 1), ("bf16", 7, 1), ("f16", 12, 2), ("bf16", 32, 1)])
+def test_many_sequences_of_some_length(kind, n, groups):
+    """More blocks of channels than an SM holds at once, sequences that end inside, at and behind a chunk of b and c."""
+    counts = [33, 70, 64, 65, 61, 40, 66, 63] * 7
+    s = Scan([(k, (i * 17) % 56, i % 5 == 0) for i, k in enumerate(counts)], 1300, n, kind, groups=groups, seed=n, gap=3)
+    a = s.upload()
+    a.max_new = max(counts)
+    run(a)
+    s.verify(a.max_new)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("shift,gap,slot_gap", [(0, 4, 0), (1, 0, 0), (0, 3, 2), (2, 6, 4), (4, 12, 1), (8, 24, 0)])
+def test_rows_at_any_place_in_few_longer_sequences(kind, shift, gap, slot_gap):
+    for gate, skip, bias, softplus in ((False, False, False, False), (True, True, True, True)):
+        s = Scan([(47, 1, False), (18, 0, True)], 72, 16, kind, gate=gate, skip=skip, bias=bias, softplus=softplus, shift=shift, gap=gap, slot_gap=slot_gap)
+        a = s.upload()
+        a.max_new = 47
+        run(a)
+        s.verify(47)
+
+
 @pytest.mark.parametrize("kind,n,channels,groups", [("f32", 16, 64, 1), ("bf16", 16, 100, 1), ("f32", 5, 33, 3), ("f16", 64, 64, 2), ("f32", 128, 24, 1)])
 def test_long_prompts_in_stretches(kind, n, channels, groups):
     """Few channels: sequences of several hundred rows are cut; their lengths end before, on and behind the cuts, and some have no second stretch."""
