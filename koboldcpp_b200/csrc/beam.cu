@@ -226,7 +226,7 @@ struct PickShared {
     Cand warps[PICK_WARPS];
     unsigned low[PICK_WARPS], high[PICK_WARPS];
     int piece[B200_BEAM_KEEP];      // where the successors are looked for
-    int n;
+    int n[2];                       // candidates of the pieces, of the successors: a count each, so that none is reset while a warp has still to read it
 };
 
 // The score of a logit of beam b.  With a reference of +inf the tokens of +inf share evenly, the others have none.
@@ -238,17 +238,17 @@ __device__ __forceinline__ double score_of(const PickShared &sh, int b, float x)
 
 // The `keep` first of the candidates that each(thread's function) names, in order, to sh.best; returns how many there are.  each(f) calls f(candidate) for all candidates of the calling
 // thread, whatever their order, and always for the same ones; `floor`: candidates with smaller scores can be left aside (at least `keep` have a score of that or more, or it is -inf).
-// (sh.n is 0 and everybody knows.)
+// (sh.n[phase] is 0 and everybody knows; no two calls share a phase.)
 template <typename F>
-__device__ __forceinline__ int first_of(PickShared &sh, int keep, double floor, F each) {
+__device__ __forceinline__ int first_of(PickShared &sh, int phase, int keep, double floor, F each) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     each([&](const Cand &c) {
         if (c.score == -(double)INFINITY || c.score < floor) return;
-        const int i = atomicAdd(&sh.n, 1);
+        const int i = atomicAdd(&sh.n[phase], 1);
         if (i < LIST) sh.list[i] = c;
     });
     __syncthreads();
-    const int n = sh.n;
+    const int n = sh.n[phase];  // (nothing changes it from here on)
     if (n <= LIST) {
         // a candidate's rank is the number of those before it: the list's own order, which is that of arrival, does not matter
         for (int i = tid; i < n; i += PICK_THREADS) {
@@ -278,7 +278,6 @@ __device__ __forceinline__ int first_of(PickShared &sh, int keep, double floor, 
             __syncthreads();
         }
     }
-    if (tid == 0) sh.n = 0;
     __syncthreads();
     return min(n, keep);
 }
@@ -294,7 +293,7 @@ __global__ void __launch_bounds__(PICK_THREADS) beam_pick_kernel(const SelectArg
     for (int i = tid; i < total; i += PICK_THREADS) cp_async4(&tops[i], a.tops + r0 * a.n_pieces + i);
     cp_async_commit();
     // ===== the logarithms of the sums, a warp a beam
-    if (tid == 0) sh.n = 0;
+    if (tid < 2) sh.n[tid] = 0;
     for (int b = warp; b < a.beams; b += PICK_WARPS) {
         const double *sums = a.sums + (r0 + b) * a.n_shares;
         const float *refs = a.refs + (r0 + b) * a.n_shares;
@@ -349,7 +348,7 @@ __global__ void __launch_bounds__(PICK_THREADS) beam_pick_kernel(const SelectArg
             floor = (double)unordered(low);
         }
     }
-    const int n_best = first_of(sh, a.keep, floor, pieces);
+    const int n_best = first_of(sh, 0, a.keep, floor, pieces);
     // ===== the successors in those pieces, a warp a piece
     for (int k = tid; k < n_best; k += PICK_THREADS) sh.piece[k] = (int)sh.best[k].at;
     floor = n_best == a.keep ? sh.best[a.keep - 1].score : -(double)INFINITY;
@@ -379,7 +378,7 @@ __global__ void __launch_bounds__(PICK_THREADS) beam_pick_kernel(const SelectArg
             }
         }
     };
-    const int n = first_of(sh, a.keep, floor, successors);
+    const int n = first_of(sh, 1, a.keep, floor, successors);
     for (int i = tid; i < a.keep; i += PICK_THREADS) {
         const int64_t to = (int64_t)blockIdx.x * a.keep + i;
         const bool there = i < n;
