@@ -218,7 +218,7 @@ __device__ __forceinline__ unsigned ordered(float f) {
 __device__ __forceinline__ float unordered(unsigned u) { return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
 
 struct PickShared {
-    double base[B200_BEAM_MAX];     // a beam's score; -inf: no successors
+    double base[B200_BEAM_MAX];     // a beam's score (base_of)
     double ref[B200_BEAM_MAX], norm[B200_BEAM_MAX];  // what is taken off its logits, one after the other
     int ended[B200_BEAM_MAX];
     Cand list[LIST];
@@ -229,6 +229,11 @@ struct PickShared {
     int n[2];                       // candidates of the pieces, of the successors: a count each, so that none is reset while a warp has still to read it
 };
 
+// A beam's score as its successors have it; ref: its row's largest logit.  -inf: it has none.  +inf counts as the largest number of 64 bits, which is +inf again once it is rounded to f32: beside a
+// logit of +inf it would make sums that are no numbers, and these have no rank.
+__device__ __forceinline__ double base_of(float s, bool ended, float ref) {
+    return s != s || (!ended && ref == NEG_INF) ? -(double)INFINITY : s == INFINITY ? 0x1.fffffffffffffp1023 : (double)s;
+}
 // The score of a logit of beam b.  With a reference of +inf the tokens of +inf share evenly, the others have none.
 __device__ __forceinline__ double score_of(const PickShared &sh, int b, float x) {
     if (x == NEG_INF || sh.base[b] == -(double)INFINITY) return -(double)INFINITY;
@@ -307,7 +312,7 @@ __global__ void __launch_bounds__(PICK_THREADS) beam_pick_kernel(const SelectArg
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
         if (lane == 0) {
-            sh.base[b] = s != s || (!ended && ref == NEG_INF) ? -(double)INFINITY : (double)s;  // (of a beam whose row was not read ref and sum are anything, and its score -inf)
+            sh.base[b] = base_of(s, ended, ref);  // (of a beam whose row was not read ref and sum are anything, and its score -inf)
             sh.ref[b] = (double)ref;
             sh.norm[b] = log(all);
             sh.ended[b] = ended;

@@ -104,3 +104,33 @@ def program(tmp_path_factory):
 def test_all_warps_see_the_same_candidates(program, n, keep, first):
     r = subprocess.run([str(program), str(n), str(keep), str(first)], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0, f"{r.stdout.strip()} threads had something else"
+
+
+SCORE = r"""
+int main() {
+    int wrong = 0;
+    auto expect = [&](float base, double ref, double norm, float x, float want) {
+        sh.base[0] = base_of(base, false, (float)ref); sh.ref[0] = ref; sh.norm[0] = norm;
+        const float got = (float)score_of(sh, 0, x);
+        if (!(got == want)) { printf("base %g ref %g norm %g logit %g: %g, not %g\n", base, ref, norm, x, got, want); wrong++; }
+    };
+    const float inf = INFINITY;
+    for (float base : {-2.5f, 0.0f, inf, -inf, 3.4028234e38f}) for (double ref : {0.0, 3.0, -7.0, (double)inf}) for (float x : {-INFINITY, -3.4028234e38f, -1.0f, 0.0f, 2.0f, 3.4028234e38f, INFINITY}) {
+        if (x > ref) continue;  // (the reference is the largest logit, rounded up)
+        const bool none = base == -inf || x == -INFINITY || (ref == inf && x < inf);
+        expect(base, ref, 0.5, x, none ? -inf : (float)(x == INFINITY ? base - 0.5 : base + (((double)x - ref) - 0.5)));
+    }
+    if (base_of(NAN, false, 0.f) != -inf || base_of(1.f, false, -inf) != -inf || base_of(1.f, true, -inf) != 1.0 || base_of(-inf, true, 0.f) != -inf) wrong++;
+    return wrong != 0;
+}
+"""
+
+
+def test_scores_are_never_no_numbers(tmp_path):
+    """Beams whose score is +inf beside logits of +inf: the other tokens are none.  (A candidate that is no number would have no rank, and leave a place that nobody writes.)"""
+    text = SOURCE.read_text()
+    (tmp_path / "score.cpp").write_text(HOST + part(text, "struct Cand {", "template <typename F>\n__device__ __forceinline__ int first_of") +
+                                        "static PickShared sh;\n" + SCORE)
+    subprocess.run(["g++", "-std=c++20", "-O1", "-pthread", str(tmp_path / "score.cpp"), "-o", str(tmp_path / "score")], check=True)
+    r = subprocess.run([str(tmp_path / "score")], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout
