@@ -543,9 +543,15 @@ int b200_op_beam_select(const b200_beam_select_args *a, void *workspace, size_t 
     const size_t size = a->type == B200_TYPE_F32 ? 4 : 2;
     OPX_REQUIRE((uintptr_t)a->logits % size == 0 && (((uintptr_t)a->score | (uintptr_t)a->ended | (uintptr_t)a->slot | (uintptr_t)a->to_score | (uintptr_t)a->to_beam | (uintptr_t)a->to_token |
                 (uintptr_t)a->to_slot) & 3) == 0, B200_ERR_INVALID, "%s: a pointer is not aligned to its type", who);
-    OPX_REQUIRE((const void *)a->to_score != a->score && (!a->slot || a->to_slot != a->slot), B200_ERR_INVALID, "%s: not in place", who);
     const SelectPlan p = select_plan(a);
     const size_t need = select_room(a, p), rows = (size_t)a->n_requests * a->n_beams;
+    // (a request's results are written while others' inputs are still read)
+    for (const void *in : {(const void *)a->score, (const void *)a->ended, (const void *)a->slot}) {
+        for (const void *out : {(const void *)a->to_score, (const void *)a->to_beam, (const void *)a->to_token, (const void *)a->to_slot}) {
+            const uintptr_t i = (uintptr_t)in, o = (uintptr_t)out;
+            OPX_REQUIRE(!in || !out || i + 4 * rows <= o || o + 4 * (size_t)a->n_requests * a->n_keep <= i, B200_ERR_INVALID, "%s: not in place", who);
+        }
+    }
     OPX_REQUIRE(workspace && workspace_bytes >= need && (uintptr_t)workspace % 8 == 0, B200_ERR_INVALID, "%s: workspace of %zu bytes, 8-byte aligned", who, need);
     double *sums = (double *)workspace;
     float *refs = (float *)(sums + rows * p.n_shares);
