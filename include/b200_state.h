@@ -21,6 +21,8 @@
 extern "C" {
 #endif
 
+#define B200_STATE_MAX_INDEX (1 << 30) /* rows of a step, channels: no more (B200_ERR_UNSUPPORTED) */
+
 /* Short causal convolution, every channel by itself: y[t][c] = act(bias[c] + sum_j w[c][j] * x[t - taps + 1 + j][c]), zeros in front of a sequence; act is silu or nothing.
  * The last taps - 1 inputs of a sequence wait in its slot of `tail` for its next rows.  dst is other memory than x.  (b200_op_short_conv has its bias in front and rows of f32.) */
 typedef struct {

@@ -756,10 +756,11 @@ static int launch_scan_type(const ScanArgs &a, const ScanPlan &p, bool states16,
     return launch_scan_rows<T, 8, 16>(a, p, st);
 }
 
-static int check_step(const int32_t *seq_info, int32_t n_seq, int32_t n_slots, int32_t n_tokens, int32_t max_new, int32_t type, const char *who) {
+static int check_step(const int32_t *seq_info, int32_t n_seq, int32_t n_slots, int32_t n_tokens, int32_t max_new, int32_t channels, int32_t type, const char *who) {
     OPX_REQUIRE(type_ok(type), B200_ERR_UNSUPPORTED, "%s: rows of type %d", who, type);
     OPX_REQUIRE(n_seq >= 0 && n_seq <= 65535 && n_slots >= 0 && n_tokens >= 0 && max_new >= 0, B200_ERR_INVALID, "%s: %d sequences, %d slots, %d rows, %d new ones at most", who, n_seq, n_slots,
                 n_tokens, max_new);
+    OPX_REQUIRE(n_tokens <= B200_STATE_MAX_INDEX && channels <= B200_STATE_MAX_INDEX, B200_ERR_UNSUPPORTED, "%s: %d rows of %d channels, %d of either at most", who, n_tokens, channels, B200_STATE_MAX_INDEX);
     OPX_REQUIRE((uintptr_t)seq_info % 4 == 0, B200_ERR_INVALID, "%s: seq_info at an odd place", who);
     OPX_REQUIRE(seq_info || (n_seq <= n_slots && (n_seq == 0 ? n_tokens == 0 : n_tokens % n_seq == 0)), B200_ERR_INVALID, "%s: without seq_info, %d rows are not %d sequences of one length in %d slots",
                 who, n_tokens, n_seq, n_slots);
@@ -769,7 +770,7 @@ static int check_step(const int32_t *seq_info, int32_t n_seq, int32_t n_slots, i
 int ssm_scan_check(const b200_ssm_scan_args *a) {
     const char *who = "b200_op_ssm_scan";
     OPX_REQUIRE(a, B200_ERR_INVALID, "%s: NULL arguments", who);
-    const int rc = check_step(a->seq_info, a->n_seq, a->n_slots, a->n_tokens, a->max_new, a->type, who);
+    const int rc = check_step(a->seq_info, a->n_seq, a->n_slots, a->n_tokens, a->max_new, a->channels, a->type, who);
     if (rc != B200_OK) return rc;
     OPX_REQUIRE(a->channels > 0 && a->d_state > 0 && a->groups > 0 && a->channels % a->groups == 0, B200_ERR_INVALID, "%s: %d channels in %d groups, %d states", who, a->channels, a->groups, a->d_state);
     OPX_REQUIRE(a->d_state <= 128, B200_ERR_UNSUPPORTED, "%s: %d states a channel, 128 at most", who, a->d_state);
@@ -812,7 +813,7 @@ bool ssm_scan_nodes_ok(const b200_tensor *s, const b200_tensor *x, const b200_te
         if (seqs > 1 && t->nb[2] != t->nb[1] * (size_t)rows) return false;
     }
     return n >= 1 && n <= 128 && ch >= 1 && seqs >= 1 && seqs <= 65535 && rows >= 1 && s->ne[3] == 1 && x->ne[0] == ch && x->ne[2] == seqs && x->ne[3] == 1 && a->ne[0] == n && a->ne[1] == ch &&
-           a->ne[2] == 1 && a->ne[3] == 1 && dt->ne[0] == ch && dt->ne[1] == rows && dt->ne[2] == seqs && dt->ne[3] == 1 && rows * seqs <= 0x7fffffff && ch <= 0x7fffffff &&
+           a->ne[2] == 1 && a->ne[3] == 1 && dt->ne[0] == ch && dt->ne[1] == rows && dt->ne[2] == seqs && dt->ne[3] == 1 && rows <= B200_STATE_MAX_INDEX && rows * seqs <= B200_STATE_MAX_INDEX && ch <= B200_STATE_MAX_INDEX &&
            opx::nelements(dst) == opx::nelements(x) + opx::nelements(s);
 }
 namespace ssm {
@@ -835,7 +836,7 @@ extern "C" {
 int b200_op_ssm_conv(const b200_ssm_conv_args *a, b200_stream_t stream) {
     const char *who = "b200_op_ssm_conv";
     OPX_REQUIRE(a, B200_ERR_INVALID, "%s: NULL arguments", who);
-    const int rc = check_step(a->seq_info, a->n_seq, a->n_slots, a->n_tokens, a->max_new, a->type, who);
+    const int rc = check_step(a->seq_info, a->n_seq, a->n_slots, a->n_tokens, a->max_new, a->channels, a->type, who);
     if (rc != B200_OK) return rc;
     OPX_REQUIRE(a->channels > 0 && a->taps >= 1, B200_ERR_INVALID, "%s: %d channels, %d taps", who, a->channels, a->taps);
     OPX_REQUIRE(a->taps <= 16, B200_ERR_UNSUPPORTED, "%s: %d taps, 16 at most", who, a->taps);
@@ -857,7 +858,7 @@ int b200_op_ssm_conv(const b200_ssm_conv_args *a, b200_stream_t stream) {
 }
 
 size_t b200_ssm_scan_workspace_bytes(const b200_ssm_scan_args *a) {
-    if (!a || a->n_seq <= 0 || a->n_tokens <= 0 || a->channels <= 0 || a->groups <= 0 || a->channels % a->groups || a->d_state <= 0 || a->d_state > 128) return 0;
+    if (!a || a->n_seq <= 0 || a->n_tokens <= 0 || a->n_tokens > B200_STATE_MAX_INDEX || a->channels <= 0 || a->channels > B200_STATE_MAX_INDEX || a->groups <= 0 || a->channels % a->groups || a->d_state <= 0 || a->d_state > 128) return 0;
     return scan_room(a, plan_of(a));
 }
 
@@ -913,7 +914,7 @@ int b200_op_ssm_conv_nodes(const b200_tensor *sx, const b200_tensor *c, const b2
 
 size_t b200_op_ssm_scan_nodes_workspace_bytes(const b200_tensor *s, const b200_tensor *x) {
     b200_ssm_scan_args a = {};
-    if (!s || !x) return 0;
+    if (!s || !x || s->ne[1] > B200_STATE_MAX_INDEX || s->ne[2] > 65535 || x->ne[1] > B200_STATE_MAX_INDEX || x->ne[1] * s->ne[2] > B200_STATE_MAX_INDEX) return 0;
     scan_node_sizes(s, x, &a);
     return b200_ssm_scan_workspace_bytes(&a);
 }
