@@ -435,6 +435,7 @@ static int launch_select(const SelectArgs &a, int rows, bool wide, cudaStream_t 
 // A CTA takes the same bytes of all slots that move, a column: it reads them all into shared memory before it writes any, so nothing is overwritten that is still wanted, whatever cycles
 // the moves make.  Columns do not touch one another.
 constexpr int REORDER_THREADS = 256, REORDER_STATES = 128, COLUMNS_BYTES = 32 * 1024;
+constexpr int64_t MOST_COLUMNS = 0x7fffffff - 0x10000;  // of a launch: a CTA's next column is one grid further, and grids are below 2^16
 constexpr int REORDER_MOST = COLUMNS_BYTES + 4 * (B200_STATE_MAX_SLOTS + 2 * B200_STATE_MAX_MOVES);
 struct ReorderArgs {
     char *base[REORDER_STATES];
@@ -586,7 +587,7 @@ int b200_op_state_reorder(const b200_slot_state *states, int32_t n_states, const
     do {  // (without states too: refused moves are counted)
         ReorderArgs r = {};
         int64_t columns = 0;
-        while (at < n_states && r.n_states < REORDER_STATES && columns + (states[at].bytes + width - 1) / width <= 0x7fffffff) {
+        while (at < n_states && r.n_states < REORDER_STATES && columns + (states[at].bytes + width - 1) / width <= MOST_COLUMNS) {
             const b200_slot_state &s = states[at++];
             r.base[r.n_states] = (char *)s.base;
             r.stride[r.n_states] = s.stride;

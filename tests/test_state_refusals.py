@@ -4,7 +4,7 @@ import ctypes as C
 import pytest
 
 import koboldcpp_b200.lib as L
-from koboldcpp_b200.lib import Tensor, lib
+from koboldcpp_b200.lib import SlotState, Tensor, lib
 from test_state_host import AT, INVALID, UNSUPPORTED, conv_args, scan_args, select_args
 
 HERE = 1 << 20  # results, far from everything else
@@ -41,3 +41,11 @@ def test_nodes_of_more_rows_than_an_index_reaches():
     t = [C.byref(Tensor.contiguous(AT, L.F32, shapes[k])) for k in shapes]
     assert lib().b200_op_ssm_scan_nodes_workspace_bytes(t[0], t[1]) == 0
     assert lib().b200_op_ssm_scan_nodes(*t, AT, 1 << 62, None) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("n,width", [(1, 4096), (8, 4096), (9, 2048), (1024, 32)])
+def test_slots_of_more_columns_than_a_launch_counts(n, width):
+    """CTAs go through the columns in steps of the grid, which is below 2^16."""
+    for columns in ((1 << 31) - 100, (1 << 31) - (1 << 16)):
+        s = (SlotState * 1)(SlotState(AT, 1 << 62, width * columns))
+        assert lib().b200_op_state_reorder(s, 1, AT, AT, n, 4, None, None) == UNSUPPORTED
