@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(REORDER_THREADS, 8) state_reorder_kernel(const
         }
     }
     __syncthreads();
-    if (a.refused && blockIdx.x == 0 && tid == 0 && n_refused) *a.refused += n_refused;
+    if (a.refused && blockIdx.x == 0 && tid == 0 && n_refused) atomicAdd(a.refused, n_refused);  // (calls on other streams may raise the same number)
     const int n = n_moves;
     if (n == 0) return;
     for (int item = blockIdx.x; item < a.first[a.n_states]; item += gridDim.x) {
