@@ -926,8 +926,9 @@ int b200_op_ssm_scan_nodes(const b200_tensor *s, const b200_tensor *x, const b20
     b200_ssm_scan_args n = {};
     scan_node_sizes(s, x, &n);
     n.x = x->data; n.dt = dt->data; n.x_stride = n.dt_stride = n.dst_stride = n.channels;
-    n.b = b->data; n.b_stride = (int64_t)(b->nb[1] / 4);
-    n.c = c->data; n.c_stride = (int64_t)(c->nb[1] / 4);
+    const bool one = n.n_tokens == 1;  // (what a single row's stride says is nothing to go by)
+    n.b = b->data; n.b_stride = one ? n.d_state : (int64_t)(b->nb[1] / 4);
+    n.c = c->data; n.c_stride = one ? n.d_state : (int64_t)(c->nb[1] / 4);
     n.a = (const float *)a->data;
     n.from = (const float *)s->data;
     n.dst = dst->data;
