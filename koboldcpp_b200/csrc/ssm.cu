@@ -366,9 +366,16 @@ __global__ void __launch_bounds__(32 * STEP_WARPS) ssm_step_kernel(const ScanArg
             const Two dd = two(dc, dc), xx = two(dxc, dxc);
             const float2 e0 = each(mul2(dd, two(rate[u].x, rate[u].y))), e1 = each(mul2(dd, two(rate[u].z, rate[u].w)));
             const Two s0 = fma2(two(ex2(e0.x), ex2(e0.y)), two(h[u].x, h[u].y), mul2(xx, two(b.x, b.y))), s1 = fma2(two(ex2(e1.x), ex2(e1.y)), two(h[u].z, h[u].w), mul2(xx, two(b.z, b.w)));
-            const float2 v0 = each(s0), v1 = each(s1), y = each(fma2(two(cc.x, cc.y), s0, mul2(two(cc.z, cc.w), s1)));
+            float2 v0 = each(s0), v1 = each(s1);
             if (left > 31 || G * (i0 + u) + g < left) store_states<VEC>(state + (i0 + u) * step, 4 * p, a.d_state, make_float4(v0.x, v0.y, v1.x, v1.y));
-            sum[i0 + u] = y.x + y.y;
+            // numbers behind d_state are no part of the sum (0 times an infinite d x is no number)
+            if constexpr (!VEC) {
+                if (4 * p + 1 >= a.d_state) v0.y = 0.f;
+                if (4 * p + 2 >= a.d_state) v1.x = 0.f;
+                if (4 * p + 3 >= a.d_state) v1.y = 0.f;
+            }
+            const float2 y = each(fma2(two(cc.x, cc.y), two(v0.x, v0.y), mul2(two(cc.z, cc.w), two(v1.x, v1.y))));
+            sum[i0 + u] = 4 * p < a.d_state ? y.x + y.y : 0.f;
         }
         if (i0 + U < L) load(i0 + U);
     }
@@ -413,7 +420,9 @@ struct ScanSizes {
 constexpr int SCAN_SHORT = 32;  // rows up to which sequences take the second way whatever the number of CTAs
 constexpr int scan_rows(int lanes, int pass) { return lanes > 1 ? 8 : pass == MANY ? 4 : 16; }
 constexpr int scan_ctas(int lanes, int pass) { return lanes > 1 || pass == MANY ? 4 : 2; }
-template <typename T, int L, int NS, int PASS>
+// PADS: lanes have numbers behind d_state, which results must not see.  (Kernels of their own: the second way through a group of rows that this takes would make the others 2 to 7 % longer, one prompt of
+// 4096 rows of 2048 channels and 16 states 101 -> 107 us; with 9 to 14 states it is 2 to 5 % longer than without, with 5 states 10 %.)
+template <typename T, int L, int NS, int PASS, bool PADS>
 __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L, PASS)) ssm_scan_kernel(const ScanArgs a) {
     using Z = ScanSizes<L, NS>;
     constexpr int CB = Z::CB, NP = Z::NP, TC = Z::TC, NQ = NS / 4, TG = scan_rows(L, PASS), MT = TG / L;  // TG: rows of a group; MT: those that a lane makes ready
@@ -526,6 +535,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L, PASS)) ssm_scan_ker
                 s.z = fmaf(ex2(d * r.z), s.z, e.z);
                 s.w = fmaf(ex2(d * r.w), s.w, e.w);
             }
+            // (numbers behind d_state: 0 times what an infinite sum of d makes of them is none)
+            if (PADS && n + 3 >= N) s = make_float4(n < N ? s.x : 0.f, n + 1 < N ? s.y : 0.f, n + 2 < N ? s.z : 0.f, 0.f);
         }
         rate[2 * i] = two(r.x, r.y); rate[2 * i + 1] = two(r.z, r.w);
         h[2 * i] = two(s.x, s.y); h[2 * i + 1] = two(s.z, s.w);
@@ -578,17 +589,17 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L, PASS)) ssm_scan_ker
                 dxs[t] = L == 1 ? dx[t / L] : __shfl_sync(0xffffffffu, dx[t / L], lane - p + t % L);
             }
             float y[TG];
-#pragma unroll
-            for (int t = 0; t < TG; t++) {
+            auto walk = [&](int t, float d_row, float dx_row, auto whole) {  // row t of the group; whole: numbers behind d_state are treated as all others
                 const ulonglong2 *b2 = reinterpret_cast<const ulonglong2 *>(&sbc[buf][0][tg + t][4 * p]), *c2 = reinterpret_cast<const ulonglong2 *>(&sbc[buf][1][tg + t][4 * p]);
-                const Two dd = two(ds[t], ds[t]), xx = two(dxs[t], dxs[t]);
                 Two sum = 0;
 #pragma unroll
                 for (int i = 0; i < NQ; i++) {
                     const ulonglong2 bv = b2[i * L];
-                    const float2 e0 = each(mul2(dd, rate[2 * i])), e1 = each(mul2(dd, rate[2 * i + 1]));
-                    h[2 * i] = fma2(two(ex2(e0.x), ex2(e0.y)), h[2 * i], mul2(xx, bv.x));
-                    h[2 * i + 1] = fma2(two(ex2(e1.x), ex2(e1.y)), h[2 * i + 1], mul2(xx, bv.y));
+                    const int n = 4 * (i * L + p);
+                    auto pair = [&](float v, int k) { return whole ? two(v, v) : two(n + k < N ? v : 0.f, n + k + 1 < N ? v : 0.f); };
+                    const float2 e0 = each(mul2(pair(d_row, 0), rate[2 * i])), e1 = each(mul2(pair(d_row, 2), rate[2 * i + 1]));
+                    h[2 * i] = fma2(two(ex2(e0.x), ex2(e0.y)), h[2 * i], mul2(pair(dx_row, 0), bv.x));
+                    h[2 * i + 1] = fma2(two(ex2(e1.x), ex2(e1.y)), h[2 * i + 1], mul2(pair(dx_row, 2), bv.y));
                     if (PASS != ENDS) {
                         const ulonglong2 cv = c2[i * L];
                         sum = i == 0 ? mul2(cv.x, h[0]) : fma2(cv.x, h[2 * i], sum);
@@ -596,7 +607,28 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L, PASS)) ssm_scan_ker
                     }
                 }
                 const float2 s = each(sum);
-                y[t] = s.x + s.y;
+                return s.x + s.y;
+            };
+            bool odd = false;  // the group has a row that the states behind d_state must not see: an infinite d x times their b of 0 is no number
+            if constexpr (PADS) {
+                float most = 0.f;
+#pragma unroll
+                for (int t = 0; t < TG; t++) most = fmaxf(most, fabsf(dxs[t]));
+                odd = most == INFINITY;
+            }
+            if (!PADS || !odd) {
+#pragma unroll
+                for (int t = 0; t < TG; t++) y[t] = walk(t, ds[t], dxs[t], std::true_type{});
+            } else if constexpr (PADS) {
+#pragma unroll 1
+                for (int t = 0; t < TG; t++) {
+                    float d_row = 0.f, dx_row = 0.f;
+#pragma unroll
+                    for (int k = 0; k < TG; k++) if (k == t) { d_row = ds[k]; dx_row = dxs[k]; }
+                    const float v = walk(t, d_row, dx_row, std::false_type{});
+#pragma unroll
+                    for (int k = 0; k < TG; k++) if (k == t) y[k] = v;
+                }
             }
             if (PASS == ENDS) continue;
             // sums over the channel's lanes: lane p ends up with the rows p, p + L, ..
@@ -729,7 +761,8 @@ template <typename T, int L, int NS, int PASS>
 static int launch_scan(const ScanArgs &a, cudaStream_t st) {
     constexpr int CB = ScanSizes<L, NS>::CB;
     const dim3 grid((unsigned)((a.per_group + CB - 1) / CB * (a.channels / a.per_group)), (unsigned)(PASS == WHOLE || PASS == MANY ? 1 : a.n_stretch), (unsigned)a.step.n_seq);
-    B200_CUDA_TRY(launch_chained(ssm_scan_kernel<T, L, NS, PASS>, grid, SCAN_THREADS, 0, st, a));
+    const bool pads = PASS != ENDS && a.d_state < NS * L;  // (the ends of stretches are stored without them)
+    B200_CUDA_TRY(launch_chained(pads ? ssm_scan_kernel<T, L, NS, PASS, PASS != ENDS> : ssm_scan_kernel<T, L, NS, PASS, false>, grid, SCAN_THREADS, 0, st, a));
     return B200_OK;
 }
 template <typename T, int L, int NS>

@@ -1,0 +1,65 @@
+"""Scans on the GPU over values at the ends of their range: what is infinite by the definition is infinite, with its sign, and what is finite stays so."""
+import numpy as np
+import pytest
+
+from test_gpu_ssm import Scan, run
+
+pytestmark = pytest.mark.gpu
+
+
+def defined(s):
+    """dst and states by the definition, row by row in 64 bits: infinities and NaN as arithmetic makes them."""
+    of = np.arange(s.ch) // (s.ch // s.groups)
+    dst, state = s.dst.copy(), s.state.copy()
+    with np.errstate(all="ignore"):
+        for first, count, slot, begins in s.info.T.tolist():
+            h = np.zeros_like(state[slot]) if begins else state[slot].copy()
+            for t in range(first, first + count):
+                d = s.dt[t] + (0 if s.bias is None else s.bias)
+                if s.softplus:
+                    d = np.maximum(d, 0) + np.log1p(np.exp(-np.abs(d)))
+                h = np.exp(d[:, None] * s.a) * h + (d * s.x[t])[:, None] * s.b[t].reshape(s.groups, s.n)[of]
+                y = (h * s.c[t].reshape(s.groups, s.n)[of]).sum(1)
+                if s.skip is not None:
+                    y = y + s.skip * s.x[t]
+                dst[t] = y if s.z is None else y * (s.z[t] / (1 + np.exp(-s.z[t])))
+            if count:
+                state[slot] = h
+    return dst, state
+
+
+def kinds(v):
+    return np.where(np.isnan(v), 3, np.where(np.isposinf(v), 1, np.where(np.isneginf(v), 2, 0)))
+
+
+def same_kinds(s):
+    want, state = defined(s)
+    got, got_state = s.d["dst"].get(), s.d_state.get().reshape(state.shape)
+    for g, w in ((got, want), (got_state, state)):
+        off = kinds(g) != kinds(w)
+        assert not off.any(), (int(off.sum()), np.argwhere(off)[:5].tolist(), g[off][:5].tolist(), w[off][:5].tolist())
+    return got, want, got_state, state
+
+
+SIZES = [1, 3, 4, 5, 7, 8, 11, 13, 16, 20, 29, 32, 41, 64, 67, 100, 127, 128]
+
+
+@pytest.mark.parametrize("n", SIZES)
+@pytest.mark.parametrize("count", [1, 5, 40, 300])
+def test_infinities_whatever_the_number_of_states(n, count):
+    """Inputs and steps that are infinite, where all states of the channel go the same way: the result is infinite with a sign, not no number, also where d_state fills no register."""
+    for gate, skip in ((False, False), (True, True)):
+        s = Scan([(count, 1, False), (count, 0, True)], 40, n, "f32", gate=gate, skip=skip, seed=n, slow=True)
+        s.b, s.c, s.state = np.abs(s.b) + 0.125, np.abs(s.c) + 0.125, np.abs(s.state)
+        s.x[:, 30:] = np.abs(s.x[:, 30:]) + 0.125
+        if gate:
+            s.z = np.abs(s.z) + 0.125
+            s.skip = np.abs(s.skip)
+        t = count // 2
+        s.x[t, 3], s.x[count + t, 5], s.x[t, 7] = np.inf, np.inf, -np.inf
+        s.dt[t, 31], s.dt[count + t, 32] = np.inf, np.inf
+        a = s.upload()
+        a.max_new = count
+        run(a)
+        got = same_kinds(s)[0]
+        assert np.isposinf(got[t:count, 3]).all() and np.isposinf(got[count + t:, 5]).all() and np.isneginf(got[t:count, 7]).all() and np.isposinf(got[t:count, 31]).all()
