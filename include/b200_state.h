@@ -40,7 +40,8 @@ B200_API int b200_op_ssm_conv(const b200_ssm_conv_args *a, b200_stream_t stream)
 /* Selective state space scan: per channel a state of d_state numbers,
  *   d = dt[t][c] + dt_bias[c], softplus != 0: d = ln(1 + e^d);   h[c][n] <- exp(d * a[c][n]) * h[c][n] + d * x[t][c] * b[t][g][n];
  *   y = sum_n c[t][g][n] * h[c][n] + skip[c] * x[t][c];   dst[t][c] = y, or y * silu(z[t][c]) with z,
- * where channel c belongs to group g = c / (channels / groups).  Everything between the rows is f32.  `from` (optional): states are read there, in slots of from_stride, instead of
+ * where channel c belongs to group g = c / (channels / groups).  Everything between the rows is f32.  Rates
+ * a of -inf and +inf count as the largest numbers of f32: a row with d = 0 leaves the state as it is.  `from` (optional): states are read there, in slots of from_stride, instead of
  * from `state` (other memory than that).  Few channels and a long sequence: the rows are shared out in stretches, whose states meet in the workspace (b200_ssm_scan_workspace_bytes bytes, 16-byte
  * aligned, 0: none). */
 typedef struct {

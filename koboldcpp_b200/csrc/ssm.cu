@@ -267,6 +267,14 @@ __device__ __forceinline__ float2 softplus2(float2 x) {
 }
 __device__ __forceinline__ float softplus(float x) { return softplus2(make_float2(x, x)).x; }
 
+// Rates of -inf and +inf count as the largest numbers of f32, so that a row with d = 0 (and those behind a sequence's last, which are walked as such) leaves their states as they are.  NaN stays.
+__device__ __forceinline__ float finite(float x) {
+    float r;
+    asm("max.NaN.f32 %0, %1, 0fFF7FFFFF;" : "=f"(r) : "f"(x));
+    asm("min.NaN.f32 %0, %0, 0f7F7FFFFF;" : "+f"(r));
+    return r;
+}
+
 // Four neighbouring states of a channel; numbers behind d_state count as zeros
 template <bool VEC>
 __device__ __forceinline__ float4 load_states(const float *row, int n0, int d_state) {
@@ -364,7 +372,7 @@ __global__ void __launch_bounds__(32 * STEP_WARPS) ssm_step_kernel(const ScanArg
             }
             const float dc = __shfl_sync(0xffffffffu, d, g * L + i0 + u), dxc = __shfl_sync(0xffffffffu, dx, g * L + i0 + u);
             const Two dd = two(dc, dc), xx = two(dxc, dxc);
-            const float2 e0 = each(mul2(dd, two(rate[u].x, rate[u].y))), e1 = each(mul2(dd, two(rate[u].z, rate[u].w)));
+            const float2 e0 = each(mul2(dd, two(finite(rate[u].x), finite(rate[u].y)))), e1 = each(mul2(dd, two(finite(rate[u].z), finite(rate[u].w))));
             const Two s0 = fma2(two(ex2(e0.x), ex2(e0.y)), two(h[u].x, h[u].y), mul2(xx, two(b.x, b.y))), s1 = fma2(two(ex2(e1.x), ex2(e1.y)), two(h[u].z, h[u].w), mul2(xx, two(b.z, b.w)));
             float2 v0 = each(s0), v1 = each(s1);
             if (left > 31 || G * (i0 + u) + g < left) store_states<VEC>(state + (i0 + u) * step, 4 * p, a.d_state, make_float4(v0.x, v0.y, v1.x, v1.y));
@@ -523,7 +531,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L, PASS)) ssm_scan_ker
             s = pieces ? load_states<true>(from, n, N) : load_states<false>(from, n, N);
         }
         if (PASS == ENDS && stretch == 0 && mine) store_end(ends - ends_row, n, s);
-        r.x *= LOG2E; r.y *= LOG2E; r.z *= LOG2E; r.w *= LOG2E;
+        r.x = finite(r.x * LOG2E); r.y = finite(r.y * LOG2E); r.z = finite(r.z * LOG2E); r.w = finite(r.w * LOG2E);
         if (PASS == ROWS) {
             s = load_end(ends - (stretch > 0 ? 0 : ends_row), n);
 #pragma unroll 4

@@ -63,3 +63,34 @@ def test_infinities_whatever_the_number_of_states(n, count):
         run(a)
         got = same_kinds(s)[0]
         assert np.isposinf(got[t:count, 3]).all() and np.isposinf(got[count + t:, 5]).all() and np.isneginf(got[t:count, 7]).all() and np.isposinf(got[t:count, 31]).all()
+
+
+@pytest.mark.parametrize("softplus", [True, False])
+@pytest.mark.parametrize("n", [5, 16, 40])
+@pytest.mark.parametrize("count", [1, 3, 18, 50, 300])
+def test_states_that_fade_at_once(n, count, softplus):
+    """a of -inf, as a type of fewer bits or an overflowing exponential leaves it: the state is what the last row put there, also where a group of rows ends behind the sequence's last."""
+    s = Scan([(count, 1, False), (count, 0, True)], 40, n, "f32", seed=n, softplus=softplus, slow=True)
+    s.a[3] = -np.inf
+    s.a[7, ::2] = -np.inf
+    s.a[9] = -3.4028234663852886e38
+    if not softplus:
+        s.dt, s.bias = np.abs(s.dt) + 2.0 ** -20, np.abs(s.bias)
+    a = s.upload()
+    a.max_new = count
+    run(a)
+    got, want, got_state, state = same_kinds(s)
+    assert np.isfinite(want).all() and np.allclose(got, want, rtol=1e-4, atol=1e-4) and np.allclose(got_state, state, rtol=1e-4, atol=1e-4)
+
+
+@pytest.mark.parametrize("n", [16, 40])
+@pytest.mark.parametrize("count", [1, 3, 18])
+def test_no_time_passes_with_a_step_of_nothing(n, count):
+    """d of 0 leaves every state as it is, whatever its rate: infinite rates count as the largest numbers of f32."""
+    s = Scan([(count, 1, False)], 40, n, "f32", seed=n, softplus=False, bias=False)
+    s.a[3], s.a[5] = -np.inf, np.inf
+    s.dt[:] = 0.0
+    a = s.upload()
+    a.max_new = count
+    run(a)
+    assert np.array_equal(s.d_state.get().reshape(s.state.shape), s.state)
