@@ -275,6 +275,14 @@ __device__ __forceinline__ float finite(float x) {
     return r;
 }
 
+// 2^(2 half) * s + e for two states.  In two steps, since a stretch over which states grow has a factor that f32 may not hold, and what it meets may be zero or small enough to stay in range.
+// (The bound keeps zeros what they are; a normal number is infinite behind it.)
+__device__ __forceinline__ Two carried(Two half, Two s, Two e) {
+    const float2 v = each(half);
+    const Two f = two(ex2(fminf(v.x, 127.f)), ex2(fminf(v.y, 127.f)));
+    return fma2(f, mul2(f, s), e);
+}
+
 // Four neighbouring states of a channel; numbers behind d_state count as zeros
 template <bool VEC>
 __device__ __forceinline__ float4 load_states(const float *row, int n0, int d_state) {
@@ -534,15 +542,15 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L, PASS)) ssm_scan_ker
         r.x = finite(r.x * LOG2E); r.y = finite(r.y * LOG2E); r.z = finite(r.z * LOG2E); r.w = finite(r.w * LOG2E);
         if (PASS == ROWS) {
             s = load_end(ends - (stretch > 0 ? 0 : ends_row), n);
+            Two lo = two(s.x, s.y), hi = two(s.z, s.w);
 #pragma unroll 4
             for (int j = 1; j < stretch; j++) {
                 const float4 e = load_end(ends + j * ends_row, n);
-                const float d = sums[(int64_t)j * a.channels];
-                s.x = fmaf(ex2(d * r.x), s.x, e.x);
-                s.y = fmaf(ex2(d * r.y), s.y, e.y);
-                s.z = fmaf(ex2(d * r.z), s.z, e.z);
-                s.w = fmaf(ex2(d * r.w), s.w, e.w);
+                const float d = 0.5f * sums[(int64_t)j * a.channels];
+                lo = carried(mul2(two(d, d), two(r.x, r.y)), lo, two(e.x, e.y));
+                hi = carried(mul2(two(d, d), two(r.z, r.w)), hi, two(e.z, e.w));
             }
+            s = make_float4(each(lo).x, each(lo).y, each(hi).x, each(hi).y);
             // (numbers behind d_state: 0 times what an infinite sum of d makes of them is none)
             if (PADS && n + 3 >= N) s = make_float4(n < N ? s.x : 0.f, n + 1 < N ? s.y : 0.f, n + 2 < N ? s.z : 0.f, 0.f);
         }

@@ -94,3 +94,28 @@ def test_no_time_passes_with_a_step_of_nothing(n, count):
     a.max_new = count
     run(a)
     assert np.array_equal(s.d_state.get().reshape(s.state.shape), s.state)
+
+
+@pytest.mark.parametrize("n", [5, 16, 40])
+@pytest.mark.parametrize("kind", ["nothing", "little"])
+def test_states_that_grow_beyond_a_stretch(n, kind):
+    """d below 0 (softplus off): a factor of more than f32 holds lies between the ends of two stretches; the states that it meets are zeros, or so small that they stay in range.
+    Per row 5 u of the state (an exponential 2^-22 + u, a product and an addition), the exponent's own rounding 2 u of 300 at most: 600 x 5 u + 600 u < 2^-12."""
+    s = Scan([(600, 0, False)], 40, n, "f32", softplus=False, bias=False, gate=False, skip=False, seed=n)
+    s.a = np.full_like(s.a, -1.0)
+    s.b, s.c = np.abs(s.b), np.abs(s.c)
+    s.x[:] = 0.0
+    if kind == "nothing":  # e^112 in 64 rows, of zeros
+        s.dt[:] = -0.25
+        s.dt[:, 5:9] = -1.75
+        s.state[:] = 0.0
+        s.x[560:, :] = -1.0  # (d is below 0: so are the products)
+    else:  # e^100 in the second 64 rows, of 1e-37
+        s.dt[:] = 0.0
+        s.dt[64:128] = -1.5625
+        s.state[:] = 1e-37
+    a = s.upload()
+    run(a)
+    got, want, got_state, state = same_kinds(s)
+    for g, w in ((got, want), (got_state, state)):
+        assert np.isfinite(w).all() and (np.abs(g - w) <= 2.0 ** -12 * np.abs(w)).all()
