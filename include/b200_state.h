@@ -43,7 +43,8 @@ B200_API int b200_op_ssm_conv(const b200_ssm_conv_args *a, b200_stream_t stream)
  * where channel c belongs to group g = c / (channels / groups).  Everything between the rows is f32.  Rates
  * a of -inf and +inf count as the largest numbers of f32: a row with d = 0 leaves the state as it is.  `from` (optional): states are read there, in slots of from_stride, instead of
  * from `state` (other memory than that).  Few channels and a long sequence: the rows are shared out in stretches, whose states meet in the workspace (b200_ssm_scan_workspace_bytes bytes, 16-byte
- * aligned, 0: none). */
+ * aligned, 0: none).  How many goes by how a step is cut, and a smaller step may need more than a larger one; B200_SSM_SCAN_WORKSPACE_MAX are enough for every step. */
+#define B200_SSM_SCAN_WORKSPACE_MAX (1 << 24)
 typedef struct {
     const void *x, *dt; int64_t x_stride, dt_stride;         /* [n_tokens][channels] */
     const void *b, *c; int64_t b_stride, c_stride;           /* [n_tokens][groups * d_state] */

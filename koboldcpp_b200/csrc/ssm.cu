@@ -245,9 +245,10 @@ struct ScanArgs {
     float *state; int64_t slot_stride;
     void *dst; int64_t dst_stride;
     int32_t channels, d_state, per_group, softplus, bc_pieces;  // bc_pieces: b and c can be read four numbers at a time
-    // stretches: rows of one, how many a sequence may have; where their end states and sums of d wait
+    // stretches: rows of one, how many a sequence may have; where end states and sums of d wait, and the states of sequences that are cut, which the last of their stretches overwrites.  A stretch's
+    // place is its first row / stretch: those that have a place are whole, so no two share one, and there are n_tokens / stretch of them whatever the number of sequences.
     int32_t stretch, n_stretch;
-    float *ends, *sums;
+    float *ends, *starts, *sums;
 };
 
 // ln(1 + e^x) = max(x, 0) + ln(1 + e^-|x|), and ln(1 + e) = e P(e) on [0, 1] with a polynomial whose relative error is smallest at its largest (fitted by weighted least squares on
@@ -452,8 +453,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L, PASS)) ssm_scan_ker
     constexpr bool ALL = PASS == WHOLE || PASS == MANY;
     const int stretch = ALL ? 0 : blockIdx.y, begin = ALL ? 0 : stretch * a.stretch, end = ALL ? q.count : min(q.count, begin + a.stretch);
     if (begin >= end) return;
-    const bool last = end == q.count;  // (of the ends nobody asks for the last one's)
-    if (PASS == ENDS && last && stretch > 0) return;
+    const bool last = end == q.count;
+    if (PASS == ENDS && last) return;  // (nobody asks for its end)
     const int64_t first = q.first + begin;
     const int rows = end - begin;
     const T *pb = (const T *)a.b + first * a.b_stride + (int64_t)group * N, *pc = (const T *)a.c + first * a.c_stride + (int64_t)group * N;
@@ -515,8 +516,9 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L, PASS)) ssm_scan_ker
     Two h[NS / 2], rate[NS / 2];
     double total = 0.0;  // (a stretch may be long: terms of one size would all be rounded the same way)
     const bool pieces = (N & 3) == 0 && ((a.slot_stride | a.from_stride) & 3) == 0 && (((uintptr_t)a.state | (uintptr_t)a.from | (uintptr_t)a.a) & 15) == 0;
-    // end states of a stretch lie as [d_state][channels], so that neighbouring lanes read neighbouring words; the stretch in front of a sequence's first is its state
+    // they lie as [d_state][channels], so that neighbouring lanes read neighbouring words
     const int64_t ends_row = (int64_t)a.channels * N;
+    const int place = ALL ? 0 : (int)(q.first / a.stretch);  // of the sequence's first stretch; the others' places follow it
     auto load_end = [&](const float *from, int n) {
         const float *q4 = from + (int64_t)n * a.channels;
         return make_float4(n < N ? q4[0] : 0.f, n + 1 < N ? q4[a.channels] : 0.f, n + 2 < N ? q4[2 * (int64_t)a.channels] : 0.f, n + 3 < N ? q4[3 * (int64_t)a.channels] : 0.f);
@@ -528,20 +530,20 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L, PASS)) ssm_scan_ker
         if (n + 2 < N) q4[2 * (int64_t)a.channels] = v.z;
         if (n + 3 < N) q4[3 * (int64_t)a.channels] = v.w;
     };
-    float *ends = a.ends + ((int64_t)blockIdx.z * (a.n_stretch + 1) + 1) * ends_row + c, *sums = a.sums + (int64_t)blockIdx.z * a.n_stretch * a.channels + c;
+    float *ends = a.ends + place * ends_row + c, *starts = a.starts + place * ends_row + c, *sums = a.sums + (int64_t)place * a.channels + c;
 #pragma unroll
     for (int i = 0; i < NQ; i++) {
         const int n = 4 * (i * L + p);  // (the channel's lanes side by side: their loads of b and c too)
         const float *pa = a.a + (int64_t)c * N;
         float4 r = pieces ? load_states<true>(pa, n, N) : load_states<false>(pa, n, N), s = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (PASS != ROWS && stretch == 0 && !q.begins) {
+        if (stretch == 0 && !q.begins && (PASS != ROWS || last)) {
             const float *from = a.from + (int64_t)q.slot * a.from_stride + (int64_t)c * N;
             s = pieces ? load_states<true>(from, n, N) : load_states<false>(from, n, N);
         }
-        if (PASS == ENDS && stretch == 0 && mine) store_end(ends - ends_row, n, s);
+        if (PASS == ENDS && stretch == 0 && mine) store_end(starts, n, s);
         r.x = finite(r.x * LOG2E); r.y = finite(r.y * LOG2E); r.z = finite(r.z * LOG2E); r.w = finite(r.w * LOG2E);
-        if (PASS == ROWS) {
-            s = load_end(ends - (stretch > 0 ? 0 : ends_row), n);
+        if (PASS == ROWS && !(stretch == 0 && last)) {
+            s = load_end(stretch > 0 ? ends : starts, n);
             Two lo = two(s.x, s.y), hi = two(s.z, s.w);
 #pragma unroll 4
             for (int j = 1; j < stretch; j++) {
@@ -557,7 +559,6 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L, PASS)) ssm_scan_ker
         rate[2 * i] = two(r.x, r.y); rate[2 * i + 1] = two(r.z, r.w);
         h[2 * i] = two(s.x, s.y); h[2 * i + 1] = two(s.z, s.w);
     }
-    if (PASS == ENDS && last) return;  // (a sequence of one stretch: its state is all that is wanted)
     keep(0, 0);
     __syncthreads();
     for (int r0 = 0, buf = 0; r0 < rows; r0 += TC, buf ^= 1) {
@@ -768,9 +769,10 @@ static ScanPlan plan_of(const b200_ssm_scan_args *a) {
     }
     return p;
 }
+// At most (4 SMs + blocks) / blocks places, of fewer than 1.25 SMs blocks of 128 / lanes channels: 13 MB.
+static size_t scan_places(const b200_ssm_scan_args *a, const ScanPlan &p) { return ((size_t)a->n_tokens + p.stretch - 1) / p.stretch; }
 static size_t scan_room(const b200_ssm_scan_args *a, const ScanPlan &p) {
-    if (p.n_stretch < 2) return 0;
-    return 4 * (size_t)a->n_seq * ((size_t)(p.n_stretch + 1) * a->channels * a->d_state + (size_t)p.n_stretch * a->channels);
+    return p.n_stretch < 2 ? 0 : 4 * scan_places(a, p) * a->channels * (2 * (size_t)a->d_state + 1);
 }
 
 template <typename T, int L, int NS, int PASS>
@@ -917,14 +919,16 @@ int b200_op_ssm_scan(const b200_ssm_scan_args *a, void *workspace, size_t worksp
     if (rc != B200_OK || a->n_seq == 0 || a->n_tokens == 0) return rc;
     const ScanPlan p = plan_of(a);
     const size_t need = scan_room(a, p);
+    OPX_REQUIRE(need <= B200_SSM_SCAN_WORKSPACE_MAX, B200_ERR_UNSUPPORTED, "%s: %zu bytes of workspace", who, need);  // (what the header promises)
     OPX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0), B200_ERR_INVALID, "%s: workspace of %zu bytes, 16-byte aligned", who, need);
     const int per_group = a->channels / a->groups, each = a->seq_info ? a->n_tokens : a->n_tokens / a->n_seq, longest = a->max_new > 0 && a->max_new < each ? a->max_new : each;
-    float *ends = (float *)workspace;
+    float *ends = need ? (float *)workspace : nullptr;
+    const size_t places = need ? scan_places(a, p) * a->channels * a->d_state : 0;
     const size_t four = 4 * type_size(a->type);
     const bool bc_pieces = on(four, {a->b, a->c}) && ((a->b_stride | a->c_stride | a->d_state) & 3) == 0;
     const ScanArgs s = {{a->seq_info, a->n_seq, a->n_slots, a->n_tokens, longest}, a->x, a->dt, a->b, a->c, a->z, a->x_stride, a->dt_stride, a->b_stride, a->c_stride, a->z_stride, a->a, a->dt_bias, a->d,
                         a->from ? a->from : a->state, a->from ? a->from_stride : a->slot_stride, a->state, a->slot_stride, a->dst, a->dst_stride, a->channels, a->d_state, per_group, a->softplus, bc_pieces,
-                        p.stretch, p.n_stretch, ends, ends ? ends + (size_t)a->n_seq * (p.n_stretch + 1) * a->channels * a->d_state : nullptr};
+                        p.stretch, p.n_stretch, ends, ends + places, ends + 2 * places};
     const bool states16 = (a->d_state & 3) == 0 && ((s.slot_stride | s.from_stride) & 3) == 0 && on(16, {s.state, s.from, a->a});
     const cudaStream_t st = (cudaStream_t)stream;
     if (a->type == B200_TYPE_F32) return launch_scan_type<float>(s, p, states16, st);

@@ -119,3 +119,24 @@ def test_states_that_grow_beyond_a_stretch(n, kind):
     got, want, got_state, state = same_kinds(s)
     for g, w in ((got, want), (got_state, state)):
         assert np.isfinite(w).all() and (np.abs(g - w) <= 2.0 ** -12 * np.abs(w)).all()
+
+
+@pytest.mark.parametrize("kind,n,groups", [("f32", 16, 1), ("bf16", 5, 3), ("f16", 64, 2)])
+@pytest.mark.parametrize("max_new", [0, 640])
+def test_single_rows_beside_prompts_in_stretches(kind, n, groups, max_new):
+    """As a server's step has them: single rows and prompts in any order, rows between them that nobody has, prompts that begin anywhere in a stretch and are a row longer or shorter than one."""
+    counts = [1, 640, 1, 1, 129, 1, 0, 128, 127, 1, 257, 1, 1, 64, 65, 1, 63]
+    rng = np.random.default_rng(n)
+    order = rng.permutation(len(counts))
+    first, at = np.zeros(len(counts), int), 3
+    for i in order:
+        first[i] = at
+        at += counts[i] + int(rng.integers(0, 3))
+    slots = rng.permutation(len(counts) + 2)[:len(counts)]
+    info = np.array([first, counts, slots, rng.integers(0, 2, len(counts))], np.int32)
+    s = Scan(info, 60, n, kind, groups=groups, seed=n, slow=True, slots=len(counts) + 2, tokens=at + 5)
+    a = s.upload()
+    a.max_new = max_new
+    ws = run(a)
+    assert ws.numel() > 16
+    s.verify(max_new)
