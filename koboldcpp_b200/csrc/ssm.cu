@@ -251,11 +251,22 @@ struct ScanArgs {
     float *ends, *starts, *sums;
 };
 
+// -|x|, and -128 below it (e^-128 is zero here; NaN stays)
+__device__ __forceinline__ float down(float x) {
+    float r;
+    asm("max.NaN.f32 %0, %1, 0fC3000000;" : "=f"(r) : "f"(-fabsf(x)));
+    return r;
+}
 // ln(1 + e^x) = max(x, 0) + ln(1 + e^-|x|), and ln(1 + e) = e P(e) on [0, 1] with a polynomial whose relative error is smallest at its largest (fitted by weighted least squares on
-// Chebyshev points; 1.8e-7 with the roundings of f32): one exponential on the special function unit and nothing else there, no overflow, no cancellation.
+// Chebyshev points; 1.8e-7 with the roundings of f32): one exponential on the special function unit and nothing else there, no overflow, no cancellation.  What the exponential's argument loses, its
+// rounding and what LOG2E has not of log2 e, is made good to first order: where e is small all of the result is e, and such steps are the usual ones of a trained layer.  (Relative error for x of
+// -12 .. -6: 2.6e-7 at most, 7.0e-8 root mean square, -5e-8 in the mean; without it 8.9e-7, 2.5e-7 and +7e-8, and more further out.  Four prompts of 2048 rows: 448 -> 456 us.)
 __device__ __forceinline__ float2 softplus2(float2 x) {
-    const Two e = two(ex2(-LOG2E * fabsf(x.x)), ex2(-LOG2E * fabsf(x.y)));
     auto both = [](float v) { return two(v, v); };
+    const Two far = two(down(x.x), down(x.y)), turn = mul2(far, both(LOG2E));
+    const float2 v = each(turn);
+    Two e = two(ex2(v.x), ex2(v.y));
+    e = fma2(e, fma2(turn, both(1.90465421e-9f), fma2(turn, both(-0x1.62e430p-1f), far)), e);
     Two p = both(0.0052326764f);
     p = fma2(p, e, both(-0.0295051672f));
     p = fma2(p, e, both(0.0782258362f));
@@ -266,7 +277,21 @@ __device__ __forceinline__ float2 softplus2(float2 x) {
     p = fma2(p, e, both(-0.499994934f));
     return each(fma2(fma2(p, e, both(1.0f)), e, two(fmaxf(x.x, 0.f), fmaxf(x.y, 0.f))));
 }
-__device__ __forceinline__ float softplus(float x) { return softplus2(make_float2(x, x)).x; }
+// .. of one value.  (Not as one of two: with that the compiler gives the kernel of single rows 64 registers and lets it ask for its states later, 25.5 -> 28.4 us for 96 rows of 8192 channels.)
+__device__ __forceinline__ float softplus(float x) {
+    const float far = down(x), turn = far * LOG2E;
+    float e = ex2(turn);
+    e = fmaf(e, fmaf(turn, 1.90465421e-9f, fmaf(turn, -0x1.62e430p-1f, far)), e);
+    float p = 0.0052326764f;
+    p = fmaf(p, e, -0.0295051672f);
+    p = fmaf(p, e, 0.0782258362f);
+    p = fmaf(p, e, -0.136632353f);
+    p = fmaf(p, e, 0.191060022f);
+    p = fmaf(p, e, -0.248429805f);
+    p = fmaf(p, e, 0.333190978f);
+    p = fmaf(p, e, -0.499994934f);
+    return fmaf(fmaf(p, e, 1.0f), e, fmaxf(x, 0.f));
+}
 
 // Rates of -inf and +inf count as the largest numbers of f32, so that a row with d = 0 (and those behind a sequence's last, which are walked as such) leaves their states as they are.  NaN stays.
 __device__ __forceinline__ float finite(float x) {
