@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 import torch
 
+import beam_check
 from koboldcpp_b200.lib import check, lib
 from test_gpu_beam import Select
 
@@ -38,3 +39,38 @@ def test_scores_and_logits_of_plus_infinity(kind, vocab):
     assert score[0, 3] == s.score[2] and (np.diff(score[0, 3:]) <= 0).all() and (beam[0, 4:] % 3 == 0).all()
     assert (beam[1] == 2).all() and token[1].tolist() == list(range(12)) and (score[1] == np.inf).all()  # (equal ones by their place)
     assert np.isfinite(score[2]).all() and np.array_equal(slot, np.take_along_axis(s.slot.reshape(3, 4), beam, 1))
+
+
+def faults(s):
+    r, b, _ = s.shape
+    got = [t[:-1].cpu().numpy().reshape(r, s.keep) for t in s.to]
+    return beam_check.faults(s.logits, s.score, s.ended, s.slot, b, s.keep, s.end, *got[:3], got[3] if s.slot is not None else None)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("requests,beams,vocab,keep", [(1, 1, 1, 1), (1, 1, 7, 3), (2, 4, 100, 8), (3, 5, 511, 5), (1, 8, 513, 16), (2, 3, 4097, 6), (1, 64, 1025, 128), (5, 4, 32003, 8), (1, 2, 200001, 4),
+                                                       (2, 32, 70000, 64), (3, 16, 9000, 128), (7, 7, 777, 7)])
+def test_every_successor(kind, requests, beams, vocab, keep):
+    for seed in range(3):
+        assert faults(Select(requests, beams, vocab, keep, kind, seed=vocab + seed, ended=0.2 if beams > 2 else 0.0, gap=seed, shift=seed).run()) == []
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_every_successor_of_beams_that_are_alike(kind):
+    """Beams a little apart, as those of one request are: the last places are close calls."""
+    for seed in range(6):
+        s = Select(4, 8, 5003, 16, kind, seed=seed)
+        s.score[:] = -3.0 + np.random.default_rng(seed).normal(size=32).astype(np.float32) * 1e-4
+        s.logits[:] = np.repeat(s.logits[::8], 8, axis=0)
+        assert faults(s.run()) == []
+
+
+def test_every_successor_where_little_is_allowed():
+    for kept in (1, 3, 40):
+        s = Select(3, 4, 3000, 20, "f16", seed=kept)
+        allowed = np.random.default_rng(kept).choice(3000, kept, replace=False)
+        mask = np.ones(3000, bool)
+        mask[allowed] = False
+        s.logits[:, mask] = -np.inf
+        s.logits[5], s.score[8:11] = np.nan, -np.inf
+        assert faults(s.run()) == []
