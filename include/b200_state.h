@@ -4,8 +4,9 @@
  * short convolution in front of it, the selection of a beam search, and what that makes necessary: slots that become what other slots held.
  *
  * A step's rows name their sequences through seq_info, int32 [4][n_seq]: a sequence's first row, its count of rows, its slot, and whether it begins (!= 0: its state and its last
- * inputs are zeros, whatever the slot holds).  Sequences with slots outside [0, n_slots), and whatever lies outside the n_tokens rows, are left out; rows that belong to no
- * sequence stay as they are.  A slot appears once in a step, and no two sequences have a row in common.  seq_info NULL: n_seq sequences of n_tokens / n_seq rows each, one behind the other, in the slots 0, 1, .., none of which begins.
+ * inputs are zeros, whatever the slot holds).  Sequences whose slot is outside [0, n_slots) or whose first row is none of the n_tokens are left out, and so are rows behind these; rows that belong
+ * to no sequence stay as they are, and so do the slots of sequences without rows, also of those that begin.  A slot appears once in a step, and no two sequences have a row in common.  seq_info
+ * NULL: n_seq sequences of n_tokens / n_seq rows each, one behind the other, in the slots 0, 1, .., none of which begins.
  * max_new: no sequence has more rows than that; those behind are left out (0: n_tokens).
  *
  * Types of rows: B200_TYPE_F32, B200_TYPE_F16, B200_TYPE_BF16, at any alignment of their own type; strides in values.  States, weights and sums are f32.  All functions
@@ -65,9 +66,10 @@ B200_API int b200_op_ssm_scan(const b200_ssm_scan_args *a, void *workspace, size
 /* ---- beam search -------------------------------------------------------------------------------------------------------------------------------------
  * Every request has n_beams beams, a row of logits each, one behind the other.  The successors of a beam that has not ended are all tokens: score[beam] + logit - ln(sum of exp(logits));
  * those of an ended one (ended != NULL and not 0 there) are end_token alone: score[beam].  The n_keep best of a request go to to_*, best first, equal ones in the order of
- * (beam, token); to_beam counts within the request, to_slot (optional) is that beam's entry of `slot`.  Scores are compared in 64 bits before they are rounded to f32.  A successor of
+ * (beam, token); to_beam counts within the request, to_slot (optional) is that beam's entry of `slot`.  Scores are compared in 64 bits before they are rounded to f32; the ln(sum) in
+ * them is a sum of f32 exponentials, good to 2^-21, so the order of successors of different beams is no better than that.  A successor of
  * score -inf is none: neither is a token whose logit is -inf or NaN, or any of a beam whose score is -inf or NaN.  (Beams of a request that has just begun: all scores but one are -inf.)
- * Where there are fewer than n_keep successors, the rest are score -inf, beam -1, token -1, slot -1.  With logits of +inf those tokens share their row evenly. */
+ * Where there are fewer than n_keep successors, the rest are score -inf, beam -1, token -1, slot -1.  The workspace (b200_beam_select_workspace_bytes bytes) is 8-byte aligned.  With logits of +inf those tokens share their row evenly. */
 #define B200_BEAM_MAX 64     /* beams of a request */
 #define B200_BEAM_KEEP 128   /* successors that are kept */
 #define B200_BEAM_VOCAB (1 << 30)

@@ -12,7 +12,7 @@ namespace beam {
 // Two launches.  The first reads the logits once: of every piece of PIECE tokens of a row (or a power of two of them) it keeps the largest, of every share of a row the sum of exponentials.
 // The second, a CTA a request, knows the logarithms of the sums then, and so every piece's best score.  The n_keep best successors all lie in the n_keep pieces whose best come first
 // (a successor elsewhere comes behind the best of each of these), so it reads those pieces again and nothing else.
-// What bounds it: the first launch memory (six instructions a token beside the loads), the second the way from one result to the next.
+// What bounds it: the first launch instructions (12.4 a token of 16 bits at odd places, issued 65 % of the time), the second the way from one result to the next: barriers, and code that is run once.
 // (The second launch is a chain of instructions, 7000 a warp of eight for 32 beams of 151936 tokens and 64 results, and its loads hide none of it: 49 us for both launches with 256 threads, 34 with 512,
 // 28 with 1024, whose 64 registers are too few for rows at odd places; four beams of 32000 tokens 10.4, 10.5 and 10.8.)
 constexpr int PIECE = 512, ROW_WARPS = 8, PICK_THREADS = 512, PICK_WARPS = PICK_THREADS / 32;

@@ -50,7 +50,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 // 2^x and 1 / x of the special function unit, off by 2^-22 and 2^-23; numbers below 2^-126 are zeros
 __device__ __forceinline__ float ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 __device__ __forceinline__ float rcp(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
-// y * sigmoid(y) (where e^-y is more than f32 holds, -0)
+// y * sigmoid(y): relative error 2^-21, and |y| 2^-23 more below 0 by the exponent's rounding; -0 below -87, where e^-y or its reciprocal leaves f32's normal numbers
 __device__ __forceinline__ float silu(float y) { return y * rcp(1.0f + ex2(-LOG2E * y)); }
 
 // two floats that are worked on by one instruction
@@ -219,7 +219,7 @@ static int launch_conv(ConvArgs a, cudaStream_t st) {
     a.rows = CONV_ROWS_MAX;
     while (a.rows > CONV_ROWS_MIN && (int64_t)across * ((a.step.n_tokens + a.rows - 1) / a.rows) < 8 * (int64_t)sm_count()) a.rows /= 2;
     const dim3 grid(across, (unsigned)((a.step.max_new + a.rows - 1) / a.rows), (unsigned)a.step.n_seq);
-    // the ring pays where there is something to wait for: 64 sequences of one row, f32: 4.5 us with it, 3.8 without; 5330 rows, bf16: 40 and 46 us
+    // the ring pays where there is something to wait for (5330 rows, bf16: 36 us with it, 51 without); for 64 sequences of one or three rows it is 4.2 to 4.4 us either way, and shared memory is left alone
     const bool ring = V * sizeof(T) >= 8 && a.step.max_new > 2 * CONV_GROUP;
     B200_CUDA_TRY(launch_chained(ring ? ssm_conv_kernel<T, K, V, EXACT, (V * sizeof(T) >= 8)> : ssm_conv_kernel<T, K, V, EXACT, false>, grid, CONV_THREADS, 0, st, a));
     return B200_OK;
@@ -348,7 +348,8 @@ __device__ __forceinline__ float4 load_row4(const T *row, int n0, int d_state, b
 
 // ===== one row a sequence.  A warp takes 32 channels; L lanes share a channel, a lane four of its states, so that a load of the warp is 512 consecutive bytes of the state.  What a channel
 // needs by itself (d, d x, z) is made by one lane and handed to the other L - 1; the sums of L channels are exchanged so that each lane ends up with one of them.  What takes longest is asked for
-// first.  What bounds it is instructions as much as memory (96 sequences of 8192 channels, 16 states: 4 TB/s); sequences one after the other in a warp, whose rates would stay, are 45 us instead of 26.
+// first.  What bounds it is waiting for memory with 38 % of an SM's warps there (96 sequences of 8192 channels, 16 states: 25.5 us, 4.2 TB/s;
+// half of the cycles between two instructions of a warp are waits for loads, instructions are issued 58 % of the time); sequences one after the other in a warp, whose rates would stay, are 45 us.
 constexpr int STEP_WARPS = 2;
 template <typename T, int L, bool VEC>
 __global__ void __launch_bounds__(32 * STEP_WARPS) ssm_step_kernel(const ScanArgs a) {
@@ -444,7 +445,7 @@ __global__ void __launch_bounds__(32 * STEP_WARPS) ssm_step_kernel(const ScanArg
 // and multiply-adds of a row are chains that run side by side.  b and c of a chunk of rows wait in shared memory, where all lanes read the same words.  Rows go in groups of TG; lane p of a channel makes d and d x of the group's rows p, p + L, ..,
 // and sends off their results; the next group's rows are loaded meanwhile.
 // What bounds it: exponentials, d_state + 3 for each row and channel at 16 a cycle and SM (four prompts of 2048 rows x 8192 channels: 283 us), and that 1024 warps make two on some schedulers and one
-// on others, where a row takes 370 cycles: 447 us.  Some of the exponentials made by multiply-adds (two or four of 16 as polynomials) gave nothing: the other instructions, 90 a row, fill up what that leaves.
+// on others: 456 us, 445 cycles a row, of which the unit has 304 to do where there are two.  Some of the exponentials made by multiply-adds (two or four of 16 as polynomials) gave nothing: the other instructions, 104 a row in all, fill up what that leaves.
 constexpr int SCAN_WARPS = 4, SCAN_THREADS = 32 * SCAN_WARPS;
 // the things that a CTA can be there for: a whole sequence, with few CTAs or with many; the state at the end of a stretch as if it began from nothing (the first one: from the sequence's state), and the sum of
 // its d; a stretch's rows, from the states and sums of those before it
@@ -456,9 +457,10 @@ struct ScanSizes {
     static constexpr int PIECES = (2 * TC * NP / 4 + SCAN_THREADS - 1) / SCAN_THREADS;  // pieces of four numbers of b or c that a thread fetches
 };
 // Rows of a group, and CTAs that an SM is to hold.  A lane that is a channel, in few CTAs: long groups in the order that the compiler gives them with 255 registers (four long prompts, 1.7 CTAs
-// an SM: 16 rows 447 us; 8 rows 460, with 168 registers 473, with 128 629).  Where there are CTAs for every place that an SM has, more places are worth more: short groups, four CTAs (128 sequences of
-// 48 rows, 8192 channels: 285 us, 351 the other way; of 5 rows, where a long group would also walk what is not there, 81 and 186).  Stretches stay with the first (one prompt of 4096 rows of 2048
-// channels: 96 us, 107 the other way; of 8192 channels: 398 and 373).  With exchanges between lanes: four CTAs (64 states: 188 us, with three 300).
+// an SM: 16 rows 455 us, 8 rows 462).  Where there are CTAs for every place that an SM has, more places are worth more: short groups, four CTAs (128 sequences of
+// 48 rows, 8192 channels: 287 us, 357 the other way; of 5 rows, where a long group would also walk what is not there, 81 and 187).  Stretches stay with the first: one prompt of 4096 rows of 2048
+// channels 103 us, 121 the other way; of 5120 channels 255 and 258; of 8192 channels 408 and 377, where the other way would be the better one.  With exchanges between lanes there is one way, four CTAs
+// and groups of 8 rows (64 states: 189 us, with three CTAs 300).
 constexpr int SCAN_SHORT = 32;  // rows up to which sequences take the second way whatever the number of CTAs
 constexpr int scan_rows(int lanes, int pass) { return lanes > 1 ? 8 : pass == MANY ? 4 : 16; }
 constexpr int scan_ctas(int lanes, int pass) { return lanes > 1 || pass == MANY ? 4 : 2; }
@@ -469,7 +471,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L, PASS)) ssm_scan_ker
     using Z = ScanSizes<L, NS>;
     constexpr int CB = Z::CB, NP = Z::NP, TC = Z::TC, NQ = NS / 4, TG = scan_rows(L, PASS), MT = TG / L;  // TG: rows of a group; MT: those that a lane makes ready
     __shared__ __align__(16) float sbc[2][2][TC][NP];  // [chunk & 1][b, c]
-    pdl_wait();  // (the kernel behind is let in at the end: CTAs of it that wait would take places in an order that leaves SMs unequal, 520 -> 610 us for four long prompts)
+    pdl_wait();  // (the kernel behind is let in at the end: its CTAs would wait in places of this one's.  Four long prompts 455 us, let in at the beginning 456)
     const int tid = threadIdx.x, lane = tid & 31, p = lane % L;
     const Seq q = seq_of(a.step, blockIdx.z);
     const int N = a.d_state, blocks = (a.per_group + CB - 1) / CB, group = blockIdx.x / blocks, in_group = (blockIdx.x - group * blocks) * CB + tid / L;
@@ -785,8 +787,9 @@ static ScanPlan plan_of(const b200_ssm_scan_args *a) {
     const double ctas = (double)((per_group + block - 1) / block) * a->groups * a->n_tokens / longest;
     p.many = longest <= SCAN_SHORT || ctas >= 3.0 * sm_count();
     if (ctas < 1.25 * sm_count() && longest >= 128) {
-        // One sequence: as many CTAs as are there at once (4096 rows of 2048 channels: 96 us; twice as many: 120).  Several, whose ends come at different times: more than that (six of 37 to 1501 rows of
-        // 5120 channels: 265 us with four an SM, 298 with two).
+        // One sequence: as many CTAs as are there at once (4096 rows of 2048 channels: 103 us; twice as many: 130).  Several: four an SM, which pays where they end at different times and there is enough
+        // of them (six of 37 to 1501 rows of 5120 channels: 272 us, 309 with two), is little either way for prompts of one length (two of 2048 rows: of 2048 channels 116 and 113, of 5120 257 and
+        // 262) and loses where channels are few (three of 100 to 2000 rows of 2048 channels: 104 and 86; three of 4096 rows of 512: 113 and 92).
         const double n = (double)(a->n_seq > 1 ? 4 : scan_ctas(lanes_of(a->d_state), ENDS)) * sm_count() / ctas;
         const int rows = (int)(longest / (n < 32 ? n : 32));
         p.stretch = ((rows < 64 ? 64 : rows) + 7) / 8 * 8;
