@@ -58,7 +58,14 @@ using Two = unsigned long long;
 __device__ __forceinline__ Two two(float lo, float hi) { Two r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi)); return r; }
 __device__ __forceinline__ float2 each(Two x) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x)); return r; }
 __device__ __forceinline__ Two fma2(Two x, Two y, Two z) { Two r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z)); return r; }
+__device__ __forceinline__ Two add2(Two x, Two y) { Two r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y)); return r; }
 __device__ __forceinline__ Two mul2(Two x, Two y) { Two r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y)); return r; }
+
+// silu of two values
+__device__ __forceinline__ Two silu2(Two z) {
+    const float2 turn = each(mul2(z, two(-LOG2E, -LOG2E))), all = each(add2(two(ex2(turn.x), ex2(turn.y)), two(1.0f, 1.0f)));
+    return mul2(z, two(rcp(all.x), rcp(all.y)));
+}
 
 // ------------------------------------------------------------------------------------------------ short convolution
 // A thread takes V channels of `rows` rows of one sequence and keeps the last K - 1 inputs in registers; rows travel in groups, asynchronously to a ring in shared memory.  The CTAs that hold a
@@ -478,6 +485,9 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L, PASS)) ssm_scan_ker
     const bool mine = in_group < a.per_group;
     const int c = group * a.per_group + min(in_group, a.per_group - 1);  // the lane's channel (those behind the group's last walk along with it and leave nothing)
     constexpr bool ALL = PASS == WHOLE || PASS == MANY;
+    // what is done to every row by itself is done to two at a time: one prompt of 4096 rows of 2048 channels 103 -> 100 us, six ragged ones 273 -> 270; short groups are better off without (128 sequences of 48
+    // rows 287 -> 291)
+    constexpr bool PAIRS = MT > 1 && PASS != MANY;
     const int stretch = ALL ? 0 : blockIdx.y, begin = ALL ? 0 : stretch * a.stretch, end = ALL ? q.count : min(q.count, begin + a.stretch);
     if (begin >= end) return;
     const bool last = end == q.count;
@@ -597,7 +607,17 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L, PASS)) ssm_scan_ker
             for (int j = 0; j < MT; j++) {
                 x[j] = wide(nx[j]);
                 if (PASS != ENDS) z[j] = wide(nz[j]);
-                d[j] = wide(ndt[j]) + bias;
+                d[j] = wide(ndt[j]);
+            }
+            if constexpr (!PAIRS) {
+#pragma unroll
+                for (int j = 0; j < MT; j++) d[j] += bias;
+            } else {
+#pragma unroll
+                for (int j = 0; j < MT; j += 2) {
+                    const float2 v = each(add2(two(d[j], d[j + 1]), two(bias, bias)));
+                    d[j] = v.x; d[j + 1] = v.y;
+                }
             }
             if (a.softplus) {
                 if constexpr (MT == 1) {
@@ -615,9 +635,15 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L, PASS)) ssm_scan_ker
 #pragma unroll
                 for (int j = 0; j < MT; j++) if (r0 + tg + j * L + p >= rows) d[j] = 0.f;
             }
+            if constexpr (!PAIRS) {
 #pragma unroll
-            for (int j = 0; j < MT; j++) {
-                dx[j] = d[j] * x[j];
+                for (int j = 0; j < MT; j++) dx[j] = d[j] * x[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < MT; j += 2) {
+                    const float2 v = each(mul2(two(d[j], d[j + 1]), two(x[j], x[j + 1])));
+                    dx[j] = v.x; dx[j + 1] = v.y;
+                }
             }
             if (PASS == ENDS) {
                 float some = d[0];
@@ -687,12 +713,28 @@ __global__ void __launch_bounds__(SCAN_THREADS, scan_ctas(L, PASS)) ssm_scan_ker
             }
             // (0 times an x that is not finite would be no number: no skip is no product)
             if (a.d) {
+                if constexpr (!PAIRS) {
 #pragma unroll
-                for (int j = 0; j < MT; j++) y[j * L] = fmaf(skip, x[j], y[j * L]);
+                    for (int j = 0; j < MT; j++) y[j * L] = fmaf(skip, x[j], y[j * L]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < MT; j += 2) {
+                        const float2 v = each(fma2(two(skip, skip), two(x[j], x[j + 1]), two(y[j * L], y[j * L + L])));
+                        y[j * L] = v.x; y[j * L + L] = v.y;
+                    }
+                }
             }
             if (pz) {
+                if constexpr (!PAIRS) {
 #pragma unroll
-                for (int j = 0; j < MT; j++) y[j * L] *= silu(z[j]);
+                    for (int j = 0; j < MT; j++) y[j * L] *= silu(z[j]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < MT; j += 2) {
+                        const float2 v = each(mul2(two(y[j * L], y[j * L + L]), silu2(two(z[j], z[j + 1]))));
+                        y[j * L] = v.x; y[j * L + L] = v.y;
+                    }
+                }
             }
             if (mine && full) {
 #pragma unroll
