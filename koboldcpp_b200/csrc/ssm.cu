@@ -309,10 +309,10 @@ __device__ __forceinline__ float finite(float x) {
 }
 
 // 2^(2 half) * s + e for two states.  In two steps, since a stretch over which states grow has a factor that f32 may not hold, and what it meets may be zero or small enough to stay in range.
-// (The bound keeps zeros what they are; a normal number is infinite behind it.)
+// (The bounds keep zeros and infinities what they are; a normal number is infinite behind the upper one, and below 2^-124 behind the lower.)
 __device__ __forceinline__ Two carried(Two half, Two s, Two e) {
     const float2 v = each(half);
-    const Two f = two(ex2(fminf(v.x, 127.f)), ex2(fminf(v.y, 127.f)));
+    const Two f = two(ex2(fmaxf(fminf(v.x, 127.f), -126.f)), ex2(fmaxf(fminf(v.y, 127.f), -126.f)));
     return fma2(f, mul2(f, s), e);
 }
 

@@ -140,3 +140,16 @@ def test_single_rows_beside_prompts_in_stretches(kind, n, groups, max_new):
     ws = run(a)
     assert ws.numel() > 16
     s.verify(max_new)
+
+
+@pytest.mark.parametrize("n", [5, 16, 40])
+def test_infinite_states_that_fade_over_a_stretch(n):
+    """A factor of e^-5 a row: an infinite state stays so, however many rows there are, and a finite one leaves nothing behind."""
+    s = Scan([(300, 1, False)], 40, n, "f32", bias=False, gate=False, skip=False, seed=n)
+    s.dt[:], s.a[:] = 5.0, -1.0
+    s.b, s.c = np.abs(s.b) + 0.125, np.abs(s.c) + 0.125
+    s.state[1, 3], s.state[1, 4], s.state[1, 5] = np.inf, -np.inf, 3e38
+    run(s.upload())
+    got, want, got_state, state = same_kinds(s)
+    there = np.isfinite(want)
+    assert there[:, 5].all() and np.allclose(got[there], want[there], rtol=1e-4, atol=1e-4) and np.allclose(got_state[1, 5], state[1, 5], rtol=1e-4, atol=1e-4)
