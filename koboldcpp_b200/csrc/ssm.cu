@@ -267,7 +267,7 @@ __device__ __forceinline__ float down(float x) {
 // ln(1 + e^x) = max(x, 0) + ln(1 + e^-|x|), and ln(1 + e) = e P(e) on [0, 1] with a polynomial whose relative error is smallest at its largest (fitted by weighted least squares on
 // Chebyshev points; 1.8e-7 with the roundings of f32): one exponential on the special function unit and nothing else there, no overflow, no cancellation.  What the exponential's argument loses, its
 // rounding and what LOG2E has not of log2 e, is made good to first order: where e is small all of the result is e, and such steps are the usual ones of a trained layer.  (Relative error for x of
-// -12 .. -6: 2.6e-7 at most, 7.0e-8 root mean square, -5e-8 in the mean; without it 8.9e-7, 2.5e-7 and +7e-8, and more further out.  Four prompts of 2048 rows: 448 -> 456 us.)
+// -12 .. -6: 2.6e-7 at most, 7.0e-8 root mean square, -5e-8 in the mean; without it 8.9e-7, 2.5e-7 and +7e-8, and more further out.  Four prompts of 2048 rows: 448 -> 455 us.)
 __device__ __forceinline__ float2 softplus2(float2 x) {
     auto both = [](float v) { return two(v, v); };
     const Two far = two(down(x.x), down(x.y)), turn = mul2(far, both(LOG2E));
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(32 * STEP_WARPS) ssm_step_kernel(const ScanArg
 // and multiply-adds of a row are chains that run side by side.  b and c of a chunk of rows wait in shared memory, where all lanes read the same words.  Rows go in groups of TG; lane p of a channel makes d and d x of the group's rows p, p + L, ..,
 // and sends off their results; the next group's rows are loaded meanwhile.
 // What bounds it: exponentials, d_state + 3 for each row and channel at 16 a cycle and SM (four prompts of 2048 rows x 8192 channels: 283 us), and that 1024 warps make two on some schedulers and one
-// on others: 456 us, 445 cycles a row, of which the unit has 304 to do where there are two.  Some of the exponentials made by multiply-adds (two or four of 16 as polynomials) gave nothing: the other instructions, 104 a row in all, fill up what that leaves.
+// on others: 455 us, 445 cycles a row, of which the unit has 304 to do where there are two.  Some of the exponentials made by multiply-adds (two or four of 16 as polynomials) gave nothing: the other instructions, 100 a row in all, fill up what that leaves.
 constexpr int SCAN_WARPS = 4, SCAN_THREADS = 32 * SCAN_WARPS;
 // the things that a CTA can be there for: a whole sequence, with few CTAs or with many; the state at the end of a stretch as if it began from nothing (the first one: from the sequence's state), and the sum of
 // its d; a stretch's rows, from the states and sums of those before it
@@ -466,7 +466,7 @@ struct ScanSizes {
 // Rows of a group, and CTAs that an SM is to hold.  A lane that is a channel, in few CTAs: long groups in the order that the compiler gives them with 255 registers (four long prompts, 1.7 CTAs
 // an SM: 16 rows 455 us, 8 rows 462).  Where there are CTAs for every place that an SM has, more places are worth more: short groups, four CTAs (128 sequences of
 // 48 rows, 8192 channels: 287 us, 357 the other way; of 5 rows, where a long group would also walk what is not there, 81 and 187).  Stretches stay with the first: one prompt of 4096 rows of 2048
-// channels 103 us, 121 the other way; of 5120 channels 255 and 258; of 8192 channels 408 and 377, where the other way would be the better one.  With exchanges between lanes there is one way, four CTAs
+// channels 100 us, 122 the other way; of 5120 channels 250 and 259; of 8192 channels 405 and 378, where the other way would be the better one.  With exchanges between lanes there is one way, four CTAs
 // and groups of 8 rows (64 states: 189 us, with three CTAs 300).
 constexpr int SCAN_SHORT = 32;  // rows up to which sequences take the second way whatever the number of CTAs
 constexpr int scan_rows(int lanes, int pass) { return lanes > 1 ? 8 : pass == MANY ? 4 : 16; }
@@ -829,9 +829,10 @@ static ScanPlan plan_of(const b200_ssm_scan_args *a) {
     const double ctas = (double)((per_group + block - 1) / block) * a->groups * a->n_tokens / longest;
     p.many = longest <= SCAN_SHORT || ctas >= 3.0 * sm_count();
     if (ctas < 1.25 * sm_count() && longest >= 128) {
-        // One sequence: as many CTAs as are there at once (4096 rows of 2048 channels: 103 us; twice as many: 130).  Several: four an SM, which pays where they end at different times and there is enough
-        // of them (six of 37 to 1501 rows of 5120 channels: 272 us, 309 with two), is little either way for prompts of one length (two of 2048 rows: of 2048 channels 116 and 113, of 5120 257 and
-        // 262) and loses where channels are few (three of 100 to 2000 rows of 2048 channels: 104 and 86; three of 4096 rows of 512: 113 and 92).
+        // One sequence: as many CTAs as are there at once (4096 rows of 2048 channels: 100 us, twice as many 126; of 5120 channels 250 and 272; of 8192 channels
+        // 405 and 375, where more would be better).  Several: four an SM, which pays where they end at different times and there is enough
+        // of them (six of 37 to 1501 rows of 5120 channels: 270 us, 306 with two), is little either way for prompts of one length (two of 2048 rows: of 2048 channels 115 and 112, of 5120 256 and
+        // 260) and loses where channels are few (three of 100 to 2000 rows of 2048 channels: 103 and 86; three of 4096 rows of 512: 112 and 91).
         const double n = (double)(a->n_seq > 1 ? 4 : scan_ctas(lanes_of(a->d_state), ENDS)) * sm_count() / ctas;
         const int rows = (int)(longest / (n < 32 ? n : 32));
         p.stretch = ((rows < 64 ? 64 : rows) + 7) / 8 * 8;
